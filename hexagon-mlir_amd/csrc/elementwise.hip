@@ -211,24 +211,7 @@ void rope_kernel(const T* __restrict__ x, T* __restrict__ y, int batch, int seq,
 #pragma unroll
   for (int p = 0; p < N / 2; ++p) {
     if (p > 0) freq *= pair_ratio;
-    // the angle m*freq in double, reduced in double to a quarter turn number q and a remainder in [-pi/4, pi/4]
-    // (so it is accurate to fp32 for any m), then fp32 polynomials for the sine and cosine of the remainder (the
-    // single-precision minimax coefficients of the Cephes library, errors near 1e-7) and the quadrant's swap and
-    // signs: about half the instructions of sincosf, which reduces its argument once more
-    double turns = (double)m * freq * 0.15915494309189533577;        // 1 / (2 pi)
-    turns -= floor(turns);
-    const double q = rint(turns * 4.0);                              // 0 .. 4
-    const float rem = (float)((turns - 0.25 * q) * 6.28318530717958647692);
-    const int qi = (int)q & 3;
-    const float z = rem * rem;
-    const float sp = fmaf(rem * z, fmaf(z, fmaf(z, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), rem);
-    const float cp = fmaf(z * z, fmaf(z, fmaf(z, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f),
-                          fmaf(z, -0.5f, 1.0f));
-    float s = (qi & 1) ? cp : sp, c = (qi & 1) ? sp : cp;
-    if (qi & 2) s = -s;
-    if (qi == 1 || qi == 2) c = -c;
-    cs[p] = c;
-    sn[p] = s;
+    sincos_turns((double)m * freq * 0.15915494309189533577, sn[p], cs[p]);        // 1 / (2 pi)
   }
   const int rows = batch * heads;                    // < 2^31: checked by the launcher
   // one row in flight per thread: with the next row's load issued ahead the kernel measured 5 % slower.

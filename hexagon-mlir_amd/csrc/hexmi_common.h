@@ -102,6 +102,26 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(a, b);
 }
 
+// Sine and cosine of `turns` whole turns. The angle is reduced in double to a quarter turn number q and a remainder in
+// [-pi/4, pi/4] (so it is accurate to fp32 however many turns), then fp32 polynomials for the sine and cosine of the remainder
+// (the single-precision minimax coefficients of the Cephes library, errors near 1e-7) and the quadrant's swap and signs: about
+// half the instructions of sincosf, which reduces its argument once more.
+__device__ __forceinline__ void sincos_turns(double turns, float& sn, float& cs) {
+  turns -= floor(turns);
+  const double q = rint(turns * 4.0);                              // 0 .. 4
+  const float rem = (float)((turns - 0.25 * q) * 6.28318530717958647692);
+  const int qi = (int)q & 3;
+  const float z = rem * rem;
+  const float sp = fmaf(rem * z, fmaf(z, fmaf(z, -1.9515295891e-4f, 8.3321608736e-3f), -1.6666654611e-1f), rem);
+  const float cp = fmaf(z * z, fmaf(z, fmaf(z, 2.443315711809948e-5f, -1.388731625493765e-3f), 4.166664568298827e-2f),
+                        fmaf(z, -0.5f, 1.0f));
+  float s = (qi & 1) ? cp : sp, c = (qi & 1) ? sp : cp;
+  if (qi & 2) s = -s;
+  if (qi == 1 || qi == 2) c = -c;
+  sn = s;
+  cs = c;
+}
+
 // ---- int8 -> fp16 (weight-only quantisation) --------------------------------
 // 4 int8 (one dword) -> 4 fp16 in two dwords, exact (|w| <= 128 has at most eight significant bits): one
 // v_cvt_f16_i16 per weight, its source the sign-extended byte picked by the instruction's operand selector and its

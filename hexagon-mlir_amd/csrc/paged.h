@@ -1,0 +1,70 @@
+// What the kernels of a paged cache share: whole-number division by an argument, the tokens of a batch, where a position stands.
+#pragma once
+#include "hexmi_common.h"
+
+namespace hexmi {
+
+// n / d for 0 <= n < 2^31, by a product (d from 1): with l = ceil(log2 d), m = ceil(2^(31 + l) / d) is below 2^32 and exceeds
+// 2^(31 + l) / d by less than 2^l / d <= 2^(31 + l) / (d n), so the floor is right.
+struct Divider {
+  uint32_t m, shift;
+};
+inline Divider divider(int64_t d) {
+  uint32_t l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return {(uint32_t)(((uint64_t(1) << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), 31 + l};
+}
+#if defined(__HIPCC__)
+__device__ __forceinline__ int divided(int n, const Divider& d) { return (int)(((uint64_t)(uint32_t)n * d.m) >> d.shift); }
+#endif
+
+// hexmi_paged_batch as the kernels take it: sizes below 2^31 (batch_fits), strides in elements.
+struct Pages {
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  const int32_t *table, *lengths, *starts;
+  int64_t table_row;
+  int num_pages, page_size, table_cols, sequences, tokens, kv_heads;
+  Divider size;
+};
+inline Pages pages_of(const hexmi_paged_batch& b) {
+  return {b.k_page, b.k_head, b.k_slot, b.v_page, b.v_head, b.v_slot, b.page_table, b.lengths, b.starts, b.table_row, (int)b.num_pages,
+          (int)b.page_size, (int)b.table_cols, (int)b.sequences, (int)b.tokens, (int)b.kv_heads, divider(b.page_size)};
+}
+// HEXMI_OK, or why a batch is refused (pointers aside)
+inline int check_batch(const hexmi_paged_batch& b) {
+  if (b.num_pages < 1 || b.page_size < 1 || b.kv_heads < 1 || b.dim < 1 || b.table_cols < 0 || b.sequences < 0 || b.tokens < 0 ||
+      (b.sequences > 1 && b.table_row < b.table_cols))
+    return HEXMI_EINVAL;
+  if (!b.starts && b.sequences != b.tokens) return HEXMI_EINVAL;
+  constexpr int64_t most = 0x7fffffff;
+  if (b.num_pages > most || b.page_size > most || b.kv_heads > 65535 || b.table_cols > most || b.sequences > most / 2 || b.tokens > most / 2 ||
+      (b.table_cols > 0 && b.page_size > (most - 1024) / b.table_cols))
+    return HEXMI_ENOTSUP;
+  return HEXMI_OK;
+}
+
+#if defined(__HIPCC__)
+// The sequence of row t: the last b with starts[b] <= t, by the 64 lanes of a wave together (t the same for all): 64 places are asked
+// at once, so 64 sequences take one read and 4096 two. -1: none (below starts[0], from starts[sequences] on).
+__device__ __forceinline__ int sequence_of(const Pages& p, int t, int lane) {
+  int lo = 0, hi = p.sequences + 1;                       // among starts[0 .. sequences]
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const bool below = at < hi && p.starts[at] <= t;
+    const int n = __popcll(__ballot(below));
+    if (n == 0) return -1;
+    lo += (n - 1) * step;
+    hi = lo + step < hi ? lo + step : hi;
+    if (step == 1) break;
+  }
+  return lo < p.sequences && p.starts[lo] <= t ? lo : -1;
+}
+
+// The positions of sequence b that have a place in the table, whatever lengths holds.
+__device__ __forceinline__ int length_of(const Pages& p, int b) {
+  const int most = p.table_cols * p.page_size, n = p.lengths[b];
+  return n < 0 ? 0 : n < most ? n : most;
+}
+#endif
+
+}  // namespace hexmi

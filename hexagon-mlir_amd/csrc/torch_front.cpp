@@ -315,6 +315,155 @@ PyObject* binary(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// rows of heads [tokens, heads, dim] where they stand, the columns adjacent; heads counts from one
+const at::Tensor* head_rows(PyObject* o, at::ScalarType type) {
+  const at::Tensor* t = dense(o);
+  return t && t->dim() == 3 && t->scalar_type() == type && (t->stride(2) == 1 || t->size(2) == 1) ? t : nullptr;
+}
+int64_t stride(const at::Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+hexmi_head_rows rows_of(const at::Tensor* x, at::Tensor* out, const at::Tensor* weight) {
+  return {in(x), out ? out->mutable_data_ptr() : nullptr, in(weight), x->size(1), stride(*x, 0), stride(*x, 1),
+          out ? out->stride(0) : 0, out ? out->stride(1) : 0};
+}
+// inv_freq or None, eps, pairs
+bool rotation_of(PyObject* freq, PyObject* eps, PyObject* pairs, const at::Tensor& like, int64_t dim, hexmi_rotation& r) {
+  double e;
+  if (!number(eps, e) || !PyUnicode_CheckExact(pairs)) return false;
+  const bool halves = PyUnicode_CompareWithASCIIString(pairs, "halves") == 0;
+  if (!halves && PyUnicode_CompareWithASCIIString(pairs, "adjacent") != 0) return false;
+  r = {nullptr, 0, halves ? HEXMI_PAIRS_HALVES : HEXMI_PAIRS_ADJACENT, (float)e};
+  if (freq == Py_None) return true;
+  const at::Tensor* f = contiguous(freq);
+  if (!f || f->dim() != 1 || f->scalar_type() != at::kDouble || f->device() != like.device() || 2 * f->size(0) > dim) return false;
+  r.inv_freq = static_cast<const double*>(in(f));
+  r.columns = 2 * f->size(0);
+  return true;
+}
+const at::Tensor* index(PyObject* o, int64_t dims, const at::Tensor& like) {
+  const at::Tensor* t = contiguous(o);
+  return t && t->dim() == dims && t->scalar_type() == at::kInt && t->device() == like.device() ? t : nullptr;
+}
+// k_pages, v_pages, page_table, lengths, starts or None
+bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, hexmi_paged_batch& b) {
+  const at::Tensor *k = dense(a[0]), *v = k ? dense(a[1]) : nullptr;
+  if (!v || k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != rows.scalar_type() || v->scalar_type() != k->scalar_type() ||
+      k->device() != rows.device() || v->device() != k->device() || k->size(3) != dim || k->stride(3) != 1 || v->stride(3) != 1)
+    return false;
+  const at::Tensor *table = index(a[2], 2, rows), *lengths = index(a[3], 1, rows), *starts = nullptr;
+  if (!table || !lengths || table->size(0) != lengths->size(0)) return false;
+  if (a[4] != Py_None) {
+    starts = index(a[4], 1, rows);
+    if (!starts || starts->size(0) != lengths->size(0) + 1) return false;
+  } else if (lengths->size(0) != rows.size(0)) {
+    return false;
+  }
+  b = {k->mutable_data_ptr(), v->mutable_data_ptr(), stride(*k, 0), stride(*k, 1), stride(*k, 2), stride(*v, 0), stride(*v, 1), stride(*v, 2),
+       k->size(0), k->size(2), k->size(1), dim, static_cast<const int32_t*>(in(table)), table->size(1), table->size(1),
+       static_cast<const int32_t*>(in(lengths)), static_cast<const int32_t*>(in(starts)), lengths->size(0), rows.size(0)};
+  return true;
+}
+PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
+  PyObject* x = THPVariable_Wrap(std::move(a));
+  PyObject* y = x ? THPVariable_Wrap(std::move(b)) : nullptr;
+  PyObject* r = y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return r;
+}
+
+// qk_norm_rope(q, k or None, q_weight or None, k_weight or None, inv_freq or None, positions or None, eps, pairs)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* q = n == 8 ? dense(v[0]) : nullptr;
+    if (!q || !code_of(q->scalar_type()) || !(q = head_rows(v[0], q->scalar_type()))) HEXMI_NOT_PLAIN;
+    const at::ScalarType type = q->scalar_type();
+    const int64_t T = q->size(0), D = q->size(2);
+    const at::Tensor *k = nullptr, *qw, *kw, *pos = nullptr;
+    if (v[1] != Py_None && (!(k = head_rows(v[1], type)) || k->size(0) != T || k->size(2) != D || k->device() != q->device())) HEXMI_NOT_PLAIN;
+    hexmi_rotation turn;
+    if (!optional(v[2], qw, {D}, type, *q) || !optional(v[3], kw, {D}, type, *q) || (kw && !k) ||
+        !rotation_of(v[4], v[6], v[7], *q, D, turn)) HEXMI_NOT_PLAIN;
+    if (v[5] != Py_None) {
+      pos = contiguous(v[5]);
+      if (!pos || pos->dim() != 1 || pos->size(0) != T || pos->device() != q->device() ||
+          (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) HEXMI_NOT_PLAIN;
+    }
+    if (turn.columns && !pos) HEXMI_NOT_PLAIN;
+    const Launch at(*q);
+    if (!at.ok) HEXMI_NOT_PLAIN;
+    at::Tensor qo = fresh(q->sizes(), type, *q), ko;
+    hexmi_head_rows qr = rows_of(q, &qo, qw), kr = {};
+    if (k) {
+      ko = fresh(k->sizes(), type, *k);
+      kr = rows_of(k, &ko, kw);
+    }
+    const int status = unlocked(hexmi_qk_norm_rope, &qr, k ? &kr : nullptr, &turn, in(pos), pos && pos->scalar_type() == at::kLong ? 1 : 0, T, D,
+                                code_of(type), at.stream);
+    if (status != HEXMI_OK || !k) return finish(status, "hexmi_qk_norm_rope", std::move(qo));
+    return pair(std::move(qo), std::move(ko));
+  });
+}
+
+// paged_append(k, v, k_pages, v_pages, page_table, lengths, starts or None, k_weight or None, inv_freq or None, eps, pairs, q or None,
+// q_weight or None): q's rows, or True
+PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* k = n == 13 ? dense(a[0]) : nullptr;
+    if (!k || (k->scalar_type() != at::kHalf && k->scalar_type() != at::kBFloat16) || !(k = head_rows(a[0], k->scalar_type()))) HEXMI_NOT_PLAIN;
+    const at::ScalarType type = k->scalar_type();
+    const int64_t D = k->size(2);
+    const at::Tensor *v = head_rows(a[1], type), *q = nullptr, *kw, *qw;
+    hexmi_paged_batch batch;
+    hexmi_rotation turn;
+    if (!v || v->sizes() != k->sizes() || v->device() != k->device() || !batch_of(a + 2, *k, D, batch) || batch.kv_heads != k->size(1) ||
+        !optional(a[7], kw, {D}, type, *k) || !rotation_of(a[8], a[9], a[10], *k, D, turn) || !optional(a[12], qw, {D}, type, *k))
+      HEXMI_NOT_PLAIN;
+    if (a[11] != Py_None) {
+      q = head_rows(a[11], type);
+      if (!q || q->size(0) != k->size(0) || q->size(2) != D || q->device() != k->device()) HEXMI_NOT_PLAIN;
+    } else if (qw) {
+      HEXMI_NOT_PLAIN;
+    }
+    const Launch at(*k);
+    if (!at.ok) HEXMI_NOT_PLAIN;
+    const hexmi_head_rows kr = rows_of(k, nullptr, kw), vr = rows_of(v, nullptr, nullptr);
+    hexmi_head_rows qr = {};
+    at::Tensor qo;
+    if (q) {
+      qo = fresh(q->sizes(), type, *q);
+      qr = rows_of(q, &qo, qw);
+    }
+    const int status = unlocked(hexmi_paged_append, &kr, &vr, q ? &qr : nullptr, &turn, &batch, code_of(type), at.stream);
+    if (status != HEXMI_OK || q) return finish(status, "hexmi_paged_append", std::move(qo));
+    Py_RETURN_TRUE;
+  });
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, lengths, starts or None, sm_scale or None, shared_pages or None)
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* q = n == 8 ? dense(a[0]) : nullptr;
+    if (!q || (q->scalar_type() != at::kHalf && q->scalar_type() != at::kBFloat16) || !(q = head_rows(a[0], q->scalar_type()))) HEXMI_NOT_PLAIN;
+    const int64_t H = q->size(1), D = q->size(2);
+    if (D % 8 != 0 || D > 256 || stride(*q, 0) % 8 != 0 || stride(*q, 1) % 8 != 0 || reinterpret_cast<uintptr_t>(in(q)) % 16 != 0) HEXMI_NOT_PLAIN;
+    hexmi_paged_batch batch;
+    if (!batch_of(a + 1, *q, D, batch) || H % batch.kv_heads != 0) HEXMI_NOT_PLAIN;
+    double scale = 1.0 / std::sqrt((double)D);
+    if ((a[6] != Py_None && !number(a[6], scale)) || !(scale > 0.0 && scale < 3e38)) HEXMI_NOT_PLAIN;
+    const at::Tensor* shared = nullptr;
+    if (a[7] != Py_None && (!(shared = index(a[7], 1, *q)) || shared->size(0) > batch.table_cols)) HEXMI_NOT_PLAIN;
+    const Launch at(*q);
+    if (!at.ok) HEXMI_NOT_PLAIN;
+    at::Tensor out = fresh(q->sizes(), q->scalar_type(), *q);
+    const hexmi_head_rows qr = rows_of(q, &out, nullptr);
+    const int64_t pages = shared ? shared->size(0) : 0, bytes = hexmi_paged_attention_workspace(&batch, H, pages);
+    const at::Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, *q) : at::Tensor();
+    return finish(unlocked(hexmi_paged_attention, &qr, &batch, static_cast<const int32_t*>(in(shared)), pages, (float)scale,
+                           code_of(q->scalar_type()), bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, at.stream),
+                  "hexmi_paged_attention", std::move(out));
+  });
+}
+
 // set_check(f): f(status, what) raises for a status that is not OK
 PyObject* set_check(PyObject*, PyObject* f) {
   Py_INCREF(f);
@@ -366,7 +515,8 @@ PyMODINIT_FUNC PyInit__front() {
 #define HEXMI_OPERATOR(f) add_operator(m, #f, f)
   if (!(HEXMI_OPERATOR(softmax) && HEXMI_OPERATOR(rms_norm) && HEXMI_OPERATOR(layer_norm) && HEXMI_OPERATOR(matmul) &&
         HEXMI_OPERATOR(w8a16_matmul) && HEXMI_OPERATOR(flash_attention) && HEXMI_OPERATOR(attention) && HEXMI_OPERATOR(unary) &&
-        HEXMI_OPERATOR(binary) && PyModule_AddStringConstant(m, "torch_version", HEXMI_TORCH_VERSION) == 0))
+        HEXMI_OPERATOR(binary) && HEXMI_OPERATOR(qk_norm_rope) && HEXMI_OPERATOR(paged_append) && HEXMI_OPERATOR(paged_attention) &&
+        PyModule_AddStringConstant(m, "torch_version", HEXMI_TORCH_VERSION) == 0))
     Py_CLEAR(m);
 #undef HEXMI_OPERATOR
   return m;

@@ -25,6 +25,25 @@ class HexmiError(RuntimeError):
 _c = ctypes
 _i64, _int, _f32, _f64, _ptr = _c.c_int64, _c.c_int, _c.c_float, _c.c_double, _c.c_void_p
 
+
+class HeadRows(_c.Structure):           # hexmi_head_rows
+    _fields_ = [("x", _ptr), ("out", _ptr), ("weight", _ptr), ("heads", _i64), ("token", _i64), ("head", _i64), ("out_token", _i64),
+                ("out_head", _i64)]
+
+
+class Rotation(_c.Structure):           # hexmi_rotation
+    _fields_ = [("inv_freq", _ptr), ("columns", _i64), ("pairs", _c.c_int32), ("eps", _f32)]
+
+
+class PagedBatch(_c.Structure):         # hexmi_paged_batch
+    _fields_ = [("k_pages", _ptr), ("v_pages", _ptr)] + [
+        (n, _i64) for n in ("k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot", "num_pages", "page_size", "kv_heads", "dim")] + [
+        ("page_table", _ptr), ("table_row", _i64), ("table_cols", _i64), ("lengths", _ptr), ("starts", _ptr), ("sequences", _i64),
+        ("tokens", _i64)]
+
+
+_rows, _batch, _rotation = _c.POINTER(HeadRows), _c.POINTER(PagedBatch), _c.POINTER(Rotation)
+
 # name -> (restype, argtypes); must list every symbol of include/hexmi.h (the operator ABI)
 SIGNATURES = {
     "hexmi_version": (_c.c_char_p, []),
@@ -72,6 +91,10 @@ SIGNATURES = {
     "hexmi_block_sum_static": (_int, [_ptr, _ptr, _i64, _i64, _int, _ptr]),
     "hexmi_rope": (_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _f64, _int, _ptr]),
     "hexmi_attention": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _int, _int, _ptr]),
+    "hexmi_qk_norm_rope": (_int, [_rows, _rows, _rotation, _ptr, _int, _i64, _i64, _int, _ptr]),
+    "hexmi_paged_append": (_int, [_rows, _rows, _rows, _rotation, _batch, _int, _ptr]),
+    "hexmi_paged_attention_workspace": (_i64, [_batch, _i64, _i64]),
+    "hexmi_paged_attention": (_int, [_rows, _batch, _ptr, _i64, _f32, _int, _ptr, _i64, _ptr]),
 }
 
 # measurement probes of include/hexmi_calibrate.h: exported by the library, not part of the operator ABI

@@ -86,6 +86,13 @@ _LIBDEF.define("binary(int op, Tensor a, Tensor b, Tensor(a!) out) -> ()")
 _LIBDEF.define("block_sum(Tensor x, int block, Tensor(a!) out) -> ()")
 _LIBDEF.define("rope(Tensor x, float theta, Tensor(a!) out) -> ()")
 _LIBDEF.define("attention(Tensor q, Tensor k, Tensor v, Tensor? mask, float sm_scale, Tensor(a!) out) -> ()")
+_LIBDEF.define("qk_norm_rope(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor? positions, float eps, "
+               "str pairs, Tensor(a!) q_out, Tensor(b!)? k_out) -> ()")
+_LIBDEF.define("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor lengths, "
+               "Tensor? starts, Tensor? k_weight, Tensor? inv_freq, float eps, str pairs, Tensor? q, Tensor? q_weight, "
+               "Tensor(c!)? q_out) -> ()")
+_LIBDEF.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lengths, Tensor? starts, "
+               "float sm_scale, Tensor? shared_pages, Tensor(a!) out) -> ()")
 
 
 def _row_workspace(rows, cols, block_cols, x):
@@ -263,13 +270,67 @@ def _rope_impl(x, theta, out):
         _lib.check(_lib.lib().hexmi_rope(_p(x), _p(out), B, L, H, D, theta, _dt(x), _stream()), "hexmi_rope")
 
 
+_PAIRS = {"adjacent": 0, "halves": 1}
+
+
+def _strides(t):
+    """A tensor's strides; a dimension of one has none that matters."""
+    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+
+
+def _head_rows(x, out=None, weight=None):
+    """hexmi_head_rows of x [tokens, heads, dim] (and of out, where its rows go)."""
+    if x is None:
+        return None
+    xs, os = _strides(x), (0, 0) if out is None else _strides(out)
+    return _lib.HeadRows(_p(x), _p(out), _p(weight), x.shape[1], xs[0], xs[1], os[0], os[1])
+
+
+def _rotation(inv_freq, eps, pairs):
+    return _lib.Rotation(_p(inv_freq), 0 if inv_freq is None else 2 * inv_freq.numel(), _PAIRS[pairs], eps)
+
+
+def _paged_batch(tokens, k_pages, v_pages, page_table, lengths, starts):
+    n, heads, size, dim = k_pages.shape
+    ks, vs = _strides(k_pages), _strides(v_pages)
+    return _lib.PagedBatch(_p(k_pages), _p(v_pages), *ks[:3], *vs[:3], n, size, heads, dim, _p(page_table), page_table.stride(0),
+                           page_table.shape[1], _p(lengths), _p(starts), lengths.shape[0], tokens)
+
+
+def _qk_norm_rope_impl(q, k, q_weight, k_weight, inv_freq, positions, eps, pairs, q_out, k_out):
+    with _on(q.device):
+        _lib.check(_lib.lib().hexmi_qk_norm_rope(_head_rows(q, q_out, q_weight), _head_rows(k, k_out, k_weight),
+                                                 _rotation(inv_freq, eps, pairs), _p(positions),
+                                                 1 if positions is not None and positions.dtype == torch.int64 else 0, q.shape[0],
+                                                 q.shape[2], _dt(q), _stream()), "hexmi_qk_norm_rope")
+
+
+def _paged_append_impl(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight, q_out):
+    with _on(k_pages.device):
+        _lib.check(_lib.lib().hexmi_paged_append(_head_rows(k, None, k_weight), _head_rows(v), _head_rows(q, q_out, q_weight),
+                                                 _rotation(inv_freq, eps, pairs),
+                                                 _paged_batch(k.shape[0], k_pages, v_pages, page_table, lengths, starts), _dt(k),
+                                                 _stream()), "hexmi_paged_append")
+
+
+def _paged_attention_impl(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages, out):
+    batch = _paged_batch(q.shape[0], k_pages, v_pages, page_table, lengths, starts)
+    shared = 0 if shared_pages is None else shared_pages.shape[0]
+    with _on(q.device):
+        need = _lib.lib().hexmi_paged_attention_workspace(batch, q.shape[1], shared)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.check(_lib.lib().hexmi_paged_attention(_head_rows(q, out), batch, _p(shared_pages), shared, sm_scale, _dt(q), _p(ws), need,
+                                                    _stream()), "hexmi_paged_attention")
+
+
 for _name, _fn in (("softmax", _softmax_impl), ("rms_norm", _rms_norm_impl), ("layer_norm", _layer_norm_impl),
                    ("matmul", _matmul_impl), ("linear", _linear_impl), ("add_matmul_softmax", _add_matmul_softmax_impl),
                    ("w8a16_matmul", _w8a16_impl), ("dequant_w8", _dequant_impl), ("pack_w8", _pack_impl),
                    ("w8a16_matmul_packed", _w8a16_packed_impl),
                    ("flash_attention", _flash_impl), ("attention", _attention_impl),
                    ("unary", _unary_impl), ("binary", _binary_impl), ("block_sum", _block_sum_impl),
-                   ("rope", _rope_impl)):
+                   ("rope", _rope_impl), ("qk_norm_rope", _qk_norm_rope_impl), ("paged_append", _paged_append_impl),
+                   ("paged_attention", _paged_attention_impl)):
     _LIBDEF.impl(_name, _fn, "CUDA")
 
 
@@ -350,7 +411,8 @@ class _Front:
 
     def __getattr__(self, name):
         _lib.lib()
-        names = ("softmax", "rms_norm", "layer_norm", "matmul", "w8a16_matmul", "flash_attention", "attention", "unary", "binary")
+        names = ("softmax", "rms_norm", "layer_norm", "matmul", "w8a16_matmul", "flash_attention", "attention", "unary", "binary",
+                 "qk_norm_rope", "paged_append", "paged_attention")
         if name not in names:
             raise AttributeError(name)
         try:
@@ -744,6 +806,237 @@ def rope(x, theta=10000.0, out=None):
     xd = _stage(x, dev)
     od = _out_like(out, x.shape, x.dtype, dev)
     _rope_impl(xd, float(theta), od)
+    return _finish(od, out)
+
+
+def rope_frequencies(columns, theta=10000.0, device=None):
+    """The angles per position, theta^(-2i / columns), of a rotation of `columns` columns of a head, as the float64 tensor that
+    `qk_norm_rope` and `paged_append` take (`compute_thetas`, test/python/triton/test_rope.py:43-57): made once by a program, on the
+    GPU, and scaled there for contexts longer than a model's own."""
+    if columns < 2 or columns % 2 != 0:
+        raise ValueError("hexmi.rope_frequencies: columns must be even and positive")
+    if not theta > 0:
+        raise ValueError("hexmi.rope_frequencies: theta must be positive")
+    i = torch.arange(0, columns, 2, dtype=torch.float64)
+    return (float(theta) ** (-i / columns)).to(_device() if device is None else device)
+
+
+def _rows_of_heads(t, dev):
+    """t [tokens, heads, dim] on the device, its columns adjacent: slices of one projection are read where they stand."""
+    if t is None:
+        return None
+    if t.device.type != "cuda":
+        t = t.to(dev, non_blocking=False)
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _apart(a, b):
+    """Whether two tensors share no memory: their spans lie apart, or they are column slices of the same rows."""
+    if not _overlaps(a, b):
+        return True
+    pitch = a.stride(0)
+    if pitch != b.stride(0) or a.element_size() != b.element_size() or (a.data_ptr() - b.data_ptr()) % a.element_size():
+        return False
+    wide = [sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) + 1 for t in (a, b)]
+    ahead = (a.data_ptr() - b.data_ptr()) // a.element_size() % pitch if pitch else 0
+    return ahead >= wide[1] and ahead + wide[0] <= pitch
+
+
+def _rows_out(name, out, x, others, dev):
+    """Where rows like x's are computed: out where it is a device tensor that shares no memory with what is read (but for x itself, row
+    for row), or fresh memory."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("hexmi.%s: out must be %s of %s" % (name, tuple(x.shape), x.dtype))
+    own = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+    plain = out.device == dev and (out.stride(2) == 1 or out.shape[2] == 1) and all(s > 0 or n == 1 for n, s in zip(out.shape, out.stride()))
+    if plain and out.numel() and (own or _apart(out, x)) and all(_apart(out, t) for t in others if t is not None and t.numel()):
+        return out
+    return torch.empty(x.shape, dtype=x.dtype, device=dev)
+
+
+def _head_operands(name, x, weight, dim, dtype):
+    if x.dim() != 3 or x.shape[1] < 1 or x.shape[2] != dim or dim < 1:
+        raise ValueError("hexmi.%s: rows of heads are [tokens, heads, %s]" % (name, dim))
+    if x.dtype != dtype:
+        raise TypeError("hexmi.%s: operands must share one type" % name)
+    if weight is not None and (weight.shape != (dim,) or weight.dtype != dtype):
+        raise ValueError("hexmi.%s: a weight must be [%d] of %s" % (name, dim, dtype))
+
+
+def _check_rotation(name, inv_freq, pairs, dim):
+    if pairs not in _PAIRS:
+        raise ValueError("hexmi.%s: pairs are 'adjacent' or 'halves'" % name)
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64:
+            raise TypeError("hexmi.%s: inv_freq is float64 (hexmi.rope_frequencies makes it)" % name)
+        if inv_freq.dim() != 1 or 2 * inv_freq.numel() > dim:
+            raise ValueError("hexmi.%s: inv_freq is [rotated columns / 2], at most %d" % (name, dim // 2))
+
+
+def _one_device(name, dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device.type == "cuda" and t.device != dev:
+            raise ValueError("hexmi.%s: operands are on %s and %s" % (name, dev, t.device))
+
+
+def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, inv_freq=None, positions=None, eps=1e-5, pairs="adjacent", q_out=None,
+                 k_out=None):
+    """RMS norm of every head's row of q [tokens, heads, dim] and k [tokens, kv heads, dim] (each where it has a weight [dim]) and their
+    rotation by the tokens' positions, in one pass and with one rounding: `rms_norm` and `rope` (test/python/triton/test_rms_norm.py:37-63,
+    test_rope.py:97-197) at any positions.
+
+    inv_freq (float64, `rope_frequencies`) turns 2 * len(inv_freq) leading columns, in pairs of columns (2i, 2i + 1) ("adjacent") or
+    (i, i + len(inv_freq)) ("halves"); None: no rotation. positions: int32 or int64 [tokens]. q and k may be slices of one projection;
+    q_out and k_out may be q and k. Returns q's rows, or with k the pair."""
+    if q_out is None and k_out is None and not _THROUGH_DISPATCHER:
+        y = _front.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, eps, pairs)
+        if y is not None:
+            return y
+    name = "qk_norm_rope"
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError("hexmi.qk_norm_rope: float16, bfloat16 or float32")
+    dim = q.shape[-1]
+    _head_operands(name, q, q_weight, dim, q.dtype)
+    _check_rotation(name, inv_freq, pairs, dim)
+    if k is not None:
+        _head_operands(name, k, k_weight, dim, q.dtype)
+        if k.shape[0] != q.shape[0]:
+            raise ValueError("hexmi.qk_norm_rope: q and k have %d and %d tokens" % (q.shape[0], k.shape[0]))
+    elif k_weight is not None or k_out is not None:
+        raise ValueError("hexmi.qk_norm_rope: k_weight and k_out go with k")
+    if inv_freq is not None and positions is None:
+        raise ValueError("hexmi.qk_norm_rope: a rotation needs positions")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (q.shape[0],)):
+        raise ValueError("hexmi.qk_norm_rope: positions must be int32 or int64 [%d]" % q.shape[0])
+    dev = _device() if q.device.type != "cuda" else q.device
+    _one_device(name, dev, k, q_weight, k_weight, inv_freq, positions)
+    qd, kd = _rows_of_heads(q, dev), _rows_of_heads(k, dev)
+    qw, kw, fd, pd = _stage(q_weight, dev), _stage(k_weight, dev), _stage(inv_freq, dev), _stage(positions, dev)
+    qo = _rows_out(name, q_out, qd, (kd, qw, kw, fd, pd), dev)
+    ko = None if k is None else _rows_out(name, k_out, kd, (qd, qw, kw, fd, pd), dev)
+    if ko is not None and qo.numel() and not _apart(qo, ko):
+        raise ValueError("hexmi.qk_norm_rope: q_out and k_out share memory")
+    if q.shape[0]:
+        args = (qd, kd, qw, kw, fd, pd, float(eps), pairs, qo, ko)
+        _run(name, _qk_norm_rope_impl, args, *args)
+    q_done = _finish(qo, q_out)
+    return q_done if k is None else (q_done, _finish(ko, k_out))
+
+
+def _paged_operands(name, tokens, k_pages, v_pages, page_table, lengths, starts):
+    """Checks a paged cache and its batch and returns (page_table, lengths, starts) on its device."""
+    if k_pages.device.type != "cuda" or v_pages.device != k_pages.device:
+        raise ValueError("hexmi.%s: the pages stay on the GPU" % name)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.numel() == 0:
+        raise ValueError("hexmi.%s: k_pages and v_pages are [pages, kv heads, page size, dim]" % name)
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("hexmi.%s: a key's columns must be adjacent" % name)
+    for what, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1), ("starts", starts, 1)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != dims):
+            raise ValueError("hexmi.%s: %s must be an int32 tensor of %d dimension%s" % (name, what, dims, "s" if dims > 1 else ""))
+    n = lengths.shape[0]
+    if page_table.shape[0] != n:
+        raise ValueError("hexmi.%s: page_table has a row and lengths a value for each sequence" % name)
+    if starts is None and n != tokens:
+        raise ValueError("hexmi.%s: without starts every sequence has one new token (%d sequences, %d tokens)" % (name, n, tokens))
+    if starts is not None and starts.shape[0] != n + 1:
+        raise ValueError("hexmi.%s: starts must be [%d]" % (name, n + 1))
+    dev = k_pages.device
+    _one_device(name, dev, page_table, lengths, starts)
+    table = page_table.to(dev)
+    if table.numel() and (table.stride(1) != 1 and table.shape[1] > 1 or table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+        table = table.contiguous()
+    return table, _stage(lengths, dev), _stage(starts, dev)
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_weight=None, inv_freq=None, eps=1e-5, pairs="adjacent",
+                 q=None, q_weight=None, q_out=None):
+    """Puts the keys and values of new tokens, [tokens, kv heads, dim], into the pages of their sequences, the keys normed (with k_weight)
+    and rotated (with inv_freq) by their positions on the way, as `qk_norm_rope` does; with q [tokens, heads, dim], its rows too, which
+    are returned.
+
+    k_pages, v_pages [pages, kv heads, page size, dim] are changed in place (any strides: a cache that keeps the heads of a token side by
+    side is a transposed view). page_table int32 [sequences, columns]: the pages of each sequence; an entry that is no page's number (-1,
+    say) is none, and a token there is left out. lengths int32 [sequences]: the positions of each sequence, the new tokens included, which
+    are its last. starts int32 [sequences + 1]: sequence b's tokens are the rows starts[b] .. starts[b + 1] - 1; rows of no sequence
+    (padding behind the last) leave nothing, and zeros in q's result. None: one token a sequence. What the index tensors hold is
+    read on the GPU only, so the call can be captured into a graph and replayed as they change."""
+    if q_out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight)
+        if y is not None:
+            return y if q is not None else None
+    name = "paged_append"
+    if k.dtype not in (torch.float16, torch.bfloat16) or k_pages.dtype != k.dtype:
+        raise TypeError("hexmi.paged_append: keys and pages must both be float16 or both bfloat16")
+    if k_pages.dim() != 4 or k.dim() != 3 or k.shape[1:] != (k_pages.shape[1], k_pages.shape[3]) or v.shape != k.shape:
+        raise ValueError("hexmi.paged_append: k and v are [tokens, kv heads, dim], the pages [pages, kv heads, page size, dim]")
+    dim, tokens = k.shape[2], k.shape[0]
+    _head_operands(name, k, k_weight, dim, k.dtype)
+    _head_operands(name, v, None, dim, k.dtype)
+    _check_rotation(name, inv_freq, pairs, dim)
+    if q is not None:
+        _head_operands(name, q, q_weight, dim, k.dtype)
+        if q.shape[0] != tokens:
+            raise ValueError("hexmi.paged_append: q and k have %d and %d tokens" % (q.shape[0], tokens))
+    elif q_weight is not None or q_out is not None:
+        raise ValueError("hexmi.paged_append: q_weight and q_out go with q")
+    table, lens, begin = _paged_operands(name, tokens, k_pages, v_pages, page_table, lengths, starts)
+    dev = k_pages.device
+    _one_device(name, dev, k, v, q, k_weight, q_weight, inv_freq)
+    kd, vd, qd = _rows_of_heads(k, dev), _rows_of_heads(v, dev), _rows_of_heads(q, dev)
+    kw, qw, fd = _stage(k_weight, dev), _stage(q_weight, dev), _stage(inv_freq, dev)
+    qo = None if q is None else _rows_out(name, q_out, qd, (kd, vd, kw, qw, fd, table, lens, begin), dev)
+    if tokens:
+        args = (kd, vd, k_pages, v_pages, table, lens, begin, kw, fd, float(eps), pairs, qd, qw, qo)
+        _run(name, _paged_append_impl, args, *args)
+    return None if q is None else _finish(qo, q_out)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_scale=None, shared_pages=None, out=None):
+    """Attention of new tokens q [tokens, heads, dim] over a paged cache: row (t, h) is softmax(sm_scale * Q K^T) V over the keys of
+    kv head h // (heads // kv heads) at the positions of its sequence up to its own (`attention` with a cache and masks of its own;
+    test/python/triton/test_flash_attention.py:37-168). The cache and the batch are `paged_append`'s, which comes first: lengths counts
+    the new tokens. One token a sequence (starts None) is a decode step, runs of tokens are prompts or pieces of them, and a batch may
+    hold both.
+
+    shared_pages int32 [n]: the first n pages of every sequence are these (a prompt that all have in common), and their keys are gone
+    through once for all of them; the result is the same without, if the table names them.
+
+    A row without any key, and a row of no sequence, is zeros. What the pages hold past a sequence's length is not used, whatever it is;
+    the keys and values of its own positions have to be finite. 16-bit, dim a multiple of 8 up to 256."""
+    if out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages)
+        if y is not None:
+            return y
+    name = "paged_attention"
+    if q.dtype not in (torch.float16, torch.bfloat16) or k_pages.dtype != q.dtype:
+        raise TypeError("hexmi.paged_attention: queries and pages must both be float16 or both bfloat16")
+    if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3] or q.shape[1] < 1 or q.shape[1] % max(k_pages.shape[1], 1) != 0:
+        raise ValueError("hexmi.paged_attention: q is [tokens, heads, dim], the pages [pages, kv heads, page size, dim], and kv heads "
+                         "divides heads")
+    if q.shape[2] % 8 != 0 or q.shape[2] > 256:
+        raise ValueError("hexmi.paged_attention: dim must be a multiple of 8 up to 256")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[2])
+    if not 0 < sm_scale < 3e38:
+        raise ValueError("hexmi.paged_attention: sm_scale must be positive")
+    if shared_pages is not None and (shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] > page_table.shape[-1]):
+        raise ValueError("hexmi.paged_attention: shared_pages must be an int32 tensor of one dimension, no longer than the table is wide")
+    table, lens, begin = _paged_operands(name, q.shape[0], k_pages, v_pages, page_table, lengths, starts)
+    dev = k_pages.device
+    _one_device(name, dev, q, shared_pages, out)
+    qd = _rows_of_heads(q, dev)
+    if qd.data_ptr() % 16 or any(s % 8 for s in _strides(qd)[:2]):
+        qd = qd.clone(memory_format=torch.contiguous_format)
+    sd = _stage(shared_pages, dev)
+    od = _out_like(out, q.shape, q.dtype, dev)
+    if out is not None and od is out and od.numel() and (od.data_ptr() % 16 or _overlaps(od, qd, k_pages, v_pages)):
+        od = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if q.shape[0]:
+        args = (qd, k_pages, v_pages, table, lens, begin, float(sm_scale), sd, od)
+        _run(name, _paged_attention_impl, args, *args)
     return _finish(od, out)
 
 

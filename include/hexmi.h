@@ -508,6 +508,102 @@ int hexmi_rope(const void *x, void *y, int64_t batch, int64_t seq,
                int64_t heads, int64_t feat, double theta, int dtype,
                hexmi_stream_t stream);
 
+/* Heads by position, a paged cache of keys and values, attention over it ---- */
+
+/* Rows of heads where they stand: head h of token t is the dim adjacent
+ * elements at x + t * token + h * head (strides in elements; slices of one
+ * projection are such rows). out: the same with out_token, out_head; it may be
+ * x itself with the strides of x, and must not overlap the rows otherwise.
+ * weight: [dim], the scale of the rows' RMS norm, or NULL: no norm. */
+typedef struct hexmi_head_rows {
+  const void *x;
+  void *out;
+  const void *weight;
+  int64_t heads, token, head, out_token, out_head;
+} hexmi_head_rows;
+
+/* How rows turn with their position p: columns (even, at most dim; 0: not at
+ * all) leading columns in pairs by the angle p * inv_freq[i], inv_freq:
+ * columns / 2 doubles in DEVICE memory, radians per position. Pairs are columns
+ * (2i, 2i + 1) or, halves, (i, i + columns / 2); (x, y) becomes
+ * (x cos - y sin, y cos + x sin). The angle is reduced in 64 bits, so far
+ * positions lose nothing. eps: of the norms. */
+typedef enum hexmi_pairs { HEXMI_PAIRS_ADJACENT = 0, HEXMI_PAIRS_HALVES = 1 } hexmi_pairs;
+typedef struct hexmi_rotation {
+  const double *inv_freq;
+  int64_t columns;
+  int32_t pairs;
+  float eps;
+} hexmi_rotation;
+
+/* A paged cache and the batch that uses it. Key (value) of head h at slot s of
+ * page p: the dim adjacent elements at k_pages + p * k_page + h * k_head +
+ * s * k_slot (strides in elements). Position i of sequence b stands in page
+ * page_table[b * table_row + i / page_size], slot i % page_size; a table entry
+ * outside 0 .. num_pages - 1 is no page. lengths [sequences]: the positions of
+ * each sequence, new tokens included. starts [sequences + 1] (not falling), or
+ * NULL for one new token each: the new tokens of sequence b are the rows
+ * starts[b] .. starts[b + 1] - 1 of the operands, at its last positions. A row
+ * below starts[0] or from starts[sequences] on belongs to no sequence; without
+ * starts, tokens == sequences. Positions past the table's columns have no page.
+ * The index arrays are read by the kernels and not checked on the host:
+ * whatever they hold, nothing outside the operands is touched. */
+typedef struct hexmi_paged_batch {
+  void *k_pages, *v_pages;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  int64_t num_pages, page_size, kv_heads, dim;
+  const int32_t *page_table;
+  int64_t table_row, table_cols;
+  const int32_t *lengths, *starts;
+  int64_t sequences, tokens;
+} hexmi_paged_batch;
+
+/* RMS norm of every head's row (where it has a weight) and its rotation by the
+ * token's position, one rounding: hexmi_rms_norm and hexmi_rope over [tokens *
+ * heads, dim] in one pass, at any positions (int32 or, positions_64, int64
+ * [tokens]; may be NULL where columns is 0). k may be NULL. dtype: HEXMI_F16,
+ * HEXMI_BF16 or HEXMI_F32. dim up to 512; fastest on 16-byte boundaries with
+ * dim and, for halves, columns / 2 multiples of 8.
+ * The rotation is rope_kernel of test/python/triton/test_rope.py:97-197, the
+ * norm rms_norm_fwd_kernel of test_rms_norm.py:37-63. */
+int hexmi_qk_norm_rope(const hexmi_head_rows *q, const hexmi_head_rows *k,
+                       const hexmi_rotation *rotation, const void *positions,
+                       int positions_64, int64_t tokens, int64_t dim, int dtype,
+                       hexmi_stream_t stream);
+
+/* Keys and values of the new tokens into their pages, the keys normed and
+ * rotated by their positions on the way (k->out, v->out and v->weight are not
+ * used), and, with q, the queries' rows normed and rotated into q->out. A
+ * token without a page leaves no key and no value; q->out of a row of no
+ * sequence is zeros. Two tokens of one slot: either's. HEXMI_F16, HEXMI_BF16. */
+int hexmi_paged_append(const hexmi_head_rows *k, const hexmi_head_rows *v,
+                       const hexmi_head_rows *q, const hexmi_rotation *rotation,
+                       const hexmi_paged_batch *batch, int dtype,
+                       hexmi_stream_t stream);
+
+/* Attention of the new tokens over the pages of their sequences: row (t, h) is
+ * softmax(sm_scale * q k) v over the keys of head h / (heads / kv_heads) from
+ * position 0 to the token's own. Keys without a page are left out; a row
+ * without any key, and one of no sequence, is zeros. What stands in the pages
+ * past a sequence's length is not used, whatever it is (infinities and NaN
+ * too); keys and values of its own positions have to be finite.
+ * shared_pages [shared]: positions 0 .. shared * page_size - 1 of every sequence
+ * are these pages, and what the table says there is not read: their keys are
+ * gone through once for all sequences. 16-bit (HEXMI_F16, HEXMI_BF16), dim a
+ * multiple of 8 up to 256, rows of q, out and pages on 16-byte boundaries,
+ * heads a multiple of kv_heads, sm_scale > 0; scores, sums and maxima are fp32,
+ * probabilities are rounded to the dtype for the product with v.
+ * hexmi_paged_attention_workspace: the bytes of scratch (16-byte aligned, not
+ * initialised, no state between calls) that a call takes; 0: none. Two calls
+ * that overlap in time need one each. */
+int64_t hexmi_paged_attention_workspace(const hexmi_paged_batch *batch,
+                                        int64_t heads, int64_t shared);
+int hexmi_paged_attention(const hexmi_head_rows *q,
+                          const hexmi_paged_batch *batch,
+                          const int32_t *shared_pages, int64_t shared,
+                          float sm_scale, int dtype, void *workspace,
+                          int64_t workspace_bytes, hexmi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
