@@ -67,4 +67,32 @@ __device__ __forceinline__ int length_of(const Pages& p, int b) {
 }
 #endif
 
+// What attention over the pages takes beside them (paged_attn.hip, paged_decode.hip).
+struct PagedAttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_token, q_head, out_token, out_head;
+  const int32_t* shared;                       // the pages of the positions below `prefix`
+  int prefix, heads, group, dim;               // group: query heads of a key head
+  float scale;                                 // sm_scale * log2 e
+  Divider by_group;
+};
+// Sums that several workgroups hold of a row: slot i of row (token * heads + head) has the row's unnormalised output, dim floats at
+// o + (i * rows + row) * dim, and (maximum in log2 units, sum) at ml[i * rows + row]; sum 0: no key, and o is not written.
+struct RowSums {
+  float* o;
+  float2* ml;
+  int64_t rows;
+  int slots;
+};
+// One new token a sequence: how the keys are shared out (workers; 0: every unit of sequence, key head and 16 query heads whole), and
+// the launch behind a prefix whose sums are there (slots 0: none).
+struct PagedDecodePlan {
+  int workers, row_tiles, rows;
+};
+PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix);
+int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim);
+int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const RowSums& prefix,
+                 hipStream_t s);
+
 }  // namespace hexmi

@@ -320,12 +320,19 @@ def test_index_tensors_that_make_no_sense_touch_nothing_outside(hexmi, ragged):
     table = torch.tensor([[-(1 << 31), (1 << 31) - 1, 5]] * B, dtype=torch.int32, device="cuda")
     starts = torch.tensor([3, -9, 1 << 30, 2, 70], dtype=torch.int32, device="cuda") if ragged else None
     before = [p.clone() for p in pages]
-    assert (hexmi.paged_attention(q, *pages, table, lengths, starts) == 0).all()          # no page is one
+    around = torch.full((18, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    out = around[6:12]
+    hexmi.paged_attention(q, *pages, table, lengths, starts, out=out)
+    assert (around[:6] == 7).all() and (around[12:] == 7).all()
+    # no page is one: zeros, but in rows that starts which fall give to nobody
+    assert ((out == 0) | (out == 7 if ragged else False)).all()
     assert hexmi.paged_append(k, k, *pages, table, lengths, starts) is None
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(pages, before))
     shared = torch.tensor([-1, 99], dtype=torch.int32, device="cuda")
-    assert (hexmi.paged_attention(q, *pages, table, lengths, starts, shared_pages=shared) == 0).all()
+    hexmi.paged_attention(q, *pages, table, lengths, starts, shared_pages=shared, out=out)
+    torch.cuda.synchronize()
+    assert (around[:6] == 7).all() and (around[12:] == 7).all() and (ragged or (out == 0).all())
 
 
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
