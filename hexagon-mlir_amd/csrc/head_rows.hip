@@ -10,6 +10,7 @@ namespace hexmi {
 namespace {
 
 constexpr int kMaxDim = 512;
+constexpr int kWavesWanted = 8192;               // a token's rows are shared by several waves up to so many in all
 
 // the three kinds of rows, in the order in which they are numbered: queries, keys, values
 struct Kind {
@@ -131,8 +132,235 @@ void head_rows_any_kernel(HeadArgs a, Pages p) {
   }
 }
 
+// Eight columns of a row as they stand in memory.
+template <typename T> struct alignas(16) Eight {
+  static constexpr int kWords = 8 * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p) {
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i)
+    *reinterpret_cast<u32x4*>(r.w + 4 * i) = *(reinterpret_cast<const u32x4*>(p) + i);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, const Eight<T>& r) {
+#pragma unroll
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i)
+    reinterpret_cast<u32x4*>(p)[i] = *reinterpret_cast<const u32x4*>(r.w + 4 * i);
+}
+template <typename T>
+__device__ __forceinline__ float column(const Eight<T>& r, int e) {
+  return to_f32<T>(reinterpret_cast<const T*>(r.w)[e]);
+}
+// the sum over the LPR lanes of a row, in all of them
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+  v += dpp_move<0xB1>(v);
+  v += dpp_move<0x4E>(v);
+  v += dpp_move<0x141>(v);
+  float a, b;
+  if constexpr (LPR >= 16) v += dpp_move<0x140>(v);
+  if constexpr (LPR >= 32) {
+    swap16(v, a, b);
+    v = a + b;
+  }
+  if constexpr (LPR == 64) {
+    swap32(v, a, b);
+    v = a + b;
+  }
+  return v;
+}
+
+// Rows on 16-byte boundaries, dim a multiple of 8. LPR lanes take a row, eight columns each, and the 64 / LPR rows of a wave are of one
+// token: its angles are worked out once and serve every head. The pair of a column is in the same lane (adjacent) or comes out of LDS
+// (halves), in one piece where columns / 2 is a multiple of 8 (PIECES: a lane's columns are all of one half, or none turns). The next rows are asked for before these are worked on.
+// What a launch is bound by: its latency up to a few hundred tokens (4 tokens x 40 heads of 128 4.8 us, 64 tokens into a cache 4.6), then the
+// rows in flight: 8192 tokens x 40 heads of 128 bf16, normed and turned, 40 us (4.2 TB/s; a copy of that size 33). Measured there: an
+// angle worked out by every lane that needs it 50 us, pointers and strides chosen by the lane 62, no row asked for ahead 49, two ahead 42,
+// 16384 waves 46, five waves a SIMD with what spills 44.
+template <typename T, int LPR, bool HALVES, bool PIECES, bool PAGED>
+__global__ __launch_bounds__(256, 4)
+void head_rows_kernel(HeadArgs a, Pages p, int waves_per_token) {
+  constexpr int kRowsAtOnce = kWave / LPR, kAngles = HALVES ? 8 : 4;
+  __shared__ __attribute__((aligned(16))) f32x2 angle[4][LPR * 4 + 4];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c0 = lane % LPR * 8, group = lane / LPR, half = a.columns / 2;
+  const bool live = c0 < a.dim, turns = c0 < a.columns;
+  __shared__ __attribute__((aligned(16))) T beside[HALVES ? 4 : 1][HALVES ? kWave * 8 : 8];
+  auto other = [&](int c) __attribute__((always_inline)) { return c >= a.columns ? c : c < half ? c + half : c - half; };
+  Eight<T> weight[2], other_weight[2];                              // of queries and keys, at these columns and at their pairs'
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (a.kind[k].weight) {
+      weight[k] = {};
+      if (live) weight[k] = load_eight(static_cast<const T*>(a.kind[k].weight) + c0);
+      if (HALVES) {
+        const T* w = static_cast<const T*>(a.kind[k].weight);
+        other_weight[k] = {};
+        if (PIECES && turns) other_weight[k] = load_eight(w + other(c0));
+        if (!PIECES && turns) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e < a.dim) reinterpret_cast<T*>(other_weight[k].w)[e] = w[other(c0 + e)];
+        }
+      }
+    }
+  const int q_chunks = (a.heads[0] + kRowsAtOnce - 1) / kRowsAtOnce, k_chunks = (a.heads[1] + kRowsAtOnce - 1) / kRowsAtOnce;
+  const int chunks = q_chunks + k_chunks + (a.heads[2] + kRowsAtOnce - 1) / kRowsAtOnce;
+  const int64_t all = (int64_t)a.tokens * waves_per_token;
+  for (int64_t at_wave = (int64_t)blockIdx.x * 4 + wave; at_wave < all; at_wave += (int64_t)gridDim.x * 4) {
+    const int t = (int)(at_wave / waves_per_token), share = (int)(at_wave - (int64_t)t * waves_per_token);
+    const Place at = place_of<PAGED>(a, p, t, lane);
+    // every angle of the token once, a lane each, and from LDS to the lanes whose columns turn by it
+    const int pairs = a.columns / 2;
+    for (int i = lane; i < pairs; i += kWave) {
+      float sn, cs;
+      sincos_turns((double)at.position * a.inv_freq[i] * 0.15915494309189533577, sn, cs);      // 1 / (2 pi)
+      angle[wave][i] = f32x2{cs, sn};
+    }
+    asm volatile("" ::: "memory");                                  // a wave's LDS accesses are in order
+    float cs[kAngles], sn[kAngles];                                 // halves: the sign of the sine says which one of a pair
+    if (turns) {
+#pragma unroll
+      for (int e = 0; e < kAngles; ++e) {
+        const int c = PIECES ? c0 : c0 + e;
+        const bool second = HALVES && c >= half;
+        const int i = !HALVES ? c0 / 2 + e : PIECES ? (second ? c0 - half : c0) + e : c >= a.columns ? 0 : second ? c - half : c;
+        const f32x2 v = angle[wave][i];                             // past the last pair: not used
+        cs[e] = v[0];
+        sn[e] = HALVES && !second ? -v[1] : v[1];
+      }
+    }
+    asm volatile("" ::: "memory");
+    // the chunk's kind is the wave's, so its pointers and strides are scalars
+    auto kind_at = [&](int chunk, int& h) __attribute__((always_inline)) {
+      const int k = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;
+      h = (chunk - (k == 0 ? 0 : k == 1 ? q_chunks : q_chunks + k_chunks)) * kRowsAtOnce + group;
+      return k;
+    };
+    auto fetch = [&](int chunk) __attribute__((always_inline)) {    // lanes without a row of it: the kind's last row
+      int h;
+      const int k = kind_at(chunk < chunks ? chunk : chunks - 1, h);
+      const Kind& kind = a.kind[k];
+      h = h < a.heads[k] ? h : a.heads[k] - 1;
+      return load_eight(static_cast<const T*>(kind.x) + t * kind.token + h * kind.head + (live ? c0 : 0));
+    };
+    Eight<T> next = fetch(share);
+    for (int chunk = share; chunk < chunks; chunk += waves_per_token) {
+      int h;
+      const int k = kind_at(chunk, h);
+      const Kind& kind = a.kind[k];
+      const bool is_row = live && h < a.heads[k];
+      Eight<T> x = next;
+      if (!live) x = {};
+      next = fetch(chunk + waves_per_token);
+      T* out = static_cast<T*>(kind.out);
+      if (PAGED && k != 0) {
+        if (at.page < 0) continue;
+        out += k == 1 ? at.page * p.k_page + at.slot * p.k_slot + h * p.k_head : at.page * p.v_page + at.slot * p.v_slot + h * p.v_head;
+      } else {
+        out += t * kind.out_token + h * kind.out_head;
+      }
+      if (k == 2) {                                                 // values as they are
+        if (is_row) store_eight(out + c0, x);
+        continue;
+      }
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = column(x, e);
+      Eight<T> pair_x = {};
+      if constexpr (HALVES) {
+        *reinterpret_cast<Eight<T>*>(&beside[wave][lane * 8]) = x;
+        asm volatile("" ::: "memory");
+        const T* row = &beside[wave][group * LPR * 8];
+        if constexpr (PIECES) {
+          if (turns) pair_x = *reinterpret_cast<const Eight<T>*>(row + other(c0));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(pair_x.w)[e] = row[turns ? other(c0 + e) : 0];
+        }
+        asm volatile("" ::: "memory");
+      }
+      float scale = 1.0f;
+      const bool norm = kind.weight != nullptr;
+      const Eight<T> wt = k == 0 ? weight[0] : weight[1], other_wt = k == 0 ? other_weight[0] : other_weight[1];
+      if (norm) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(y[e], y[e], sum);
+        const float mean = fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps), r = __builtin_amdgcn_rsqf(mean);
+        scale = r == 0.0f ? 0.0f : r * fmaf(-0.5f * mean * r, r, 1.5f);          // one Newton step; an infinite mean stays 0
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = y[e] * scale * column(wt, e);
+      }
+      if (turns) {
+        if constexpr (HALVES) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float o = column(pair_x, e);
+            if (norm) o = o * scale * column(other_wt, e);
+            const float turned = fmaf(y[e], cs[e], o * sn[e]);
+            y[e] = PIECES || c0 + e < a.columns ? turned : y[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (c0 + 2 * e >= a.columns) continue;
+            const float u = y[2 * e], v = y[2 * e + 1];
+            y[2 * e] = fmaf(u, cs[e], -(v * sn[e]));
+            y[2 * e + 1] = fmaf(v, cs[e], u * sn[e]);
+          }
+        }
+      }
+      if (!is_row) continue;
+      Eight<T> r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(r.w)[e] = from_f32<T>(PAGED && at.none ? 0.0f : y[e]);
+      store_eight(out + c0, r);
+    }
+  }
+}
+
+// whether head_rows_kernel takes the rows
+template <typename T, bool PAGED>
+bool takes(const HeadArgs& a, const Pages& p) {
+  constexpr int n = 16 / (int)sizeof(T);
+  if (a.dim % 8 != 0) return false;
+  for (int k = 0; k < 3; ++k) {
+    if (a.heads[k] == 0) continue;
+    const Kind& r = a.kind[k];
+    if (!aligned_to(r.x, 16) || !aligned_to(r.out, 16) || !aligned_to(r.weight, 16) || r.token % n != 0 || r.head % n != 0) return false;
+    if (PAGED && k != 0) continue;
+    if (r.out_token % n != 0 || r.out_head % n != 0) return false;
+  }
+  if (PAGED)
+    for (int64_t s : {p.k_page, p.k_head, p.k_slot, p.v_page, p.v_head, p.v_slot})
+      if (s % n != 0) return false;
+  return true;
+}
+
+template <typename T, int LPR, bool PAGED>
+int launch_rows(const HeadArgs& a, const Pages& p, hipStream_t s) {
+  constexpr int at_once = kWave / LPR;
+  int64_t most = 0;                            // chunks of a token's rows
+  for (int k = 0; k < 3; ++k) most += (a.heads[k] + at_once - 1) / at_once;
+  const int64_t wanted = kWavesWanted / a.tokens, per_token = wanted < 1 ? 1 : wanted < most ? wanted : most;
+  const int64_t blocks = (a.tokens * per_token + 3) / 4;
+  const dim3 grid((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22));
+  if (!a.halves || a.columns == 0) hipLaunchKernelGGL((head_rows_kernel<T, LPR, false, false, PAGED>), grid, dim3(256), 0, s, a, p, (int)per_token);
+  else if (a.columns % 16 == 0) hipLaunchKernelGGL((head_rows_kernel<T, LPR, true, true, PAGED>), grid, dim3(256), 0, s, a, p, (int)per_token);
+  else hipLaunchKernelGGL((head_rows_kernel<T, LPR, true, false, PAGED>), grid, dim3(256), 0, s, a, p, (int)per_token);
+  return launch_status();
+}
+
 template <typename T, bool PAGED>
 int launch(const HeadArgs& a, const Pages& p, hipStream_t s) {
+  if (takes<T, PAGED>(a, p))
+    return a.dim <= 64 ? launch_rows<T, 8, PAGED>(a, p, s) : a.dim <= 128 ? launch_rows<T, 16, PAGED>(a, p, s)
+         : a.dim <= 256 ? launch_rows<T, 32, PAGED>(a, p, s) : launch_rows<T, 64, PAGED>(a, p, s);
   const int64_t rows = (int64_t)a.tokens * a.rows, blocks = (rows + 3) / 4;
   hipLaunchKernelGGL((head_rows_any_kernel<T, PAGED>), dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), 0, s, a, p);
   return launch_status();

@@ -563,7 +563,7 @@ typedef struct hexmi_paged_batch {
  * heads, dim] in one pass, at any positions (int32 or, positions_64, int64
  * [tokens]; may be NULL where columns is 0). k may be NULL. dtype: HEXMI_F16,
  * HEXMI_BF16 or HEXMI_F32. dim up to 512; fastest on 16-byte boundaries with
- * dim and, for halves, columns / 2 multiples of 8.
+ * dim a multiple of 8 (other rows take five times as long).
  * The rotation is rope_kernel of test/python/triton/test_rope.py:97-197, the
  * norm rms_norm_fwd_kernel of test_rms_norm.py:37-63. */
 int hexmi_qk_norm_rope(const hexmi_head_rows *q, const hexmi_head_rows *k,
