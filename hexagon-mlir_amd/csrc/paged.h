@@ -86,7 +86,8 @@ struct RowSums {
   int slots;
 };
 // One new token a sequence: how the keys are shared out (workers; 0: every unit of sequence, key head and 16 query heads whole), and
-// the launch behind a prefix whose sums are there (slots 0: none).
+// the launch behind a prefix whose sums are there, in all slots of `prefix` but the last, which is for a unit's own sums (slots 0: no
+// prefix).
 struct PagedDecodePlan {
   int workers, row_tiles, rows;
 };

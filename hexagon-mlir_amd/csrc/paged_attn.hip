@@ -18,9 +18,10 @@ namespace {
 
 constexpr int kTileWaves = 4, kRows = kTileWaves * 32;
 
+// One launch: the prefix for all rows (the first workgroups), and every sequence's keys behind it.
 struct TileArgs {
-  bool shared;                                 // the prefix for all rows; otherwise every sequence's keys behind it
-  int tiles, splits, slot;                     // tiles of a key head; parts of its keys, whose sums go to slots slot ..
+  int shared_tiles, shared_splits;             // tiles of a key head; parts of the prefix, whose sums go to slots 0 .. (0: no prefix)
+  int tiles, splits;                           // of the sequences' own keys, whose sums go to the slots behind (0: decode, not here)
   RowSums sums;                                // slots 0: the result goes to out
 };
 
@@ -65,89 +66,43 @@ void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
   const int dim = PADDED ? a.dim : COLS;
 
-  // Workgroup -> (key head, tile, part). Workgroup ids go round robin to the 8 XCDs (one L2 each): every XCD gets a run of the list of all,
-  // key head by key head, a sequence's last (longest) tiles first.
-  const unsigned id = blockIdx.x, xcd = id % 8, each = gridDim.x / 8, more = gridDim.x % 8;
+  // Workgroup -> (prefix or not, key head, tile, part). Workgroup ids go round robin to the 8 XCDs (one L2 each): every XCD gets a run of
+  // the list, key head by key head, a sequence's last (longest) tiles first.
+  const unsigned shared_grid = (unsigned)(w.shared_tiles * w.shared_splits * p.kv_heads);
+  const bool shared = blockIdx.x < shared_grid;
+  const int tiles = shared ? w.shared_tiles : w.tiles, splits = shared ? w.shared_splits : w.splits;
+  const unsigned id = shared ? blockIdx.x : blockIdx.x - shared_grid, count = shared ? shared_grid : gridDim.x - shared_grid;
+  const unsigned xcd = id % 8, each = count / 8, more = count % 8;
   const unsigned unit = xcd * each + (xcd < more ? xcd : more) + id / 8;
-  const int part = unit % w.splits, tile = w.tiles - 1 - (int)(unit / w.splits % w.tiles), kvh = unit / w.splits / w.tiles;
+  const int part = unit % splits, tile = tiles - 1 - (int)(unit / splits % tiles), kvh = unit / splits / tiles;
 
-  int token0 = 0, rows, row0, new_tokens = 0, b = -1;
+  int token0 = 0, rows, row0, new_tokens = 0, begin = 0, end;
   int64_t length = 0;
+  bool none = false;                                                // rows of no sequence
   const int most = p.table_cols * p.page_size;
-  if (w.shared) {
+  const int32_t* table;
+  if (shared) {
     row0 = tile * kRows;
     rows = p.tokens * a.group;
+    end = a.prefix;
+    table = a.shared;
   } else {
-    b = __builtin_amdgcn_readfirstlane(sequence_of_tile(p, a.group, tile, lane));
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile(p, a.group, tile, lane));
     token0 = first_row(p, b);
     new_tokens = first_row(p, b + 1) - token0;
     row0 = (tile - first_tile(p, a.group, b)) * kRows;
     rows = new_tokens * a.group;                                    // negative where starts fall: nothing
-    if (b >= 0 && b < p.sequences) length = p.lengths[b];
-  }
-  if (row0 < 0 || row0 >= rows) return;
-  // this lane's row: its token and the keys it sees
-  const int wave_row = row0 + wave * 32, row = wave_row + lane % 32;
-  const bool live = row < rows;
-  const int in_seq = divided(live ? row : rows - 1, a.by_group), head = kvh * a.group + (live ? row : rows - 1) - in_seq * a.group;
-  const int token = token0 + in_seq;
-  int keys = 0, begin = 0, end;
-  const int32_t* table;
-  if (w.shared) {
-    int s = token;                                                  // the row's sequence: this lane's own search
-    if (p.starts) {
-      s = -1;
-      int hi = p.sequences + 1;                                     // the last one with starts[s] <= token, among 0 .. sequences
-      int lo = 0;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.starts[mid] <= token) lo = mid;
-        else hi = mid;
-      }
-      if (lo < p.sequences && p.starts[lo] <= token) s = lo;
-    }
-    if (live && s >= 0) keys = keys_of(p.lengths[s], p.starts ? p.starts[s + 1] - token : 1, 0, most);
-    keys = keys < a.prefix ? keys : a.prefix;
-    end = a.prefix;
-    table = a.shared;
-  } else {
-    const bool none = b < 0 || b >= p.sequences;
-    keys = none || !live ? 0 : keys_of(length, new_tokens, in_seq, most);
+    if (row0 < 0 || row0 >= rows) return;
+    none = b < 0 || b >= p.sequences;
+    if (!none) length = p.lengths[b];
     const int last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
     end = none ? 0 : keys_of(length, new_tokens, divided(last, a.by_group), most);
     begin = a.prefix;
     table = p.table + (none ? 0 : b) * p.table_row;
   }
   end = __builtin_amdgcn_readfirstlane(end);
-  const int blocks = end > begin ? (end - begin + kBlockN - 1) / kBlockN : 0, share = (blocks + w.splits - 1) / w.splits;
+  const int blocks = end > begin ? (end - begin + kBlockN - 1) / kBlockN : 0, share = (blocks + splits - 1) / splits;
   const int block0 = part * share, block1 = block0 + share < blocks ? block0 + share : blocks;
-  // the wave's rows together: beyond the most that one sees a block is nothing to it, up to the least none is hidden
-  int most_keys = keys, least_keys = live ? keys : 0x7fffffff;
-#pragma unroll
-  for (int x = 1; x < 32; x *= 2) {
-    const int m1 = __shfl_xor(most_keys, x), m2 = __shfl_xor(least_keys, x);
-    most_keys = most_keys > m1 ? most_keys : m1;
-    least_keys = least_keys < m2 ? least_keys : m2;
-  }
-  most_keys = __builtin_amdgcn_readfirstlane(most_keys);
-  least_keys = __builtin_amdgcn_readfirstlane(least_keys);
-
-  Frag qf[DS];                                                      // row lane % 32, columns 16 ds + 8 half ..
-  {
-    const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
-#pragma unroll
-    for (int ds = 0; ds < DS; ++ds) {
-      const int c = ds * 16 + half * 8;
-      if (!PADDED || c < dim) qf[ds] = *reinterpret_cast<const Frag*>(q + c);
-      else qf[ds] = Frag{};
-    }
-  }
-  f32x16 o_acc[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.0f;
-  float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
 
   // ---- copies: instruction j of a wave takes kRowStep / 4 rows, a lane 16 bytes of one
   const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
@@ -172,6 +127,65 @@ void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
       *reinterpret_cast<u32x4*>(to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
     }
   };
+  int page = -1, next = -1;
+  if (block0 < block1) {                                            // on their way while the rows are looked up
+    page = find(block0);
+    next = find(block0 + 1);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) copy(j, false, block0, page, k_lds0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) copy(j, true, block0, page, v_lds0);
+  }
+
+  // this lane's row: its token, its queries and the keys it sees
+  const int wave_row = row0 + wave * 32, row = wave_row + lane % 32;
+  const bool live = row < rows;
+  const int in_seq = divided(live ? row : rows - 1, a.by_group), head = kvh * a.group + (live ? row : rows - 1) - in_seq * a.group;
+  const int token = token0 + in_seq;
+  Frag qf[DS];                                                      // row lane % 32, columns 16 ds + 8 half ..
+  {
+    const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      const int c = ds * 16 + half * 8;
+      if (!PADDED || c < dim) qf[ds] = *reinterpret_cast<const Frag*>(q + c);
+      else qf[ds] = Frag{};
+    }
+  }
+  int keys = 0;
+  if (shared) {
+    int s = token;                                                  // the row's sequence: this lane's own search
+    if (p.starts) {
+      int lo = 0, hi = p.sequences + 1;                             // the last one with starts[s] <= token, among 0 .. sequences
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.starts[mid] <= token) lo = mid;
+        else hi = mid;
+      }
+      s = lo < p.sequences && p.starts[lo] <= token ? lo : -1;
+    }
+    if (live && s >= 0) keys = keys_of(p.lengths[s], p.starts ? p.starts[s + 1] - token : 1, 0, most);
+    keys = keys < a.prefix ? keys : a.prefix;
+  } else if (live && !none) {
+    keys = keys_of(length, new_tokens, in_seq, most);
+  }
+  // the wave's rows together: beyond the most that one sees a block is nothing to it, up to the least none is hidden
+  int most_keys = keys, least_keys = live ? keys : 0x7fffffff;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) {
+    const int m1 = __shfl_xor(most_keys, x), m2 = __shfl_xor(least_keys, x);
+    most_keys = most_keys > m1 ? most_keys : m1;
+    least_keys = least_keys < m2 ? least_keys : m2;
+  }
+  most_keys = __builtin_amdgcn_readfirstlane(most_keys);
+  least_keys = __builtin_amdgcn_readfirstlane(least_keys);
+
+  f32x16 o_acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.0f;
+  float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
 
   auto process = [&](int block, uint64_t there, int next_page, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
     const int key0 = begin + block * kBlockN;
@@ -281,34 +295,27 @@ void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
     pv(vf1);
   };
 
-  if (block0 < block1) {
-    int page = find(block0), next = find(block0 + 1);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) copy(j, false, block0, page, k_lds0);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) copy(j, true, block0, page, v_lds0);
-    for (int block = block0; block < block1; block += 2) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      uint64_t there = __ballot(page >= 0);
-      page = next;
-      next = find(block + 2);
-      process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
-      if (block + 1 >= block1) break;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      there = __ballot(page >= 0);
-      page = next;
-      next = find(block + 3);
-      process(block + 1, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
-    }
+  for (int block = block0; block < block1; block += 2) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint64_t there = __ballot(page >= 0);
+    page = next;
+    next = find(block + 2);
+    process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
+    if (block + 1 >= block1) break;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    there = __ballot(page >= 0);
+    page = next;
+    next = find(block + 3);
+    process(block + 1, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
   }
 
   // ---- o_acc[dt][r] is column 32 dt + 8 (r / 4) + 4 half + r % 4 of the row's sum
   const float l = l_i + other_half(l_i);
   if (!live) return;
   if (w.sums.slots) {
-    const int64_t at = (w.slot + part) * w.sums.rows + (int64_t)token * a.heads + head;
+    const int64_t at = (int64_t)(part + (shared ? 0 : w.shared_splits)) * w.sums.rows + (int64_t)token * a.heads + head;
     if (half == 0) w.sums.ml[at] = float2{m_i, l};
     if (!(l > 0.0f)) return;
     float* out = w.sums.o + at * dim;
@@ -333,31 +340,44 @@ void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
     }
 }
 
-// A row's sums of all slots joined: 32 threads a row, a thread the columns d and, past 128, d + 128.
+// A row's sums of all slots (at most 32) joined: 32 threads a row, a thread the columns d and, past 128, d + 128.
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
   const int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   if (row >= sums.rows) return;
   const int d = threadIdx.x % 32 * 4;
-  float top = -INFINITY, sum = 0.0f;
-  for (int x = 0; x < sums.slots; ++x) {
-    const float2 ml = sums.ml[x * sums.rows + row];
-    if (ml.y > 0.0f) top = fmaxf(top, ml.x);
-  }
+  // lane x of the 32 has slot x's maximum and sum, and all four slots' columns are asked for at once
+  constexpr int kSlots = 4;
+  const int lane = threadIdx.x % kWave, own = lane % 32;
+  const float2 ml = own < sums.slots ? sums.ml[own * sums.rows + row] : float2{-INFINITY, 0.0f};
+  float top = ml.y > 0.0f ? ml.x : -INFINITY;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+  const float f = ml.y > 0.0f ? __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;
+  float sum = ml.y * f;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
   f32x4 out[2] = {};
-  for (int x = 0; x < sums.slots; ++x) {
-    const float2 ml = sums.ml[x * sums.rows + row];
-    if (!(ml.y > 0.0f)) continue;
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
+  for (int x0 = 0; x0 < sums.slots; x0 += kSlots) {
+    f32x4 o[kSlots][2];
+    float fx[kSlots];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (d + h * 128 < a.dim) {
-        const f32x4 ox = *reinterpret_cast<const f32x4*>(sums.o + (x * sums.rows + row) * a.dim + d + h * 128);
+    for (int x = 0; x < kSlots; ++x) {
+      fx[x] = __shfl(f, (lane & 32) + x0 + x);                      // 0: nothing there, and its columns are not read
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[h][e] = fmaf(ox[e], f, out[h][e]);
+      for (int h = 0; h < 2; ++h) {
+        o[x][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (fx[x] > 0.0f && d + h * 128 < a.dim)
+          o[x][h] = *reinterpret_cast<const f32x4*>(sums.o + ((x0 + x) * sums.rows + row) * a.dim + d + h * 128);
       }
+    }
+#pragma unroll
+    for (int x = 0; x < kSlots; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[h][e] = fmaf(o[x][h][e], fx[x], out[h][e]);
   }
   const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
@@ -369,7 +389,7 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
 
 template <typename T>
 int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipStream_t s) {
-  const unsigned grid = (unsigned)((int64_t)w.tiles * w.splits * p.kv_heads);
+  const unsigned grid = (unsigned)(((int64_t)w.tiles * w.splits + (int64_t)w.shared_tiles * w.shared_splits) * p.kv_heads);
 #define HEXMI_PAGED_TILE(D, COLS)                                                                                                         \
   do {                                                                                                                                    \
     if (a.dim == COLS) hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, false>), dim3(grid), dim3(kTileWaves * kWave), 0, s, a, p, w);   \
@@ -391,12 +411,13 @@ struct Plan {
   int64_t tiles;
   PagedDecodePlan one;
   int64_t rows, sum_bytes, decode_bytes;
-  int slots() const { return prefix_splits + (decode || (prefix_splits == 0 && splits == 1) ? 0 : splits); }
+  int slots() const { return prefix_splits == 0 && (decode || splits == 1) ? 0 : prefix_splits + (decode ? 1 : splits); }
 };
-// Parts of the keys for tiles of which there are `units`: two workgroups a compute unit, no part below four blocks.
+// Parts of the keys for tiles of which there are `units`: two workgroups a compute unit, no part below four blocks. A row has 32 slots for
+// the sums of its parts, of the prefix and its own together.
 int parts_of(int64_t units, int64_t keys) {
   const int64_t blocks = (keys + kBlockN - 1) / kBlockN, wanted = 2 * (int64_t)hexmi_num_cus() / units;
-  const int64_t most = blocks / 4 < 32 ? blocks / 4 : 32;
+  const int64_t most = blocks / 4 < 16 ? blocks / 4 : 16;
   return (int)(wanted < most ? (wanted > 1 ? wanted : 1) : (most > 1 ? most : 1));
 }
 Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
@@ -437,7 +458,7 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   const Plan plan = plan_of(b, heads, shared);
-  return plan.tiles * plan.splits * b.kv_heads <= limit / (kTileWaves * kWave) ? HEXMI_OK : HEXMI_ENOTSUP;
+  return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads <= limit / (kTileWaves * kWave) ? HEXMI_OK : HEXMI_ENOTSUP;
 }
 }  // namespace
 
@@ -475,9 +496,11 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   hipStream_t s = as_stream(stream);
   begin_call();
   auto tiles = [&](const TileArgs& w) { return dtype == HEXMI_F16 ? launch_tiles<f16>(a, p, w, s) : launch_tiles<bf16>(a, p, w, s); };
-  if (plan.prefix_splits > 0 && (rc = tiles({true, plan.prefix_tiles, plan.prefix_splits, 0, sums})) != HEXMI_OK) return rc;
-  if (plan.decode) return paged_decode(plan.one, a, p, dtype, workspace, sums, s);
-  if ((rc = tiles({false, (int)plan.tiles, plan.splits, plan.prefix_splits, sums})) != HEXMI_OK || sums.slots == 0) return rc;
+  if (plan.decode) {
+    if (plan.prefix_splits > 0 && (rc = tiles({plan.prefix_tiles, plan.prefix_splits, 0, 0, sums})) != HEXMI_OK) return rc;
+    return paged_decode(plan.one, a, p, dtype, workspace, sums, s);
+  }
+  if ((rc = tiles({plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums})) != HEXMI_OK || sums.slots == 0) return rc;
   const unsigned blocks = (unsigned)((plan.rows + 7) / 8);
   if (dtype == HEXMI_F16) hipLaunchKernelGGL((paged_join_kernel<f16>), dim3(blocks), dim3(256), 0, s, a, sums);
   else hipLaunchKernelGGL((paged_join_kernel<bf16>), dim3(blocks), dim3(256), 0, s, a, sums);

@@ -311,16 +311,11 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
         if (d == 0) w.part_ml[slot * 16 + r] = float2{top, sum};
         continue;
       }
-      const int64_t row = (int64_t)b * a.heads + head0 + r;
-      for (int x = 0; x < w.prefix.slots; ++x) {                     // the prefix's sums of this row
-        const float2 ml = w.prefix.ml[x * w.prefix.rows + row];
-        if (!(ml.y > 0.0f)) continue;
-        const f32x4 ox = *reinterpret_cast<const f32x4*>(w.prefix.o + (x * w.prefix.rows + row) * dim + d);
-        const float new_top = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(ml.x - new_top), old = __builtin_amdgcn_exp2f(top - new_top);
-        sum = fmaf(ml.y, f, sum * old);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = fmaf(ox[e], f, out[e] * old);
-        top = new_top;
+      if (w.prefix.slots) {                                          // to be joined with the prefix's
+        const int64_t at = (w.prefix.slots - 1) * w.prefix.rows + (int64_t)b * a.heads + head0 + r;
+        *reinterpret_cast<f32x4*>(w.prefix.o + at * dim + d) = out;
+        if (d == 0) w.prefix.ml[at] = float2{top, sum};
+        continue;
       }
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
       store4o<T>(static_cast<T*>(a.out) + b * a.out_token + (head0 + r) * a.out_head + d, out[0] * inv, out[1] * inv, out[2] * inv, out[3] * inv);
@@ -331,23 +326,43 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
 }
 
 // The units that several workers share: block (w, row) looks at the boundary between workers w and w + 1, and takes the unit that it
-// falls into if no earlier boundary does.
+// falls into if no earlier boundary does. Behind a prefix every unit is joined with its sums: block (unit, row).
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   __shared__ float o_lds[8][256 + 4];
   __shared__ float m_lds[8], l_lds[8];
   const int lane = threadIdx.x % kWave, units = p.kv_heads * w.row_tiles;
-  const int total = all_blocks(p, a.prefix, lane) * units, at = run_start(total, w.workers, blockIdx.x + 1);
-  if (at >= total) return;
-  int before;
-  const int b = sequence_at(p, a.prefix, units, at, lane, before);
-  const int blocks = blocks_of(p, b, a.prefix), u = (at - before * units) / blocks, first = before * units + u * blocks;
-  if (at == first || run_start(total, w.workers, blockIdx.x) > first) return;
+  int total = 0, b, u, first = 0, blocks = 1;
+  if (w.prefix.slots) {
+    b = blockIdx.x / units;
+    u = blockIdx.x - b * units;
+    if (w.workers) {
+      int before = 0;
+      for (int x = lane; x < p.sequences; x += kWave) {
+        const int n = blocks_of(p, x, a.prefix);
+        total += n;
+        if (x < b) before += n;
+      }
+      total = wave_sum_int(total) * units;
+      blocks = blocks_of(p, b, a.prefix);
+      first = wave_sum_int(before) * units + u * blocks;
+    }
+  } else {
+    total = all_blocks(p, a.prefix, lane) * units;
+    const int at = run_start(total, w.workers, blockIdx.x + 1);
+    if (at >= total) return;
+    int before;
+    b = sequence_at(p, a.prefix, units, at, lane, before);
+    blocks = blocks_of(p, b, a.prefix);
+    u = (at - before * units) / blocks;
+    first = before * units + u * blocks;
+    if (at == first || run_start(total, w.workers, blockIdx.x) > first) return;
+  }
   const int kvh = u / w.row_tiles, row0 = (u - kvh * w.row_tiles) * 16, r = blockIdx.y;
   if (r >= a.group - row0) return;
   const int head = kvh * a.group + row0 + r;
-  const int w0 = worker_of(total, w.workers, first), w1 = worker_of(total, w.workers, first + blocks - 1);
+  const int w0 = w.workers ? worker_of(total, w.workers, first) : 0, w1 = w.workers ? worker_of(total, w.workers, first + blocks - 1) : 0;
   const int64_t row = (int64_t)b * a.heads + head;
   // eight groups of 32 threads take every eighth set of sums, a thread the columns d and, past 128, d + 128
   const int group = threadIdx.x / 32, d = threadIdx.x % 32 * 4;
@@ -366,11 +381,11 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
         for (int e = 0; e < 4; ++e) out[h][e] = fmaf(ox[e], f, out[h][e] * old);
       }
   };
-  for (int x = w0 + group; x <= w1; x += 8) {
-    const int64_t slot = (int64_t)x * 2 + (x == w0 && run_start(total, w.workers, x) <= first ? 1 : 0);
+  for (int x = w0 + group; x <= w1 && w0 < w1; x += 8) {
+    const int64_t slot = (int64_t)x * 2 + (x == w0 ? 1 : 0);
     take(w.part_ml[slot * 16 + r], w.part_o + (slot * 16 + r) * a.dim);
   }
-  for (int x = group; x < w.prefix.slots; x += 8) take(w.prefix.ml[x * w.prefix.rows + row], w.prefix.o + (x * w.prefix.rows + row) * a.dim);
+  for (int x = group; x < w.prefix.slots - (w0 < w1 ? 1 : 0); x += 8) take(w.prefix.ml[x * w.prefix.rows + row], w.prefix.o + (x * w.prefix.rows + row) * a.dim);
 #pragma unroll
   for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(&o_lds[group][d + h * 128]) = out[h];
   if (d == 0) {
@@ -406,8 +421,9 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
   else HEXMI_PAGED_DECODE(256, 256);
 #undef HEXMI_PAGED_DECODE
   const int rc = launch_status();
-  if (rc != HEXMI_OK || plan.workers < 2) return rc;
-  hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
+  if (rc != HEXMI_OK || (plan.workers < 2 && w.prefix.slots == 0)) return rc;
+  const unsigned joins = w.prefix.slots ? (unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles) : plan.workers - 1;
+  hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(joins, plan.rows), dim3(256), 0, s, a, p, w);
   return launch_status();
 }
 
