@@ -45,41 +45,53 @@ __device__ __forceinline__ float sum_of_quarters(float v) {
 }
 
 // blocks of a sequence's unit: one at least, so that a row without keys is written too
-__device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) {
-  const int keys = length_of(p, b) - prefix;
-  return keys > kBlockKeys ? (keys + kBlockKeys - 1) / kBlockKeys : 1;
-}
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-  for (int x = 1; x < kWave; x *= 2) v += __shfl_xor(v, x);
+__device__ __forceinline__ int blocks_of_keys(int keys) { return keys > kBlockKeys ? (keys + kBlockKeys - 1) / kBlockKeys : 1; }
+__device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) { return blocks_of_keys(length_of(p, b) - prefix); }
+// the sum over the lanes up to this one
+__device__ __forceinline__ int sum_up_to(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);     // row_shr:1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);    // row_bcast:15 into the second and fourth 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);    // row_bcast:31 into the upper 32
   return v;
 }
-__device__ __forceinline__ int all_blocks(const Pages& p, int prefix, int lane) {
-  int n = 0;
-  for (int b = lane; b < p.sequences; b += kWave) n += blocks_of(p, b, prefix);
-  return wave_sum_int(n);
+__device__ __forceinline__ int of_last_lane(int v) { return __builtin_amdgcn_readlane(v, kWave - 1); }
+
+// The list of all blocks, sequence by sequence: lengths, blocks and sums of blocks of the first 64 sequences are a lane's each, read once;
+// those of further ones are read again where they are needed.
+struct BlockList {
+  int length, blocks, up_to;                   // lane b: of sequence b, and of all up to it
+  int of_64, all;                              // blocks of the first 64 sequences, of all (one unit's)
+};
+__device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int lane) {
+  BlockList l;
+  l.length = lane < p.sequences ? length_of(p, lane) : 0;
+  l.blocks = lane < p.sequences ? blocks_of_keys(l.length - prefix) : 0;
+  l.up_to = sum_up_to(l.blocks);
+  l.of_64 = of_last_lane(l.up_to);
+  int more = 0;
+  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of(p, b0 + lane, prefix) : 0;
+  l.all = l.of_64 + (p.sequences > kWave ? of_last_lane(sum_up_to(more)) : 0);
+  return l;
 }
-// The sequence that block `at` of the list of all blocks belongs to, with `units` units a sequence, and the blocks (of one unit)
-// before it.
-__device__ __forceinline__ int sequence_at(const Pages& p, int prefix, int units, int at, int lane, int& before) {
+// The sequence that block `at` of the list belongs to, with `units` units a sequence, and the blocks (of one unit) before it.
+__device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, int units, int at, int lane, int& before) {
   before = 0;
-  for (int b0 = 0; b0 < p.sequences; b0 += kWave) {
-    const int b = b0 + lane, n = b < p.sequences ? blocks_of(p, b, prefix) : 0;
-    int sum = n;
-#pragma unroll
-    for (int x = 1; x < kWave; x *= 2) {
-      const int below = __shfl_up(sum, x);
-      if (lane >= x) sum += below;
-    }
+  for (int b0 = 0;; b0 += kWave) {
+    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of(p, b0 + lane, prefix) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
     const uint64_t past = __ballot((before + sum) * units > at);
-    if (past) {
-      const int first = __ffsll((unsigned long long)past) - 1;
-      before += __shfl(sum - n, first);
+    if (past || b0 + kWave >= p.sequences) {   // `at` is below the end: there is one
+      const int first = past ? __ffsll((unsigned long long)past) - 1 : 0;
+      before += __builtin_amdgcn_readlane(sum - n, first);
       return b0 + first;
     }
-    before += __shfl(sum, kWave - 1);
+    before += of_last_lane(sum);
   }
-  return p.sequences;                          // at is past the end: callers do not ask
+}
+__device__ __forceinline__ int length_at(const BlockList& l, const Pages& p, int b) {
+  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.length, b & (kWave - 1)) : length_of(p, b));
 }
 // worker w's run of `total` blocks
 __device__ __forceinline__ int run_start(int total, int workers, int w) {
@@ -95,9 +107,14 @@ __device__ __forceinline__ int worker_of(int total, int workers, int at) {
 // 32 bytes) stand on all banks once
 template <int D> __device__ __forceinline__ int swz_pairs(int row) { return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; }
 
+// A unit that a worker begins and others go on with: its sequence, unit and last worker (none: last < 0).
+struct Shared {
+  int sequence, unit, last, pad;
+};
 struct DecodeArgs {
   float* part_o;                               // [workers][2][16][dim]
   float2* part_ml;                             // [workers][2][16]
+  Shared* begun;                               // [workers]
   int workers, row_tiles;
   RowSums prefix;
 };
@@ -109,37 +126,43 @@ __global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
 void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   typedef typename MfmaT<T>::Frag Frag;
   constexpr int DS = COLS / 32, DT = COLS / 16, CPR = D / 8, kPitch = COLS + 4;
-  constexpr int kWaveBytes = kTileKeys * D * 2 > 16 * kPitch * 4 ? kTileKeys * D * 2 : 16 * kPitch * 4;
+  constexpr int kSumBytes = (16 * kPitch * 4 + D * 2 - 1) / (D * 2) * (D * 2);      // a wave's part starts at a row's multiple
+  constexpr int kWaveBytes = kTileKeys * D * 2 > kSumBytes ? kTileKeys * D * 2 : kSumBytes;
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kWaveBytes];
   __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane / 16, n = lane % 16;
   const int dim = PADDED ? a.dim : COLS;
-  T* v_lds = reinterpret_cast<T*>(lds + wave * kWaveBytes);
+  // This lane's bytes of V in LDS, rows of D columns in 16-byte chunks: chunk g of row n, where it puts, and columns 4 (n % 4) .. of row
+  // 4 g + n / 4, from where it takes (ds_read_b64_tr_b16: a group of 16 lanes asks for 4 rows x 16 columns, and a lane gets a column).
+  // Other chunks are these with the chunk's number XORed in.
+  const int put_at = wave * kWaveBytes + n * (D * 2) + (g ^ swz_pairs<D>(n)) * 16;
+  const int take_row = 4 * g + (n >> 2), take_at = wave * kWaveBytes + take_row * (D * 2) + (((n & 3) >> 1) ^ swz_pairs<D>(take_row)) * 16 + (n & 1) * 8;
   float* o_lds = reinterpret_cast<float*>(lds + wave * kWaveBytes);
   const int units = p.kv_heads * w.row_tiles;
 
-  int cur, end, b, before, start = 0;
+  BlockList list;
+  int cur, end, b, before = 0, total = 0;
   if (w.workers == 0) {                        // a unit each
     b = blockIdx.x / units;
-    before = 0;
-    const int u = blockIdx.x - b * units, blocks = blocks_of(p, b, a.prefix);
+    list.length = 0;
+    const int u = blockIdx.x - b * units, blocks = __builtin_amdgcn_readfirstlane(blocks_of(p, b, a.prefix));
     cur = u * blocks;
     end = cur + blocks;
-    start = cur;
   } else {
-    const int total = all_blocks(p, a.prefix, lane) * units;
+    list = block_list(p, a.prefix, lane);
+    total = list.all * units;
     cur = run_start(total, w.workers, blockIdx.x);
     end = run_start(total, w.workers, blockIdx.x + 1);
+    if (wave == 0 && lane == 0) w.begun[blockIdx.x].last = -1;
     if (cur >= end) return;
-    start = cur;
-    b = sequence_at(p, a.prefix, units, cur, lane, before);
+    b = sequence_at(list, p, a.prefix, units, cur, lane, before);
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  before = __builtin_amdgcn_readfirstlane(before);
+  const int start = cur;
 
   while (cur < end) {
-    const int length = length_of(p, b), blocks = blocks_of(p, b, a.prefix), local = cur - before * units;
+    const int length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
+    const int blocks = blocks_of_keys(length - a.prefix), local = cur - before * units;
     if (local >= blocks * units) {             // on to the next sequence
       before += blocks;
       ++b;
@@ -177,35 +200,35 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     const int32_t* table = p.table + b * p.table_row;
     const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
     const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
-    struct Keys { int page[2], slot[2]; };
-    auto find = [&](int key0) __attribute__((always_inline)) {       // where keys key0 + n and key0 + 16 + n stand
+    // where keys key0 + n and key0 + 16 + n stand; past the end: the last key again, without weight
+    struct Keys { int page[2]; };
+    auto clamped = [&](int key) __attribute__((always_inline)) { return key < key_end ? key : key_end - 1; };
+    auto find = [&](int key0) __attribute__((always_inline)) {
       Keys k;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        int key = key0 + t * 16 + n;
-        key = key < key_end ? key : key_end - 1;                     // past the end: the last key again, without weight
-        const int column = divided(key, p.size);
-        k.page[t] = table[column];
-        k.slot[t] = key - column * p.page_size;
-      }
+      for (int t = 0; t < 2; ++t) k.page[t] = table[divided(clamped(key0 + t * 16 + n), p.size)];
       return k;
     };
     auto there = [&](int page) __attribute__((always_inline)) { return page >= 0 && page < p.num_pages; };
-    u32x4 kr[2][DS], vr[2][DS];
-    auto load = [&](const Keys& at, const T* base, int64_t page, int64_t slot, u32x4 (*r)[DS]) __attribute__((always_inline)) {
+    auto load = [&](const Keys& at, int key0, const T* base, int64_t page_stride, int64_t slot_stride, u32x4 (*r)[DS]) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const T* row = base + (there(at.page[t]) ? at.page[t] : 0) * page + at.slot[t] * slot;
+        const int key = clamped(key0 + t * 16 + n), slot = key - divided(key, p.size) * p.page_size;
+        const T* row = base + (there(at.page[t]) ? at.page[t] : 0) * page_stride + slot * slot_stride;
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) r[t][ds] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + col[ds]));
+        for (int ds = 0; ds < DS; ++ds) r[t][ds] = *reinterpret_cast<const u32x4*>(row + col[ds]);
       }
     };
     if (key_first < key_end) {
+      u32x4 kr[2][DS], vr[2][DS];
       Keys now = find(key_first), next = find(key_first + kBlockKeys);
-      load(now, k_head, p.k_page, p.k_slot, kr);
-      load(now, v_head, p.v_page, p.v_slot, vr);
+      load(now, key_first, k_head, p.k_page, p.k_slot, kr);
+      load(now, key_first, v_head, p.v_page, p.v_slot, vr);
       for (int key0 = key_first; key0 < key_end; key0 += kBlockKeys) {
         __builtin_amdgcn_sched_barrier(0);
+        // what the constants of a chunk are XORed into; kept from becoming a register each
+        int to = put_at, from = take_at;
+        asm volatile("" : "+v"(to), "+v"(from));
         f32x4 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -216,7 +239,7 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
         const bool ok0 = there(now.page[0]) && key0 + n < key_end, ok1 = there(now.page[1]) && key0 + 16 + n < key_end;
         const bool whole = __ballot(ok0 && ok1) == ~0ull;
         __builtin_amdgcn_sched_barrier(0);
-        load(next, k_head, p.k_page, p.k_slot, kr);                  // past the last tile: its last key again
+        load(next, key0 + kBlockKeys, k_head, p.k_page, p.k_slot, kr);
         __builtin_amdgcn_sched_barrier(0);
         if (!whole) {                                                // what stands where no key is may be anything: no weight, and zeros of V
           const uint32_t k0 = (uint32_t)__ballot(ok0), k1 = (uint32_t)__ballot(ok1);
@@ -234,14 +257,9 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int ds = 0; ds < DS; ++ds) {
-            const int row = t * 16 + n;
-            *reinterpret_cast<u32x4*>(v_lds + (row * CPR + ((ds * 4 + g) ^ swz_pairs<D>(row))) * 8) = vr[t][ds];
-          }
+          for (int ds = 0; ds < DS; ++ds) *reinterpret_cast<u32x4*>(lds + (to ^ (ds * 64)) + t * (16 * D * 2)) = vr[t][ds];
         __builtin_amdgcn_sched_barrier(0);
-        load(next, v_head, p.v_page, p.v_slot, vr);
-        now = next;
-        next = find(key0 + 2 * kBlockKeys);
+        load(next, key0 + kBlockKeys, v_head, p.v_page, p.v_slot, vr);
         __builtin_amdgcn_sched_barrier(0);
         // online softmax, the reference maximum up to kRescaleLag behind the true one (flash_attn.hip)
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -267,14 +285,15 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
         for (int dt = 0; dt < DT; ++dt) {
           union { i16x4 h[2]; Frag f; } v;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int row = t * 16 + 4 * g + (n >> 2), c = (dt * 2 + ((n & 3) >> 1)) ^ swz_pairs<D>(row);
+          for (int t = 0; t < 2; ++t)
             v.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4*)(v_lds + (row * CPR + c) * 8 + (n & 1) * 4));
-          }
+                (__attribute__((address_space(3))) i16x4*)(lds + (from ^ (dt * 32)) + t * (16 * D * 2)));
           o[dt] = Mfma16<T>::run(v.f, pf, o[dt]);
+          if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // no more than four pieces of V in registers
         }
         asm volatile("" ::: "memory");
+        now = next;
+        next = find(key0 + 2 * kBlockKeys);
       }
     }
 
@@ -288,7 +307,9 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     }
     __syncthreads();
     const bool mine = block0 == 0 && count == blocks;
-    const int slot = blockIdx.x * 2 + (cur == start && block0 != 0 ? 0 : 1);
+    const int slot = blockIdx.x * 2 + (block0 != 0 ? 0 : 1);         // what another began, or what it begins
+    if (threadIdx.x == 0 && w.workers && block0 == 0 && !mine)
+      w.begun[blockIdx.x] = Shared{b, u, worker_of(total, w.workers, cur + blocks - 1), 0};
     for (int i = threadIdx.x; i < rows * (COLS / 4); i += kWaves * kWave) {
       const int r = i / (COLS / 4), d = i % (COLS / 4) * 4;
       if (PADDED && d >= dim) continue;
@@ -325,44 +346,39 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   }
 }
 
-// The units that several workers share: block (w, row) looks at the boundary between workers w and w + 1, and takes the unit that it
-// falls into if no earlier boundary does. Behind a prefix every unit is joined with its sums: block (unit, row).
+// The units that several workers share: block (w, row) takes the one that worker w began. Behind a prefix every unit is joined with its
+// sums: block (unit, row).
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   __shared__ float o_lds[8][256 + 4];
   __shared__ float m_lds[8], l_lds[8];
-  const int lane = threadIdx.x % kWave, units = p.kv_heads * w.row_tiles;
-  int total = 0, b, u, first = 0, blocks = 1;
+  const int units = p.kv_heads * w.row_tiles, r = blockIdx.y;
+  int b, u, w0 = 0, w1 = 0;
   if (w.prefix.slots) {
     b = blockIdx.x / units;
     u = blockIdx.x - b * units;
     if (w.workers) {
+      const int lane = threadIdx.x % kWave;
+      const BlockList list = block_list(p, a.prefix, lane);
       int before = 0;
-      for (int x = lane; x < p.sequences; x += kWave) {
-        const int n = blocks_of(p, x, a.prefix);
-        total += n;
-        if (x < b) before += n;
-      }
-      total = wave_sum_int(total) * units;
-      blocks = blocks_of(p, b, a.prefix);
-      first = wave_sum_int(before) * units + u * blocks;
+      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of(p, x, a.prefix);
+      const int blocks = blocks_of_keys(length_at(list, p, b) - a.prefix), total = list.all * units;
+      const int first = of_last_lane(sum_up_to(before)) * units + u * blocks;
+      w0 = worker_of(total, w.workers, first);
+      w1 = worker_of(total, w.workers, first + blocks - 1);
     }
   } else {
-    total = all_blocks(p, a.prefix, lane) * units;
-    const int at = run_start(total, w.workers, blockIdx.x + 1);
-    if (at >= total) return;
-    int before;
-    b = sequence_at(p, a.prefix, units, at, lane, before);
-    blocks = blocks_of(p, b, a.prefix);
-    u = (at - before * units) / blocks;
-    first = before * units + u * blocks;
-    if (at == first || run_start(total, w.workers, blockIdx.x) > first) return;
+    const Shared begun = w.begun[blockIdx.x];
+    if (begun.last < 0) return;
+    b = begun.sequence;
+    u = begun.unit;
+    w0 = blockIdx.x;
+    w1 = begun.last;
   }
-  const int kvh = u / w.row_tiles, row0 = (u - kvh * w.row_tiles) * 16, r = blockIdx.y;
+  const int kvh = u / w.row_tiles, row0 = (u - kvh * w.row_tiles) * 16;
   if (r >= a.group - row0) return;
   const int head = kvh * a.group + row0 + r;
-  const int w0 = w.workers ? worker_of(total, w.workers, first) : 0, w1 = w.workers ? worker_of(total, w.workers, first + blocks - 1) : 0;
   const int64_t row = (int64_t)b * a.heads + head;
   // eight groups of 32 threads take every eighth set of sums, a thread the columns d and, past 128, d + 128
   const int group = threadIdx.x / 32, d = threadIdx.x % 32 * 4;
@@ -434,18 +450,23 @@ PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int
   const int64_t most = b.table_cols * b.page_size - prefix, blocks = most > kBlockKeys ? (most + kBlockKeys - 1) / kBlockKeys : 1;
   const int rows = (int)(group < 16 ? group : 16);
   if (blocks <= 1) return {0, (int)tiles, rows};
-  const int64_t workers = 2 * (int64_t)hexmi_num_cus();
-  return {(int)(units * blocks < workers ? units * blocks : workers), (int)tiles, rows};
+  // A block each while they are fewer than the compute units; then four and more, so that a worker's sums are few beside its keys, on as
+  // many workgroups as a compute unit holds. One and two a compute unit, heads of 128: 1 sequence x 16000 keys x 8 heads 21.9 / 24.5 us,
+  // 3 x 5000 15.2 / 17.0; 128 x 500 58 / 52, 16 x 2048 x 32 97.7 / 93.5. Heads of 256, of which it holds one: 16 x 2048 x 8 56 / 60.
+  const int64_t cus = hexmi_num_cus(), all = units * blocks, held = cus * (b.dim <= 96 ? 3 : b.dim <= 128 ? 2 : 1);
+  const int64_t fours = all / 4 < cus ? cus : all / 4, workers = all < cus ? all : fours < held ? fours : held;
+  return {(int)(workers < 1 ? 1 : workers), (int)tiles, rows};
 }
 
 int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim) {
-  return (int64_t)plan.workers * 2 * 16 * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
+  return (int64_t)plan.workers * (2 * 16 * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2)) + (int64_t)sizeof(Shared));
 }
 
 int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const RowSums& prefix,
                  hipStream_t s) {
   float* o = static_cast<float*>(workspace);
-  const DecodeArgs w = {o, reinterpret_cast<float2*>(o + (int64_t)plan.workers * 2 * 16 * a.dim), plan.workers, plan.row_tiles, prefix};
+  float2* ml = reinterpret_cast<float2*>(o + (int64_t)plan.workers * 2 * 16 * a.dim);
+  const DecodeArgs w = {o, ml, reinterpret_cast<Shared*>(ml + (int64_t)plan.workers * 2 * 16), plan.workers, plan.row_tiles, prefix};
   return dtype == HEXMI_F16 ? launch<f16>(plan, a, p, w, s) : launch<bf16>(plan, a, p, w, s);
 }
 
