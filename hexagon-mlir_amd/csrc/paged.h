@@ -85,15 +85,35 @@ struct RowSums {
   int64_t rows;
   int slots;
 };
-// One new token a sequence: how the keys are shared out (workers; 0: every unit of sequence, key head and 16 query heads whole), and
-// the launch behind a prefix whose sums are there, in all slots of `prefix` but the last, which is for a unit's own sums (slots 0: no
-// prefix).
+// One launch: the prefix for all rows (the first workgroups), and every sequence's keys behind it.
+struct TileArgs {
+  int shared_tiles, shared_splits;             // tiles of a key head; parts of the prefix, whose sums go to slots 0 .. (0: no prefix)
+  int tiles, splits;                           // of the sequences' own keys, whose sums go to the slots behind (0: decode, not here)
+  RowSums sums;                                // slots 0: the result goes to out
+};
+
+// One new token a sequence: how the keys are shared out (workers; 0: every unit of sequence, key head and 16 query heads whole).
 struct PagedDecodePlan {
   int workers, row_tiles, rows;
 };
+// A unit that a worker begins and others go on with: its sequence, unit and last worker (none: last < 0).
+struct BegunUnit {
+  int sequence, unit, last, pad;
+};
+struct DecodeArgs {
+  float* part_o;                               // [workers][2][16][dim]
+  float2* part_ml;                             // [workers][2][16]
+  BegunUnit* begun;                               // [workers]
+  int workers, row_tiles;
+  RowSums prefix;                              // slots: the prefix's and, last, one for a unit's own sums (0: no prefix)
+};
 PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix);
 int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim);
-int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const RowSums& prefix,
+// tiles: of the prefix (shared_splits 0: none), whose sums' last slot is for the sequences' own keys
+int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const TileArgs& tiles,
                  hipStream_t s);
+// the prefix's tiles and `grid` workers in one launch (paged_shared.hip)
+int paged_shared_decode(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
+                        hipStream_t s);
 
 }  // namespace hexmi

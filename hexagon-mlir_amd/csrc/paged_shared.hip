@@ -1,0 +1,51 @@
+// A decode step behind a prefix that all sequences share: the prefix's tiles (paged_tile.h), which the matrix cores bind, and the workers on
+// the sequences' own keys (paged_decode.h), which wait for memory, in one launch side by side. Their sums are joined by
+// paged_decode_join_kernel. 32 sequences x 200 keys behind 8192 (32 heads over 8, of 128): one launch after the other 37 us, this way 23.
+#include "paged_decode.h"
+#include "paged_tile.h"
+
+namespace hexmi {
+namespace {
+
+static_assert(kWaves == kTileWaves, "one workgroup size");
+
+template <typename T, int D, int COLS, bool PADDED>
+__global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
+void paged_shared_decode_kernel(PagedAttnArgs a, Pages p, TileArgs tiles, DecodeArgs w, unsigned tile_grid) {
+  constexpr int kTile = kBlockN * D, kTileBytes = 4 * kTile * 2, kDecodeBytes = kWaves * decode_wave_bytes(D, COLS);
+  __shared__ __attribute__((aligned(16))) char lds[kTileBytes > kDecodeBytes ? kTileBytes : kDecodeBytes];
+  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
+  if (blockIdx.x < tile_grid) {
+    T* t = reinterpret_cast<T*>(lds);
+    paged_tile<T, D, COLS, PADDED>(a, p, tiles, blockIdx.x, tile_grid, t, t + kTile, t + 2 * kTile, t + 3 * kTile);
+  } else {
+    paged_decode_worker<T, D, COLS, PADDED>(a, p, w, blockIdx.x - tile_grid, lds, m_lds, l_lds);
+  }
+}
+
+template <typename T>
+int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned workers, hipStream_t s) {
+  const unsigned tile_grid = (unsigned)((int64_t)tiles.shared_tiles * tiles.shared_splits * p.kv_heads), grid = tile_grid + workers;
+#define HEXMI_PAGED_SHARED(D, COLS)                                                                                                      \
+  do {                                                                                                                                   \
+    if (a.dim == COLS)                                                                                                                   \
+      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, false>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, tiles, w, tile_grid); \
+    else                                                                                                                                 \
+      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, true>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, tiles, w, tile_grid);  \
+  } while (0)
+  if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64);
+  else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96);
+  else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128);
+  else HEXMI_PAGED_SHARED(256, 256);
+#undef HEXMI_PAGED_SHARED
+  return launch_status();
+}
+
+}  // namespace
+
+int paged_shared_decode(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
+                        hipStream_t s) {
+  return dtype == HEXMI_F16 ? launch<f16>(a, p, tiles, w, grid, s) : launch<bf16>(a, p, tiles, w, grid, s);
+}
+
+}  // namespace hexmi

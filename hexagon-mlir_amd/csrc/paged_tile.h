@@ -1,0 +1,334 @@
+// A tile of query rows over the pages of a cache (paged_attn.hip, paged_shared.hip).
+//
+// The query rows of a key head, (token, head of its group) one behind the other, are cut into tiles of kRows; a workgroup of four waves
+// takes a tile, 32 rows a wave, and walks the keys up to its last token's own in blocks of 64, as flash_attn.hip does: S^T = K Q^T with
+// v_mfma_f32_32x32x16, online softmax in registers, O^T += V^T P^T with V read transposed from LDS. What differs is where things stand:
+// a block's 64 pages are looked up a block ahead, a lane each, a key's row is copied into LDS from wherever its page is, and a block
+// carries a bit a key that says whether it is one. Heads that share their keys share a tile, so a step of decode in a batch with
+// prompts reads its keys once too; a wave whose rows are none only copies.
+//
+// The prefix is one sequence that all rows of the batch attend: its keys go through LDS once for kRows rows, whatever sequences they are
+// of. Its sums, and those of tiles whose keys are cut over several workgroups because there are few, go through the workspace.
+#pragma once
+#include "flash_attn_tiles.h"
+#include "paged.h"
+
+namespace hexmi {
+namespace {
+
+constexpr int kTileWaves = 4, kRows = kTileWaves * 32;
+
+// The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences, where -1 and `sequences` are the
+// rows of no sequence before the first and behind the last. floor(x / r) + 1 >= ceil(n / r) + floor(x0 / r) for x = x0 + n, so
+// a sequence's tiles end before the next one's begin; some numbers are no tile.
+__device__ __forceinline__ int first_row(const Pages& p, int b) {
+  const int s = b < 0 ? 0 : b > p.sequences ? p.tokens : p.starts[b];
+  return s < 0 ? 0 : s < p.tokens ? s : p.tokens;
+}
+__device__ __forceinline__ int first_tile(const Pages& p, int group, int b) { return b < 0 ? 0 : first_row(p, b) * group / kRows + b + 1; }
+__device__ __forceinline__ int sequence_of_tile(const Pages& p, int group, int tile, int lane) {
+  int lo = -1, hi = p.sequences + 1;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const int n = __popcll(__ballot(at < hi && first_tile(p, group, at) <= tile));
+    lo += (n > 0 ? n - 1 : 0) * step;
+    hi = lo + step < hi ? lo + step : hi;
+    if (step == 1) break;
+  }
+  return lo;
+}
+
+// keys that token i of a sequence's n sees, whatever the index tensors hold
+__device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
+  const int64_t keys = length - n + i + 1;
+  return keys < 0 ? 0 : keys < most ? (int)keys : most;
+}
+
+// D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
+// columns lie past the head copies the head's first ones instead: the query has zeros there, and what comes of V there is not stored.
+// A workgroup's tile: number `block` of a launch whose tiles are `grid` workgroups; k_lds0 .. v_lds1: 64 rows of D each.
+template <typename T, int D, int COLS, bool PADDED>
+__device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, unsigned block_id, unsigned grid,
+                                           T* k_lds0, T* k_lds1, T* v_lds0, T* v_lds1) {
+  typedef typename MfmaT<T>::Frag Frag;
+  constexpr int DS = COLS / 16, DT = COLS / 32, CPR = D / 8;
+  constexpr int NI = kBlockN * CPR / kWave / kTileWaves, kRowStep = kTileWaves * kWave / CPR;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
+  const int dim = PADDED ? a.dim : COLS;
+
+  // Workgroup -> (prefix or not, key head, tile, part). Workgroup ids go round robin to the 8 XCDs (one L2 each): every XCD gets a run of
+  // the list, key head by key head, a sequence's last (longest) tiles first.
+  const unsigned shared_grid = (unsigned)(w.shared_tiles * w.shared_splits * p.kv_heads);
+  const bool shared = block_id < shared_grid;
+  const int tiles = shared ? w.shared_tiles : w.tiles, splits = shared ? w.shared_splits : w.splits;
+  const unsigned id = shared ? block_id : block_id - shared_grid, count = shared ? shared_grid : grid - shared_grid;
+  const unsigned xcd = id % 8, each = count / 8, more = count % 8;
+  const unsigned unit = xcd * each + (xcd < more ? xcd : more) + id / 8;
+  const int part = unit % splits, tile = tiles - 1 - (int)(unit / splits % tiles), kvh = unit / splits / tiles;
+
+  int token0 = 0, rows, row0, new_tokens = 0, begin = 0, end;
+  int64_t length = 0;
+  bool none = false;                                                // rows of no sequence
+  const int most = p.table_cols * p.page_size;
+  const int32_t* table;
+  if (shared) {
+    row0 = tile * kRows;
+    rows = p.tokens * a.group;
+    end = a.prefix;
+    table = a.shared;
+  } else {
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile(p, a.group, tile, lane));
+    token0 = first_row(p, b);
+    new_tokens = first_row(p, b + 1) - token0;
+    row0 = (tile - first_tile(p, a.group, b)) * kRows;
+    rows = new_tokens * a.group;                                    // negative where starts fall: nothing
+    if (row0 < 0 || row0 >= rows) return;
+    none = b < 0 || b >= p.sequences;
+    if (!none) length = p.lengths[b];
+    const int last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
+    end = none ? 0 : keys_of(length, new_tokens, divided(last, a.by_group), most);
+    begin = a.prefix;
+    table = p.table + (none ? 0 : b) * p.table_row;
+  }
+  end = __builtin_amdgcn_readfirstlane(end);
+  const int blocks = end > begin ? (end - begin + kBlockN - 1) / kBlockN : 0, share = (blocks + splits - 1) / splits;
+  const int block0 = part * share, block1 = block0 + share < blocks ? block0 + share : blocks;
+
+  // ---- copies: instruction j of a wave takes kRowStep / 4 rows, a lane 16 bytes of one
+  const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
+  const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
+  const int lin = wave * kWave + lane, copy_row = lin / CPR, lds_at = wave * kWave * 8;
+  auto find = [&](int block) __attribute__((always_inline)) {       // the page of key 64 block + lane, -1: none
+    const int key = begin + block * kBlockN + lane;
+    if (block >= block1 || key >= end) return -1;
+    const int page = table[divided(key, p.size)];
+    return page < p.num_pages ? page : -1;
+  };
+  auto copy = [&](int j, bool v, int block, int page_of_lane, T* lds) __attribute__((always_inline)) {
+    const int r = copy_row + j * kRowStep, key = begin + block * kBlockN + r, page = __shfl(page_of_lane, r);
+    int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
+    if (PADDED && c >= dim) c = 0;
+    T* to = lds + lds_at + j * (kTileWaves * kWave * 8);
+    if (page >= 0) {
+      const int slot = key - divided(key, p.size) * p.page_size;
+      const T* from = v ? v_head + page * p.v_page + slot * p.v_slot + c : k_head + page * p.k_page + slot * p.k_slot + c;
+      __builtin_amdgcn_global_load_lds(HEXMI_GLB(from), HEXMI_LDS(to), 16, 0, 0);
+    } else if (v) {                                                 // no key: whatever the cache holds, zeros of V (its score is dropped)
+      *reinterpret_cast<u32x4*>(to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  int page = -1, next = -1;
+  if (block0 < block1) {                                            // on their way while the rows are looked up
+    page = find(block0);
+    next = find(block0 + 1);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) copy(j, false, block0, page, k_lds0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) copy(j, true, block0, page, v_lds0);
+  }
+
+  // this lane's row: its token, its queries and the keys it sees
+  const int wave_row = row0 + wave * 32, row = wave_row + lane % 32;
+  const bool live = row < rows;
+  const int in_seq = divided(live ? row : rows - 1, a.by_group), head = kvh * a.group + (live ? row : rows - 1) - in_seq * a.group;
+  const int token = token0 + in_seq;
+  Frag qf[DS];                                                      // row lane % 32, columns 16 ds + 8 half ..
+  {
+    const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      const int c = ds * 16 + half * 8;
+      if (!PADDED || c < dim) qf[ds] = *reinterpret_cast<const Frag*>(q + c);
+      else qf[ds] = Frag{};
+    }
+  }
+  int keys = 0;
+  if (shared) {
+    int s = token;                                                  // the row's sequence: this lane's own search
+    if (p.starts) {
+      int lo = 0, hi = p.sequences + 1;                             // the last one with starts[s] <= token, among 0 .. sequences
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.starts[mid] <= token) lo = mid;
+        else hi = mid;
+      }
+      s = lo < p.sequences && p.starts[lo] <= token ? lo : -1;
+    }
+    if (live && s >= 0) keys = keys_of(p.lengths[s], p.starts ? p.starts[s + 1] - token : 1, 0, most);
+    keys = keys < a.prefix ? keys : a.prefix;
+  } else if (live && !none) {
+    keys = keys_of(length, new_tokens, in_seq, most);
+  }
+  // the wave's rows together: beyond the most that one sees a block is nothing to it, up to the least none is hidden
+  int most_keys = keys, least_keys = live ? keys : 0x7fffffff;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) {
+    const int m1 = __shfl_xor(most_keys, x), m2 = __shfl_xor(least_keys, x);
+    most_keys = most_keys > m1 ? most_keys : m1;
+    least_keys = least_keys < m2 ? least_keys : m2;
+  }
+  most_keys = __builtin_amdgcn_readfirstlane(most_keys);
+  least_keys = __builtin_amdgcn_readfirstlane(least_keys);
+
+  f32x16 o_acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.0f;
+  float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
+
+  auto process = [&](int block, uint64_t there, int next_page, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    const int key0 = begin + block * kBlockN;
+    if (block + 1 < block1) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) copy(j, false, block + 1, next_page, k_dst);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) copy(j, true, block + 1, next_page, v_dst);
+    }
+    if (key0 >= most_keys) return;                                  // wave-uniform; the barriers are outside
+    f32x16 s[2];
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[jt][r] = 0.0f;
+    {
+      constexpr int kAhead = 3;
+      auto read_k = [&](int jt, int ds) __attribute__((always_inline)) {
+        const int r = jt * 32 + lane % 32, c = (ds * 2 + half) ^ swz_ktile<D == 64 ? 64 : 128>(r);
+        return *reinterpret_cast<const Frag*>(k_src + (r * CPR + c) * 8);
+      };
+      Frag kf[2][DS];
+#pragma unroll
+      for (int ds = 0; ds < kAhead && ds < DS; ++ds) {
+        kf[0][ds] = read_k(0, ds);
+        kf[1][ds] = read_k(1, ds);
+      }
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) {
+        if (ds + kAhead < DS) {
+          kf[0][ds + kAhead] = read_k(0, ds + kAhead);
+          kf[1][ds + kAhead] = read_k(1, ds + kAhead);
+        }
+        s[0] = MfmaT<T>::run(kf[0][ds], qf[ds], s[0]);
+        s[1] = MfmaT<T>::run(kf[1][ds], qf[ds], s[1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    struct VFrags { Frag f[2][DT]; };
+    auto read_v = [&](int jt, VFrags& vf) __attribute__((always_inline)) {
+      const int g = lane / 16, i16 = lane % 16;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          union { i16x4 h[2]; Frag f; } u;
+#pragma unroll
+          for (int pp = 0; pp < 2; ++pp) {
+            const int r = jt * 32 + hf * 16 + 8 * pp + 4 * (g >> 1) + (i16 >> 2), col = dt * 32 + (g & 1) * 16 + (i16 & 3) * 4;
+            const int c = (col / 8) ^ swz_vtile<D == 64 ? 64 : 128>(r);
+            u.h[pp] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(v_src + (r * CPR + c) * 8 + col % 8));
+          }
+          vf.f[hf][dt] = u.f;
+        }
+    };
+    VFrags vf0, vf1;
+    read_v(0, vf0);
+    __builtin_amdgcn_sched_barrier(0);
+    // s[jt][r] is the score of key key0 + 32 jt + 8 (r / 4) + 4 half + r % 4
+    if (there != ~0ull || key0 + kBlockN > least_keys) {
+      const uint32_t bits[2] = {(uint32_t)there >> (4 * half), (uint32_t)(there >> 32) >> (4 * half)};
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = 8 * (r / 4) + r % 4;
+          if (!(bits[jt] >> at & 1) || key0 + jt * 32 + at + 4 * half >= keys) s[jt][r] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx1 = fmaxf(mx1, s[1][r]);
+    mx = fmaxf(mx, mx1);
+    mx = fmaxf(mx, other_half(mx)) * a.scale;
+    const bool grow = mx > m_i + kRescaleLag;                       // the reference maximum may lag (flash_attn.hip)
+    if (__ballot(grow) != 0) {
+      const float m_new = grow ? mx : m_i, alpha = grow ? __builtin_amdgcn_exp2f(m_i - m_new) : 1.0f;
+      l_i *= alpha;
+      m_i = m_new;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+      neg_m = m_i == -INFINITY ? 0.0f : -m_i;
+    }
+    Frag pf[2];
+    auto exp_tile = [&](const f32x16& t) __attribute__((always_inline)) {
+      float pr[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(fmaf(t[r], a.scale, neg_m));
+      pf[0] = MfmaT<T>::pack(&pr[0]);
+      pf[1] = MfmaT<T>::pack(&pr[8]);
+      l_i = MfmaT<T>::sum8(pf[1], MfmaT<T>::sum8(pf[0], l_i));      // the sum of what the product multiplies
+    };
+    auto pv = [&](const VFrags& vf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o_acc[dt] = MfmaT<T>::run(vf.f[hf][dt], pf[hf], o_acc[dt]);
+    };
+    read_v(1, vf1);
+    exp_tile(s[0]);
+    pv(vf0);
+    exp_tile(s[1]);
+    pv(vf1);
+  };
+
+  for (int block = block0; block < block1; block += 2) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint64_t there = __ballot(page >= 0);
+    page = next;
+    next = find(block + 2);
+    process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
+    if (block + 1 >= block1) break;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    there = __ballot(page >= 0);
+    page = next;
+    next = find(block + 3);
+    process(block + 1, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
+  }
+
+  // ---- o_acc[dt][r] is column 32 dt + 8 (r / 4) + 4 half + r % 4 of the row's sum
+  const float l = l_i + other_half(l_i);
+  if (!live) return;
+  if (w.sums.slots) {
+    const int64_t at = (int64_t)(part + (shared ? 0 : w.shared_splits)) * w.sums.rows + (int64_t)token * a.heads + head;
+    if (half == 0) w.sums.ml[at] = float2{m_i, l};
+    if (!(l > 0.0f)) return;
+    float* out = w.sums.o + at * dim;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int d = dt * 32 + 8 * q4 + 4 * half;
+        if (!PADDED || d < dim) store4<float>(out + d, o_acc[dt][q4 * 4], o_acc[dt][q4 * 4 + 1], o_acc[dt][q4 * 4 + 2], o_acc[dt][q4 * 4 + 3]);
+      }
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  T* out = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = dt * 32 + 8 * q4 + 4 * half;
+      if (!PADDED || d < dim)
+        store4o<T>(out + d, o_acc[dt][q4 * 4] * inv, o_acc[dt][q4 * 4 + 1] * inv, o_acc[dt][q4 * 4 + 2] * inv, o_acc[dt][q4 * 4 + 3] * inv);
+    }
+}
+
+}  // namespace
+}  // namespace hexmi
