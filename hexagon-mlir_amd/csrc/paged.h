@@ -87,6 +87,7 @@ struct RowSums {
 };
 // One launch: the prefix for all rows (the first workgroups), and every sequence's keys behind it.
 struct TileArgs {
+  bool deep;                                   // DeepTile (paged_tile.h), or WideTile
   int shared_tiles, shared_splits;             // tiles of a key head; parts of the prefix, whose sums go to slots 0 .. (0: no prefix)
   int tiles, splits;                           // of the sequences' own keys, whose sums go to the slots behind (0: decode, not here)
   RowSums sums;                                // slots 0: the result goes to out
@@ -112,7 +113,8 @@ int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim);
 // tiles: of the prefix (shared_splits 0: none), whose sums' last slot is for the sequences' own keys
 int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const TileArgs& tiles,
                  hipStream_t s);
-// the prefix's tiles and `grid` workers in one launch (paged_shared.hip)
+// the prefix's tiles and `grid` workers in one launch (paged_shared.hip), of as many waves as the tiles have
+inline int paged_shared_waves(bool deep, int64_t dim) { return deep && dim <= 128 ? 8 : 4; }
 int paged_shared_decode(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
                         hipStream_t s);
 

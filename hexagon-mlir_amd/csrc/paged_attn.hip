@@ -1,3 +1,9 @@
+#ifndef DEEP_BELOW
+#define DEEP_BELOW 1
+#endif
+#ifndef DEEP_KEYS
+#define DEEP_KEYS 512
+#endif
 // Attention over a paged cache of keys and values (fp16 / bf16): runs of new tokens of many sequences over the positions before them, and
 // the prefix that all sequences share: what a call launches, the tiles of ragged batches (paged_tile.h) and the join of their sums.
 #include "paged_tile.h"
@@ -5,14 +11,12 @@
 namespace hexmi {
 namespace {
 
-template <typename T, int D, int COLS, bool PADDED>
-__global__ __launch_bounds__(kTileWaves * kWave, D == 256 ? 1 : 2)
+template <typename T, int D, int COLS, bool PADDED, typename Shape>
+__global__ __launch_bounds__(Shape::kThreads, D == 256 || Shape::kGroups > 1 ? 1 : 2)
 void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
-  __shared__ __attribute__((aligned(16))) T k_lds0[kBlockN * D];
-  __shared__ __attribute__((aligned(16))) T k_lds1[kBlockN * D];
-  __shared__ __attribute__((aligned(16))) T v_lds0[kBlockN * D];
-  __shared__ __attribute__((aligned(16))) T v_lds1[kBlockN * D];
-  paged_tile<T, D, COLS, PADDED>(a, p, w, blockIdx.x, gridDim.x, k_lds0, k_lds1, v_lds0, v_lds1);
+  __shared__ __attribute__((aligned(16))) T lds[Shape::lds_elements(D)];
+  __shared__ float m_lds[Shape::kGroups][Shape::kRows], l_lds[Shape::kGroups][Shape::kRows];
+  paged_tile<T, D, COLS, PADDED, Shape>(a, p, w, blockIdx.x, gridDim.x, lds, m_lds, l_lds);
 }
 
 // A row's sums of all slots (at most 32) joined: 32 threads a row, a thread the columns d and, past 128, d + 128.
@@ -65,15 +69,22 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
 template <typename T>
 int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipStream_t s) {
   const unsigned grid = (unsigned)(((int64_t)w.tiles * w.splits + (int64_t)w.shared_tiles * w.shared_splits) * p.kv_heads);
-#define HEXMI_PAGED_TILE(D, COLS)                                                                                                         \
+#define HEXMI_PAGED_TILE(D, COLS, Shape)                                                                                                  \
   do {                                                                                                                                    \
-    if (a.dim == COLS) hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, false>), dim3(grid), dim3(kTileWaves * kWave), 0, s, a, p, w);   \
-    else hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, true>), dim3(grid), dim3(kTileWaves * kWave), 0, s, a, p, w);                  \
+    if (a.dim == COLS) hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, false, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w); \
+    else hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, true, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);              \
   } while (0)
-  if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64);
-  else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96);
-  else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128);
-  else HEXMI_PAGED_TILE(256, 256);
+  if (w.deep) {
+    if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, DeepTile);
+    else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, DeepTile);
+    else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128, DeepTile);
+    else HEXMI_PAGED_TILE(256, 256, DeepTile256);
+  } else {
+    if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, WideTile);
+    else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, WideTile);
+    else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128, WideTile);
+    else HEXMI_PAGED_TILE(256, 256, WideTile);
+  }
 #undef HEXMI_PAGED_TILE
   return launch_status();
 }
@@ -81,36 +92,39 @@ int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipS
 // What a call launches: the prefix's tiles (prefix_splits 0: none), then one token a sequence (decode) or tiles of the sequences' own keys
 // (splits), then the join of the tiles' sums.
 struct Plan {
-  bool decode;
+  bool decode, deep;
   int prefix_tiles, prefix_splits, splits;
   int64_t tiles;
   PagedDecodePlan one;
   int64_t rows, sum_bytes, decode_bytes;
   int slots() const { return prefix_splits == 0 && (decode || splits == 1) ? 0 : prefix_splits + (decode ? 1 : splits); }
 };
-// Parts of the keys for tiles of which there are `units`: two workgroups a compute unit, no part below four blocks. A row has 32 slots for
-// the sums of its parts, of the prefix and its own together.
-int parts_of(int64_t units, int64_t keys, int limit) {
-  const int64_t blocks = (keys + kBlockN - 1) / kBlockN, wanted = 2 * (int64_t)hexmi_num_cus() / units;
-  const int64_t most = blocks / 4 < limit ? blocks / 4 : limit;
-  return (int)(wanted < most ? (wanted > 1 ? wanted : 1) : (most > 1 ? most : 1));
+// Parts of the keys for `units` tiles: `wanted` workgroups, no part below `least` keys. A row has 32 slots for the sums of its parts, of the
+// prefix and its own together.
+int parts_of(int64_t units, int64_t keys, int64_t wanted, int64_t least, int64_t limit) {
+  const int64_t most = keys / least < limit ? keys / least : limit, parts = wanted / units < most ? wanted / units : most;
+  return parts > 1 ? (int)parts : 1;
 }
 Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   Plan plan = {};
-  const int64_t group = heads / b.kv_heads, prefix = shared * b.page_size, rows = b.tokens * group;
-  const int64_t own = b.table_cols * b.page_size - prefix, full = (rows + kRows - 1) / kRows;
+  const int64_t group = heads / b.kv_heads, prefix = shared * b.page_size, rows = b.tokens * group, cus = hexmi_num_cus();
+  const int64_t own = b.table_cols * b.page_size - prefix;
   plan.decode = b.starts == nullptr;
   plan.rows = b.tokens * heads;
+  const int64_t wide = (rows + WideTile::kRows - 1) / WideTile::kRows * b.kv_heads;
+  plan.deep = wide < DEEP_BELOW * cus;
+  const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
+  const int64_t wanted = plan.deep ? cus : 2 * cus, least = plan.deep ? DEEP_KEYS : 256;
   if (shared > 0) {
     plan.prefix_tiles = (int)full;
-    plan.prefix_splits = parts_of(full * b.kv_heads, prefix, plan.decode ? 31 : 16);
+    plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);
   }
   if (plan.decode) {
     plan.one = plan_paged_decode(b, heads, prefix);
     plan.decode_bytes = (paged_decode_workspace(plan.one, b.dim) + 15) / 16 * 16;
   } else {
-    plan.tiles = rows / kRows + b.sequences + 2;
-    plan.splits = parts_of(full * b.kv_heads, own, 16);
+    plan.tiles = rows / tile_rows + b.sequences + 2;
+    plan.splits = parts_of(full * b.kv_heads, own, wanted, least, 16);
   }
   plan.sum_bytes = plan.slots() * plan.rows * (b.dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
   return plan;
@@ -133,7 +147,7 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   const Plan plan = plan_of(b, heads, shared);
-  return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads <= limit / (kTileWaves * kWave) ? HEXMI_OK : HEXMI_ENOTSUP;
+  return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
 }
 }  // namespace
 
@@ -158,6 +172,7 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
                              batch->v_head, batch->v_slot};
   for (int64_t s : strides)
     if (s % 8 != 0) return HEXMI_ENOTSUP;
+  if (batch->k_slot < 0 || batch->k_slot > 1 << 26 || batch->v_slot < 0 || batch->v_slot > 1 << 26) return HEXMI_ENOTSUP;      // 32-bit offsets within a page
   if (!aligned_to(q->x, 16) || !aligned_to(q->out, 16) || !aligned_to(batch->k_pages, 16) || !aligned_to(batch->v_pages, 16)) return HEXMI_ENOTSUP;
   const Plan plan = plan_of(*batch, q->heads, shared);
   const int64_t need = plan.decode_bytes + plan.sum_bytes;
@@ -171,8 +186,8 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   hipStream_t s = as_stream(stream);
   begin_call();
   auto tiles = [&](const TileArgs& w) { return dtype == HEXMI_F16 ? launch_tiles<f16>(a, p, w, s) : launch_tiles<bf16>(a, p, w, s); };
-  if (plan.decode) return paged_decode(plan.one, a, p, dtype, workspace, {plan.prefix_tiles, plan.prefix_splits, 0, 0, sums}, s);
-  if ((rc = tiles({plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums})) != HEXMI_OK || sums.slots == 0) return rc;
+  if (plan.decode) return paged_decode(plan.one, a, p, dtype, workspace, {plan.deep, plan.prefix_tiles, plan.prefix_splits, 0, 0, sums}, s);
+  if ((rc = tiles({plan.deep, plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums})) != HEXMI_OK || sums.slots == 0) return rc;
   const unsigned blocks = (unsigned)((plan.rows + 7) / 8);
   if (dtype == HEXMI_F16) hipLaunchKernelGGL((paged_join_kernel<f16>), dim3(blocks), dim3(256), 0, s, a, sums);
   else hipLaunchKernelGGL((paged_join_kernel<bf16>), dim3(blocks), dim3(256), 0, s, a, sums);

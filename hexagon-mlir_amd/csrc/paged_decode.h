@@ -9,7 +9,7 @@
 // Keys and values of the next 32 are asked for as soon as the registers of these are free, so a wave has 16 KiB (heads of 128) on the way
 // at nearly all times, eight waves a compute unit.
 //
-// The work is cut evenly whatever the lengths are: the blocks of kBlockKeys keys of all sequences and key heads, one behind the other,
+// The work is cut evenly whatever the lengths are: the blocks of keys of all sequences and key heads, one behind the other,
 // are dealt to the workers (workgroups) in equal runs. A worker that has all of a unit (sequence, key head, 16 query heads) writes
 // its rows; of a unit that several share every worker leaves its sums, at most two sets, which a second launch joins in the order of
 // the keys. Nothing is added atomically.
@@ -20,7 +20,7 @@
 namespace hexmi {
 namespace {
 
-constexpr int kWaves = 4, kTileKeys = 32, kBlockKeys = kWaves * kTileKeys;
+constexpr int kTileKeys = 32;                  // of a wave; a workgroup's W waves take a block of W * kTileKeys
 
 template <typename T> struct Mfma16;
 template <> struct Mfma16<f16> {
@@ -46,8 +46,10 @@ __device__ __forceinline__ float sum_of_quarters(float v) {
 }
 
 // blocks of a sequence's unit: one at least, so that a row without keys is written too
-__device__ __forceinline__ int blocks_of_keys(int keys) { return keys > kBlockKeys ? (keys + kBlockKeys - 1) / kBlockKeys : 1; }
-__device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) { return blocks_of_keys(length_of(p, b) - prefix); }
+template <int W> __device__ __forceinline__ int blocks_of_keys(int keys) {
+  return keys > W * kTileKeys ? (keys + W * kTileKeys - 1) / (W * kTileKeys) : 1;
+}
+template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) { return blocks_of_keys<W>(length_of(p, b) - prefix); }
 // the sum over the lanes up to this one
 __device__ __forceinline__ int sum_up_to(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);     // row_shr:1, 2, 4, 8: within 16 lanes
@@ -66,22 +68,24 @@ struct BlockList {
   int length, blocks, up_to;                   // lane b: of sequence b, and of all up to it
   int of_64, all;                              // blocks of the first 64 sequences, of all (one unit's)
 };
+template <int W>
 __device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int lane) {
   BlockList l;
   l.length = lane < p.sequences ? length_of(p, lane) : 0;
-  l.blocks = lane < p.sequences ? blocks_of_keys(l.length - prefix) : 0;
+  l.blocks = lane < p.sequences ? blocks_of_keys<W>(l.length - prefix) : 0;
   l.up_to = sum_up_to(l.blocks);
   l.of_64 = of_last_lane(l.up_to);
   int more = 0;
-  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of(p, b0 + lane, prefix) : 0;
+  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix) : 0;
   l.all = l.of_64 + (p.sequences > kWave ? of_last_lane(sum_up_to(more)) : 0);
   return l;
 }
 // The sequence that block `at` of the list belongs to, with `units` units a sequence, and the blocks (of one unit) before it.
+template <int W>
 __device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, int units, int at, int lane, int& before) {
   before = 0;
   for (int b0 = 0;; b0 += kWave) {
-    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of(p, b0 + lane, prefix) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
+    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
     const uint64_t past = __ballot((before + sum) * units > at);
     if (past || b0 + kWave >= p.sequences) {   // `at` is below the end: there is one
       const int first = past ? __ffsll((unsigned long long)past) - 1 : 0;
@@ -117,12 +121,12 @@ constexpr int decode_wave_bytes(int d, int cols) {
 // D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
 // columns lie past the head reads the head's first ones instead: the query has zeros there, and what comes of V there is not stored.
 // worker: of w.workers, or the unit where that is 0.
-template <typename T, int D, int COLS, bool PADDED>
+template <typename T, int D, int COLS, bool PADDED, int W>
 __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned worker, char* lds,
                                                     float (*m_lds)[16], float (*l_lds)[16]) {
   typedef typename MfmaT<T>::Frag Frag;
   constexpr int DS = COLS / 32, DT = COLS / 16, CPR = D / 8, kPitch = COLS + 4;
-  constexpr int kWaveBytes = decode_wave_bytes(D, COLS);
+  constexpr int kWaveBytes = decode_wave_bytes(D, COLS), kBlock = W * kTileKeys;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane / 16, n = lane % 16;
   const int dim = PADDED ? a.dim : COLS;
@@ -139,23 +143,23 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
   if (w.workers == 0) {                        // a unit each
     b = worker / units;
     list.length = 0;
-    const int u = worker - b * units, blocks = __builtin_amdgcn_readfirstlane(blocks_of(p, b, a.prefix));
+    const int u = worker - b * units, blocks = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix));
     cur = u * blocks;
     end = cur + blocks;
   } else {
-    list = block_list(p, a.prefix, lane);
+    list = block_list<W>(p, a.prefix, lane);
     total = list.all * units;
     cur = run_start(total, w.workers, worker);
     end = run_start(total, w.workers, worker + 1);
     if (wave == 0 && lane == 0) w.begun[worker].last = -1;
     if (cur >= end) return;
-    b = sequence_at(list, p, a.prefix, units, cur, lane, before);
+    b = sequence_at<W>(list, p, a.prefix, units, cur, lane, before);
   }
   const int start = cur;
 
   while (cur < end) {
     const int length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
-    const int blocks = blocks_of_keys(length - a.prefix), local = cur - before * units;
+    const int blocks = blocks_of_keys<W>(length - a.prefix), local = cur - before * units;
     if (local >= blocks * units) {             // on to the next sequence
       before += blocks;
       ++b;
@@ -187,8 +191,8 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     float m = -INFINITY, neg_m = 0.0f, l = 0.0f;
 
     // ---- keys: this wave's tiles of the run
-    const int key_first = a.prefix + (block0 * kWaves + wave) * kTileKeys;
-    int key_end = a.prefix + (block0 + count) * kBlockKeys;
+    const int key_first = a.prefix + (block0 * W + wave) * kTileKeys;
+    int key_end = a.prefix + (block0 + count) * kBlock;
     key_end = key_end < length ? key_end : length;
     const int32_t* table = p.table + b * p.table_row;
     const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
@@ -214,10 +218,10 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     };
     if (key_first < key_end) {
       u32x4 kr[2][DS], vr[2][DS];
-      Keys now = find(key_first), next = find(key_first + kBlockKeys);
+      Keys now = find(key_first), next = find(key_first + kBlock);
       load(now, key_first, k_head, p.k_page, p.k_slot, kr);
       load(now, key_first, v_head, p.v_page, p.v_slot, vr);
-      for (int key0 = key_first; key0 < key_end; key0 += kBlockKeys) {
+      for (int key0 = key_first; key0 < key_end; key0 += kBlock) {
         __builtin_amdgcn_sched_barrier(0);
         // what the constants of a chunk are XORed into; kept from becoming a register each
         int to = put_at, from = take_at;
@@ -232,7 +236,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         const bool ok0 = there(now.page[0]) && key0 + n < key_end, ok1 = there(now.page[1]) && key0 + 16 + n < key_end;
         const bool whole = __ballot(ok0 && ok1) == ~0ull;
         __builtin_amdgcn_sched_barrier(0);
-        load(next, key0 + kBlockKeys, k_head, p.k_page, p.k_slot, kr);
+        load(next, key0 + kBlock, k_head, p.k_page, p.k_slot, kr);
         __builtin_amdgcn_sched_barrier(0);
         if (!whole) {                                                // what stands where no key is may be anything: no weight, and zeros of V
           const uint32_t k0 = (uint32_t)__ballot(ok0), k1 = (uint32_t)__ballot(ok1);
@@ -252,7 +256,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
 #pragma unroll
           for (int ds = 0; ds < DS; ++ds) *reinterpret_cast<u32x4*>(lds + (to ^ (ds * 64)) + t * (16 * D * 2)) = vr[t][ds];
         __builtin_amdgcn_sched_barrier(0);
-        load(next, key0 + kBlockKeys, v_head, p.v_page, p.v_slot, vr);
+        load(next, key0 + kBlock, v_head, p.v_page, p.v_slot, vr);
         __builtin_amdgcn_sched_barrier(0);
         // online softmax, the reference maximum up to kRescaleLag behind the true one (flash_attn.hip)
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -286,7 +290,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         }
         asm volatile("" ::: "memory");
         now = next;
-        next = find(key0 + 2 * kBlockKeys);
+        next = find(key0 + 2 * kBlock);
       }
     }
 
@@ -303,16 +307,16 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     const int slot = worker * 2 + (block0 != 0 ? 0 : 1);         // what another began, or what it begins
     if (threadIdx.x == 0 && w.workers && block0 == 0 && !mine)
       w.begun[worker] = BegunUnit{b, u, worker_of(total, w.workers, cur + blocks - 1), 0};
-    for (int i = threadIdx.x; i < rows * (COLS / 4); i += kWaves * kWave) {
+    for (int i = threadIdx.x; i < rows * (COLS / 4); i += W * kWave) {
       const int r = i / (COLS / 4), d = i % (COLS / 4) * 4;
       if (PADDED && d >= dim) continue;
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int x = 0; x < kWaves; ++x) top = fmaxf(top, m_lds[x][r]);
+      for (int x = 0; x < W; ++x) top = fmaxf(top, m_lds[x][r]);
       f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
       if (top != -INFINITY) {
 #pragma unroll
-        for (int x = 0; x < kWaves; ++x) {
+        for (int x = 0; x < W; ++x) {
           const float f = __builtin_amdgcn_exp2f(m_lds[x][r] - top);
           const f32x4 ox = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * kWaveBytes) + r * kPitch + d);
           sum = fmaf(l_lds[x][r], f, sum);

@@ -5,17 +5,19 @@
 namespace hexmi {
 namespace {
 
+constexpr int kWaves = 4, kBlockKeys = kWaves * kTileKeys;
+
 template <typename T, int D, int COLS, bool PADDED>
 __global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
 void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   __shared__ __attribute__((aligned(16))) char lds[kWaves * decode_wave_bytes(D, COLS)];
   __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
-  paged_decode_worker<T, D, COLS, PADDED>(a, p, w, blockIdx.x, lds, m_lds, l_lds);
+  paged_decode_worker<T, D, COLS, PADDED, kWaves>(a, p, w, blockIdx.x, lds, m_lds, l_lds);
 }
 
 // The units that several workers share: block (w, row) takes the one that worker w began. Behind a prefix every unit is joined with its
 // sums: block (unit, row).
-template <typename T>
+template <typename T, int W>
 __global__ __launch_bounds__(256)
 void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   __shared__ float o_lds[8][256 + 4];
@@ -27,10 +29,10 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     u = blockIdx.x - b * units;
     if (w.workers) {
       const int lane = threadIdx.x % kWave;
-      const BlockList list = block_list(p, a.prefix, lane);
+      const BlockList list = block_list<W>(p, a.prefix, lane);
       int before = 0;
-      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of(p, x, a.prefix);
-      const int blocks = blocks_of_keys(length_at(list, p, b) - a.prefix), total = list.all * units;
+      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<W>(p, x, a.prefix);
+      const int blocks = blocks_of_keys<W>(length_at(list, p, b) - a.prefix), total = list.all * units;
       const int first = of_last_lane(sum_up_to(before)) * units + u * blocks;
       w0 = worker_of(total, w.workers, first);
       w1 = worker_of(total, w.workers, first + blocks - 1);
@@ -97,8 +99,9 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
   if (tiles.shared_splits) {
     const int rc = paged_shared_decode(a, p, tiles, w, grid, dtype, s);
     if (rc != HEXMI_OK) return rc;
-    hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3((unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles), plan.rows), dim3(256), 0,
-                       s, a, p, w);
+    const dim3 units((unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles), plan.rows);
+    if (paged_shared_waves(tiles.deep, a.dim) == 8) hipLaunchKernelGGL((paged_decode_join_kernel<T, 8>), units, dim3(256), 0, s, a, p, w);
+    else hipLaunchKernelGGL((paged_decode_join_kernel<T, 4>), units, dim3(256), 0, s, a, p, w);
     return launch_status();
   }
 #define HEXMI_PAGED_DECODE(D, COLS)                                                                                                      \
@@ -113,7 +116,7 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
 #undef HEXMI_PAGED_DECODE
   const int rc = launch_status();
   if (rc != HEXMI_OK || plan.workers < 2) return rc;
-  hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
+  hipLaunchKernelGGL((paged_decode_join_kernel<T, kWaves>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
   return launch_status();
 }
 

@@ -7,36 +7,44 @@
 namespace hexmi {
 namespace {
 
-static_assert(kWaves == kTileWaves, "one workgroup size");
-
-template <typename T, int D, int COLS, bool PADDED>
-__global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
+template <typename T, int D, int COLS, bool PADDED, typename Shape>
+__global__ __launch_bounds__(Shape::kThreads, D == 256 || Shape::kGroups > 1 ? 1 : 2)
 void paged_shared_decode_kernel(PagedAttnArgs a, Pages p, TileArgs tiles, DecodeArgs w, unsigned tile_grid) {
-  constexpr int kTile = kBlockN * D, kTileBytes = 4 * kTile * 2, kDecodeBytes = kWaves * decode_wave_bytes(D, COLS);
+  constexpr int W = Shape::kThreads / kWave, kTileBytes = Shape::lds_elements(D) * 2, kDecodeBytes = W * decode_wave_bytes(D, COLS);
   __shared__ __attribute__((aligned(16))) char lds[kTileBytes > kDecodeBytes ? kTileBytes : kDecodeBytes];
-  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
-  if (blockIdx.x < tile_grid) {
-    T* t = reinterpret_cast<T*>(lds);
-    paged_tile<T, D, COLS, PADDED>(a, p, tiles, blockIdx.x, tile_grid, t, t + kTile, t + 2 * kTile, t + 3 * kTile);
-  } else {
-    paged_decode_worker<T, D, COLS, PADDED>(a, p, w, blockIdx.x - tile_grid, lds, m_lds, l_lds);
-  }
+  __shared__ union Statistics {
+    float tile[2][Shape::kGroups][Shape::kRows];
+    float worker[2][W][16];
+  } ml;
+  if (blockIdx.x < tile_grid)
+    paged_tile<T, D, COLS, PADDED, Shape>(a, p, tiles, blockIdx.x, tile_grid, reinterpret_cast<T*>(lds), ml.tile[0], ml.tile[1]);
+  else
+    paged_decode_worker<T, D, COLS, PADDED, W>(a, p, w, blockIdx.x - tile_grid, lds, ml.worker[0], ml.worker[1]);
 }
 
 template <typename T>
 int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned workers, hipStream_t s) {
   const unsigned tile_grid = (unsigned)((int64_t)tiles.shared_tiles * tiles.shared_splits * p.kv_heads), grid = tile_grid + workers;
-#define HEXMI_PAGED_SHARED(D, COLS)                                                                                                      \
+#define HEXMI_PAGED_SHARED(D, COLS, Shape)                                                                                               \
   do {                                                                                                                                   \
     if (a.dim == COLS)                                                                                                                   \
-      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, false>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, tiles, w, tile_grid); \
+      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, false, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, tiles, w,  \
+                         tile_grid);                                                                                                     \
     else                                                                                                                                 \
-      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, true>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, tiles, w, tile_grid);  \
+      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, true, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, tiles, w,   \
+                         tile_grid);                                                                                                     \
   } while (0)
-  if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64);
-  else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96);
-  else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128);
-  else HEXMI_PAGED_SHARED(256, 256);
+  if (tiles.deep) {
+    if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, DeepTile);
+    else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, DeepTile);
+    else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128, DeepTile);
+    else HEXMI_PAGED_SHARED(256, 256, DeepTile256);
+  } else {
+    if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, WideTile);
+    else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, WideTile);
+    else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128, WideTile);
+    else HEXMI_PAGED_SHARED(256, 256, WideTile);
+  }
 #undef HEXMI_PAGED_SHARED
   return launch_status();
 }

@@ -16,7 +16,16 @@
 namespace hexmi {
 namespace {
 
-constexpr int kTileWaves = 4, kRows = kTileWaves * 32;
+// KEYS a block, ROW_WAVES waves of 32 rows each, GROUPS of such waves that take every GROUPS-th block each, with LDS of their own.
+template <int KEYS, int ROW_WAVES, int GROUPS> struct TileShape {
+  static constexpr int kKeys = KEYS, kRowWaves = ROW_WAVES, kGroups = GROUPS, kRows = ROW_WAVES * 32, kThreads = ROW_WAVES * GROUPS * kWave;
+  // LDS of D columns of 16 bits: K and V of two blocks a group, later the groups' sums in 32 bits
+  static constexpr int lds_elements(int d) { return GROUPS * 4 * KEYS * d; }
+  static_assert(4 * KEYS * 2 == kRows * 4, "a group's sums take the place of its blocks");
+};
+typedef TileShape<64, 4, 1> WideTile;          // many tiles: 128 rows, two workgroups a compute unit
+typedef TileShape<32, 2, 4> DeepTile;          // few: 64 rows, the chain of a tile's blocks a quarter as long, one workgroup a compute unit
+typedef TileShape<32, 2, 2> DeepTile256;       // ... heads of 256 columns, whose blocks are as large again
 
 // The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences, where -1 and `sequences` are the
 // rows of no sequence before the first and behind the last. floor(x / r) + 1 >= ceil(n / r) + floor(x0 / r) for x = x0 + n, so
@@ -25,12 +34,14 @@ __device__ __forceinline__ int first_row(const Pages& p, int b) {
   const int s = b < 0 ? 0 : b > p.sequences ? p.tokens : p.starts[b];
   return s < 0 ? 0 : s < p.tokens ? s : p.tokens;
 }
-__device__ __forceinline__ int first_tile(const Pages& p, int group, int b) { return b < 0 ? 0 : first_row(p, b) * group / kRows + b + 1; }
+template <int ROWS>
+__device__ __forceinline__ int first_tile(const Pages& p, int group, int b) { return b < 0 ? 0 : first_row(p, b) * group / ROWS + b + 1; }
+template <int ROWS>
 __device__ __forceinline__ int sequence_of_tile(const Pages& p, int group, int tile, int lane) {
   int lo = -1, hi = p.sequences + 1;
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-    const int n = __popcll(__ballot(at < hi && first_tile(p, group, at) <= tile));
+    const int n = __popcll(__ballot(at < hi && first_tile<ROWS>(p, group, at) <= tile));
     lo += (n > 0 ? n - 1 : 0) * step;
     hi = lo + step < hi ? lo + step : hi;
     if (step == 1) break;
@@ -46,14 +57,19 @@ __device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
 
 // D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
 // columns lie past the head copies the head's first ones instead: the query has zeros there, and what comes of V there is not stored.
-// A workgroup's tile: number `block` of a launch whose tiles are `grid` workgroups; k_lds0 .. v_lds1: 64 rows of D each.
-template <typename T, int D, int COLS, bool PADDED>
+// A workgroup's tile: number block_id of a launch whose tiles are `grid` workgroups; lds: Shape::lds_elements(D); m_lds, l_lds: of every
+// group's rows.
+template <typename T, int D, int COLS, bool PADDED, typename Shape>
 __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, unsigned block_id, unsigned grid,
-                                           T* k_lds0, T* k_lds1, T* v_lds0, T* v_lds1) {
+                                           T* lds, float (*m_lds)[Shape::kRows], float (*l_lds)[Shape::kRows]) {
   typedef typename MfmaT<T>::Frag Frag;
+  constexpr int kKeys = Shape::kKeys, kRowWaves = Shape::kRowWaves, kGroups = Shape::kGroups, kRows = Shape::kRows, JT = kKeys / 32;
   constexpr int DS = COLS / 16, DT = COLS / 32, CPR = D / 8;
-  constexpr int NI = kBlockN * CPR / kWave / kTileWaves, kRowStep = kTileWaves * kWave / CPR;
+  constexpr int NI = kKeys * CPR / kWave / kRowWaves, kRowStep = kRowWaves * kWave / CPR;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
+  const int group = wave / kRowWaves, row_wave = wave % kRowWaves;
+  constexpr int kTile = kKeys * D;
+  T *k_lds0 = lds + group * 4 * kTile, *k_lds1 = k_lds0 + kTile, *v_lds0 = k_lds1 + kTile, *v_lds1 = v_lds0 + kTile;
   const int dim = PADDED ? a.dim : COLS;
 
   // Workgroup -> (prefix or not, key head, tile, part). Workgroup ids go round robin to the 8 XCDs (one L2 each): every XCD gets a run of
@@ -77,10 +93,10 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     end = a.prefix;
     table = a.shared;
   } else {
-    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile(p, a.group, tile, lane));
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile<kRows>(p, a.group, tile, lane));
     token0 = first_row(p, b);
     new_tokens = first_row(p, b + 1) - token0;
-    row0 = (tile - first_tile(p, a.group, b)) * kRows;
+    row0 = (tile - first_tile<kRows>(p, a.group, b)) * kRows;
     rows = new_tokens * a.group;                                    // negative where starts fall: nothing
     if (row0 < 0 || row0 >= rows) return;
     none = b < 0 || b >= p.sequences;
@@ -91,44 +107,68 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     table = p.table + (none ? 0 : b) * p.table_row;
   }
   end = __builtin_amdgcn_readfirstlane(end);
-  const int blocks = end > begin ? (end - begin + kBlockN - 1) / kBlockN : 0, share = (blocks + splits - 1) / splits;
+  const int blocks = end > begin ? (end - begin + kKeys - 1) / kKeys : 0, share = (blocks + splits - 1) / splits;
   const int block0 = part * share, block1 = block0 + share < blocks ? block0 + share : blocks;
 
-  // ---- copies: instruction j of a wave takes kRowStep / 4 rows, a lane 16 bytes of one
+  const int first = block0 + group;                                 // this group's blocks: first, first + kGroups, ..
+
+  // ---- copies: instruction j of a wave takes kRowsOfOne rows, a lane 16 bytes of one
   const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
   const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
-  const int lin = wave * kWave + lane, copy_row = lin / CPR, lds_at = wave * kWave * 8;
-  auto find = [&](int block) __attribute__((always_inline)) {       // the page of key 64 block + lane, -1: none
-    const int key = begin + block * kBlockN + lane;
+  const int lin = row_wave * kWave + lane, copy_row = lin / CPR, lds_at = row_wave * kWave * 8;
+  auto find = [&](int block) __attribute__((always_inline)) {       // the page of key kKeys block + lane, -1: none
+    const int key = begin + block * kKeys + lane % kKeys;
     if (block >= block1 || key >= end) return -1;
     const int page = table[divided(key, p.size)];
     return page < p.num_pages ? page : -1;
   };
-  auto copy = [&](int j, bool v, int block, int page_of_lane, T* lds) __attribute__((always_inline)) {
-    const int r = copy_row + j * kRowStep, key = begin + block * kBlockN + r, page = __shfl(page_of_lane, r);
-    int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
-    if (PADDED && c >= dim) c = 0;
-    T* to = lds + lds_at + j * (kTileWaves * kWave * 8);
-    if (page >= 0) {
+  // One block into LDS. Where every key is there and the rows of an instruction share a page, the page, and so the place, is the wave's
+  // (scalar arithmetic), and a lane adds what it is off in it; any other block goes row by row.
+  constexpr int kRowsOfOne = kWave / CPR;
+  const bool one_page = p.page_size % kRowsOfOne == 0;
+  auto column = [&](bool v, int r) __attribute__((always_inline)) {
+    const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
+    return PADDED && c >= dim ? 0 : c;
+  };
+  auto copy = [&](int block, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int64_t page_stride = v ? p.v_page : p.k_page, slot_stride = v ? p.v_slot : p.k_slot;
+        T* dst = v ? v_dst : k_dst;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const int row = row_wave * kRowsOfOne + j * kRowStep, key = begin + block * kKeys + row;
+          const int page = __builtin_amdgcn_readlane(page_of_lane, row), slot = key - divided(key, p.size) * p.page_size;
+          const T* from = (v ? v_head : k_head) + page * page_stride + slot * slot_stride;
+          const int off = lane / CPR * (int)slot_stride + column(v, copy_row + j * kRowStep);
+          __builtin_amdgcn_global_load_lds(HEXMI_GLB(from + off), HEXMI_LDS(dst + lds_at + j * (kRowWaves * kWave * 8)), 16, 0, 0);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int r = copy_row + j * kRowStep, key = begin + block * kKeys + r, page = __shfl(page_of_lane, r);
       const int slot = key - divided(key, p.size) * p.page_size;
-      const T* from = v ? v_head + page * p.v_page + slot * p.v_slot + c : k_head + page * p.k_page + slot * p.k_slot + c;
-      __builtin_amdgcn_global_load_lds(HEXMI_GLB(from), HEXMI_LDS(to), 16, 0, 0);
-    } else if (v) {                                                 // no key: whatever the cache holds, zeros of V (its score is dropped)
-      *reinterpret_cast<u32x4*>(to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
+      T *k_to = k_dst + lds_at + j * (kRowWaves * kWave * 8), *v_to = v_dst + lds_at + j * (kRowWaves * kWave * 8);
+      if (page >= 0) {
+        __builtin_amdgcn_global_load_lds(HEXMI_GLB(k_head + page * p.k_page + slot * p.k_slot + column(false, r)), HEXMI_LDS(k_to), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(HEXMI_GLB(v_head + page * p.v_page + slot * p.v_slot + column(true, r)), HEXMI_LDS(v_to), 16, 0, 0);
+      } else {                                                      // no key: whatever the cache holds, zeros of V (its score is dropped)
+        *reinterpret_cast<u32x4*>(v_to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
+      }
     }
   };
   int page = -1, next = -1;
-  if (block0 < block1) {                                            // on their way while the rows are looked up
-    page = find(block0);
-    next = find(block0 + 1);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) copy(j, false, block0, page, k_lds0);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) copy(j, true, block0, page, v_lds0);
+  if (first < block1) {                                             // on their way while the rows are looked up
+    page = find(first);
+    next = find(first + kGroups);
+    copy(first, page, k_lds0, v_lds0);
   }
 
   // this lane's row: its token, its queries and the keys it sees
-  const int wave_row = row0 + wave * 32, row = wave_row + lane % 32;
+  const int wave_row = row0 + row_wave * 32, row = wave_row + lane % 32;
   const bool live = row < rows;
   const int in_seq = divided(live ? row : rows - 1, a.by_group), head = kvh * a.group + (live ? row : rows - 1) - in_seq * a.group;
   const int token = token0 + in_seq;
@@ -178,17 +218,12 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
 
   auto process = [&](int block, uint64_t there, int next_page, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
-    const int key0 = begin + block * kBlockN;
-    if (block + 1 < block1) {
+    const int key0 = begin + block * kKeys;
+    if (block + kGroups < block1) copy(block + kGroups, next_page, k_dst, v_dst);
+    if (block >= block1 || key0 >= most_keys) return;               // wave-uniform; the barriers are outside
+    f32x16 s[JT];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) copy(j, false, block + 1, next_page, k_dst);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) copy(j, true, block + 1, next_page, v_dst);
-    }
-    if (key0 >= most_keys) return;                                  // wave-uniform; the barriers are outside
-    f32x16 s[2];
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
+    for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[jt][r] = 0.0f;
     {
@@ -197,20 +232,18 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
         const int r = jt * 32 + lane % 32, c = (ds * 2 + half) ^ swz_ktile<D == 64 ? 64 : 128>(r);
         return *reinterpret_cast<const Frag*>(k_src + (r * CPR + c) * 8);
       };
-      Frag kf[2][DS];
+      Frag kf[JT][DS];
 #pragma unroll
-      for (int ds = 0; ds < kAhead && ds < DS; ++ds) {
-        kf[0][ds] = read_k(0, ds);
-        kf[1][ds] = read_k(1, ds);
-      }
+      for (int ds = 0; ds < kAhead && ds < DS; ++ds)
+#pragma unroll
+        for (int jt = 0; jt < JT; ++jt) kf[jt][ds] = read_k(jt, ds);
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds) {
-        if (ds + kAhead < DS) {
-          kf[0][ds + kAhead] = read_k(0, ds + kAhead);
-          kf[1][ds + kAhead] = read_k(1, ds + kAhead);
-        }
-        s[0] = MfmaT<T>::run(kf[0][ds], qf[ds], s[0]);
-        s[1] = MfmaT<T>::run(kf[1][ds], qf[ds], s[1]);
+        if (ds + kAhead < DS)
+#pragma unroll
+          for (int jt = 0; jt < JT; ++jt) kf[jt][ds + kAhead] = read_k(jt, ds + kAhead);
+#pragma unroll
+        for (int jt = 0; jt < JT; ++jt) s[jt] = MfmaT<T>::run(kf[jt][ds], qf[ds], s[jt]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -235,10 +268,10 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     read_v(0, vf0);
     __builtin_amdgcn_sched_barrier(0);
     // s[jt][r] is the score of key key0 + 32 jt + 8 (r / 4) + 4 half + r % 4
-    if (there != ~0ull || key0 + kBlockN > least_keys) {
+    if (there != ~0ull || key0 + kKeys > least_keys) {
       const uint32_t bits[2] = {(uint32_t)there >> (4 * half), (uint32_t)(there >> 32) >> (4 * half)};
 #pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
+      for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r / 4) + r % 4;
@@ -249,7 +282,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx1 = fmaxf(mx1, s[1][r]);
+    for (int r = 0; r < 16; ++r) mx1 = fmaxf(mx1, s[JT - 1][r]);
     mx = fmaxf(mx, mx1);
     mx = fmaxf(mx, other_half(mx)) * a.scale;
     const bool grow = mx > m_i + kRescaleLag;                       // the reference maximum may lag (flash_attn.hip)
@@ -278,56 +311,108 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o_acc[dt] = MfmaT<T>::run(vf.f[hf][dt], pf[hf], o_acc[dt]);
     };
-    read_v(1, vf1);
+    if constexpr (JT == 2) read_v(1, vf1);
     exp_tile(s[0]);
     pv(vf0);
-    exp_tile(s[1]);
-    pv(vf1);
+    if constexpr (JT == 2) {
+      exp_tile(s[1]);
+      pv(vf1);
+    }
   };
 
-  for (int block = block0; block < block1; block += 2) {
+  for (int block = first, at = block0; at < block1; block += 2 * kGroups, at += 2 * kGroups) {      // as many turns for every group
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     uint64_t there = __ballot(page >= 0);
     page = next;
-    next = find(block + 2);
+    next = find(block + 2 * kGroups);
     process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
-    if (block + 1 >= block1) break;
+    if (at + kGroups >= block1) break;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     there = __ballot(page >= 0);
     page = next;
-    next = find(block + 3);
-    process(block + 1, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
+    next = find(block + 3 * kGroups);
+    process(block + kGroups, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
   }
+  __syncthreads();
 
-  // ---- o_acc[dt][r] is column 32 dt + 8 (r / 4) + 4 half + r % 4 of the row's sum
+  // ---- o_acc[dt][r] is column 32 dt + 8 (r / 4) + 4 half + r % 4 of the row's sum. A lane holds four columns of its row at a time; they
+  // leave as whole rows, through the LDS that held the blocks (16-byte chunks XOR swizzled by the row), where the groups' sums meet.
   const float l = l_i + other_half(l_i);
-  if (!live) return;
-  if (w.sums.slots) {
-    const int64_t at = (int64_t)(part + (shared ? 0 : w.shared_splits)) * w.sums.rows + (int64_t)token * a.heads + head;
-    if (half == 0) w.sums.ml[at] = float2{m_i, l};
-    if (!(l > 0.0f)) return;
-    float* out = w.sums.o + at * dim;
+  const bool parts = w.sums.slots != 0;
+  const float own = kGroups > 1 || parts ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+  const int64_t slot = (int64_t)(part + (shared ? 0 : w.shared_splits)) * w.sums.rows;
+  float* sums = reinterpret_cast<float*>(lds);
+  auto at_lds = [&](int g, int r, int chunk) __attribute__((always_inline)) {
+    return sums + (g * kRows + r) * D + (chunk ^ (r & (D == 64 ? 15 : 31))) * 4;
+  };
+  if (kGroups > 1 || wave_row < rows) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int d = dt * 32 + 8 * q4 + 4 * half;
-        if (!PADDED || d < dim) store4<float>(out + d, o_acc[dt][q4 * 4], o_acc[dt][q4 * 4 + 1], o_acc[dt][q4 * 4 + 2], o_acc[dt][q4 * 4 + 3]);
-      }
-    return;
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(at_lds(group, row_wave * 32 + lane % 32, dt * 8 + 2 * q4 + half)) =
+            f32x4{o_acc[dt][q4 * 4] * own, o_acc[dt][q4 * 4 + 1] * own, o_acc[dt][q4 * 4 + 2] * own, o_acc[dt][q4 * 4 + 3] * own};
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  T* out = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int d = dt * 32 + 8 * q4 + 4 * half;
-      if (!PADDED || d < dim)
-        store4o<T>(out + d, o_acc[dt][q4 * 4] * inv, o_acc[dt][q4 * 4 + 1] * inv, o_acc[dt][q4 * 4 + 2] * inv, o_acc[dt][q4 * 4 + 3] * inv);
+  if constexpr (kGroups > 1) {
+    if (half == 0) {
+      m_lds[group][row_wave * 32 + lane] = m_i;
+      l_lds[group][row_wave * 32 + lane] = l;
     }
+    __syncthreads();
+  } else {
+    if (parts && live && half == 0) w.sums.ml[slot + (int64_t)token * a.heads + head] = float2{m_i, l};
+    asm volatile("" ::: "memory");                                  // a wave's LDS accesses are in order
+  }
+  constexpr int kLanes = D / 8, kRowsAtOnce = kWave / kLanes, kWaveRows = kRows / (kRowWaves * kGroups);      // eight columns a lane
+  const int d = lane % kLanes * 8;
+#pragma unroll 2
+  for (int r0 = 0; r0 < kWaveRows; r0 += kRowsAtOnce) {
+    const int r = wave * kWaveRows + r0 + lane / kLanes, at = row0 + r;
+    if (at >= rows || d >= dim) continue;
+    const int i = divided(at, a.by_group), t = token0 + i, h = kvh * a.group + at - i * a.group;
+    const int64_t to = slot + (int64_t)t * a.heads + h;
+    float v[8];
+    if constexpr (kGroups == 1) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(at_lds(0, r, d / 4)), hi = *reinterpret_cast<const f32x4*>(at_lds(0, r, d / 4 + 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = lo[e];
+        v[e + 4] = hi[e];
+      }
+    } else {
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) top = fmaxf(top, m_lds[g][r]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      if (top != -INFINITY) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const float f = __builtin_amdgcn_exp2f(m_lds[g][r] - top);
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4)), hi = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4 + 1));
+          sum = fmaf(l_lds[g][r], f, sum);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = fmaf(lo[e], f, v[e]);
+            v[e + 4] = fmaf(hi[e], f, v[e + 4]);
+          }
+        }
+      }
+      if (parts && d == 0) w.sums.ml[to] = float2{top, sum};
+      const float inv = parts ? 1.0f : sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= inv;
+    }
+    if (parts) {
+      float* out = w.sums.o + to * dim + d;
+      *reinterpret_cast<f32x4*>(out) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(out + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+      *reinterpret_cast<Frag*>(static_cast<T*>(a.out) + t * a.out_token + h * a.out_head + d) = MfmaT<T>::pack(v);
+    }
+  }
 }
 
 }  // namespace
