@@ -60,6 +60,14 @@ __device__ __forceinline__ int sequence_of(const Pages& p, int t, int lane) {
   return lo < p.sequences && p.starts[lo] <= t ? lo : -1;
 }
 
+// The rows of sequence b, from the first of them to the first of b + 1: -1 and `sequences` are the rows of no sequence before the first and
+// behind the last; all within the operands, whatever starts holds.
+__device__ __forceinline__ int first_row(const Pages& p, int b) {
+  const int s = b < 0 ? 0 : b > p.sequences ? p.tokens : p.starts ? p.starts[b] : b;
+  return s < 0 ? 0 : s < p.tokens ? s : p.tokens;
+}
+__device__ __forceinline__ int new_tokens_of(const Pages& p, int b) { return p.starts ? first_row(p, b + 1) - first_row(p, b) : 1; }
+
 // The positions of sequence b that have a place in the table, whatever lengths holds.
 __device__ __forceinline__ int length_of(const Pages& p, int b) {
   const int most = p.table_cols * p.page_size, n = p.lengths[b];
@@ -88,6 +96,7 @@ struct RowSums {
 // One launch: the prefix for all rows (the first workgroups), and every sequence's keys behind it.
 struct TileArgs {
   bool deep;                                   // DeepTile (paged_tile.h), or WideTile
+  bool workers;                                // sequences of one new token are the workers' (paged_decode.h)
   int shared_tiles, shared_splits;             // tiles of a key head; parts of the prefix, whose sums go to slots 0 .. (0: no prefix)
   int tiles, splits;                           // of the sequences' own keys, whose sums go to the slots behind (0: decode, not here)
   RowSums sums;                                // slots 0: the result goes to out
@@ -106,15 +115,17 @@ struct DecodeArgs {
   float2* part_ml;                             // [workers][2][16]
   BegunUnit* begun;                               // [workers]
   int workers, row_tiles;
-  RowSums prefix;                              // slots: the prefix's and, last, one for a unit's own sums (0: no prefix)
+  RowSums sums;                                // slots 0: rows go to out
+  int own;                                     // otherwise the slot of the sequences' own keys
+  bool join_all;                               // own is the last slot, and every unit is joined with the prefix's sums
 };
 PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix);
 int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim);
-// tiles: of the prefix (shared_splits 0: none), whose sums' last slot is for the sequences' own keys
+// One new token a sequence, or those sequences of a batch that have one, with the tiles (none: splits and shared_splits 0) of the prefix and the
+// others. Rows whose sums are to be joined (tiles.sums) are left there, but for one token a sequence throughout.
 int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const TileArgs& tiles,
                  hipStream_t s);
-// the prefix's tiles and `grid` workers in one launch (paged_shared.hip), of as many waves as the tiles have
-inline int paged_shared_waves(bool deep, int64_t dim) { return deep && dim <= 128 ? 8 : 4; }
+// tiles and `grid` workers in one launch (paged_shared.hip)
 int paged_shared_decode(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
                         hipStream_t s);
 

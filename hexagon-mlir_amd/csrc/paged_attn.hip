@@ -92,7 +92,7 @@ int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipS
 // What a call launches: the prefix's tiles (prefix_splits 0: none), then one token a sequence (decode) or tiles of the sequences' own keys
 // (splits), then the join of the tiles' sums.
 struct Plan {
-  bool decode, deep;
+  bool decode, deep, workers;                  // one token a sequence; DeepTile; sequences of one new token apart
   int prefix_tiles, prefix_splits, splits;
   int64_t tiles;
   PagedDecodePlan one;
@@ -112,17 +112,19 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   plan.decode = b.starts == nullptr;
   plan.rows = b.tokens * heads;
   const int64_t wide = (rows + WideTile::kRows - 1) / WideTile::kRows * b.kv_heads;
-  plan.deep = wide < DEEP_BELOW * cus;
+  plan.deep = !plan.decode && wide < DEEP_BELOW * cus;
+  plan.workers = plan.decode || b.sequences > 1 || b.tokens == 1;
   const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
   const int64_t wanted = plan.deep ? cus : 2 * cus, least = plan.deep ? DEEP_KEYS : 256;
   if (shared > 0) {
     plan.prefix_tiles = (int)full;
     plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);
   }
-  if (plan.decode) {
+  if (plan.workers) {
     plan.one = plan_paged_decode(b, heads, prefix);
     plan.decode_bytes = (paged_decode_workspace(plan.one, b.dim) + 15) / 16 * 16;
-  } else {
+  }
+  if (!plan.decode) {
     plan.tiles = rows / tile_rows + b.sequences + 2;
     plan.splits = parts_of(full * b.kv_heads, own, wanted, least, 16);
   }
@@ -147,7 +149,8 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   const Plan plan = plan_of(b, heads, shared);
-  return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
+  const int64_t workers = b.sequences > limit / 1024 / units ? limit : b.sequences * units;
+  return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads + workers <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
 }
 }  // namespace
 
@@ -185,9 +188,10 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   const RowSums sums = {o, reinterpret_cast<float2*>(o + plan.slots() * plan.rows * batch->dim), plan.rows, plan.slots()};
   hipStream_t s = as_stream(stream);
   begin_call();
-  auto tiles = [&](const TileArgs& w) { return dtype == HEXMI_F16 ? launch_tiles<f16>(a, p, w, s) : launch_tiles<bf16>(a, p, w, s); };
-  if (plan.decode) return paged_decode(plan.one, a, p, dtype, workspace, {plan.deep, plan.prefix_tiles, plan.prefix_splits, 0, 0, sums}, s);
-  if ((rc = tiles({plan.deep, plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums})) != HEXMI_OK || sums.slots == 0) return rc;
+  const TileArgs tiles = {plan.deep, plan.workers, plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums};
+  rc = plan.workers ? paged_decode(plan.one, a, p, dtype, workspace, tiles, s)
+       : dtype == HEXMI_F16 ? launch_tiles<f16>(a, p, tiles, s) : launch_tiles<bf16>(a, p, tiles, s);
+  if (rc != HEXMI_OK || plan.decode || sums.slots == 0) return rc;
   const unsigned blocks = (unsigned)((plan.rows + 7) / 8);
   if (dtype == HEXMI_F16) hipLaunchKernelGGL((paged_join_kernel<f16>), dim3(blocks), dim3(256), 0, s, a, sums);
   else hipLaunchKernelGGL((paged_join_kernel<bf16>), dim3(blocks), dim3(256), 0, s, a, sums);

@@ -49,7 +49,10 @@ __device__ __forceinline__ float sum_of_quarters(float v) {
 template <int W> __device__ __forceinline__ int blocks_of_keys(int keys) {
   return keys > W * kTileKeys ? (keys + W * kTileKeys - 1) / (W * kTileKeys) : 1;
 }
-template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) { return blocks_of_keys<W>(length_of(p, b) - prefix); }
+// of sequence b, none where it has other than one new token (the tiles take those)
+template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) {
+  return new_tokens_of(p, b) == 1 ? blocks_of_keys<W>(length_of(p, b) - prefix) : 0;
+}
 // the sum over the lanes up to this one
 __device__ __forceinline__ int sum_up_to(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);     // row_shr:1, 2, 4, 8: within 16 lanes
@@ -65,14 +68,14 @@ __device__ __forceinline__ int of_last_lane(int v) { return __builtin_amdgcn_rea
 // The list of all blocks, sequence by sequence: lengths, blocks and sums of blocks of the first 64 sequences are a lane's each, read once;
 // those of further ones are read again where they are needed.
 struct BlockList {
-  int length, blocks, up_to;                   // lane b: of sequence b, and of all up to it
+  int length, blocks, up_to;                   // lane b: of sequence b (no blocks: not a worker's), and of all up to it
   int of_64, all;                              // blocks of the first 64 sequences, of all (one unit's)
 };
 template <int W>
 __device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int lane) {
   BlockList l;
   l.length = lane < p.sequences ? length_of(p, lane) : 0;
-  l.blocks = lane < p.sequences ? blocks_of_keys<W>(l.length - prefix) : 0;
+  l.blocks = lane < p.sequences && new_tokens_of(p, lane) == 1 ? blocks_of_keys<W>(l.length - prefix) : 0;
   l.up_to = sum_up_to(l.blocks);
   l.of_64 = of_last_lane(l.up_to);
   int more = 0;
@@ -98,6 +101,9 @@ __device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, i
 __device__ __forceinline__ int length_at(const BlockList& l, const Pages& p, int b) {
   return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.length, b & (kWave - 1)) : length_of(p, b));
 }
+template <int W> __device__ __forceinline__ int blocks_at(const BlockList& l, const Pages& p, int prefix, int b) {
+  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.blocks, b & (kWave - 1)) : blocks_of<W>(p, b, prefix));
+}
 // worker w's run of `total` blocks
 __device__ __forceinline__ int run_start(int total, int workers, int w) {
   const int each = total / workers, more = total % workers;
@@ -116,6 +122,15 @@ template <int D> __device__ __forceinline__ int swz_pairs(int row) { return D ==
 constexpr int decode_wave_bytes(int d, int cols) {
   const int sums = (16 * (cols + 4) * 4 + d * 2 - 1) / (d * 2) * (d * 2), tile = kTileKeys * d * 2;
   return tile > sums ? tile : sums;
+}
+
+// A row's four columns from d on into the slot for sequences' own keys; of the slots behind it, which only tiles fill, that they are empty.
+__device__ __forceinline__ void keep_sums(const DecodeArgs& w, int64_t row, int dim, int d, const f32x4& out, float2 ml) {
+  const int64_t at = w.own * w.sums.rows + row;
+  *reinterpret_cast<f32x4*>(w.sums.o + at * dim + d) = out;
+  if (d != 0) return;
+  w.sums.ml[at] = ml;
+  for (int x = w.own + 1; x < w.sums.slots; ++x) w.sums.ml[x * w.sums.rows + row] = float2{-INFINITY, 0.0f};
 }
 
 // D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
@@ -140,12 +155,13 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
 
   BlockList list;
   int cur, end, b, before = 0, total = 0;
+  int unit = 0;
   if (w.workers == 0) {                        // a unit each
     b = worker / units;
+    unit = worker - b * units;
     list.length = 0;
-    const int u = worker - b * units, blocks = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix));
-    cur = u * blocks;
-    end = cur + blocks;
+    cur = 0;
+    end = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix));
   } else {
     list = block_list<W>(p, a.prefix, lane);
     total = list.all * units;
@@ -159,23 +175,24 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
 
   while (cur < end) {
     const int length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
-    const int blocks = blocks_of_keys<W>(length - a.prefix), local = cur - before * units;
+    const int blocks = w.workers ? blocks_at<W>(list, p, a.prefix, b) : end - cur, local = cur - before * units;
     if (local >= blocks * units) {             // on to the next sequence
       before += blocks;
       ++b;
       continue;
     }
-    const int u = local / blocks, block0 = local - u * blocks;
+    const int in_list = local / blocks, u = w.workers ? in_list : unit, block0 = local - in_list * blocks;
     const int count = end - cur < blocks - block0 ? end - cur : blocks - block0;
     const int kvh = u / w.row_tiles, row0 = (u - kvh * w.row_tiles) * 16;
     const int rows = a.group - row0 < 16 ? a.group - row0 : 16;
     const int head0 = kvh * a.group + row0;
+    const int token = __builtin_amdgcn_readfirstlane(first_row(p, b));
 
     // ---- queries: the B operand, head n's columns 32 ds + 8 g ..
     Frag qf[DS];
     int col[DS];
     {
-      const T* q = static_cast<const T*>(a.q) + b * a.q_token + (head0 + (n < rows ? n : rows - 1)) * a.q_head;
+      const T* q = static_cast<const T*>(a.q) + token * a.q_token + (head0 + (n < rows ? n : rows - 1)) * a.q_head;
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds) {
         const int c = ds * 32 + g * 8;
@@ -329,14 +346,12 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         if (d == 0) w.part_ml[slot * 16 + r] = float2{top, sum};
         continue;
       }
-      if (w.prefix.slots) {                                          // to be joined with the prefix's
-        const int64_t at = (w.prefix.slots - 1) * w.prefix.rows + (int64_t)b * a.heads + head0 + r;
-        *reinterpret_cast<f32x4*>(w.prefix.o + at * dim + d) = out;
-        if (d == 0) w.prefix.ml[at] = float2{top, sum};
+      if (w.sums.slots) {                                            // to be joined with others
+        keep_sums(w, (int64_t)token * a.heads + head0 + r, dim, d, out, float2{top, sum});
         continue;
       }
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-      store4o<T>(static_cast<T*>(a.out) + b * a.out_token + (head0 + r) * a.out_head + d, out[0] * inv, out[1] * inv, out[2] * inv, out[3] * inv);
+      store4o<T>(static_cast<T*>(a.out) + token * a.out_token + (head0 + r) * a.out_head + d, out[0] * inv, out[1] * inv, out[2] * inv, out[3] * inv);
     }
     __syncthreads();                                                 // before the LDS holds V again
     cur += count;

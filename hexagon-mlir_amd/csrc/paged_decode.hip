@@ -15,24 +15,24 @@ void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   paged_decode_worker<T, D, COLS, PADDED, kWaves>(a, p, w, blockIdx.x, lds, m_lds, l_lds);
 }
 
-// The units that several workers share: block (w, row) takes the one that worker w began. Behind a prefix every unit is joined with its
-// sums: block (unit, row).
-template <typename T, int W>
+// The units that several workers share: block (w, row) takes the one that worker w began. With join_all every unit is joined with the
+// prefix's sums: block (unit, row).
+template <typename T>
 __global__ __launch_bounds__(256)
 void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   __shared__ float o_lds[8][256 + 4];
   __shared__ float m_lds[8], l_lds[8];
   const int units = p.kv_heads * w.row_tiles, r = blockIdx.y;
   int b, u, w0 = 0, w1 = 0;
-  if (w.prefix.slots) {
+  if (w.join_all) {
     b = blockIdx.x / units;
     u = blockIdx.x - b * units;
     if (w.workers) {
       const int lane = threadIdx.x % kWave;
-      const BlockList list = block_list<W>(p, a.prefix, lane);
+      const BlockList list = block_list<kWaves>(p, a.prefix, lane);
       int before = 0;
-      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<W>(p, x, a.prefix);
-      const int blocks = blocks_of_keys<W>(length_at(list, p, b) - a.prefix), total = list.all * units;
+      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<kWaves>(p, x, a.prefix);
+      const int blocks = blocks_at<kWaves>(list, p, a.prefix, b), total = list.all * units;
       const int first = of_last_lane(sum_up_to(before)) * units + u * blocks;
       w0 = worker_of(total, w.workers, first);
       w1 = worker_of(total, w.workers, first + blocks - 1);
@@ -48,7 +48,8 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   const int kvh = u / w.row_tiles, row0 = (u - kvh * w.row_tiles) * 16;
   if (r >= a.group - row0) return;
   const int head = kvh * a.group + row0 + r;
-  const int64_t row = (int64_t)b * a.heads + head;
+  const int token = first_row(p, b);
+  const int64_t row = (int64_t)token * a.heads + head;
   // eight groups of 32 threads take every eighth set of sums, a thread the columns d and, past 128, d + 128
   const int group = threadIdx.x / 32, d = threadIdx.x % 32 * 4;
   float top = -INFINITY, sum = 0.0f;
@@ -70,7 +71,8 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     const int64_t slot = (int64_t)x * 2 + (x == w0 ? 1 : 0);
     take(w.part_ml[slot * 16 + r], w.part_o + (slot * 16 + r) * a.dim);
   }
-  for (int x = group; x < w.prefix.slots - (w0 < w1 ? 1 : 0); x += 8) take(w.prefix.ml[x * w.prefix.rows + row], w.prefix.o + (x * w.prefix.rows + row) * a.dim);
+  const int beside = !w.join_all ? 0 : w0 < w1 ? w.own : w.own + 1;
+  for (int x = group; x < beside; x += 8) take(w.sums.ml[x * w.sums.rows + row], w.sums.o + (x * w.sums.rows + row) * a.dim);
 #pragma unroll
   for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(&o_lds[group][d + h * 128]) = out[h];
   if (d == 0) {
@@ -89,19 +91,25 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
       l = fmaf(l_lds[x], f, l);
       o = fmaf(o_lds[x][c], f, o);
     }
-  static_cast<T*>(a.out)[b * a.out_token + head * a.out_head + c] = from_f32<T>(l > 0.0f ? o / l : 0.0f);
+  if (w.sums.slots && !w.join_all) {                                // a set of sums like a tile's
+    const int64_t at = w.own * w.sums.rows + row;
+    w.sums.o[at * a.dim + c] = o;
+    if (c == 0) w.sums.ml[at] = float2{top, l};
+    if (c > w.own && c < w.sums.slots) w.sums.ml[c * w.sums.rows + row] = float2{-INFINITY, 0.0f};
+    return;
+  }
+  static_cast<T*>(a.out)[token * a.out_token + head * a.out_head + c] = from_f32<T>(l > 0.0f ? o / l : 0.0f);
 }
 
 template <typename T>
 int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, const TileArgs& tiles, int dtype,
            hipStream_t s) {
   const unsigned grid = plan.workers ? plan.workers : (unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles);
-  if (tiles.shared_splits) {
+  if (tiles.shared_splits || tiles.splits) {
     const int rc = paged_shared_decode(a, p, tiles, w, grid, dtype, s);
-    if (rc != HEXMI_OK) return rc;
-    const dim3 units((unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles), plan.rows);
-    if (paged_shared_waves(tiles.deep, a.dim) == 8) hipLaunchKernelGGL((paged_decode_join_kernel<T, 8>), units, dim3(256), 0, s, a, p, w);
-    else hipLaunchKernelGGL((paged_decode_join_kernel<T, 4>), units, dim3(256), 0, s, a, p, w);
+    if (rc != HEXMI_OK || (!w.join_all && plan.workers < 2)) return rc;
+    const dim3 joins(w.join_all ? (unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles) : plan.workers - 1, plan.rows);
+    hipLaunchKernelGGL((paged_decode_join_kernel<T>), joins, dim3(256), 0, s, a, p, w);
     return launch_status();
   }
 #define HEXMI_PAGED_DECODE(D, COLS)                                                                                                      \
@@ -116,7 +124,7 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
 #undef HEXMI_PAGED_DECODE
   const int rc = launch_status();
   if (rc != HEXMI_OK || plan.workers < 2) return rc;
-  hipLaunchKernelGGL((paged_decode_join_kernel<T, kWaves>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
+  hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
   return launch_status();
 }
 
@@ -130,7 +138,7 @@ PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int
   // A block each while they are fewer than the compute units; then four and more, so that a worker's sums are few beside its keys, on as
   // many workgroups as a compute unit holds. One and two a compute unit, heads of 128: 1 sequence x 16000 keys x 8 heads 21.9 / 24.5 us,
   // 3 x 5000 15.2 / 17.0; 128 x 500 58 / 52, 16 x 2048 x 32 97.7 / 93.5. Heads of 256, of which it holds one: 16 x 2048 x 8 56 / 60.
-  const int64_t cus = hexmi_num_cus(), all = units * blocks, held = cus * (prefix > 0 ? 1 : b.dim <= 96 ? 3 : b.dim <= 128 ? 2 : 1);
+  const int64_t cus = hexmi_num_cus(), all = units * blocks, held = cus * (prefix > 0 || b.starts ? 1 : b.dim <= 96 ? 3 : b.dim <= 128 ? 2 : 1);
   const int64_t fours = all / 4 < cus ? cus : all / 4, workers = all < cus ? all : fours < held ? fours : held;
   return {(int)(workers < 1 ? 1 : workers), (int)tiles, rows};
 }
@@ -143,7 +151,8 @@ int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Page
                  hipStream_t s) {
   float* o = static_cast<float*>(workspace);
   float2* ml = reinterpret_cast<float2*>(o + (int64_t)plan.workers * 2 * 16 * a.dim);
-  const DecodeArgs w = {o, ml, reinterpret_cast<BegunUnit*>(ml + (int64_t)plan.workers * 2 * 16), plan.workers, plan.row_tiles, tiles.sums};
+  const DecodeArgs w = {o, ml, reinterpret_cast<BegunUnit*>(ml + (int64_t)plan.workers * 2 * 16), plan.workers,
+                        plan.row_tiles, tiles.sums, tiles.shared_splits, p.starts == nullptr && tiles.shared_splits > 0};
   return dtype == HEXMI_F16 ? launch<f16>(plan, a, p, w, tiles, dtype, s) : launch<bf16>(plan, a, p, w, tiles, dtype, s);
 }
 

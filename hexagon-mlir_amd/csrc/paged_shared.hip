@@ -1,6 +1,6 @@
-// A decode step behind a prefix that all sequences share: the prefix's tiles (paged_tile.h), which the matrix cores bind, and the workers on
-// the sequences' own keys (paged_decode.h), which wait for memory, in one launch side by side. Their sums are joined by
-// paged_decode_join_kernel. 32 sequences x 200 keys behind 8192 (32 heads over 8, of 128): one launch after the other 37 us, this way 23.
+// Tiles (paged_tile.h), which the matrix cores bind, and workers on sequences of one new token (paged_decode.h), which wait for memory, in one
+// launch side by side: a decode step behind a prefix that all sequences share, whose sums paged_decode_join_kernel joins, and a batch of
+// prompts and decode steps. 32 sequences x 200 keys behind 8192 (32 heads over 8, of 128): one launch after the other 37 us, this way 23.
 #include "paged_decode.h"
 #include "paged_tile.h"
 
@@ -24,7 +24,8 @@ void paged_shared_decode_kernel(PagedAttnArgs a, Pages p, TileArgs tiles, Decode
 
 template <typename T>
 int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned workers, hipStream_t s) {
-  const unsigned tile_grid = (unsigned)((int64_t)tiles.shared_tiles * tiles.shared_splits * p.kv_heads), grid = tile_grid + workers;
+  const unsigned tile_grid = (unsigned)(((int64_t)tiles.shared_tiles * tiles.shared_splits + (int64_t)tiles.tiles * tiles.splits) * p.kv_heads);
+  const unsigned grid = tile_grid + workers;
 #define HEXMI_PAGED_SHARED(D, COLS, Shape)                                                                                               \
   do {                                                                                                                                   \
     if (a.dim == COLS)                                                                                                                   \

@@ -27,13 +27,9 @@ typedef TileShape<64, 4, 1> WideTile;          // many tiles: 128 rows, two work
 typedef TileShape<32, 2, 4> DeepTile;          // few: 64 rows, the chain of a tile's blocks a quarter as long, one workgroup a compute unit
 typedef TileShape<32, 2, 2> DeepTile256;       // ... heads of 256 columns, whose blocks are as large again
 
-// The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences, where -1 and `sequences` are the
-// rows of no sequence before the first and behind the last. floor(x / r) + 1 >= ceil(n / r) + floor(x0 / r) for x = x0 + n, so
-// a sequence's tiles end before the next one's begin; some numbers are no tile.
-__device__ __forceinline__ int first_row(const Pages& p, int b) {
-  const int s = b < 0 ? 0 : b > p.sequences ? p.tokens : p.starts[b];
-  return s < 0 ? 0 : s < p.tokens ? s : p.tokens;
-}
+// The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences (first_row).
+// floor(x / r) + 1 >= ceil(n / r) + floor(x0 / r) for x = x0 + n, so a sequence's tiles end before the next one's begin; some numbers are
+// no tile.
 template <int ROWS>
 __device__ __forceinline__ int first_tile(const Pages& p, int group, int b) { return b < 0 ? 0 : first_row(p, b) * group / ROWS + b + 1; }
 template <int ROWS>
@@ -100,6 +96,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     rows = new_tokens * a.group;                                    // negative where starts fall: nothing
     if (row0 < 0 || row0 >= rows) return;
     none = b < 0 || b >= p.sequences;
+    if (w.workers && new_tokens == 1 && !none) return;
     if (!none) length = p.lengths[b];
     const int last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
     end = none ? 0 : keys_of(length, new_tokens, divided(last, a.by_group), most);
