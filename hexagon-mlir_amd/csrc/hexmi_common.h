@@ -231,6 +231,23 @@ __device__ __forceinline__ void copy_ptr_to_lds_asm(const char* src, char* lds) 
 #endif
 }
 
+// Two of the same, each from a wave-uniform address and a lane's own offset in bytes (below 2^31); the second goes STEP bytes further on.
+template <int STEP>
+__device__ __forceinline__ void copy_two_to_lds_asm(const char* base0, int off0, const char* base1, int off1, char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto uniform = [](const char* p) __attribute__((always_inline)) {
+    const uint64_t b = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b), hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    return (uint64_t)hi << 32 | lo;
+  };
+  const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)(lds)));
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
+               "s_add_u32 m0, %1, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved) : "s"(dst), "v"(off0), "s"(uniform(base0)), "v"(off1), "s"(uniform(base1)), "i"(STEP) : "memory", "scc");
+#endif
+}
+
 // sixteen 16-bit columns in two chunks, from column `by` (0 .. 7) on: eight of them
 __device__ __forceinline__ u32x4 shift_columns(const u32x4& lo, const u32x4& hi, int by) {
   auto pick = [](bool second, uint32_t v0, uint32_t v1) { return second ? v1 : v0; };    // (values, not places: no scratch)

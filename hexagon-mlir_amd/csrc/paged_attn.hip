@@ -12,7 +12,7 @@ namespace hexmi {
 namespace {
 
 template <typename T, int D, int COLS, bool PADDED, typename Shape>
-__global__ __launch_bounds__(Shape::kThreads, D == 256 || Shape::kGroups > 1 ? 1 : 2)
+__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : 2)
 void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
   __shared__ __attribute__((aligned(16))) T lds[Shape::lds_elements(D)];
   __shared__ float m_lds[Shape::kGroups][Shape::kRows], l_lds[Shape::kGroups][Shape::kRows];
@@ -78,7 +78,7 @@ int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipS
     if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, DeepTile);
     else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, DeepTile);
     else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128, DeepTile);
-    else HEXMI_PAGED_TILE(256, 256, DeepTile256);
+    else HEXMI_PAGED_TILE(256, 256, DeepTile);
   } else {
     if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, WideTile);
     else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, WideTile);
@@ -115,7 +115,7 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   plan.deep = !plan.decode && wide < DEEP_BELOW * cus;
   plan.workers = plan.decode || b.sequences > 1 || b.tokens == 1;
   const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
-  const int64_t wanted = plan.deep ? cus : 2 * cus, least = plan.deep ? DEEP_KEYS : 256;
+  const int64_t wanted = 2 * cus, least = plan.deep ? DEEP_KEYS : 256;
   if (shared > 0) {
     plan.prefix_tiles = (int)full;
     plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);

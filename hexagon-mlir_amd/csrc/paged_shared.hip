@@ -8,7 +8,7 @@ namespace hexmi {
 namespace {
 
 template <typename T, int D, int COLS, bool PADDED, typename Shape>
-__global__ __launch_bounds__(Shape::kThreads, D == 256 || Shape::kGroups > 1 ? 1 : 2)
+__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : 2)
 void paged_shared_decode_kernel(PagedAttnArgs a, Pages p, TileArgs tiles, DecodeArgs w, unsigned tile_grid) {
   constexpr int W = Shape::kThreads / kWave, kTileBytes = Shape::lds_elements(D) * 2, kDecodeBytes = W * decode_wave_bytes(D, COLS);
   __shared__ __attribute__((aligned(16))) char lds[kTileBytes > kDecodeBytes ? kTileBytes : kDecodeBytes];
@@ -39,7 +39,7 @@ int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const 
     if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, DeepTile);
     else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, DeepTile);
     else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128, DeepTile);
-    else HEXMI_PAGED_SHARED(256, 256, DeepTile256);
+    else HEXMI_PAGED_SHARED(256, 256, DeepTile);
   } else {
     if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, WideTile);
     else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, WideTile);

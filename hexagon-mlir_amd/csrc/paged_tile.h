@@ -24,8 +24,7 @@ template <int KEYS, int ROW_WAVES, int GROUPS> struct TileShape {
   static_assert(4 * KEYS * 2 == kRows * 4, "a group's sums take the place of its blocks");
 };
 typedef TileShape<64, 4, 1> WideTile;          // many tiles: 128 rows, two workgroups a compute unit
-typedef TileShape<32, 2, 4> DeepTile;          // few: 64 rows, the chain of a tile's blocks a quarter as long, one workgroup a compute unit
-typedef TileShape<32, 2, 2> DeepTile256;       // ... heads of 256 columns, whose blocks are as large again
+typedef TileShape<32, 2, 2> DeepTile;          // few: 64 rows, the chain of a tile's keys half as long
 
 // The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences (first_row).
 // floor(x / r) + 1 >= ceil(n / r) + floor(x0 / r) for x = x0 + n, so a sequence's tiles end before the next one's begin; some numbers are
@@ -113,13 +112,17 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
   const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
   const int lin = row_wave * kWave + lane, copy_row = lin / CPR, lds_at = row_wave * kWave * 8;
-  auto find = [&](int block) __attribute__((always_inline)) {       // the page of key kKeys block + lane, -1: none
+  // The table's entry for key kKeys block + lane. No branch: it is asked for a block ahead, and what it is worth is looked at then (a load
+  // behind a branch would be waited for where the branch ends).
+  auto find = [&](int block) __attribute__((always_inline)) {
     const int key = begin + block * kKeys + lane % kKeys;
-    if (block >= block1 || key >= end) return -1;
-    const int page = table[divided(key, p.size)];
-    return page < p.num_pages ? page : -1;
+    return table[divided(key < end ? key : end - 1, p.size)];       // end > begin: only asked then
   };
-  // One block into LDS. Where every key is there and the rows of an instruction share a page, the page, and so the place, is the wave's
+  auto page_at = [&](int block, int entry) __attribute__((always_inline)) {     // -1: no key there
+    return block < block1 && begin + block * kKeys + lane % kKeys < end && entry >= 0 && entry < p.num_pages ? entry : -1;
+  };
+  // One block into LDS, by copies that the compiler does not know of: it would wait for all of them before it reads LDS transposed, in the
+  // middle of the block before. They are waited for ahead of the barrier that ends that block. Where every key is there and the rows of an instruction share a page, the page, and so the place, is the wave's
   // (scalar arithmetic), and a lane adds what it is off in it; any other block goes row by row.
   constexpr int kRowsOfOne = kWave / CPR;
   const bool one_page = p.page_size % kRowsOfOne == 0;
@@ -129,19 +132,27 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   };
   auto copy = [&](int block, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
+      // a lane works out where its key stands, for all of the block's at once; an instruction takes its first row's
+      const int key_of_lane = begin + block * kKeys + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
+      const int64_t k_at = page_of_lane * p.k_page + slot_of_lane * p.k_slot, v_at = page_of_lane * p.v_page + slot_of_lane * p.v_slot;
+      auto first_of = [&](int64_t at, int j) __attribute__((always_inline)) {
+        const int row = row_wave * kRowsOfOne + j * kRowStep;
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, row), hi = __builtin_amdgcn_readlane((int)(at >> 32), row);
+        return (int64_t)((uint64_t)hi << 32 | lo);
+      };
+      constexpr int kStep = kRowWaves * kWave * 16;                 // bytes of LDS between a wave's instructions
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int64_t page_stride = v ? p.v_page : p.k_page, slot_stride = v ? p.v_slot : p.k_slot;
-        T* dst = v ? v_dst : k_dst;
+      for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const int row = row_wave * kRowsOfOne + j * kRowStep, key = begin + block * kKeys + row;
-          const int page = __builtin_amdgcn_readlane(page_of_lane, row), slot = key - divided(key, p.size) * p.page_size;
-          const T* from = (v ? v_head : k_head) + page * page_stride + slot * slot_stride;
-          const int off = lane / CPR * (int)slot_stride + column(v, copy_row + j * kRowStep);
-          __builtin_amdgcn_global_load_lds(HEXMI_GLB(from + off), HEXMI_LDS(dst + lds_at + j * (kRowWaves * kWave * 8)), 16, 0, 0);
+        for (int j = 0; j < NI; j += 2) {
+          const T* head = v ? v_head : k_head;
+          const int64_t at = v ? v_at : k_at;
+          const int step = lane / CPR * (int)(v ? p.v_slot : p.k_slot);
+          copy_two_to_lds_asm<kStep>(reinterpret_cast<const char*>(head + first_of(at, j)), (step + column(v, copy_row + j * kRowStep)) * 2,
+                                     reinterpret_cast<const char*>(head + first_of(at, j + 1)),
+                                     (step + column(v, copy_row + (j + 1) * kRowStep)) * 2,
+                                     reinterpret_cast<char*>((v ? v_dst : k_dst) + lds_at) + j * kStep);
         }
-      }
       return;
     }
 #pragma unroll
@@ -150,18 +161,19 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       const int slot = key - divided(key, p.size) * p.page_size;
       T *k_to = k_dst + lds_at + j * (kRowWaves * kWave * 8), *v_to = v_dst + lds_at + j * (kRowWaves * kWave * 8);
       if (page >= 0) {
-        __builtin_amdgcn_global_load_lds(HEXMI_GLB(k_head + page * p.k_page + slot * p.k_slot + column(false, r)), HEXMI_LDS(k_to), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(HEXMI_GLB(v_head + page * p.v_page + slot * p.v_slot + column(true, r)), HEXMI_LDS(v_to), 16, 0, 0);
+        copy_ptr_to_lds_asm(reinterpret_cast<const char*>(k_head + page * p.k_page + slot * p.k_slot + column(false, r)), reinterpret_cast<char*>(k_to));
+        copy_ptr_to_lds_asm(reinterpret_cast<const char*>(v_head + page * p.v_page + slot * p.v_slot + column(true, r)), reinterpret_cast<char*>(v_to));
       } else {                                                      // no key: whatever the cache holds, zeros of V (its score is dropped)
         *reinterpret_cast<u32x4*>(v_to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
       }
     }
   };
   int page = -1, next = -1;
-  if (first < block1) {                                             // on their way while the rows are looked up
+  if (block0 < block1) {                                            // on their way while the rows are looked up
     page = find(first);
     next = find(first + kGroups);
-    copy(first, page, k_lds0, v_lds0);
+    page = page_at(first, page);
+    if (first < block1) copy(first, page, k_lds0, v_lds0);
   }
 
   // this lane's row: its token, its queries and the keys it sees
@@ -317,18 +329,25 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     }
   };
 
+  // the queries are here before the walk begins: their first use must not wait inside it, with copies on their way
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) {
+    u32x4 f = __builtin_bit_cast(u32x4, qf[ds]);
+    asm volatile("" : "+v"(f));
+    qf[ds] = __builtin_bit_cast(Frag, f);
+  }
   for (int block = first, at = block0; at < block1; block += 2 * kGroups, at += 2 * kGroups) {      // as many turns for every group
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     uint64_t there = __ballot(page >= 0);
-    page = next;
+    page = page_at(block + kGroups, next);
     next = find(block + 2 * kGroups);
     process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
     if (at + kGroups >= block1) break;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     there = __ballot(page >= 0);
-    page = next;
+    page = page_at(block + 2 * kGroups, next);
     next = find(block + 3 * kGroups);
     process(block + kGroups, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
   }
