@@ -1,9 +1,3 @@
-#ifndef DEEP_BELOW
-#define DEEP_BELOW 1
-#endif
-#ifndef DEEP_KEYS
-#define DEEP_KEYS 512
-#endif
 // Attention over a paged cache of keys and values (fp16 / bf16): runs of new tokens of many sequences over the positions before them, and
 // the prefix that all sequences share: what a call launches, the tiles of ragged batches (paged_tile.h) and the join of their sums.
 #include "paged_tile.h"
@@ -77,8 +71,7 @@ int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipS
   if (w.deep) {
     if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, DeepTile);
     else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, DeepTile);
-    else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128, DeepTile);
-    else HEXMI_PAGED_TILE(256, 256, DeepTile);
+    else HEXMI_PAGED_TILE(128, 128, DeepTile);
   } else {
     if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, WideTile);
     else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, WideTile);
@@ -112,10 +105,10 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   plan.decode = b.starts == nullptr;
   plan.rows = b.tokens * heads;
   const int64_t wide = (rows + WideTile::kRows - 1) / WideTile::kRows * b.kv_heads;
-  plan.deep = !plan.decode && wide < DEEP_BELOW * cus;
+  plan.deep = !plan.decode && b.dim <= 128 && wide < cus;
   plan.workers = plan.decode || b.sequences > 1 || b.tokens == 1;
   const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
-  const int64_t wanted = 2 * cus, least = plan.deep ? DEEP_KEYS : 256;
+  const int64_t wanted = 2 * cus, least = plan.deep ? 512 : 256;
   if (shared > 0) {
     plan.prefix_tiles = (int)full;
     plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);

@@ -38,8 +38,7 @@ int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const 
   if (tiles.deep) {
     if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, DeepTile);
     else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, DeepTile);
-    else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128, DeepTile);
-    else HEXMI_PAGED_SHARED(256, 256, DeepTile);
+    else HEXMI_PAGED_SHARED(128, 128, DeepTile);
   } else {
     if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, WideTile);
     else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, WideTile);

@@ -256,22 +256,25 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    struct VFrags { Frag f[2][DT]; };
+    // fragments of V: of a 32-key tile they are read ahead of its probabilities, but for heads of 256 columns, whose registers they are
+    constexpr int kPieces = D == 256 ? 1 : 2 * DT;
+    struct VFrags { Frag f[kPieces]; };
+    auto read_piece = [&](int jt, int piece) __attribute__((always_inline)) {
+      const int g = lane / 16, i16 = lane % 16, hf = piece / DT, dt = piece % DT;
+      union { i16x4 h[2]; Frag f; } u;
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp) {
+        const int r = jt * 32 + hf * 16 + 8 * pp + 4 * (g >> 1) + (i16 >> 2), col = dt * 32 + (g & 1) * 16 + (i16 & 3) * 4;
+        const int c = (col / 8) ^ swz_vtile<D == 64 ? 64 : 128>(r);
+        u.h[pp] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(v_src + (r * CPR + c) * 8 + col % 8));
+      }
+      return u.f;
+    };
     auto read_v = [&](int jt, VFrags& vf) __attribute__((always_inline)) {
-      const int g = lane / 16, i16 = lane % 16;
+      if constexpr (kPieces > 1) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          union { i16x4 h[2]; Frag f; } u;
-#pragma unroll
-          for (int pp = 0; pp < 2; ++pp) {
-            const int r = jt * 32 + hf * 16 + 8 * pp + 4 * (g >> 1) + (i16 >> 2), col = dt * 32 + (g & 1) * 16 + (i16 & 3) * 4;
-            const int c = (col / 8) ^ swz_vtile<D == 64 ? 64 : 128>(r);
-            u.h[pp] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(v_src + (r * CPR + c) * 8 + col % 8));
-          }
-          vf.f[hf][dt] = u.f;
-        }
+        for (int piece = 0; piece < kPieces; ++piece) vf.f[piece] = read_piece(jt, piece);
+      }
     };
     VFrags vf0, vf1;
     read_v(0, vf0);
@@ -314,18 +317,19 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       pf[1] = MfmaT<T>::pack(&pr[8]);
       l_i = MfmaT<T>::sum8(pf[1], MfmaT<T>::sum8(pf[0], l_i));      // the sum of what the product multiplies
     };
-    auto pv = [&](const VFrags& vf) __attribute__((always_inline)) {
+    auto pv = [&](int jt, const VFrags& vf) __attribute__((always_inline)) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o_acc[dt] = MfmaT<T>::run(vf.f[hf][dt], pf[hf], o_acc[dt]);
+      for (int piece = 0; piece < 2 * DT; ++piece) {
+        o_acc[piece % DT] = MfmaT<T>::run(kPieces > 1 ? vf.f[piece % kPieces] : read_piece(jt, piece), pf[piece / DT], o_acc[piece % DT]);
+        if (kPieces == 1 && piece % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
     };
     if constexpr (JT == 2) read_v(1, vf1);
     exp_tile(s[0]);
-    pv(vf0);
+    pv(0, vf0);
     if constexpr (JT == 2) {
       exp_tile(s[1]);
-      pv(vf1);
+      pv(1, vf1);
     }
   };
 
