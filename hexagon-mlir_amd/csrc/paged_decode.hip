@@ -54,25 +54,44 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   const int group = threadIdx.x / 32, d = threadIdx.x % 32 * 4;
   float top = -INFINITY, sum = 0.0f;
   f32x4 out[2] = {};
-  auto take = [&](float2 ml, const float* o) __attribute__((always_inline)) {
-    if (!(ml.y > 0.0f)) return;
-    const float new_top = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(ml.x - new_top), old = __builtin_amdgcn_exp2f(top - new_top);
-    sum = fmaf(ml.y, f, sum * old);
-    top = new_top;
+  // n sets of sums, this group's four at a time on their way: place(x, ml, o) says where set x stands
+  auto take = [&](int n, auto place) __attribute__((always_inline)) {
+    for (int x0 = group; x0 < n; x0 += 32) {
+      float2 ml[4];
+      f32x4 ox[4][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (d + h * 128 < a.dim) {
-        const f32x4 ox = *reinterpret_cast<const f32x4*>(o + d + h * 128);
+      for (int i = 0; i < 4; ++i) {
+        const float2* at_ml;
+        const float* at_o;
+        place(x0 + 8 * i < n ? x0 + 8 * i : x0, at_ml, at_o);
+        ml[i] = *at_ml;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[h][e] = fmaf(ox[e], f, out[h][e] * old);
+        for (int h = 0; h < 2; ++h) ox[i][h] = d + h * 128 < a.dim ? *reinterpret_cast<const f32x4*>(at_o + d + h * 128) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (x0 + 8 * i >= n || !(ml[i].y > 0.0f)) continue;          // nothing there: its columns may be anything
+        const float new_top = fmaxf(top, ml[i].x), f = __builtin_amdgcn_exp2f(ml[i].x - new_top), old = __builtin_amdgcn_exp2f(top - new_top);
+        sum = fmaf(ml[i].y, f, sum * old);
+        top = new_top;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[h][e] = fmaf(ox[i][h][e], f, out[h][e] * old);
+      }
+    }
   };
-  for (int x = w0 + group; x <= w1 && w0 < w1; x += 8) {
-    const int64_t slot = (int64_t)x * 2 + (x == w0 ? 1 : 0);
-    take(w.part_ml[slot * 16 + r], w.part_o + (slot * 16 + r) * a.dim);
-  }
-  const int beside = !w.join_all ? 0 : w0 < w1 ? w.own : w.own + 1;
-  for (int x = group; x < beside; x += 8) take(w.sums.ml[x * w.sums.rows + row], w.sums.o + (x * w.sums.rows + row) * a.dim);
+  if (w0 < w1)
+    take(w1 - w0 + 1, [&](int x, const float2*& ml, const float*& o) {
+      const int64_t slot = (int64_t)(w0 + x) * 2 + (x == 0 ? 1 : 0);
+      ml = w.part_ml + slot * 16 + r;
+      o = w.part_o + (slot * 16 + r) * a.dim;
+    });
+  if (w.join_all)
+    take(w0 < w1 ? w.own : w.own + 1, [&](int x, const float2*& ml, const float*& o) {
+      ml = w.sums.ml + x * w.sums.rows + row;
+      o = w.sums.o + (x * w.sums.rows + row) * a.dim;
+    });
 #pragma unroll
   for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(&o_lds[group][d + h * 128]) = out[h];
   if (d == 0) {
