@@ -24,10 +24,10 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
   constexpr int kSlots = 4;
   const int lane = threadIdx.x % kWave, own = lane % 32;
   const float2 ml = own < sums.slots ? sums.ml[own * sums.rows + row] : float2{-INFINITY, 0.0f};
-  float top = ml.y > 0.0f ? ml.x : -INFINITY;
+  float top = ml.y != 0.0f ? ml.x : -INFINITY;
 #pragma unroll
   for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-  const float f = ml.y > 0.0f ? __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;
+  const float f = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;      // NaN in a part makes it NaN
   float sum = ml.y * f;
 #pragma unroll
   for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
@@ -41,7 +41,7 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         o[x][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (fx[x] > 0.0f && d + h * 128 < a.dim)
+        if (fx[x] != 0.0f && d + h * 128 < a.dim)
           o[x][h] = *reinterpret_cast<const f32x4*>(sums.o + ((x0 + x) * sums.rows + row) * a.dim + d + h * 128);
       }
     }
@@ -53,7 +53,7 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
         for (int e = 0; e < 4; ++e) out[h][e] = fmaf(o[x][h][e], fx[x], out[h][e]);
   }
   const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   T* to = static_cast<T*>(a.out) + token * a.out_token + head * a.out_head;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -142,6 +142,7 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   const Plan plan = plan_of(b, heads, shared);
+  if (plan.slots() > 0 && plan.rows > limit / 32) return HEXMI_ENOTSUP;         // 32 threads a row join them
   const int64_t workers = b.sequences > limit / 1024 / units ? limit : b.sequences * units;
   return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads + workers <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
 }

@@ -331,15 +331,14 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
 #pragma unroll
       for (int x = 0; x < W; ++x) top = fmaxf(top, m_lds[x][r]);
       f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (top != -INFINITY) {
+      const float base = top == -INFINITY ? 0.0f : top;             // no key: sums of 0; a NaN among the scores stays one
 #pragma unroll
-        for (int x = 0; x < W; ++x) {
-          const float f = __builtin_amdgcn_exp2f(m_lds[x][r] - top);
-          const f32x4 ox = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * kWaveBytes) + r * kPitch + d);
-          sum = fmaf(l_lds[x][r], f, sum);
+      for (int x = 0; x < W; ++x) {
+        const float f = __builtin_amdgcn_exp2f(m_lds[x][r] - base);
+        const f32x4 ox = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * kWaveBytes) + r * kPitch + d);
+        sum = fmaf(l_lds[x][r], f, sum);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[e] = fmaf(ox[e], f, out[e]);
-        }
+        for (int e = 0; e < 4; ++e) out[e] = fmaf(ox[e], f, out[e]);
       }
       if (!mine) {
         *reinterpret_cast<f32x4*>(w.part_o + ((int64_t)slot * 16 + r) * dim + d) = out;
@@ -350,7 +349,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         keep_sums(w, (int64_t)token * a.heads + head0 + r, dim, d, out, float2{top, sum});
         continue;
       }
-      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       store4o<T>(static_cast<T*>(a.out) + token * a.out_token + (head0 + r) * a.out_head + d, out[0] * inv, out[1] * inv, out[2] * inv, out[3] * inv);
     }
     __syncthreads();                                                 // before the LDS holds V again

@@ -70,7 +70,7 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (x0 + 8 * i >= n || !(ml[i].y > 0.0f)) continue;          // nothing there: its columns may be anything
+        if (x0 + 8 * i >= n || ml[i].y == 0.0f) continue;            // nothing there: its columns may be anything
         const float new_top = fmaxf(top, ml[i].x), f = __builtin_amdgcn_exp2f(ml[i].x - new_top), old = __builtin_amdgcn_exp2f(top - new_top);
         sum = fmaf(ml[i].y, f, sum * old);
         top = new_top;
@@ -104,20 +104,22 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
   top = -INFINITY;
   for (int x = 0; x < 8; ++x) top = fmaxf(top, m_lds[x]);
   float l = 0.0f, o = 0.0f;
-  if (top != -INFINITY)
-    for (int x = 0; x < 8; ++x) {
-      const float f = __builtin_amdgcn_exp2f(m_lds[x] - top);
-      l = fmaf(l_lds[x], f, l);
-      o = fmaf(o_lds[x][c], f, o);
-    }
+  const float base = top == -INFINITY ? 0.0f : top;                 // no key: sums of 0; a NaN among the scores stays one
+  for (int x = 0; x < 8; ++x) {
+    const float f = __builtin_amdgcn_exp2f(m_lds[x] - base);
+    l = fmaf(l_lds[x], f, l);
+    o = fmaf(o_lds[x][c], f, o);
+  }
   if (w.sums.slots && !w.join_all) {                                // a set of sums like a tile's
     const int64_t at = w.own * w.sums.rows + row;
     w.sums.o[at * a.dim + c] = o;
-    if (c == 0) w.sums.ml[at] = float2{top, l};
-    if (c > w.own && c < w.sums.slots) w.sums.ml[c * w.sums.rows + row] = float2{-INFINITY, 0.0f};
+    if (c == 0) {
+      w.sums.ml[at] = float2{top, l};
+      for (int x = w.own + 1; x < w.sums.slots; ++x) w.sums.ml[x * w.sums.rows + row] = float2{-INFINITY, 0.0f};
+    }
     return;
   }
-  static_cast<T*>(a.out)[token * a.out_token + head * a.out_head + c] = from_f32<T>(l > 0.0f ? o / l : 0.0f);
+  static_cast<T*>(a.out)[token * a.out_token + head * a.out_head + c] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
 }
 
 template <typename T>

@@ -361,7 +361,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   // leave as whole rows, through the LDS that held the blocks (16-byte chunks XOR swizzled by the row), where the groups' sums meet.
   const float l = l_i + other_half(l_i);
   const bool parts = w.sums.slots != 0;
-  const float own = kGroups > 1 || parts ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+  const float own = kGroups > 1 || parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t slot = (int64_t)(part + (shared ? 0 : w.shared_splits)) * w.sums.rows;
   float* sums = reinterpret_cast<float*>(lds);
   auto at_lds = [&](int g, int r, int chunk) __attribute__((always_inline)) {
@@ -407,21 +407,20 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       for (int g = 0; g < kGroups; ++g) top = fmaxf(top, m_lds[g][r]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      if (top != -INFINITY) {
+      const float base = top == -INFINITY ? 0.0f : top;             // no key: sums of 0; a NaN among the scores stays one
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const float f = __builtin_amdgcn_exp2f(m_lds[g][r] - top);
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4)), hi = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4 + 1));
-          sum = fmaf(l_lds[g][r], f, sum);
+      for (int g = 0; g < kGroups; ++g) {
+        const float f = __builtin_amdgcn_exp2f(m_lds[g][r] - base);
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4)), hi = *reinterpret_cast<const f32x4*>(at_lds(g, r, d / 4 + 1));
+        sum = fmaf(l_lds[g][r], f, sum);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = fmaf(lo[e], f, v[e]);
-            v[e + 4] = fmaf(hi[e], f, v[e + 4]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          v[e] = fmaf(lo[e], f, v[e]);
+          v[e + 4] = fmaf(hi[e], f, v[e + 4]);
         }
       }
       if (parts && d == 0) w.sums.ml[to] = float2{top, sum};
-      const float inv = parts ? 1.0f : sum > 0.0f ? 1.0f / sum : 0.0f;
+      const float inv = parts ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= inv;
     }

@@ -177,3 +177,11 @@ def test_division_by_a_product():
         for n in [0, d - 1, d, (1 << 31) - 1] + [k * d + e for k in (1, 2, 7, ((1 << 31) - 1) // d) for e in (-1, 0, 1)] + [rng.randrange(1 << 31) for _ in range(20)]:
             if 0 <= n < 1 << 31:
                 assert n * m >> 31 + shift == n // d, (n, d)
+
+
+def test_more_rows_than_a_join_takes_are_refused():
+    f = _lib.lib().hexmi_paged_attention
+    big = dict(tokens=1 << 22, starts=4096)
+    assert f(c_rows(heads=32), c_batch(**big), 4096, 1, 1.0, _lib.F16, 4096, 1 << 60, None) == _lib.ENOTSUP       # behind a prefix
+    assert _lib.lib().hexmi_paged_attention_workspace(c_batch(**big), 32, 1) == 0
+    assert f(c_rows(heads=32), c_batch(**big), 4096, 1, 1.0, _lib.F16, None, 0, None) == _lib.ENOTSUP

@@ -8,6 +8,7 @@ Tolerances, derived: u = eps / 2 is a rounding to the type, e = 2^-24 one to fp3
            joining of parts by 16 e. fp16 probabilities below 2^-14 of a row's largest are off by 2^-25 of it each. The result: u |o|.
 """
 import math
+import sys
 
 import pytest
 import torch
@@ -550,3 +551,41 @@ def test_a_layer_over_the_cache(hexmi):
         assert got.shape == want.shape and d == n
         rel = (got - want).norm() / want.norm()
         assert rel <= 12 * half_step(dtype), rel
+
+
+@pytest.mark.parametrize("dim", [8, 24])
+def test_joins_read_no_sums_that_nobody_left(hexmi, dim):
+    """More parts than a narrow head has columns, in a workspace full of large numbers: sequences of one token, whose keys several workers
+    share, leave word that the parts of longer runs are empty."""
+    c = Cache([3, 1, 1, 2], [6000, 5000, 4001, 9000], 2, 1, dim, 16, torch.float16, seed=71, shared=4000)
+    ops, lib = sys.modules["hexmi.ops"], sys.modules["hexmi._lib"].lib()
+    batch = ops._paged_batch(c.q.shape[0], c.k_pages, c.v_pages, c.page_table, c.lengths_d, c.starts)
+    need, out = lib.hexmi_paged_attention_workspace(batch, 2, c.shared_pages.numel()), torch.empty_like(c.q)
+    junk = torch.full((need // 4 + 4,), 1e30, device="cuda")
+    assert need > 0
+    assert lib.hexmi_paged_attention(ops._head_rows(c.q, out), batch, c.shared_pages.data_ptr(), c.shared_pages.numel(), 1 / math.sqrt(dim),
+                                     sys.modules["hexmi._lib"].F16, junk.data_ptr(), need, None) == 0
+    torch.cuda.synchronize()
+    c.check(out)
+
+
+@pytest.mark.parametrize("new, context, heads, kv, dim, shared", [
+    ([1], [9000], 8, 2, 128, 0), ([1] * 3, [200, 40, 700], 8, 2, 64, 0), ([1, 1], [5000, 4300], 8, 2, 128, 4096), ([1, 1], [100, 20], 4, 4, 256, 0),
+    ([6, 1, 1], [3000, 5000, 80], 8, 2, 128, 0), ([6, 1, 1], [7000, 5000, 4100], 8, 2, 64, 4096), ([300, 40], [0, 700], 16, 2, 128, 0),
+    ([700, 900], [0, 700], 32, 32, 64, 0), ([70, 200], [500, 0], 4, 1, 256, 0),
+])
+def test_nan_among_a_sequence_s_keys_shows(hexmi, new, context, heads, kv, dim, shared):
+    """A NaN in a key of the first sequence makes NaN of its rows, however its keys are cut up, and of no other sequence's; in a value, of
+    that column."""
+    for where in ("k", "v"):
+        c = Cache(new, context, heads, kv, dim, 16, torch.float16, seed=72, shared=shared)
+        at = c.lengths[0] - new[0] if shared else (c.lengths[0] - new[0]) // 2     # seen by all its new tokens, behind the prefix
+        pages = c.k_pages if where == "k" else c.v_pages
+        pages[c.table[0][at // 16].item(), kv - 1, at % 16, 3] = math.nan
+        got = hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages)
+        mine = got[:new[0], heads - heads // kv:]                                 # the heads of the last key head
+        assert torch.isnan(mine if where == "k" else mine[..., 3]).all(), where
+        got[:new[0], heads - heads // kv:] = 0
+        out, bound = c.attention64()
+        out[:new[0], heads - heads // kv:] = 0
+        assert ((got.cpu().double() - out).abs() <= bound).all(), where
