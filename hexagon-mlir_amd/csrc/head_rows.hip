@@ -291,8 +291,12 @@ void head_rows_kernel(HeadArgs a, Pages p, int waves_per_token) {
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(y[e], y[e], sum);
-        const float mean = fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps), r = __builtin_amdgcn_rsqf(mean);
+        float mean = fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps);
+        const bool tiny = mean < 0x1p-100f;                         // the root's instruction takes no subnormal numbers
+        mean = tiny ? mean * 0x1p60f : mean;
+        const float r = __builtin_amdgcn_rsqf(mean);
         scale = r == 0.0f ? 0.0f : r * fmaf(-0.5f * mean * r, r, 1.5f);          // one Newton step; an infinite mean stays 0
+        scale = tiny ? scale * 0x1p30f : scale;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = y[e] * scale * column(wt, e);
       }

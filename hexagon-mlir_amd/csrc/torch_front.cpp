@@ -362,6 +362,10 @@ bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, hexmi_pag
        static_cast<const int32_t*>(in(lengths)), static_cast<const int32_t*>(in(starts)), lengths->size(0), rows.size(0)};
   return true;
 }
+bool in_storage_of(const void* p, const at::Tensor& t) {
+  const auto* base = static_cast<const char*>(t.storage().data());
+  return p >= base && p < base + t.storage().nbytes();
+}
 PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
   PyObject* x = THPVariable_Wrap(std::move(a));
   PyObject* y = x ? THPVariable_Wrap(std::move(b)) : nullptr;
@@ -424,6 +428,10 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else if (qw) {
       HEXMI_NOT_PLAIN;
     }
+    for (const at::Tensor* t : {k, v, q})                           // rows of the pages themselves: ops.py copies them first
+      for (const void* pages : {batch.k_pages, batch.v_pages})
+        if (t && t->numel() && in_storage_of(pages, *t)) HEXMI_NOT_PLAIN;
+    if (batch.k_pages == batch.v_pages) HEXMI_NOT_PLAIN;
     const Launch at(*k);
     if (!at.ok) HEXMI_NOT_PLAIN;
     const hexmi_head_rows kr = rows_of(k, nullptr, kw), vr = rows_of(v, nullptr, nullptr);
@@ -449,7 +457,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     hexmi_paged_batch batch;
     if (!batch_of(a + 1, *q, D, batch) || H % batch.kv_heads != 0) HEXMI_NOT_PLAIN;
     double scale = 1.0 / std::sqrt((double)D);
-    if ((a[6] != Py_None && !number(a[6], scale)) || !(scale > 0.0 && scale < 3e38)) HEXMI_NOT_PLAIN;
+    if ((a[6] != Py_None && !number(a[6], scale)) || !(scale > 0.0 && scale <= 2e38)) HEXMI_NOT_PLAIN;
     const at::Tensor* shared = nullptr;
     if (a[7] != Py_None && (!(shared = index(a[7], 1, *q)) || shared->size(0) > batch.table_cols)) HEXMI_NOT_PLAIN;
     const Launch at(*q);

@@ -985,9 +985,13 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     table, lens, begin = _paged_operands(name, tokens, k_pages, v_pages, page_table, lengths, starts)
     dev = k_pages.device
     _one_device(name, dev, k, v, q, k_weight, q_weight, inv_freq)
-    kd, vd, qd = _rows_of_heads(k, dev), _rows_of_heads(v, dev), _rows_of_heads(q, dev)
+    if k_pages.data_ptr() == v_pages.data_ptr():
+        raise ValueError("hexmi.paged_append: keys and values need pages of their own")
+    # rows that stand in the pages themselves (one sequence's going to another) are read before any is written
+    kd, vd, qd = (t.clone() if t is not None and t.numel() and _overlaps(t, k_pages, v_pages) else t
+                  for t in (_rows_of_heads(k, dev), _rows_of_heads(v, dev), _rows_of_heads(q, dev)))
     kw, qw, fd = _stage(k_weight, dev), _stage(q_weight, dev), _stage(inv_freq, dev)
-    qo = None if q is None else _rows_out(name, q_out, qd, (kd, vd, kw, qw, fd, table, lens, begin), dev)
+    qo = None if q is None else _rows_out(name, q_out, qd, (kd, vd, kw, qw, fd, table, lens, begin, k_pages, v_pages), dev)
     if tokens:
         args = (kd, vd, k_pages, v_pages, table, lens, begin, kw, fd, float(eps), pairs, qd, qw, qo)
         _run(name, _paged_append_impl, args, *args)
@@ -1020,7 +1024,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
         raise ValueError("hexmi.paged_attention: dim must be a multiple of 8 up to 256")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[2])
-    if not 0 < sm_scale < 3e38:
+    if not 0 < sm_scale <= 2e38:
         raise ValueError("hexmi.paged_attention: sm_scale must be positive")
     if shared_pages is not None and (shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] > page_table.shape[-1]):
         raise ValueError("hexmi.paged_attention: shared_pages must be an int32 tensor of one dimension, no longer than the table is wide")

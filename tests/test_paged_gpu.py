@@ -589,3 +589,35 @@ def test_nan_among_a_sequence_s_keys_shows(hexmi, new, context, heads, kv, dim, 
         out, bound = c.attention64()
         out[:new[0], heads - heads // kv:] = 0
         assert ((got.cpu().double() - out).abs() <= bound).all(), where
+
+
+@pytest.mark.parametrize("dim, offset", [(64, 0), (128, 0), (64, 1)])
+def test_rows_whose_squares_are_subnormal(hexmi, dim, offset):
+    """eps 0 and squares of 1e-40: a square is off by 2^-150 at most, the mean's product by as much, and the root halves that."""
+    g = _gen(73)
+    x = ((1 + torch.rand(1 + 9 * 3 * dim, generator=g)) * 1e-20)[offset:][:9 * 3 * dim].view(9, 3, dim).cuda()
+    w = torch.ones(dim, device="cuda")
+    want, size = rows64(x, w, None, None, 0.0, "adjacent")
+    got = hexmi.qk_norm_rope(x, None, w, eps=0.0).cpu().double()
+    least = x.cpu().double().square().mean(-1).min().item()
+    assert ((got - want).abs() <= (24 * E + 2.0 ** -150 / least) * size).all()
+
+
+def test_append_of_rows_that_stand_in_the_pages(hexmi):
+    """One sequence's keys and values go to another's pages, in the same call as others to theirs; queries land outside the pages."""
+    g = _gen(74)
+    pages = [torch.randn(6, 16, 2, 64, generator=g).half().cuda().transpose(1, 2) for _ in range(2)]
+    before = [p.clone() for p in pages]
+    table = torch.tensor([[1], [2], [3]], dtype=torch.int32, device="cuda")
+    lengths, starts = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([16, 16, 16], [0, 16, 32, 48]))
+    rows = [p.transpose(1, 2).flatten(0, 1)[:48] for p in pages]                  # pages 0, 1, 2: every one but the first read and written
+    assert rows[0].data_ptr() == pages[0].data_ptr()
+    hexmi.paged_append(*rows, *pages, table, lengths, starts)
+    for p, b in zip(pages, before):
+        assert torch.equal(p[1:4], b[:3]) and torch.equal(p[0], b[0]) and torch.equal(p[4:], b[4:])
+    q_out = pages[0].transpose(1, 2).flatten(0, 1)[80:]                           # the last page: kept until the keys are in
+    q = torch.randn(16, 2, 64, generator=g).half().cuda()
+    got = hexmi.paged_append(q, q, *pages, torch.tensor([[4]], dtype=torch.int32, device="cuda"), lengths[:1], starts[:2], q=q, q_out=q_out)
+    assert torch.equal(got, q) and torch.equal(pages[0][4].transpose(0, 1), q) and torch.equal(q_out, q)
+    with pytest.raises(ValueError, match="pages of their own"):
+        hexmi.paged_append(q, q, pages[0], pages[0], table[:1], lengths[:1], starts[:2])
