@@ -1009,7 +1009,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
     through once for all of them; the result is the same without, if the table names them.
 
     A row without any key, and a row of no sequence, is zeros. What the pages hold past a sequence's length is not used, whatever it is;
-    the keys and values of its own positions have to be finite. 16-bit, dim a multiple of 8 up to 256."""
+    the keys and values of its own positions, and of all of the shared pages, have to be finite (a NaN among them reaches any row of the
+    sequence). 16-bit, dim a multiple of 8 up to 256."""
     if out is None and not _THROUGH_DISPATCHER:
         y = _front.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages)
         if y is not None:

@@ -563,7 +563,8 @@ typedef struct hexmi_paged_batch {
  * heads, dim] in one pass, at any positions (int32 or, positions_64, int64
  * [tokens]; may be NULL where columns is 0). k may be NULL. dtype: HEXMI_F16,
  * HEXMI_BF16 or HEXMI_F32. dim up to 512; fastest on 16-byte boundaries with
- * dim a multiple of 8 (other rows take five times as long).
+ * dim a multiple of 8 (other rows take five times as long). out may be x itself,
+ * and shares no memory with anything else that is read.
  * The rotation is rope_kernel of test/python/triton/test_rope.py:97-197, the
  * norm rms_norm_fwd_kernel of test_rms_norm.py:37-63. */
 int hexmi_qk_norm_rope(const hexmi_head_rows *q, const hexmi_head_rows *k,
@@ -575,7 +576,8 @@ int hexmi_qk_norm_rope(const hexmi_head_rows *q, const hexmi_head_rows *k,
  * rotated by their positions on the way (k->out, v->out and v->weight are not
  * used), and, with q, the queries' rows normed and rotated into q->out. A
  * token without a page leaves no key and no value; q->out of a row of no
- * sequence is zeros. Two tokens of one slot: either's. HEXMI_F16, HEXMI_BF16. */
+ * sequence is zeros. Two tokens of one slot: either's. What is read and what is
+ * written share no memory, but for q->x as q->out. HEXMI_F16, HEXMI_BF16. */
 int hexmi_paged_append(const hexmi_head_rows *k, const hexmi_head_rows *v,
                        const hexmi_head_rows *q, const hexmi_rotation *rotation,
                        const hexmi_paged_batch *batch, int dtype,
@@ -586,12 +588,17 @@ int hexmi_paged_append(const hexmi_head_rows *k, const hexmi_head_rows *v,
  * position 0 to the token's own. Keys without a page are left out; a row
  * without any key, and one of no sequence, is zeros. What stands in the pages
  * past a sequence's length is not used, whatever it is (infinities and NaN
- * too); keys and values of its own positions have to be finite.
+ * too). Keys and values of its own positions, and of all of the shared pages,
+ * have to be finite: a NaN among them reaches any row of the sequence (of all
+ * sequences), also those before its position.
  * shared_pages [shared]: positions 0 .. shared * page_size - 1 of every sequence
  * are these pages, and what the table says there is not read: their keys are
  * gone through once for all sequences. 16-bit (HEXMI_F16, HEXMI_BF16), dim a
  * multiple of 8 up to 256, rows of q, out and pages on 16-byte boundaries,
- * heads a multiple of kv_heads, sm_scale > 0; scores, sums and maxima are fp32,
+ * slots of a page in rising order (strides up to 2^26), heads a multiple of
+ * kv_heads, 0 < sm_scale <= 2e38, tokens * heads below 2^31 (2^26 where parts
+ * of the keys are joined: behind shared pages, and few tokens); out may not
+ * share memory with what is read; scores, sums and maxima are fp32,
  * probabilities are rounded to the dtype for the product with v.
  * hexmi_paged_attention_workspace: the bytes of scratch (16-byte aligned, not
  * initialised, no state between calls) that a call takes; 0: none. Two calls

@@ -8,6 +8,7 @@ Tolerances, derived: u = eps / 2 is a rounding to the type, e = 2^-24 one to fp3
            joining of parts by 16 e. fp16 probabilities below 2^-14 of a row's largest are off by 2^-25 of it each. The result: u |o|.
 """
 import math
+import random
 import sys
 
 import pytest
@@ -621,3 +622,34 @@ def test_append_of_rows_that_stand_in_the_pages(hexmi):
     assert torch.equal(got, q) and torch.equal(pages[0][4].transpose(0, 1), q) and torch.equal(q_out, q)
     with pytest.raises(ValueError, match="pages of their own"):
         hexmi.paged_append(q, q, pages[0], pages[0], table[:1], lengths[:1], starts[:2])
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_batches_of_any_kind(hexmi, seed):
+    """Sizes, orders and kinds of batch drawn together."""
+    r = random.Random(seed)
+    kind = ("decode", "mixed", "mixed", "prompts", "singles")[seed % 5]
+    dim, kv, group = r.choice([8, 24, 64, 64, 80, 96, 128, 128, 136, 200, 256]), r.choice([1, 2, 3, 8]), r.choice([1, 2, 4, 5, 7, 16, 17, 33])
+    page, B = r.choice([1, 3, 8, 16, 16, 24, 64, 100, 256]), r.choice([1, 2, 3, 9, 20, 70])
+    shared = r.choice([0, page * r.randint(1, 1 + 600 // page), page * r.randint(1, 1 + 4000 // page)])
+    new = [1 if kind in ("decode", "singles") else r.choice([0, 1, 1, r.randint(1, 90)]) for _ in range(B)] if kind != "prompts" else [
+        r.randint(1, 600 // B + 2) for _ in range(B)]
+    context = [shared] + [shared + r.randint(0, 300) if r.random() < 0.9 else r.randint(0, shared) for _ in range(B - 1)]
+    c = Cache(new, context, kv * group, kv, dim, page, r.choice([torch.float16, torch.bfloat16]), r.choice(["head", "token"]), seed=seed,
+              padding=0 if kind == "decode" else r.choice([0, 3]), ragged=kind != "decode", shared=shared)
+    c.check(hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages), what=(kind, new, context, shared, page, c.heads, kv, dim))
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_rows_of_any_kind(hexmi, seed):
+    r, g = random.Random(seed), _gen(seed)
+    D, H, K, T = r.choice([1, 2, 8, 30, 64, 72, 128, 130, 256, 320, 512]), r.randint(1, 40), r.randint(1, 9), r.choice([1, 2, 17, 300])
+    dtype, pairs, R = r.choice(list(DTYPES.values())), r.choice(["adjacent", "halves"]), 2 * r.randint(0, D // 2)
+    wide = torch.randn(T, (H + K) * D + r.choice([0, 1, 8]), generator=g).to(dtype).cuda()[:, :(H + K) * D].unflatten(1, (H + K, D))
+    q, k = wide[:, :H], wide[:, H:]
+    qw, kw = (torch.randn(D, generator=g).to(dtype).cuda() if r.random() < 0.7 else None for _ in range(2))
+    freq = hexmi.rope_frequencies(R, r.choice([1e4, 5e5])) if R else None
+    pos = torch.randint(0, 1 << 17, (T,), generator=g).cuda()
+    got = hexmi.qk_norm_rope(q, k, qw, kw, freq, pos, 1e-6, pairs)
+    for x, w, y in ((q, qw, got[0]), (k, kw, got[1])):
+        check_rows(y, rows64(x, w, freq, pos, 1e-6, pairs), (D, H, K, T, R, pairs))
