@@ -105,10 +105,18 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   plan.decode = b.starts == nullptr;
   plan.rows = b.tokens * heads;
   const int64_t wide = (rows + WideTile::kRows - 1) / WideTile::kRows * b.kv_heads;
-  plan.deep = !plan.decode && b.dim <= 128 && wide < cus;
+  // Tiles of 64 rows, two groups on the keys, where those of 128 would be fewer than the compute units, and up to half as many again over few
+  // keys: 64 / 128 rows, 32 heads of 128 over 8, us: 100 tokens 9.4 / 10.4, 400 14.9 / 17.4, 8 x 4 behind 1000 .. 3000 24.7 / 27.2, 509 behind
+  // 2046 beside 15 single ones 31 / 49 (alone 46 / 43.5), 1000 26 / 31, 1400 37 / 39.5; but 1800 53 / 50, 32 x 1 .. 300 behind up to 4000
+  // 159 / 144: there what a block's keys are worth in rows counts.
+  plan.deep = !plan.decode && b.dim <= 128 && (wide < cus || (wide < cus * 3 / 2 && own <= 2048));
+  // Sequences of one new token to workers, where some may be: 509 tokens beside 15 single ones 31 us, as tiles 41; the launch with both costs a
+  // batch without any 1.5 (8 x 4 tokens).
   plan.workers = plan.decode || b.sequences > 1 || b.tokens == 1;
   const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
-  const int64_t wanted = 2 * cus, least = plan.deep ? 512 : 256;
+  // Two workgroups a compute unit (three, four: no better), no part below 512 keys, which a join costs: 256 / 512 / 1024, us: 1000 tokens
+  // of 128 columns 37 / 31 / 31, of 256 67 / 60 / 60, 100 behind 1500 - / 22 / 33, 500 behind 3000 of 256 121 / 119 / 136.
+  const int64_t wanted = 2 * cus, least = 512;
   if (shared > 0) {
     plan.prefix_tiles = (int)full;
     plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);

@@ -44,6 +44,28 @@ __device__ __forceinline__ int sequence_of_tile(const Pages& p, int group, int t
   return lo;
 }
 
+// The sequence of a tile, its rows from `first` to `next`, and its length. Where the sequences are a lane each, starts and lengths come in
+// one trip to memory.
+struct Run {
+  int sequence, first, next;
+  int64_t length;
+};
+template <int ROWS>
+__device__ __forceinline__ Run run_of_tile(const Pages& p, int group, int tile, int lane) {
+  Run run;
+  if (p.sequences > 0 && p.sequences <= kWave - 3) {                // lanes of -1 .. sequences + 1
+    const int at = lane - 1, s = p.starts[at < 0 ? 0 : at < p.sequences ? at : p.sequences];
+    const int length = p.lengths[at < 0 ? 0 : at < p.sequences ? at : p.sequences - 1];
+    const int row = at < 0 || s < 0 ? 0 : at > p.sequences || s > p.tokens ? p.tokens : s;
+    const int n = __popcll(__ballot(at <= p.sequences && (at < 0 ? 0 : row * group / ROWS + at + 1) <= tile));      // lane 0 is one
+    run = {n - 2, __builtin_amdgcn_readlane(row, n - 1), __builtin_amdgcn_readlane(row, n), __builtin_amdgcn_readlane(length, n - 1)};
+  } else {
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile<ROWS>(p, group, tile, lane));
+    run = {b, first_row(p, b), first_row(p, b + 1), b >= 0 && b < p.sequences ? p.lengths[b] : 0};
+  }
+  return run;
+}
+
 // keys that token i of a sequence's n sees, whatever the index tensors hold
 __device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
   const int64_t keys = length - n + i + 1;
@@ -88,15 +110,16 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     end = a.prefix;
     table = a.shared;
   } else {
-    const int b = __builtin_amdgcn_readfirstlane(sequence_of_tile<kRows>(p, a.group, tile, lane));
-    token0 = first_row(p, b);
-    new_tokens = first_row(p, b + 1) - token0;
-    row0 = (tile - first_tile<kRows>(p, a.group, b)) * kRows;
+    const Run run = run_of_tile<kRows>(p, a.group, tile, lane);
+    const int b = run.sequence;
+    token0 = run.first;
+    new_tokens = run.next - token0;
+    row0 = (tile - (b < 0 ? 0 : token0 * a.group / kRows + b + 1)) * kRows;
     rows = new_tokens * a.group;                                    // negative where starts fall: nothing
     if (row0 < 0 || row0 >= rows) return;
     none = b < 0 || b >= p.sequences;
     if (w.workers && new_tokens == 1 && !none) return;
-    if (!none) length = p.lengths[b];
+    if (!none) length = run.length;
     const int last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
     end = none ? 0 : keys_of(length, new_tokens, divided(last, a.by_group), most);
     begin = a.prefix;
