@@ -10,7 +10,9 @@ namespace hexmi {
 namespace {
 
 constexpr int kMaxDim = 512;
-constexpr int kWavesWanted = 8192;               // a token's rows are shared by several waves up to so many in all
+// A token's rows are shared by several waves up to so many in all: what the card holds at once, four a SIMD. 2048 / 4096 / 8192, 40 heads of 128
+// bf16, us: 256 tokens 6.1 / 5.7 / 5.7, 1000 10.7 / 10.5 / 13.1, 2000 15.4 / 13.7 / 16.4, 1500 into a cache 19.0 / 14.7 / 17.8.
+constexpr int kWavesWanted = 4096;
 
 // the three kinds of rows, in the order in which they are numbered: queries, keys, values
 struct Kind {
@@ -176,11 +178,12 @@ __device__ __forceinline__ float row_sum(float v) {
 
 // Rows on 16-byte boundaries, dim a multiple of 8. LPR lanes take a row, eight columns each, and the 64 / LPR rows of a wave are of one
 // token: its angles are worked out once and serve every head. The pair of a column is in the same lane (adjacent) or comes out of LDS
-// (halves), in one piece where columns / 2 is a multiple of 8 (PIECES: a lane's columns are all of one half, or none turns). The next rows are asked for before these are worked on.
-// What a launch is bound by: its latency up to a few hundred tokens (4 tokens x 40 heads of 128 4.8 us, 64 tokens into a cache 4.6), then the
+// (halves), in one piece where columns / 2 is a multiple of 8 (PIECES: a lane's columns are all of one half, or none turns). The next rows
+// are asked for before these are worked on.
+// What a launch is bound by: its latency up to a few hundred tokens (4 tokens x 40 heads of 128 4.9 us, 64 tokens into a cache 4.6), then the
 // rows in flight: 8192 tokens x 40 heads of 128 bf16, normed and turned, 40 us (4.2 TB/s; a copy of that size 33). Measured there: an
 // angle worked out by every lane that needs it 50 us, pointers and strides chosen by the lane 62, no row asked for ahead 49, two ahead 42,
-// 16384 waves 46, five waves a SIMD with what spills 44.
+// 16384 waves 46, five waves a SIMD with what spills 44, nontemporal stores 41, and loads 43.
 template <typename T, int LPR, bool HALVES, bool PIECES, bool PAGED>
 __global__ __launch_bounds__(256, 4)
 void head_rows_kernel(HeadArgs a, Pages p, int waves_per_token) {

@@ -7,7 +7,9 @@
 //                  product is free: slot 8 g + 4 t + i is key 16 t + 4 g + i); V passes through a wave's own LDS and is read transposed
 //                  (ds_read_b64_tr_b16).
 // Keys and values of the next 32 are asked for as soon as the registers of these are free, so a wave has 16 KiB (heads of 128) on the way
-// at nearly all times, eight waves a compute unit.
+// at nearly all times, eight waves a compute unit: 16 sequences x 2048 keys x 32 heads of 128 97 us, 5.5 TB/s (a copy reaches 5.1, read and
+// written), 64 of 100 to 16384 over 8 heads 177. Two tiles ahead, twelve waves a compute unit, and rows of keys fetched whole through LDS
+// changed nothing there.
 //
 // The work is cut evenly whatever the lengths are: the blocks of keys of all sequences and key heads, one behind the other,
 // are dealt to the workers (workgroups) in equal runs. A worker that has all of a unit (sequence, key head, 16 query heads) writes

@@ -9,6 +9,12 @@
 //
 // The prefix is one sequence that all rows of the batch attend: its keys go through LDS once for kRows rows, whatever sequences they are
 // of. Its sums, and those of tiles whose keys are cut over several workgroups because there are few, go through the workspace.
+//
+// What bounds it. Prompts of 4 x 4096, 32 heads over 8 of 128, bf16: 587 us, 0.93 PFLOP/s (a matrix product of 8192^3 1.12). Without the
+// copies it takes 432 us, with nothing but them 332: a wave reads all of a block out of LDS for its 32 rows, as many cycles as the matrix
+// instructions take, and two workgroups a compute unit hide that in part. Measured on the way: copies that the compiler knows of (it waits
+// for them before it reads LDS transposed) 609; a lane's own address for every row 687. Few rows are bound by what is one behind the other:
+// launch and look-up about 5 us, 1 to 2 us a block, the join 4 to 5.
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"
@@ -145,8 +151,9 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     return block < block1 && begin + block * kKeys + lane % kKeys < end && entry >= 0 && entry < p.num_pages ? entry : -1;
   };
   // One block into LDS, by copies that the compiler does not know of: it would wait for all of them before it reads LDS transposed, in the
-  // middle of the block before. They are waited for ahead of the barrier that ends that block. Where every key is there and the rows of an instruction share a page, the page, and so the place, is the wave's
-  // (scalar arithmetic), and a lane adds what it is off in it; any other block goes row by row.
+  // middle of the block before. They are waited for ahead of the barrier that ends that block. Where every key is there and the rows of an
+  // instruction share a page, the page, and so the place, is the wave's (scalar arithmetic), and a lane adds what it is off in it; any other
+  // block goes row by row.
   constexpr int kRowsOfOne = kWave / CPR;
   const bool one_page = p.page_size % kRowsOfOne == 0;
   auto column = [&](bool v, int r) __attribute__((always_inline)) {
