@@ -6,7 +6,7 @@ namespace hexmi {
 namespace {
 
 template <typename T, int D, int COLS, bool PADDED, typename Shape>
-__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : 2)
+__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : D == 64 ? 3 : 2)
 void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
   __shared__ __attribute__((aligned(16))) T lds[Shape::lds_elements(D)];
   __shared__ float m_lds[Shape::kGroups][Shape::kRows], l_lds[Shape::kGroups][Shape::kRows];
@@ -114,12 +114,18 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   // batch without any 1.5 (8 x 4 tokens).
   plan.workers = plan.decode || b.sequences > 1 || b.tokens == 1;
   const int64_t tile_rows = plan.deep ? DeepTile::kRows : WideTile::kRows, full = (rows + tile_rows - 1) / tile_rows;
-  // Two workgroups a compute unit (three, four: no better), no part below 512 keys, which a join costs: 256 / 512 / 1024, us: 1000 tokens
-  // of 128 columns 37 / 31 / 31, of 256 67 / 60 / 60, 100 behind 1500 - / 22 / 33, 500 behind 3000 of 256 121 / 119 / 136.
-  const int64_t wanted = 2 * cus, least = 512;
+  // As many workgroups as the card holds at once (heads of 256, one and two a compute unit: 500 behind 3000 101 / 116 us; heads of 64, two and
+  // three: 2 x 700 behind 3000 60 / 51), and no part below 512 keys, which a join costs: 256 / 512 / 1024, us: 1000 tokens of 128 columns
+  // 37 / 31 / 31, of 256 67 / 60 / 60, 100 behind 1500 - / 22 / 33.
+  const int64_t wanted = (b.dim <= 64 ? 3 : b.dim <= 128 ? 2 : 1) * cus, least = 512;
   if (shared > 0) {
+    // Behind a prefix there is a join in any case. Its parts may be of 256 keys in ragged batches (256 / 512: 4 x 20 tokens behind 992
+    // 19 / 28 us, 16 x 1 .. 40 behind 3008 of 64 columns 32 / 30); of 128 in a decode step (128 / 256 / 512, us: 16 sequences behind 1008
+    // 18.6 / 21 / 34, 32 behind 4000 20.3 / 21.1 / 25.7, of 256 columns 28 / 32 / 43), as long as all rows have 16384 sets of sums to
+    // join at most: 32 x 32 heads behind 8192 in 16 parts 27, in 31 29; 64 x 32 heads behind 2000 in 8 28, in 15 30.
+    const int64_t rows_there = plan.rows > 0 ? plan.rows : 1, sets = 16384 / rows_there;
     plan.prefix_tiles = (int)full;
-    plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, least, plan.decode ? 31 : 16);
+    plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, plan.decode ? 128 : 256, plan.decode ? (sets < 31 ? sets : 31) : 16);
   }
   if (plan.workers) {
     plan.one = plan_paged_decode(b, heads, prefix);

@@ -29,7 +29,7 @@ template <int KEYS, int ROW_WAVES, int GROUPS> struct TileShape {
   static constexpr int lds_elements(int d) { return GROUPS * 4 * KEYS * d; }
   static_assert(4 * KEYS * 2 == kRows * 4, "a group's sums take the place of its blocks");
 };
-typedef TileShape<64, 4, 1> WideTile;          // many tiles: 128 rows, two workgroups a compute unit
+typedef TileShape<64, 4, 1> WideTile;          // many tiles: 128 rows; two workgroups a compute unit (heads of 64 three)
 typedef TileShape<32, 2, 2> DeepTile;          // few: 64 rows, the chain of a tile's keys half as long
 
 // The tiles of a key head: those of sequence b are numbered from first_tile(b) on, b = -1 .. sequences (first_row).
