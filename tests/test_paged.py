@@ -185,3 +185,10 @@ def test_more_rows_than_a_join_takes_are_refused():
     assert f(c_rows(heads=32), c_batch(**big), 4096, 1, 1.0, _lib.F16, 4096, 1 << 60, None) == _lib.ENOTSUP       # behind a prefix
     assert _lib.lib().hexmi_paged_attention_workspace(c_batch(**big), 32, 1) == 0
     assert f(c_rows(heads=32), c_batch(**big), 4096, 1, 1.0, _lib.F16, None, 0, None) == _lib.ENOTSUP
+
+
+@pytest.mark.parametrize("slot", [-64, (1 << 26) + 8])
+@pytest.mark.parametrize("which", ["k_slot", "v_slot"])
+def test_slots_that_32_bit_offsets_do_not_reach_are_refused(which, slot):
+    f = _lib.lib().hexmi_paged_attention
+    assert f(c_rows(heads=4), c_batch(**{which: slot}), None, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
