@@ -75,6 +75,26 @@ __device__ __forceinline__ int length_of(const Pages& p, int b) {
 }
 #endif
 
+// How attention holds a head: D columns of a row in LDS, COLS <= D of them multiplied (a multiple of 32), PADDED: the head is narrower than COLS.
+template <int D_, int COLS_, bool PADDED_> struct HeadWidth {
+  static constexpr int D = D_, COLS = COLS_;
+  static constexpr bool PADDED = PADDED_;
+};
+template <int D, int COLS, typename F> int with_columns(int64_t dim, F&& f) {
+  return dim == COLS ? f(HeadWidth<D, COLS, false>{}) : f(HeadWidth<D, COLS, true>{});
+}
+// f of the width that heads of dim columns go by, up to MOST (128 or 256)
+template <int MOST, typename F> int with_width(int64_t dim, F&& f) {
+  if (dim <= 64) return with_columns<64, 64>(dim, f);
+  if (dim <= 96) return with_columns<128, 96>(dim, f);
+  if constexpr (MOST == 128) return with_columns<128, 128>(dim, f);
+  else return dim <= 128 ? with_columns<128, 128>(dim, f) : with_columns<256, 256>(dim, f);
+}
+// The first of the eight columns that a tile copies to where columns c .. c + 7 of an LDS row stand. The row is wider than the head where
+// the head is padded, and where fewer columns than the row's are multiplied (heads of 96): what stands behind the head there is no part
+// of it, and nobody multiplies it or stores what comes of it, so the head's first columns are copied.
+template <int D, int COLS, bool PADDED> constexpr int copied_column(int c, int dim) { return (PADDED || COLS < D) && c >= dim ? 0 : c; }
+
 // What attention over the pages takes beside them (paged_attn.hip, paged_decode.hip).
 struct PagedAttnArgs {
   const void *q, *k, *v;

@@ -1,5 +1,6 @@
 // Attention over a paged cache of keys and values (fp16 / bf16): runs of new tokens of many sequences over the positions before them, and
 // the prefix that all sequences share: what a call launches, the tiles of ragged batches (paged_tile.h) and the join of their sums.
+#include "hexmi_calibrate.h"
 #include "paged_tile.h"
 
 namespace hexmi {
@@ -63,23 +64,14 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
 template <typename T>
 int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipStream_t s) {
   const unsigned grid = (unsigned)(((int64_t)w.tiles * w.splits + (int64_t)w.shared_tiles * w.shared_splits) * p.kv_heads);
-#define HEXMI_PAGED_TILE(D, COLS, Shape)                                                                                                  \
-  do {                                                                                                                                    \
-    if (a.dim == COLS) hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, false, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w); \
-    else hipLaunchKernelGGL((paged_tile_kernel<T, D, COLS, true, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);              \
-  } while (0)
-  if (w.deep) {
-    if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, DeepTile);
-    else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, DeepTile);
-    else HEXMI_PAGED_TILE(128, 128, DeepTile);
-  } else {
-    if (a.dim <= 64) HEXMI_PAGED_TILE(64, 64, WideTile);
-    else if (a.dim <= 96) HEXMI_PAGED_TILE(128, 96, WideTile);
-    else if (a.dim <= 128) HEXMI_PAGED_TILE(128, 128, WideTile);
-    else HEXMI_PAGED_TILE(256, 256, WideTile);
-  }
-#undef HEXMI_PAGED_TILE
-  return launch_status();
+  auto launch = [&](auto width, auto shape) {
+    typedef decltype(width) W;
+    typedef decltype(shape) Shape;
+    hipLaunchKernelGGL((paged_tile_kernel<T, W::D, W::COLS, W::PADDED, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);
+    return launch_status();
+  };
+  return w.deep ? with_width<128>(a.dim, [&](auto width) { return launch(width, DeepTile{}); })
+                : with_width<256>(a.dim, [&](auto width) { return launch(width, WideTile{}); });
 }
 
 // What a call launches: the prefix's tiles (prefix_splits 0: none), then one token a sequence (decode) or tiles of the sequences' own keys
@@ -204,4 +196,12 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   if (dtype == HEXMI_F16) hipLaunchKernelGGL((paged_join_kernel<f16>), dim3(blocks), dim3(256), 0, s, a, sums);
   else hipLaunchKernelGGL((paged_join_kernel<bf16>), dim3(blocks), dim3(256), 0, s, a, sums);
   return launch_status();
+}
+
+extern "C" int hexmi_paged_tile_column(int64_t dim, int64_t chunk) {
+  if (dim < 8 || dim > 256 || dim % 8 != 0 || chunk < 0) return -1;
+  return with_width<256>(dim, [&](auto width) {
+    typedef decltype(width) W;
+    return chunk < W::D / 8 ? copied_column<W::D, W::COLS, W::PADDED>((int)chunk * 8, (int)dim) : -1;
+  });
 }

@@ -135,8 +135,8 @@ __device__ __forceinline__ void keep_sums(const DecodeArgs& w, int64_t row, int 
   for (int x = w.own + 1; x < w.sums.slots; ++x) w.sums.ml[x * w.sums.rows + row] = float2{-INFINITY, 0.0f};
 }
 
-// D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
-// columns lie past the head reads the head's first ones instead: the query has zeros there, and what comes of V there is not stored.
+// D, COLS, PADDED: HeadWidth. A lane whose columns lie past the head reads the head's first ones instead: the query has zeros there, and what
+// comes of V there is not stored.
 // worker: of w.workers, or the unit where that is 0.
 template <typename T, int D, int COLS, bool PADDED, int W>
 __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned worker, char* lds,

@@ -133,17 +133,11 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
     hipLaunchKernelGGL((paged_decode_join_kernel<T>), joins, dim3(256), 0, s, a, p, w);
     return launch_status();
   }
-#define HEXMI_PAGED_DECODE(D, COLS)                                                                                                      \
-  do {                                                                                                                                   \
-    if (a.dim == COLS) hipLaunchKernelGGL((paged_decode_kernel<T, D, COLS, false>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);    \
-    else hipLaunchKernelGGL((paged_decode_kernel<T, D, COLS, true>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);                   \
-  } while (0)
-  if (a.dim <= 64) HEXMI_PAGED_DECODE(64, 64);
-  else if (a.dim <= 96) HEXMI_PAGED_DECODE(128, 96);
-  else if (a.dim <= 128) HEXMI_PAGED_DECODE(128, 128);
-  else HEXMI_PAGED_DECODE(256, 256);
-#undef HEXMI_PAGED_DECODE
-  const int rc = launch_status();
+  const int rc = with_width<256>(a.dim, [&](auto width) {
+    typedef decltype(width) W;
+    hipLaunchKernelGGL((paged_decode_kernel<T, W::D, W::COLS, W::PADDED>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);
+    return launch_status();
+  });
   if (rc != HEXMI_OK || plan.workers < 2) return rc;
   hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
   return launch_status();

@@ -28,27 +28,15 @@ template <typename T>
 int launch(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned workers, hipStream_t s) {
   const unsigned tile_grid = (unsigned)(((int64_t)tiles.shared_tiles * tiles.shared_splits + (int64_t)tiles.tiles * tiles.splits) * p.kv_heads);
   const unsigned grid = tile_grid + workers;
-#define HEXMI_PAGED_SHARED(D, COLS, Shape)                                                                                               \
-  do {                                                                                                                                   \
-    if (a.dim == COLS)                                                                                                                   \
-      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, false, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, tiles, w,  \
-                         tile_grid);                                                                                                     \
-    else                                                                                                                                 \
-      hipLaunchKernelGGL((paged_shared_decode_kernel<T, D, COLS, true, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, tiles, w,   \
-                         tile_grid);                                                                                                     \
-  } while (0)
-  if (tiles.deep) {
-    if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, DeepTile);
-    else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, DeepTile);
-    else HEXMI_PAGED_SHARED(128, 128, DeepTile);
-  } else {
-    if (a.dim <= 64) HEXMI_PAGED_SHARED(64, 64, WideTile);
-    else if (a.dim <= 96) HEXMI_PAGED_SHARED(128, 96, WideTile);
-    else if (a.dim <= 128) HEXMI_PAGED_SHARED(128, 128, WideTile);
-    else HEXMI_PAGED_SHARED(256, 256, WideTile);
-  }
-#undef HEXMI_PAGED_SHARED
-  return launch_status();
+  auto launch = [&](auto width, auto shape) {
+    typedef decltype(width) W;
+    typedef decltype(shape) Shape;
+    hipLaunchKernelGGL((paged_shared_decode_kernel<T, W::D, W::COLS, W::PADDED, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, tiles,
+                       w, tile_grid);
+    return launch_status();
+  };
+  return tiles.deep ? with_width<128>(a.dim, [&](auto width) { return launch(width, DeepTile{}); })
+                    : with_width<256>(a.dim, [&](auto width) { return launch(width, WideTile{}); });
 }
 
 }  // namespace

@@ -78,8 +78,8 @@ __device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
   return keys < 0 ? 0 : keys < most ? (int)keys : most;
 }
 
-// D: columns of a row in LDS; COLS <= D, a multiple of 32: columns that are multiplied; PADDED: a head is narrower than COLS. A lane whose
-// columns lie past the head copies the head's first ones instead: the query has zeros there, and what comes of V there is not stored.
+// D, COLS, PADDED: HeadWidth. A lane whose columns lie past the head copies the head's first ones instead (copied_column): the query has
+// zeros there or they are not multiplied, and what comes of V there is not stored.
 // A workgroup's tile: number block_id of a launch whose tiles are `grid` workgroups; lds: Shape::lds_elements(D); m_lds, l_lds: of every
 // group's rows.
 template <typename T, int D, int COLS, bool PADDED, typename Shape>
@@ -158,7 +158,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   const bool one_page = p.page_size % kRowsOfOne == 0;
   auto column = [&](bool v, int r) __attribute__((always_inline)) {
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
-    return PADDED && c >= dim ? 0 : c;
+    return copied_column<D, COLS, PADDED>(c, dim);
   };
   auto copy = [&](int block, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {

@@ -105,6 +105,7 @@ PROBE_SIGNATURES = {
     "hexmi_lds_read_pattern": (_int, [_int, _i64, _ptr, _ptr]),
     "hexmi_l2_stream": (_int, [_int, _int, _i64, _i64, _ptr, _ptr, _ptr]),
     "hexmi_gemm_w8a16_kernel": (_int, [_i64, _i64, _i64, _int, _int]),
+    "hexmi_paged_tile_column": (_int, [_i64, _i64]),
 }
 
 _lib = None

@@ -38,6 +38,12 @@ extern "C" {
 int hexmi_gemm_w8a16_kernel(int64_t M, int64_t N, int64_t K, int zero_points,
                             int per_tensor);
 
+/* Which columns of a key or value hexmi_paged_attention's tiles copy into 16-byte
+ * chunk `chunk` of its row in LDS, for heads of dim columns: the first of eight,
+ * all of them the head's. A row's chunks may be more than the head's. -1: a row
+ * has no such chunk, or dim is refused. No device is asked. */
+int hexmi_paged_tile_column(int64_t dim, int64_t chunk);
+
 /* A stream of nothing but MFMAs (operands and accumulators in registers, no
  * memory traffic): what the matrix cores of this GPU sustain for one
  * instruction shape on operands of the caller's choice. It has no counterpart

@@ -192,3 +192,16 @@ def test_more_rows_than_a_join_takes_are_refused():
 def test_slots_that_32_bit_offsets_do_not_reach_are_refused(which, slot):
     f = _lib.lib().hexmi_paged_attention
     assert f(c_rows(heads=4), c_batch(**{which: slot}), None, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
+
+
+@pytest.mark.parametrize("dim", range(8, 257, 8))
+def test_tiles_copy_no_columns_past_a_head(dim):
+    """What a tile copies of a key's row stands within the row, whatever the LDS row is wide: behind the last row of the pages there is
+    nothing."""
+    column = _lib.lib().hexmi_paged_tile_column
+    chunks = [column(dim, c) for c in range(40)]
+    row = chunks.index(-1)
+    assert set(chunks[row:]) == {-1} and row * 8 >= dim
+    assert chunks[:dim // 8] == list(range(0, dim, 8))                # the head's own chunks hold its own columns
+    assert all(0 <= c and c + 8 <= dim for c in chunks[:row])
+    assert all(column(d, 0) == -1 for d in (0, -8, dim + 1, 264)) and column(dim, -1) == -1
