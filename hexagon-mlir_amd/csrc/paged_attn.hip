@@ -147,6 +147,7 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   const int64_t blocks = (b.table_cols * b.page_size + 127) / 128 + 1;
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
+  if (b.tokens == 0) return HEXMI_OK;          // nothing to launch: there is no plan of it (plan_of divides by the tiles)
   const Plan plan = plan_of(b, heads, shared);
   if (plan.slots() > 0 && plan.rows > limit / 32) return HEXMI_ENOTSUP;         // 32 threads a row join them
   const int64_t workers = b.sequences > limit / 1024 / units ? limit : b.sequences * units;

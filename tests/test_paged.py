@@ -205,3 +205,16 @@ def test_tiles_copy_no_columns_past_a_head(dim):
     assert chunks[:dim // 8] == list(range(0, dim, 8))                # the head's own chunks hold its own columns
     assert all(0 <= c and c + 8 <= dim for c in chunks[:row])
     assert all(column(d, 0) == -1 for d in (0, -8, dim + 1, 264)) and column(dim, -1) == -1
+
+
+@pytest.mark.parametrize("sequences", [0, 1, 2, 70])
+@pytest.mark.parametrize("shared", [0, 1])
+@pytest.mark.parametrize("starts", [None, 4096])
+def test_a_batch_without_new_tokens_is_nothing(sequences, shared, starts):
+    """A step in which no sequence has a new token: no workspace, and nothing is launched."""
+    lib = _lib.lib()
+    b = c_batch(tokens=0, sequences=sequences if starts else 0, starts=starts)
+    assert lib.hexmi_paged_attention_workspace(b, 4, shared) == 0
+    assert lib.hexmi_paged_attention(c_rows(heads=4), b, 4096, shared, 1.0, _lib.F16, None, 0, None) == _lib.OK
+    assert lib.hexmi_paged_append(c_rows(), c_rows(), c_rows(heads=4), _lib.Rotation(**TURN), b, _lib.F16, None) == _lib.OK
+    assert lib.hexmi_paged_attention(c_rows(heads=3), b, 4096, shared, 1.0, _lib.F16, None, 0, None) == _lib.EINVAL      # refused as any other

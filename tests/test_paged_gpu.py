@@ -653,3 +653,15 @@ def test_rows_of_any_kind(hexmi, seed):
     got = hexmi.qk_norm_rope(q, k, qw, kw, freq, pos, 1e-6, pairs)
     for x, w, y in ((q, qw, got[0]), (k, kw, got[1])):
         check_rows(y, rows64(x, w, freq, pos, 1e-6, pairs), (D, H, K, T, R, pairs))
+
+
+def test_a_step_without_new_tokens(hexmi):
+    """Sequences, and no new token of any: nothing is computed, through the operator and through the registered one."""
+    c = Cache([0, 0, 0], [70, 0, 5], 4, 2, 64, 16, torch.float16, seed=75, ragged=True, shared=0)
+    before, k = c.k_pages.clone(), torch.empty(0, 2, 64, dtype=torch.float16, device="cuda")
+    out = torch.empty_like(c.q)
+    assert c.q.shape[0] == 0 and hexmi.paged_attention(c.q, *c.batch()).shape == c.q.shape
+    torch.ops.hexmi.paged_attention(c.q, *c.batch(), 0.125, None, out)
+    hexmi.paged_append(k, k, *c.batch())
+    torch.cuda.synchronize()
+    assert torch.equal(c.k_pages.view(torch.int16), before.view(torch.int16))
