@@ -57,7 +57,7 @@ __device__ __forceinline__ Place place_of(const HeadArgs& a, const Pages& p, int
       b = sequence_of(p, t, lane);
       at.none = b < 0;
       if (at.none) return at;
-      behind = p.starts[b + 1] - t;
+      behind = first_row(p, b + 1) - t;
     }
     const int64_t position = (int64_t)p.lengths[b] - behind;
     at.position = position;

@@ -61,7 +61,7 @@ __device__ __forceinline__ int sequence_of(const Pages& p, int t, int lane) {
 }
 
 // The rows of sequence b, from the first of them to the first of b + 1: -1 and `sequences` are the rows of no sequence before the first and
-// behind the last; all within the operands, whatever starts holds.
+// behind the last; all within the operands, whatever starts holds. A sequence's end, and so its tokens' positions, go by this everywhere.
 __device__ __forceinline__ int first_row(const Pages& p, int b) {
   const int s = b < 0 ? 0 : b > p.sequences ? p.tokens : p.starts ? p.starts[b] : b;
   return s < 0 ? 0 : s < p.tokens ? s : p.tokens;

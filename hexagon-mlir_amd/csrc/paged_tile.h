@@ -233,7 +233,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       }
       s = lo < p.sequences && p.starts[lo] <= token ? lo : -1;
     }
-    if (live && s >= 0) keys = keys_of(p.lengths[s], p.starts ? p.starts[s + 1] - token : 1, 0, most);
+    if (live && s >= 0) keys = keys_of(p.lengths[s], first_row(p, s + 1) - token, 0, most);
     keys = keys < a.prefix ? keys : a.prefix;
   } else if (live && !none) {
     keys = keys_of(length, new_tokens, in_seq, most);

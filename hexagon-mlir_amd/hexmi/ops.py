@@ -960,8 +960,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     k_pages, v_pages [pages, kv heads, page size, dim] are changed in place (any strides: a cache that keeps the heads of a token side by
     side is a transposed view). page_table int32 [sequences, columns]: the pages of each sequence; an entry that is no page's number (-1,
     say) is none, and a token there is left out. lengths int32 [sequences]: the positions of each sequence, the new tokens included, which
-    are its last. starts int32 [sequences + 1]: sequence b's tokens are the rows starts[b] .. starts[b + 1] - 1; rows of no sequence
-    (padding behind the last) leave nothing, and zeros in q's result. None: one token a sequence. What the index tensors hold is
+    are its last. starts int32 [sequences + 1]: sequence b's tokens are the rows starts[b] .. starts[b + 1] - 1 (of those
+    that there are); rows of no sequence (padding behind the last) leave nothing, and zeros in q's result. None: one token a sequence. What the index tensors hold is
     read on the GPU only, so the call can be captured into a graph and replayed as they change."""
     if q_out is None and not _THROUGH_DISPATCHER:
         y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight)

@@ -543,9 +543,10 @@ typedef struct hexmi_rotation {
  * outside 0 .. num_pages - 1 is no page. lengths [sequences]: the positions of
  * each sequence, new tokens included. starts [sequences + 1] (not falling), or
  * NULL for one new token each: the new tokens of sequence b are the rows
- * starts[b] .. starts[b + 1] - 1 of the operands, at its last positions. A row
- * below starts[0] or from starts[sequences] on belongs to no sequence; without
- * starts, tokens == sequences. Positions past the table's columns have no page.
+ * starts[b] .. starts[b + 1] - 1 of the operands, at its last positions; a value
+ * below 0 or above tokens is taken as that. A row below starts[0] or from
+ * starts[sequences] on belongs to no sequence; without starts, tokens ==
+ * sequences. Positions past the table's columns have no page.
  * The index arrays are read by the kernels and not checked on the host:
  * whatever they hold, nothing outside the operands is touched. */
 typedef struct hexmi_paged_batch {

@@ -665,3 +665,24 @@ def test_a_step_without_new_tokens(hexmi):
     hexmi.paged_append(k, k, *c.batch())
     torch.cuda.synchronize()
     assert torch.equal(c.k_pages.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("new", [[3, 9], [3, 8, 1], [2] * 70])
+def test_starts_past_the_rows_there_are(hexmi, new):
+    """starts that begin below the first row and end behind the last: a sequence's new tokens are those of its rows that there are, at
+    its last positions, for what is appended, behind a prefix and without one alike."""
+    prefix, T = 64, sum(new)
+    c = Cache(new, [prefix + 1] * len(new), 4, 2, 64, 16, torch.float16, seed=76, ragged=True, shared=prefix)
+    whole = c.starts
+    beyond = whole.clone()
+    beyond[0], beyond[-1] = -4, T + 30
+    k, freq = torch.randn(T, 2, 64, generator=_gen(77)).half().cuda(), hexmi.rope_frequencies(64)
+    results = []
+    for starts in (whole, beyond):
+        pages = c.k_pages.clone(), c.v_pages.clone()
+        q = hexmi.paged_append(k, k, *pages, c.page_table, c.lengths_d, starts, inv_freq=freq, q=c.q)
+        results.append([q] + [p.view(torch.int16) for p in pages])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    c.starts = beyond
+    c.check(hexmi.paged_attention(c.q, *c.batch()), what="each for itself")
+    c.check(hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages), what="shared")
