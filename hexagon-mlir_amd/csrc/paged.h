@@ -95,6 +95,13 @@ template <int MOST, typename F> int with_width(int64_t dim, F&& f) {
 // of it, and nobody multiplies it or stores what comes of it, so the head's first columns are copied.
 template <int D, int COLS, bool PADDED> constexpr int copied_column(int c, int dim) { return (PADDED || COLS < D) && c >= dim ? 0 : c; }
 
+// How far (log2) the reference of a softmax stands below the largest score when it is set: probabilities, which go to the matrix cores
+// rounded to T, are 2^kLift there, and up to 2^(kLift + kRescaleLag) before it is set again. fp16 has no more than 2^-24 below 1, so without
+// it a key of 2^-25 of the largest one's weight was nothing, and 2^17 of them with it; 2^15 is as far as fp16 goes, and the step is 2^-31 of the
+// largest weight so. bf16 has the exponents of fp32.
+template <typename T> constexpr float kLift = 0.0f;
+template <> inline constexpr float kLift<f16> = 7.0f;
+
 // What attention over the pages takes beside them (paged_attn.hip, paged_decode.hip).
 struct PagedAttnArgs {
   const void *q, *k, *v;

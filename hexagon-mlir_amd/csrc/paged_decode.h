@@ -277,12 +277,12 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         __builtin_amdgcn_sched_barrier(0);
         load(next, key0 + kBlock, v_head, p.v_page, p.v_slot, vr);
         __builtin_amdgcn_sched_barrier(0);
-        // online softmax, the reference maximum up to kRescaleLag behind the true one (flash_attn.hip)
+        // online softmax, the reference up to kRescaleLag further behind the true maximum than it was set (flash_attn.hip)
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = max_of_quarters(mx) * a.scale;
-        const bool grow = mx > m + kRescaleLag;
+        const bool grow = mx > m + (kLift<T> + kRescaleLag);
         if (__ballot(grow) != 0) {
-          const float m_new = grow ? mx : m, alpha = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+          const float m_new = grow ? mx - kLift<T> : m, alpha = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
           l *= alpha;
           m = m_new;
 #pragma unroll
@@ -295,7 +295,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
 #pragma unroll
         for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.scale, neg_m));
         const Frag pf = MfmaT<T>::pack(pr);
-        l = MfmaT<T>::sum8(pf, l);                                   // the sum of what the product multiplies
+        l += MfmaT<T>::sum8(pf, 0.0f);                               // the sum of what the product multiplies (these keys' first, paged_tile.h)
         asm volatile("" ::: "memory");                               // the reads below stay behind the writes above (LDS is in order)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {

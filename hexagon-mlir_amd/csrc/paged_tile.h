@@ -327,9 +327,9 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     for (int r = 0; r < 16; ++r) mx1 = fmaxf(mx1, s[JT - 1][r]);
     mx = fmaxf(mx, mx1);
     mx = fmaxf(mx, other_half(mx)) * a.scale;
-    const bool grow = mx > m_i + kRescaleLag;                       // the reference maximum may lag (flash_attn.hip)
+    const bool grow = mx > m_i + (kLift<T> + kRescaleLag);          // the reference may lag (flash_attn.hip)
     if (__ballot(grow) != 0) {
-      const float m_new = grow ? mx : m_i, alpha = grow ? __builtin_amdgcn_exp2f(m_i - m_new) : 1.0f;
+      const float m_new = grow ? mx - kLift<T> : m_i, alpha = grow ? __builtin_amdgcn_exp2f(m_i - m_new) : 1.0f;
       l_i *= alpha;
       m_i = m_new;
 #pragma unroll
@@ -345,7 +345,8 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(fmaf(t[r], a.scale, neg_m));
       pf[0] = MfmaT<T>::pack(&pr[0]);
       pf[1] = MfmaT<T>::pack(&pr[8]);
-      l_i = MfmaT<T>::sum8(pf[1], MfmaT<T>::sum8(pf[0], l_i));      // the sum of what the product multiplies
+      l_i += MfmaT<T>::sum8(pf[1], MfmaT<T>::sum8(pf[0], 0.0f));    // the sum of what the product multiplies, these keys' first: two at a
+                                                                    // time to a sum 2^25 times as large are nothing
     };
     auto pv = [&](int jt, const VFrags& vf) __attribute__((always_inline)) {
 #pragma unroll

@@ -600,7 +600,8 @@ int hexmi_paged_append(const hexmi_head_rows *k, const hexmi_head_rows *v,
  * kv_heads, 0 < sm_scale <= 2e38, tokens * heads below 2^31 (2^26 where parts
  * of the keys are joined: behind shared pages, and few tokens); out may not
  * share memory with what is read; scores, sums and maxima are fp32,
- * probabilities are rounded to the dtype for the product with v.
+ * probabilities are rounded to the dtype for the product with v (in fp16 to
+ * no coarser steps than 2^-31 of a row's largest).
  * hexmi_paged_attention_workspace: the bytes of scratch (16-byte aligned, not
  * initialised, no state between calls) that a call takes; 0: none. Two calls
  * that overlap in time need one each. */

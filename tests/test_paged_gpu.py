@@ -686,3 +686,27 @@ def test_starts_past_the_rows_there_are(hexmi, new):
     c.starts = beyond
     c.check(hexmi.paged_attention(c.q, *c.batch()), what="each for itself")
     c.check(hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages), what="shared")
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("new, shared", [(2048, 0), (1, 0), (20, 1 << 16)])
+def test_many_keys_far_below_one(hexmi, dt, new, shared):
+    """A key that all rows see first and 2^17 others of 2^-26 of its weight each: together they have 2^-9 of it. Column 0 is what comes of them
+    alone (their values are 1 there, the first's is 0), column 1 the first key's.
+    fp16 weights have steps of 2^-24 where the largest is 2^7 and more, so each is off by at most 2^-32 of it, and all by 2^17 times that. The
+    weights are powers of two, and sums of 8 and more of them whole steps of the sum that they are added to; beyond that the result's
+    rounding, and for the quotient and the order of sums in parts (2 u + 2^17 E) of what the others come to, 2^-9."""
+    dtype, L, dim, page, heads = DTYPES[dt], 1 << 17, 64, 256, 64
+    k, v = (torch.zeros(L // page, 1, page, dim, dtype=dtype, device="cuda") for _ in range(2))
+    q = torch.zeros(new, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0], k[0, 0, 0, 0] = 2.0, 13.0                             # 26 in log2 with this scale; the others' scores are 0
+    v[..., 0], v[0, 0, 0, 0], v[0, 0, 0, 1] = 1.0, 0.0, 1.0
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda")[None]
+    starts = None if new == 1 else torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    got = hexmi.paged_attention(q, k, v, table, torch.tensor([L], dtype=torch.int32, device="cuda"), starts, sm_scale=math.log(2.0),
+                                shared_pages=table[0, :shared // page] if shared else None).cpu().double()
+    others = torch.arange(L - new, L, dtype=torch.float64)[:, None] * 2.0 ** -26
+    u = half_step(dtype)
+    bound = L * 2.0 ** -32 + (2 * u + L * E) * 2.0 ** -9
+    assert (got[..., 0] - others / (1 + others)).abs().max() <= bound
+    assert (got[..., 1] - 1 / (1 + others)).abs().max() <= bound + u and (got[..., 2:] == 0).all()
