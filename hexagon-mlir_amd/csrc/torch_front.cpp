@@ -343,8 +343,8 @@ const at::Tensor* index(PyObject* o, int64_t dims, const at::Tensor& like) {
   const at::Tensor* t = contiguous(o);
   return t && t->dim() == dims && t->scalar_type() == at::kInt && t->device() == like.device() ? t : nullptr;
 }
-// k_pages, v_pages, page_table, lengths, starts or None
-bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, hexmi_paged_batch& b) {
+// k_pages, v_pages, page_table, lengths, starts or None. written: whether the pages are, and not only read
+bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, bool written, hexmi_paged_batch& b) {
   const at::Tensor *k = dense(a[0]), *v = k ? dense(a[1]) : nullptr;
   if (!v || k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != rows.scalar_type() || v->scalar_type() != k->scalar_type() ||
       k->device() != rows.device() || v->device() != k->device() || k->size(3) != dim || k->stride(3) != 1 || v->stride(3) != 1)
@@ -357,7 +357,8 @@ bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, hexmi_pag
   } else if (lengths->size(0) != rows.size(0)) {
     return false;
   }
-  b = {k->mutable_data_ptr(), v->mutable_data_ptr(), stride(*k, 0), stride(*k, 1), stride(*k, 2), stride(*v, 0), stride(*v, 1), stride(*v, 2),
+  auto pages = [&](const at::Tensor* t) { return written ? t->mutable_data_ptr() : const_cast<void*>(in(t)); };
+  b = {pages(k), pages(v), stride(*k, 0), stride(*k, 1), stride(*k, 2), stride(*v, 0), stride(*v, 1), stride(*v, 2),
        k->size(0), k->size(2), k->size(1), dim, static_cast<const int32_t*>(in(table)), table->size(1), table->size(1),
        static_cast<const int32_t*>(in(lengths)), static_cast<const int32_t*>(in(starts)), lengths->size(0), rows.size(0)};
   return true;
@@ -419,7 +420,7 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *v = head_rows(a[1], type), *q = nullptr, *kw, *qw;
     hexmi_paged_batch batch;
     hexmi_rotation turn;
-    if (!v || v->sizes() != k->sizes() || v->device() != k->device() || !batch_of(a + 2, *k, D, batch) || batch.kv_heads != k->size(1) ||
+    if (!v || v->sizes() != k->sizes() || v->device() != k->device() || !batch_of(a + 2, *k, D, true, batch) || batch.kv_heads != k->size(1) ||
         !optional(a[7], kw, {D}, type, *k) || !rotation_of(a[8], a[9], a[10], *k, D, turn) || !optional(a[12], qw, {D}, type, *k))
       HEXMI_NOT_PLAIN;
     if (a[11] != Py_None) {
@@ -455,7 +456,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t H = q->size(1), D = q->size(2);
     if (D % 8 != 0 || D > 256 || stride(*q, 0) % 8 != 0 || stride(*q, 1) % 8 != 0 || reinterpret_cast<uintptr_t>(in(q)) % 16 != 0) HEXMI_NOT_PLAIN;
     hexmi_paged_batch batch;
-    if (!batch_of(a + 1, *q, D, batch) || H % batch.kv_heads != 0) HEXMI_NOT_PLAIN;
+    if (!batch_of(a + 1, *q, D, false, batch) || H % batch.kv_heads != 0) HEXMI_NOT_PLAIN;
     double scale = 1.0 / std::sqrt((double)D);
     if ((a[6] != Py_None && !number(a[6], scale)) || !(scale > 0.0 && scale <= 2e38)) HEXMI_NOT_PLAIN;
     const at::Tensor* shared = nullptr;

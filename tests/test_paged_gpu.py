@@ -710,3 +710,20 @@ def test_many_keys_far_below_one(hexmi, dt, new, shared):
     bound = L * 2.0 ** -32 + (2 * u + L * E) * 2.0 ** -9
     assert (got[..., 0] - others / (1 + others)).abs().max() <= bound
     assert (got[..., 1] - 1 / (1 + others)).abs().max() <= bound + u and (got[..., 2:] == 0).all()
+
+
+@pytest.mark.parametrize("new, shared", [([1, 1], 0), ([5, 30], 0), ([1, 1], 64), ([5, 1], 64)])
+def test_pages_that_are_only_read_stay_shared(hexmi, new, shared):
+    """Copy-on-write pages are not copied for attention over them; an append makes them the caller's own."""
+    c = Cache(new, [70 + shared, 90 + shared], 4, 2, 64, 16, torch.float16, seed=78, shared=shared)
+    want = hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages)
+    plain = c.k_pages, c.v_pages
+    c.k_pages, c.v_pages = (torch._lazy_clone(p) for p in plain)
+    assert torch.equal(hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages), want)
+    assert all(torch._C._is_cow_tensor(p) for p in (c.k_pages, c.v_pages))
+    before = [p.clone().view(torch.int16) for p in plain]
+    k = torch.zeros(sum(new), 2, 64, dtype=torch.float16, device="cuda")
+    hexmi.paged_append(k, k, *c.batch())
+    assert not any(torch._C._is_cow_tensor(p) for p in (c.k_pages, c.v_pages))
+    assert all(torch.equal(p.view(torch.int16), b) for p, b in zip(plain, before))
+    assert not any(torch.equal(p.view(torch.int16), b) for p, b in zip((c.k_pages, c.v_pages), before))
