@@ -1037,7 +1037,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
         qd = qd.clone(memory_format=torch.contiguous_format)
     sd = _stage(shared_pages, dev)
     od = _out_like(out, q.shape, q.dtype, dev)
-    if out is not None and od is out and od.numel() and (od.data_ptr() % 16 or _overlaps(od, qd, k_pages, v_pages)):
+    read = [t for t in (qd, k_pages, v_pages, table, lens, begin, sd) if t is not None and t.numel()]
+    if out is not None and od is out and od.numel() and (od.data_ptr() % 16 or _overlaps(od, *read)):
         od = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if q.shape[0]:
         args = (qd, k_pages, v_pages, table, lens, begin, float(sm_scale), sd, od)

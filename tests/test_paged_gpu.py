@@ -727,3 +727,17 @@ def test_pages_that_are_only_read_stay_shared(hexmi, new, shared):
     assert not any(torch._C._is_cow_tensor(p) for p in (c.k_pages, c.v_pages))
     assert all(torch.equal(p.view(torch.int16), b) for p, b in zip(plain, before))
     assert not any(torch.equal(p.view(torch.int16), b) for p, b in zip((c.k_pages, c.v_pages), before))
+
+
+@pytest.mark.parametrize("name, shared", [("page_table", 0), ("lengths_d", 0), ("starts", 0), ("page_table", 64), ("lengths_d", 64), ("starts", 64),
+                                          ("shared_pages", 64)])
+def test_out_over_an_index_tensor(hexmi, name, shared):
+    """A result that lands where an index tensor stood is complete before it is written there. Tiles of the last rows, where it stands, are
+    done before those of the first are begun."""
+    c = Cache([2100, 1, 1900, 700], [shared] * 4, 32, 8, 128, 16, torch.float16, seed=79, shared=shared)
+    want = hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages)
+    out = torch.empty_like(c.q)
+    index = getattr(c, name)
+    setattr(c, name, out.view(torch.int32).flatten()[-index.numel():].view(index.shape).copy_(index))
+    assert hexmi.paged_attention(c.q, *c.batch(), shared_pages=c.shared_pages, out=out) is out
+    assert torch.equal(out, want)
