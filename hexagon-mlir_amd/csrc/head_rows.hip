@@ -183,7 +183,8 @@ __device__ __forceinline__ float row_sum(float v) {
 // What a launch is bound by: its latency up to a few hundred tokens (4 tokens x 40 heads of 128 4.9 us, 64 tokens into a cache 4.6), then the
 // rows in flight: 8192 tokens x 40 heads of 128 bf16, normed and turned, 40 us (4.2 TB/s; a copy of that size 33). Measured there: an
 // angle worked out by every lane that needs it 50 us, pointers and strides chosen by the lane 62, no row asked for ahead 49, two ahead 42,
-// 16384 waves 46, five waves a SIMD with what spills 44, nontemporal stores 41, and loads 43.
+// 16384 waves 46, five waves a SIMD with what spills 44, nontemporal stores 41, and loads 43 (into a cache, prompts of 8700 tokens: 51 plain, 49
+// and 53).
 template <typename T, int LPR, bool HALVES, bool PIECES, bool PAGED>
 __global__ __launch_bounds__(256, 4)
 void head_rows_kernel(HeadArgs a, Pages p, int waves_per_token) {

@@ -90,6 +90,10 @@ int parts_of(int64_t units, int64_t keys, int64_t wanted, int64_t least, int64_t
   const int64_t most = keys / least < limit ? keys / least : limit, parts = wanted / units < most ? wanted / units : most;
   return parts > 1 ? (int)parts : 1;
 }
+// Lengths are on the GPU, so a plan takes the table's width for them, and its rules were measured with tables no wider than the longest
+// sequence. As wide / 8192 columns of 16, 32 heads of 128 over 8, us: one prompt of 40 tokens 7.6 / 14.1, of 400 14.6 / 22.6, of 1000 26.9 / 37.2 (parts
+// that nothing fills, and their join), of 2000 54.9 / 54.8; 64 decoding behind 99 10.5 / 12.7; one behind 999, 64 behind 99 .. 16383, 509
+// tokens beside 15 single ones and 4 x 4096 are level.
 Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   Plan plan = {};
   const int64_t group = heads / b.kv_heads, prefix = shared * b.page_size, rows = b.tokens * group, cus = hexmi_num_cus();

@@ -142,7 +142,7 @@ template <typename T, int D, int COLS, bool PADDED, int W>
 __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned worker, char* lds,
                                                     float (*m_lds)[16], float (*l_lds)[16]) {
   typedef typename MfmaT<T>::Frag Frag;
-  constexpr int DS = COLS / 32, DT = COLS / 16, CPR = D / 8, kPitch = COLS + 4;
+  constexpr int DS = COLS / 32, DT = COLS / 16, kPitch = COLS + 4;
   constexpr int kWaveBytes = decode_wave_bytes(D, COLS), kBlock = W * kTileKeys;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane / 16, n = lane % 16;
@@ -294,7 +294,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         float pr[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.scale, neg_m));
-        const Frag pf = MfmaT<T>::pack(pr);
+        const Frag pf = MfmaT<T>::pack(pr);                          // 16 bits: paged_tile.h
         l += MfmaT<T>::sum8(pf, 0.0f);                               // the sum of what the product multiplies (these keys' first, paged_tile.h)
         asm volatile("" ::: "memory");                               // the reads below stay behind the writes above (LDS is in order)
 #pragma unroll

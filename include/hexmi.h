@@ -548,7 +548,10 @@ typedef struct hexmi_rotation {
  * starts[sequences] on belongs to no sequence; without starts, tokens ==
  * sequences. Positions past the table's columns have no page.
  * The index arrays are read by the kernels and not checked on the host:
- * whatever they hold, nothing outside the operands is touched. */
+ * whatever they hold, nothing outside the operands is touched. How attention
+ * cuts the work goes by table_cols, since lengths is not read: a table much
+ * wider than the longest sequence (a captured step's, as wide as any may get)
+ * costs a batch of little work 2 to 10 us, and sums in another order. */
 typedef struct hexmi_paged_batch {
   void *k_pages, *v_pages;
   int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
@@ -577,8 +580,8 @@ int hexmi_qk_norm_rope(const hexmi_head_rows *q, const hexmi_head_rows *k,
  * rotated by their positions on the way (k->out, v->out and v->weight are not
  * used), and, with q, the queries' rows normed and rotated into q->out. A
  * token without a page leaves no key and no value; q->out of a row of no
- * sequence is zeros. Two tokens of one slot: either's. What is read and what is
- * written share no memory, but for q->x as q->out. HEXMI_F16, HEXMI_BF16. */
+ * sequence is zeros. Of two tokens of one slot pieces of either are left there.
+ * What is read and what is written share no memory, but for q->x as q->out. HEXMI_F16, HEXMI_BF16. */
 int hexmi_paged_append(const hexmi_head_rows *k, const hexmi_head_rows *v,
                        const hexmi_head_rows *q, const hexmi_rotation *rotation,
                        const hexmi_paged_batch *batch, int dtype,
