@@ -4,41 +4,14 @@
 // A row x of dim columns becomes y = x / sqrt(mean(x^2) + eps) * w (where there is a weight), and pairs (a, b) of its leading columns
 // become (a cos - b sin, b cos + a sin) at the angle position * inv_freq[i], all in fp32 but for the angle, which is a double until
 // it is down to a quarter turn; one rounding at the end. Bound by HBM: every row is read once and written once.
-#include "paged.h"
+#include "head_rows.h"
 
 namespace hexmi {
 namespace {
 
-constexpr int kMaxDim = 512;
 // A token's rows are shared by several waves up to so many in all: what the card holds at once, four a SIMD. 2048 / 4096 / 8192, 40 heads of 128
 // bf16, us: 256 tokens 6.1 / 5.7 / 5.7, 1000 10.7 / 10.5 / 13.1, 2000 15.4 / 13.7 / 16.4, 1500 into a cache 19.0 / 14.7 / 17.8.
 constexpr int kWavesWanted = 4096;
-
-// the three kinds of rows, in the order in which they are numbered: queries, keys, values
-struct Kind {
-  const void* x;
-  void* out;
-  const void* weight;
-  int64_t token, head, out_token, out_head;
-};
-struct HeadArgs {
-  Kind kind[3];
-  int heads[3], rows;                          // rows of a token, all kinds
-  const double* inv_freq;
-  int columns, halves, dim;
-  float eps;
-  const void* positions;
-  int positions_64, tokens;
-};
-
-// where row h of a token belongs: its kind and the head of that kind
-__device__ __forceinline__ int kind_of(const HeadArgs& a, int& h) {
-  if (h < a.heads[0]) return 0;
-  h -= a.heads[0];
-  if (h < a.heads[1]) return 1;
-  h -= a.heads[1];
-  return 2;
-}
 
 // The position of a token, and its page where it has one (page -1: none). PAGED: the batch says so (none: no sequence).
 struct Place {
@@ -132,48 +105,6 @@ void head_rows_any_kernel(HeadArgs a, Pages p) {
       if (c < a.dim) out[c] = y[i];
     }
   }
-}
-
-// Eight columns of a row as they stand in memory.
-template <typename T> struct alignas(16) Eight {
-  static constexpr int kWords = 8 * (int)sizeof(T) / 4;
-  uint32_t w[kWords];
-};
-template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p) {
-  Eight<T> r;
-#pragma unroll
-  for (int i = 0; i < Eight<T>::kWords / 4; ++i)
-    *reinterpret_cast<u32x4*>(r.w + 4 * i) = *(reinterpret_cast<const u32x4*>(p) + i);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store_eight(T* p, const Eight<T>& r) {
-#pragma unroll
-  for (int i = 0; i < Eight<T>::kWords / 4; ++i)
-    reinterpret_cast<u32x4*>(p)[i] = *reinterpret_cast<const u32x4*>(r.w + 4 * i);
-}
-template <typename T>
-__device__ __forceinline__ float column(const Eight<T>& r, int e) {
-  return to_f32<T>(reinterpret_cast<const T*>(r.w)[e]);
-}
-// the sum over the LPR lanes of a row, in all of them
-template <int LPR>
-__device__ __forceinline__ float row_sum(float v) {
-  v += dpp_move<0xB1>(v);
-  v += dpp_move<0x4E>(v);
-  v += dpp_move<0x141>(v);
-  float a, b;
-  if constexpr (LPR >= 16) v += dpp_move<0x140>(v);
-  if constexpr (LPR >= 32) {
-    swap16(v, a, b);
-    v = a + b;
-  }
-  if constexpr (LPR == 64) {
-    swap32(v, a, b);
-    v = a + b;
-  }
-  return v;
 }
 
 // Rows on 16-byte boundaries, dim a multiple of 8. LPR lanes take a row, eight columns each, and the 64 / LPR rows of a wave are of one
@@ -295,12 +226,7 @@ void head_rows_kernel(HeadArgs a, Pages p, int waves_per_token) {
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(y[e], y[e], sum);
-        float mean = fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps);
-        const bool tiny = mean < 0x1p-100f;                         // the root's instruction takes no subnormal numbers
-        mean = tiny ? mean * 0x1p60f : mean;
-        const float r = __builtin_amdgcn_rsqf(mean);
-        scale = r == 0.0f ? 0.0f : r * fmaf(-0.5f * mean * r, r, 1.5f);          // one Newton step; an infinite mean stays 0
-        scale = tiny ? scale * 0x1p30f : scale;
+        scale = rms_scale(fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps));
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = y[e] * scale * column(wt, e);
       }
@@ -372,29 +298,6 @@ int launch(const HeadArgs& a, const Pages& p, hipStream_t s) {
   const int64_t rows = (int64_t)a.tokens * a.rows, blocks = (rows + 3) / 4;
   hipLaunchKernelGGL((head_rows_any_kernel<T, PAGED>), dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), 0, s, a, p);
   return launch_status();
-}
-
-int take(HeadArgs& a, int k, const hexmi_head_rows* r, bool needs_out) {
-  if (!r) return HEXMI_OK;
-  if (r->heads < 1 || !r->x || (needs_out && !r->out)) return HEXMI_EINVAL;
-  if (r->heads > 65535) return HEXMI_ENOTSUP;
-  a.kind[k] = {r->x, r->out, r->weight, r->token, r->head, r->out_token, r->out_head};
-  a.heads[k] = (int)r->heads;
-  a.rows += (int)r->heads;
-  return HEXMI_OK;
-}
-
-int turn(HeadArgs& a, const hexmi_rotation* r, int64_t dim) {
-  if (!r || dim < 1 || r->columns < 0 || r->columns % 2 != 0 || r->columns > dim || (r->columns > 0 && !r->inv_freq) ||
-      (r->pairs != HEXMI_PAIRS_ADJACENT && r->pairs != HEXMI_PAIRS_HALVES))
-    return HEXMI_EINVAL;
-  if (dim > kMaxDim) return HEXMI_ENOTSUP;
-  a.inv_freq = r->inv_freq;
-  a.columns = (int)r->columns;
-  a.halves = r->pairs == HEXMI_PAIRS_HALVES;
-  a.dim = (int)dim;
-  a.eps = r->eps;
-  return HEXMI_OK;
 }
 
 }  // namespace

@@ -43,7 +43,36 @@ inline int check_batch(const hexmi_paged_batch& b) {
   return HEXMI_OK;
 }
 
+// hexmi_paged_scales as the kernels take it
+struct Scales {
+  uint8_t *k, *v;
+  int64_t k_page, k_head, k_block, v_page, v_head, v_block;
+  int block;
+  Divider by_block;
+};
+inline Scales scales_of(const hexmi_paged_scales& s) {
+  return {s.k_scales, s.v_scales, s.k_page, s.k_head, s.k_block, s.v_page, s.v_head, s.v_block, (int)s.block, divider(s.block)};
+}
+constexpr int kMostBlock = 64;
+inline int check_scales(const hexmi_paged_batch& b, const hexmi_paged_scales& s) {
+  if (s.block < 1 || b.page_size % s.block != 0) return HEXMI_EINVAL;
+  if (s.block > kMostBlock) return HEXMI_ENOTSUP;
+  return s.k_scales && s.v_scales ? HEXMI_OK : HEXMI_EINVAL;
+}
+
+// The window of a call over positions 0 .. most - 1, 0 where it hides none of them (then window + sinks is below 2^31).
+inline int window_of(int64_t window, int64_t sinks, int64_t most) { return window > 0 && window < most && sinks < most - window ? (int)window : 0; }
+
 #if defined(__HIPCC__)
+// The exponents of scales, so that a number of e4m3 (2^-9 to 448) times its scale is one of T: fp16 has nothing below 2^-24, and 240 * 2^8, its
+// largest number here, is off from 65504 by 6.2 %, less than half a step of e4m3.
+template <typename T> constexpr int kLeastExponent = -117;
+template <typename T> constexpr int kMostExponent = 120;
+template <> inline constexpr int kLeastExponent<f16> = -15;
+template <> inline constexpr int kMostExponent<f16> = 8;
+// 2^e of a normal number
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
 // The sequence of row t: the last b with starts[b] <= t, by the 64 lanes of a wave together (t the same for all): 64 places are asked
 // at once, so 64 sequences take one read and 4096 two. -1: none (below starts[0], from starts[sequences] on).
 __device__ __forceinline__ int sequence_of(const Pages& p, int t, int lane) {

@@ -1,0 +1,290 @@
+// The pages of a cache: rows that go on from others' with their last page copied (fork), and the pages in use moved to the front (compact).
+// Copies, bound by HBM; what is in use is found from the table, so nothing is counted beside it.
+#include "paged.h"
+
+namespace hexmi {
+namespace {
+
+// Keys (or values) as bytes: strides in bytes, `row` bytes of a head at a slot, copied in pieces of `piece` bytes (16, or what divides all)
+struct Side {
+  char* pages;
+  int64_t page, head, slot;
+};
+struct CopyArgs {
+  Side side[2];
+  uint8_t* scales[2];
+  int64_t scale_page[2], scale_head[2], scale_block[2];
+  int block;                                   // 0: none
+  Divider by_block;
+  int pieces;                                  // of a row
+};
+
+template <typename Piece>
+__device__ __forceinline__ void copy_rows(const Side& side, int from, int to, int heads, int slots, int pieces, int first, int step) {
+  // the order of memory: slots within heads, or heads within slots
+  const bool slots_inside = side.slot < side.head;
+  const int inner = slots_inside ? slots : heads;
+  const int64_t inner_stride = slots_inside ? side.slot : side.head, outer_stride = slots_inside ? side.head : side.slot;
+  const char* src = side.pages + from * side.page;
+  char* dst = side.pages + to * side.page;
+  const int64_t all = (int64_t)heads * slots * pieces;
+  for (int64_t i = first; i < all; i += step) {
+    const int64_t r = i / pieces, o = r / inner;
+    const int64_t at = o * outer_stride + (r - o * inner) * inner_stride + (i - r * pieces) * sizeof(Piece);
+    *reinterpret_cast<Piece*>(dst + at) = *reinterpret_cast<const Piece*>(src + at);
+  }
+}
+__device__ __forceinline__ void copy_scales(const CopyArgs& c, int side, int from, int to, int heads, int blocks, int first, int step) {
+  uint8_t* s = c.scales[side];
+  for (int i = first; i < heads * blocks; i += step) {
+    const int h = i / blocks, j = i - h * blocks;
+    const int64_t at = h * c.scale_head[side] + j * c.scale_block[side];
+    s[to * c.scale_page[side] + at] = s[from * c.scale_page[side] + at];
+  }
+}
+
+// Workgroup (row, share): a share of the row's copies, keys and values, and of its entries of the table.
+template <typename Piece>
+__global__ __launch_bounds__(256)
+void fork_kernel(CopyArgs c, Pages p, const int32_t* parents, const int32_t* pages, int32_t* table_out, int64_t table_out_row, int32_t* lengths_out,
+                 int shares) {
+  const int row = blockIdx.x / shares, share = blockIdx.x - row * shares;
+  const int parent = parents[row], page = pages[row];
+  const bool is = parent >= 0 && parent < p.sequences;
+  const int length = is ? p.lengths[parent] : 0, there = is ? length_of(p, parent) : 0;
+  const int column = divided(there, p.size), filled = there - column * p.page_size;
+  const int32_t* table = p.table + (is ? parent : 0) * p.table_row;
+  int last = -1;
+  if (is && column < p.table_cols && filled > 0) last = table[column];
+  const bool last_is = last >= 0 && last < p.num_pages;
+  const bool takes = is && page >= 0 && page < p.num_pages && column < p.table_cols && (filled == 0 || last_is);
+  for (int i = share * 256 + threadIdx.x; i < p.table_cols; i += shares * 256)
+    table_out[row * table_out_row + i] = takes && i == column ? page : is ? table[i] : -1;
+  if (share == 0 && threadIdx.x == 0) lengths_out[row] = length;
+  if (!takes || filled == 0 || page == last) return;
+  const int first = share * 256 + threadIdx.x, step = shares * 256;
+  for (int side = 0; side < 2; ++side) {
+    copy_rows<Piece>(c.side[side], last, page, p.kv_heads, filled, c.pieces, first, step);
+    if (c.block) copy_scales(c, side, last, page, p.kv_heads, divided(filled + c.block - 1, c.by_block), first, step);
+  }
+}
+
+// ---- compact: mark (a bit a page), number what is to go and where to, move and rename
+struct CompactSpace {
+  uint32_t* marks;                             // [words]
+  int32_t *renamed, *sources, *targets;        // [pages]
+  int32_t* moves;                              // [1]
+};
+__host__ __device__ inline int64_t words_of(int64_t pages) { return (pages + 31) / 32; }
+
+__global__ __launch_bounds__(256)
+void clear_kernel(uint32_t* marks, int64_t words) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < words) marks[i] = 0;
+}
+
+struct View {
+  int window, sinks;                           // window 0: all
+};
+// the page that entry (b, column) of the table names, -1: none in use
+__device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, int column) {
+  const int length = length_of(p, b);
+  const int first = column * p.page_size;
+  if (first >= length) return -1;
+  if (w.window > 0 && first >= w.sinks && first + p.page_size <= length - w.window) return -1;
+  const int page = p.table[b * p.table_row + column];
+  return page >= 0 && page < p.num_pages ? page : -1;
+}
+__global__ __launch_bounds__(256)
+void mark_kernel(Pages p, View w, uint32_t* marks, int64_t entries) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
+    const int b = (int)(i / p.table_cols), page = used_page(p, w, b, (int)(i - (int64_t)b * p.table_cols));
+    if (page < 0) continue;
+    const uint32_t bit = 1u << page % 32;
+    if (!(__hip_atomic_load(marks + page / 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit)) atomicOr(marks + page / 32, bit);
+  }
+}
+
+// One workgroup: a thread takes a run of words, twice.
+__global__ __launch_bounds__(1024)
+void number_kernel(CompactSpace s, int num_pages, int32_t* count) {
+  __shared__ int sums[16], used_below, total;
+  const int words = (int)words_of(num_pages), each = (words + 1023) / 1024;
+  const int w0 = (int)threadIdx.x * each < words ? (int)threadIdx.x * each : words, w1 = w0 + each < words ? w0 + each : words;
+  int n = 0;
+  for (int w = w0; w < w1; ++w) n += __popc(s.marks[w]);
+  // the sum over the threads before this one
+  int up_to = n;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  for (int d = 1; d < kWave; d *= 2) {
+    const int v = __shfl_up(up_to, d);
+    if (lane >= d) up_to += v;
+  }
+  if (lane == kWave - 1) sums[wave] = up_to;
+  __syncthreads();
+  int before = up_to - n;
+  for (int x = 0; x < wave; ++x) before += sums[x];
+  if (threadIdx.x == 1023) total = before + n;
+  if (threadIdx.x == 0) used_below = 0;
+  __syncthreads();
+  const int front = total;
+  // used pages below `front`: the thread whose run holds it says
+  if (front / 32 >= w0 && front / 32 < w1) {
+    int below = before;
+    for (int w = w0; w < front / 32; ++w) below += __popc(s.marks[w]);
+    used_below = below + __popc(s.marks[front / 32] & ((1u << front % 32) - 1));
+  } else if (threadIdx.x == 0 && front / 32 >= words) {
+    used_below = total;                                             // all pages are in use
+  }
+  __syncthreads();
+  const int moved = used_below;
+  int used = before;
+  for (int w = w0; w < w1; ++w) {
+    const uint32_t marks = s.marks[w];
+    const int page0 = w * 32, last = num_pages - page0 < 32 ? num_pages - page0 : 32;
+    for (int i = 0; i < last; ++i) {
+      const int page = page0 + i;
+      if (marks >> i & 1) {
+        if (page >= front) s.sources[used - moved] = page;
+        ++used;
+      } else if (page < front) {
+        s.targets[page - used] = page;
+      }
+    }
+  }
+  if (threadIdx.x == 0) {
+    *s.moves = front - moved;
+    *count = front;
+  }
+}
+__global__ __launch_bounds__(256)
+void name_kernel(CompactSpace s) {
+  const int moves = *s.moves;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < moves; i += gridDim.x * 256) s.renamed[s.sources[i]] = s.targets[i];
+}
+
+template <typename Piece>
+__global__ __launch_bounds__(256)
+void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int64_t entries) {
+  const int front = *count, moves = *s.moves;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
+    const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols), page = used_page(p, w, b, column);
+    table_out[b * table_out_row + column] = page >= front ? s.renamed[page] : page;
+  }
+  for (int64_t i = blockIdx.x; i < 2 * (int64_t)moves; i += gridDim.x) {
+    const int move = (int)(i / 2), side = (int)(i - 2 * (int64_t)move), from = s.sources[move], to = s.targets[move];
+    copy_rows<Piece>(c.side[side], from, to, p.kv_heads, p.page_size, c.pieces, threadIdx.x, 256);
+    if (c.block) copy_scales(c, side, from, to, p.kv_heads, divided(p.page_size, c.by_block), threadIdx.x, 256);
+  }
+}
+
+// HEXMI_OK, or why a cache is refused; the copies' arguments and the bytes of their pieces
+int check_cache(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int dtype, int64_t table_out_row, CopyArgs& c, int& piece) {
+  if (!batch) return HEXMI_EINVAL;
+  hexmi_paged_batch b = *batch;
+  b.starts = nullptr;
+  b.tokens = b.sequences;
+  int rc = check_batch(b);
+  if (rc == HEXMI_OK && scales) rc = check_scales(b, *scales);
+  if (rc != HEXMI_OK) return rc;
+  if (dtype != HEXMI_F16 && dtype != HEXMI_BF16) return HEXMI_ENOTSUP;
+  if (!b.k_pages || !b.v_pages || (b.sequences > 0 && (!b.lengths || (b.table_cols > 0 && !b.page_table)))) return HEXMI_EINVAL;
+  const int size = scales ? 1 : 2;
+  if (b.dim > (1 << 20)) return HEXMI_ENOTSUP;
+  if (table_out_row < b.table_cols) return HEXMI_EINVAL;
+  c = {};
+  c.side[0] = {static_cast<char*>(b.k_pages), b.k_page * size, b.k_head * size, b.k_slot * size};
+  c.side[1] = {static_cast<char*>(b.v_pages), b.v_page * size, b.v_head * size, b.v_slot * size};
+  piece = 16;
+  for (const Side& s : c.side)
+    for (int64_t x : {(int64_t)reinterpret_cast<uintptr_t>(s.pages), s.page, s.head, s.slot, b.dim * size})
+      while (x % piece != 0) piece /= 2;
+  c.pieces = (int)(b.dim * size / piece);
+  if (scales) {
+    c.scales[0] = scales->k_scales;
+    c.scales[1] = scales->v_scales;
+    c.scale_page[0] = scales->k_page, c.scale_head[0] = scales->k_head, c.scale_block[0] = scales->k_block;
+    c.scale_page[1] = scales->v_page, c.scale_head[1] = scales->v_head, c.scale_block[1] = scales->v_block;
+    c.block = (int)scales->block;
+    c.by_block = divider(scales->block);
+  }
+  return HEXMI_OK;
+}
+// f of a piece's type
+template <typename F> int with_piece(int piece, F&& f) {
+  switch (piece) {
+    case 16: return f(u32x4{});
+    case 8: return f(u32x2{});
+    case 4: return f(uint32_t{});
+    case 2: return f(uint16_t{});
+    default: return f(uint8_t{});
+  }
+}
+CompactSpace space_of(void* workspace, int64_t pages) {
+  CompactSpace s;
+  s.marks = static_cast<uint32_t*>(workspace);
+  s.renamed = reinterpret_cast<int32_t*>(s.marks + words_of(pages));
+  s.sources = s.renamed + pages;
+  s.targets = s.sources + pages;
+  s.moves = s.targets + pages;
+  return s;
+}
+
+}  // namespace
+}  // namespace hexmi
+
+using namespace hexmi;
+
+extern "C" int hexmi_paged_fork(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, const int32_t* parents, const int32_t* pages,
+                                int64_t rows, int32_t* table_out, int64_t table_out_row, int32_t* lengths_out, int dtype, hexmi_stream_t stream) {
+  CopyArgs c;
+  int piece;
+  const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
+  if (rc != HEXMI_OK) return rc;
+  if (rows < 0) return HEXMI_EINVAL;
+  if (rows == 0) return HEXMI_OK;
+  if (!parents || !pages || !lengths_out || (batch->table_cols > 0 && !table_out)) return HEXMI_EINVAL;
+  // a workgroup for some KiB of a full page, as many as the card holds at once
+  const int64_t page_bytes = 2 * batch->kv_heads * batch->page_size * c.pieces * piece, most = (page_bytes + 8191) / 8192;
+  int64_t shares = 2048 / rows;
+  shares = shares < 1 ? 1 : shares < most ? shares : most;
+  if (!grid_fits(rows * shares, 256)) return HEXMI_ENOTSUP;
+  const Pages p = pages_of(*batch);
+  begin_call();
+  return with_piece(piece, [&](auto x) {
+    hipLaunchKernelGGL((fork_kernel<decltype(x)>), dim3((unsigned)(rows * shares)), dim3(256), 0, as_stream(stream), c, p, parents, pages, table_out,
+                       table_out_row, lengths_out, (int)shares);
+    return launch_status();
+  });
+}
+
+extern "C" int64_t hexmi_paged_compact_workspace(const hexmi_paged_batch* batch) {
+  if (!batch || batch->num_pages < 1 || batch->num_pages > 0x7fffffff) return 0;
+  return (words_of(batch->num_pages) + 3 * batch->num_pages + 1) * 4;
+}
+
+extern "C" int hexmi_paged_compact(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int64_t window, int64_t sinks, int32_t* table_out,
+                                   int64_t table_out_row, int32_t* count, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
+  CopyArgs c;
+  int piece;
+  const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
+  if (rc != HEXMI_OK) return rc;
+  const int64_t entries = batch->sequences * batch->table_cols;
+  if (window < 0 || sinks < 0 || !count || (entries > 0 && !table_out)) return HEXMI_EINVAL;
+  if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < hexmi_paged_compact_workspace(batch)) return HEXMI_EINVAL;
+  const Pages p = pages_of(*batch);
+  const CompactSpace space = space_of(workspace, batch->num_pages);
+  const View view = {window_of(window, sinks, batch->table_cols * batch->page_size), (int)(sinks < 0x7fffffff ? sinks : 0x7fffffff)};
+  const hipStream_t s = as_stream(stream);
+  const int64_t words = words_of(batch->num_pages);
+  auto blocks = [](int64_t n, int64_t most) { return dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)); };
+  begin_call();
+  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, space.marks, words);
+  if (entries > 0) hipLaunchKernelGGL(mark_kernel, blocks(entries, 4096), dim3(256), 0, s, p, view, space.marks, entries);
+  hipLaunchKernelGGL(number_kernel, dim3(1), dim3(1024), 0, s, space, (int)batch->num_pages, count);
+  hipLaunchKernelGGL(name_kernel, blocks(batch->num_pages, 256), dim3(256), 0, s, space);
+  return with_piece(piece, [&](auto x) {
+    hipLaunchKernelGGL((move_kernel<decltype(x)>), dim3(2048), dim3(256), 0, s, c, p, view, space, count, table_out, table_out_row, entries);
+    return launch_status();
+  });
+}

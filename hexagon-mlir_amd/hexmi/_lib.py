@@ -42,7 +42,12 @@ class PagedBatch(_c.Structure):         # hexmi_paged_batch
         ("tokens", _i64)]
 
 
+class PagedScales(_c.Structure):        # hexmi_paged_scales
+    _fields_ = [("k_scales", _ptr), ("v_scales", _ptr)] + [(n, _i64) for n in ("k_page", "k_head", "k_block", "v_page", "v_head", "v_block", "block")]
+
+
 _rows, _batch, _rotation = _c.POINTER(HeadRows), _c.POINTER(PagedBatch), _c.POINTER(Rotation)
+_scales = _c.POINTER(PagedScales)
 
 # name -> (restype, argtypes); must list every symbol of include/hexmi.h (the operator ABI)
 SIGNATURES = {
@@ -95,6 +100,12 @@ SIGNATURES = {
     "hexmi_paged_append": (_int, [_rows, _rows, _rows, _rotation, _batch, _int, _ptr]),
     "hexmi_paged_attention_workspace": (_i64, [_batch, _i64, _i64]),
     "hexmi_paged_attention": (_int, [_rows, _batch, _ptr, _i64, _f32, _int, _ptr, _i64, _ptr]),
+    "hexmi_paged_append_ex": (_int, [_rows, _rows, _rows, _rotation, _batch, _scales, _int, _ptr]),
+    "hexmi_paged_attention_ex_workspace": (_i64, [_batch, _i64, _i64, _scales, _i64, _i64]),
+    "hexmi_paged_attention_ex": (_int, [_rows, _batch, _scales, _ptr, _i64, _i64, _i64, _f32, _int, _ptr, _i64, _ptr]),
+    "hexmi_paged_fork": (_int, [_batch, _scales, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _int, _ptr]),
+    "hexmi_paged_compact_workspace": (_i64, [_batch]),
+    "hexmi_paged_compact": (_int, [_batch, _scales, _i64, _i64, _ptr, _i64, _ptr, _int, _ptr, _i64, _ptr]),
 }
 
 # measurement probes of include/hexmi_calibrate.h: exported by the library, not part of the operator ABI

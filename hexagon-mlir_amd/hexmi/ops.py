@@ -93,6 +93,15 @@ _LIBDEF.define("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) 
                "Tensor(c!)? q_out) -> ()")
 _LIBDEF.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lengths, Tensor? starts, "
                "float sm_scale, Tensor? shared_pages, Tensor(a!) out) -> ()")
+_LIBDEF.define("paged_append_ex(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!) k_scales, Tensor(d!) v_scales, "
+               "Tensor page_table, Tensor lengths, Tensor? starts, Tensor? k_weight, Tensor? inv_freq, float eps, str pairs, Tensor? q, "
+               "Tensor? q_weight, Tensor(e!)? q_out) -> ()")
+_LIBDEF.define("paged_attention_ex(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor page_table, "
+               "Tensor lengths, Tensor? starts, float sm_scale, Tensor? shared_pages, int? window, int sinks, Tensor(a!) out) -> ()")
+_LIBDEF.define("paged_fork(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
+               "Tensor lengths, Tensor parents, Tensor pages, Tensor(e!) table_out, Tensor(f!) lengths_out) -> ()")
+_LIBDEF.define("paged_compact(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
+               "Tensor lengths, int? window, int sinks, Tensor(e!) table_out, Tensor(f!) count) -> ()")
 
 
 def _row_workspace(rows, cols, block_cols, x):
@@ -323,6 +332,55 @@ def _paged_attention_impl(q, k_pages, v_pages, page_table, lengths, starts, sm_s
                                                     _stream()), "hexmi_paged_attention")
 
 
+def _paged_scales(k_pages, k_scales, v_scales):
+    """hexmi_paged_scales, or None of a cache in 16 bits."""
+    if k_scales is None:
+        return None
+    return _lib.PagedScales(_p(k_scales), _p(v_scales), *_strides(k_scales), *_strides(v_scales), k_pages.shape[2] // k_scales.shape[2])
+
+
+def _paged_append_ex_impl(k, v, k_pages, v_pages, k_scales, v_scales, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight,
+                          q_out):
+    with _on(k_pages.device):
+        _lib.check(_lib.lib().hexmi_paged_append_ex(_head_rows(k, None, k_weight), _head_rows(v), _head_rows(q, q_out, q_weight),
+                                                    _rotation(inv_freq, eps, pairs),
+                                                    _paged_batch(k.shape[0], k_pages, v_pages, page_table, lengths, starts),
+                                                    _paged_scales(k_pages, k_scales, v_scales), _dt(k), _stream()), "hexmi_paged_append_ex")
+
+
+def _paged_attention_ex_impl(q, k_pages, v_pages, k_scales, v_scales, page_table, lengths, starts, sm_scale, shared_pages, window, sinks, out):
+    batch, scales = _paged_batch(q.shape[0], k_pages, v_pages, page_table, lengths, starts), _paged_scales(k_pages, k_scales, v_scales)
+    shared, window = 0 if shared_pages is None else shared_pages.shape[0], window or 0
+    with _on(q.device):
+        need = _lib.lib().hexmi_paged_attention_ex_workspace(batch, q.shape[1], shared, scales, window, sinks)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.check(_lib.lib().hexmi_paged_attention_ex(_head_rows(q, out), batch, scales, _p(shared_pages), shared, window, sinks, sm_scale,
+                                                       _dt(q), _p(ws), need, _stream()), "hexmi_paged_attention_ex")
+
+
+def _page_type(pages, scales):
+    """The type that entries which only copy pages are told: any of 16 bits where scales say that they hold 8."""
+    return _dt(pages) if scales is None else _lib.F16
+
+
+def _paged_fork_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, parents, pages, table_out, lengths_out):
+    with _on(k_pages.device):
+        _lib.check(_lib.lib().hexmi_paged_fork(_paged_batch(lengths.shape[0], k_pages, v_pages, page_table, lengths, None),
+                                               _paged_scales(k_pages, k_scales, v_scales), _p(parents), _p(pages), parents.shape[0],
+                                               _p(table_out), table_out.stride(0), _p(lengths_out), _page_type(k_pages, k_scales), _stream()),
+                   "hexmi_paged_fork")
+
+
+def _paged_compact_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, window, sinks, table_out, count):
+    batch = _paged_batch(lengths.shape[0], k_pages, v_pages, page_table, lengths, None)
+    with _on(k_pages.device):
+        need = _lib.lib().hexmi_paged_compact_workspace(batch)
+        ws = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
+        _lib.check(_lib.lib().hexmi_paged_compact(batch, _paged_scales(k_pages, k_scales, v_scales), window or 0, sinks, _p(table_out),
+                                                  table_out.stride(0), _p(count), _page_type(k_pages, k_scales), _p(ws), need, _stream()),
+                   "hexmi_paged_compact")
+
+
 for _name, _fn in (("softmax", _softmax_impl), ("rms_norm", _rms_norm_impl), ("layer_norm", _layer_norm_impl),
                    ("matmul", _matmul_impl), ("linear", _linear_impl), ("add_matmul_softmax", _add_matmul_softmax_impl),
                    ("w8a16_matmul", _w8a16_impl), ("dequant_w8", _dequant_impl), ("pack_w8", _pack_impl),
@@ -330,7 +388,8 @@ for _name, _fn in (("softmax", _softmax_impl), ("rms_norm", _rms_norm_impl), ("l
                    ("flash_attention", _flash_impl), ("attention", _attention_impl),
                    ("unary", _unary_impl), ("binary", _binary_impl), ("block_sum", _block_sum_impl),
                    ("rope", _rope_impl), ("qk_norm_rope", _qk_norm_rope_impl), ("paged_append", _paged_append_impl),
-                   ("paged_attention", _paged_attention_impl)):
+                   ("paged_attention", _paged_attention_impl), ("paged_append_ex", _paged_append_ex_impl),
+                   ("paged_attention_ex", _paged_attention_ex_impl), ("paged_fork", _paged_fork_impl), ("paged_compact", _paged_compact_impl)):
     _LIBDEF.impl(_name, _fn, "CUDA")
 
 
@@ -856,6 +915,15 @@ def _rows_out(name, out, x, others, dev):
     return torch.empty(x.shape, dtype=x.dtype, device=dev)
 
 
+def _stands_on_boundaries(t):
+    """Whether the rows of a tensor (its last dimension) begin on 16-byte boundaries; of 16-bit numbers."""
+    return t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t)[:-1])
+
+
+def _on_boundaries(t):
+    return t if t is None or _stands_on_boundaries(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _head_operands(name, x, weight, dim, dtype):
     if x.dim() != 3 or x.shape[1] < 1 or x.shape[2] != dim or dim < 1:
         raise ValueError("hexmi.%s: rows of heads are [tokens, heads, %s]" % (name, dim))
@@ -951,8 +1019,33 @@ def _paged_operands(name, tokens, k_pages, v_pages, page_table, lengths, starts)
     return table, _stage(lengths, dev), _stage(starts, dev)
 
 
+def _check_scales(name, k_pages, k_scales, v_scales):
+    """Whether a cache is in 8 bits; its scales are checked."""
+    if k_scales is None and v_scales is None:
+        if k_pages.dtype == torch.float8_e4m3fn:
+            raise TypeError("hexmi.%s: pages of float8_e4m3fn go with k_scales and v_scales" % name)
+        return False
+    if k_scales is None or v_scales is None or k_scales.dtype != torch.uint8 or v_scales.dtype != torch.uint8 or k_pages.dtype != torch.float8_e4m3fn:
+        raise TypeError("hexmi.%s: k_scales and v_scales (uint8, both) go with pages of float8_e4m3fn" % name)
+    if (k_scales.dim() != 3 or v_scales.shape != k_scales.shape or k_pages.dim() != 4 or k_scales.shape[:2] != k_pages.shape[:2]
+            or k_scales.shape[2] < 1 or k_pages.shape[2] % k_scales.shape[2] != 0 or k_pages.shape[2] // k_scales.shape[2] > 64):
+        raise ValueError("hexmi.%s: k_scales and v_scales are [pages, kv heads, blocks of 1 to 64 slots of a page]" % name)
+    if k_scales.device != k_pages.device or v_scales.device != k_pages.device:
+        raise ValueError("hexmi.%s: the scales are where the pages are" % name)
+    return True
+
+
+def _check_window(name, window, sinks):
+    """(window, sinks) as the library takes them; numbers past any position are one as good as another."""
+    if window is None and sinks:
+        raise ValueError("hexmi.%s: sinks go with a window" % name)
+    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1) or isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError("hexmi.%s: window is a positive number or None, sinks one from 0" % name)
+    return window if window is None else min(window, 1 << 40), min(sinks, 1 << 40)
+
+
 def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_weight=None, inv_freq=None, eps=1e-5, pairs="adjacent",
-                 q=None, q_weight=None, q_out=None):
+                 q=None, q_weight=None, q_out=None, k_scales=None, v_scales=None):
     """Puts the keys and values of new tokens, [tokens, kv heads, dim], into the pages of their sequences, the keys normed (with k_weight)
     and rotated (with inv_freq) by their positions on the way, as `qk_norm_rope` does; with q [tokens, heads, dim], its rows too, which
     are returned.
@@ -962,17 +1055,25 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     say) is none, and a token there is left out. lengths int32 [sequences]: the positions of each sequence, the new tokens included, which
     are its last. starts int32 [sequences + 1]: sequence b's tokens are the rows starts[b] .. starts[b + 1] - 1 (of those
     that there are); rows of no sequence (padding behind the last) leave nothing, and zeros in q's result. None: one token a sequence. What the index tensors hold is
-    read on the GPU only, so the call can be captured into a graph and replayed as they change."""
-    if q_out is None and not _THROUGH_DISPATCHER:
+    read on the GPU only, so the call can be captured into a graph and replayed as they change.
+
+    A cache in 8 bits: pages of float8_e4m3fn, and k_scales, v_scales uint8 [pages, kv heads, blocks] (any strides, changed in place), the
+    biased exponent e + 127 of the power of two that the numbers of each page_size / blocks slots (1 to 64) of a page are multiplied by. A
+    block's exponent is the least that has the largest of the call's values in it within 448; it does not fall below what older tokens
+    of the sequence in the block have, and their numbers are rounded again where it rises. dim a multiple of 8 up to 256."""
+    if q_out is None and k_scales is None and v_scales is None and not _THROUGH_DISPATCHER:
         y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight)
         if y is not None:
             return y if q is not None else None
     name = "paged_append"
-    if k.dtype not in (torch.float16, torch.bfloat16) or k_pages.dtype != k.dtype:
+    scaled = _check_scales(name, k_pages, k_scales, v_scales)
+    if k.dtype not in (torch.float16, torch.bfloat16) or not scaled and k_pages.dtype != k.dtype:
         raise TypeError("hexmi.paged_append: keys and pages must both be float16 or both bfloat16")
     if k_pages.dim() != 4 or k.dim() != 3 or k.shape[1:] != (k_pages.shape[1], k_pages.shape[3]) or v.shape != k.shape:
         raise ValueError("hexmi.paged_append: k and v are [tokens, kv heads, dim], the pages [pages, kv heads, page size, dim]")
     dim, tokens = k.shape[2], k.shape[0]
+    if scaled and (dim % 8 != 0 or dim > 256):
+        raise ValueError("hexmi.paged_append: a cache in 8 bits takes a dim that is a multiple of 8 up to 256")
     _head_operands(name, k, k_weight, dim, k.dtype)
     _head_operands(name, v, None, dim, k.dtype)
     _check_rotation(name, inv_freq, pairs, dim)
@@ -984,21 +1085,28 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
         raise ValueError("hexmi.paged_append: q_weight and q_out go with q")
     table, lens, begin = _paged_operands(name, tokens, k_pages, v_pages, page_table, lengths, starts)
     dev = k_pages.device
-    _one_device(name, dev, k, v, q, k_weight, q_weight, inv_freq)
+    _one_device(name, dev, k, v, q, k_weight, q_weight, inv_freq, k_scales, v_scales)
     if k_pages.data_ptr() == v_pages.data_ptr():
         raise ValueError("hexmi.paged_append: keys and values need pages of their own")
     # rows that stand in the pages themselves (one sequence's going to another) are read before any is written
     kd, vd, qd = (t.clone() if t is not None and t.numel() and _overlaps(t, k_pages, v_pages) else t
                   for t in (_rows_of_heads(k, dev), _rows_of_heads(v, dev), _rows_of_heads(q, dev)))
     kw, qw, fd = _stage(k_weight, dev), _stage(q_weight, dev), _stage(inv_freq, dev)
-    qo = None if q is None else _rows_out(name, q_out, qd, (kd, vd, kw, qw, fd, table, lens, begin, k_pages, v_pages), dev)
-    if tokens:
+    qo = None if q is None else _rows_out(name, q_out, qd, (kd, vd, kw, qw, fd, table, lens, begin, k_pages, v_pages, k_scales, v_scales), dev)
+    if tokens and scaled:
+        kd, vd, qd, kw, qw = (_on_boundaries(t) for t in (kd, vd, qd, kw, qw))
+        if qo is not None and not _stands_on_boundaries(qo):
+            qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        args = (kd, vd, k_pages, v_pages, k_scales, v_scales, table, lens, begin, kw, fd, float(eps), pairs, qd, qw, qo)
+        _run("paged_append_ex", _paged_append_ex_impl, args, *args)
+    elif tokens:
         args = (kd, vd, k_pages, v_pages, table, lens, begin, kw, fd, float(eps), pairs, qd, qw, qo)
         _run(name, _paged_append_impl, args, *args)
     return None if q is None else _finish(qo, q_out)
 
 
-def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_scale=None, shared_pages=None, out=None):
+def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_scale=None, shared_pages=None, out=None, k_scales=None,
+                    v_scales=None, window=None, sinks=0):
     """Attention of new tokens q [tokens, heads, dim] over a paged cache: row (t, h) is softmax(sm_scale * Q K^T) V over the keys of
     kv head h // (heads // kv heads) at the positions of its sequence up to its own (`attention` with a cache and masks of its own;
     test/python/triton/test_flash_attention.py:37-168). The cache and the batch are `paged_append`'s, which comes first: lengths counts
@@ -1013,14 +1121,22 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
 
     A row without any key, and a row of no sequence, is zeros. What the pages hold past a sequence's length is not used, whatever it is;
     the keys and values of its own positions, and of all of the shared pages, have to be finite (a NaN among them reaches any row of the
-    sequence). 16-bit, dim a multiple of 8 up to 256."""
-    if out is None and not _THROUGH_DISPATCHER:
+    sequence). 16-bit, dim a multiple of 8 up to 256.
+
+    k_scales, v_scales: a cache in 8 bits, as `paged_append` has it. window: a token at position p sees the positions j <= p with
+    j > p - window or j < sinks; pages that hold none of what a sequence's new tokens see are not read, and their entries of the table
+    may be anything (-1, once `paged_compact` has freed them). No shared pages within a window."""
+    if out is None and k_scales is None and v_scales is None and window is None and not sinks and not _THROUGH_DISPATCHER:
         y = _front.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages)
         if y is not None:
             return y
     name = "paged_attention"
-    if q.dtype not in (torch.float16, torch.bfloat16) or k_pages.dtype != q.dtype:
+    scaled = _check_scales(name, k_pages, k_scales, v_scales)
+    window, sinks = _check_window(name, window, sinks)
+    if q.dtype not in (torch.float16, torch.bfloat16) or not scaled and k_pages.dtype != q.dtype:
         raise TypeError("hexmi.paged_attention: queries and pages must both be float16 or both bfloat16")
+    if window is not None and shared_pages is not None:
+        raise ValueError("hexmi.paged_attention: no shared pages within a window (name them in page_table)")
     if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3] or q.shape[1] < 1 or q.shape[1] % max(k_pages.shape[1], 1) != 0:
         raise ValueError("hexmi.paged_attention: q is [tokens, heads, dim], the pages [pages, kv heads, page size, dim], and kv heads "
                          "divides heads")
@@ -1040,13 +1156,81 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
         qd = qd.clone(memory_format=torch.contiguous_format)
     sd = _stage(shared_pages, dev)
     od = _out_like(out, q.shape, q.dtype, dev)
-    read = [t for t in (qd, k_pages, v_pages, table, lens, begin, sd) if t is not None and t.numel()]
+    read = [t for t in (qd, k_pages, v_pages, k_scales, v_scales, table, lens, begin, sd) if t is not None and t.numel()]
     if out is not None and od is out and od.numel() and (od.data_ptr() % 16 or _overlaps(od, *read)):
         od = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if q.shape[0]:
+    if q.shape[0] and (scaled or window is not None):
+        args = (qd, k_pages, v_pages, k_scales, v_scales, table, lens, begin, float(sm_scale), sd, window, sinks, od)
+        _run("paged_attention_ex", _paged_attention_ex_impl, args, *args)
+    elif q.shape[0]:
         args = (qd, k_pages, v_pages, table, lens, begin, float(sm_scale), sd, od)
         _run(name, _paged_attention_impl, args, *args)
     return _finish(od, out)
+
+
+def _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales):
+    """Checks a cache whose pages are copied and returns (page_table, lengths) on its device."""
+    scaled = _check_scales(name, k_pages, k_scales, v_scales)
+    if not scaled and k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("hexmi.%s: pages are float16, bfloat16 or, with scales, float8_e4m3fn" % name)
+    if k_pages.data_ptr() == v_pages.data_ptr():
+        raise ValueError("hexmi.%s: keys and values need pages of their own" % name)
+    return _paged_operands(name, lengths.shape[0] if lengths.dim() == 1 else 0, k_pages, v_pages, page_table, lengths, None)[:2]
+
+
+def _index_out(name, what, out, shape, others, dev):
+    """Where whole numbers are computed: out where it is a device tensor of adjacent columns that shares no memory with what is read, or
+    fresh memory."""
+    if out is not None:
+        if tuple(out.shape) != tuple(shape) or out.dtype != torch.int32:
+            raise ValueError("hexmi.%s: %s must be int32 %s" % (name, what, tuple(shape)))
+        if out.device == dev and out.is_contiguous() and out.numel() and not any(_overlaps(out, t) for t in others if t is not None and t.numel()):
+            return out
+    return torch.empty(shape, dtype=torch.int32, device=dev)
+
+
+def paged_fork(k_pages, v_pages, page_table, lengths, parents, pages, k_scales=None, v_scales=None, table_out=None, lengths_out=None):
+    """Rows that go on from a batch's, as a step of a beam search has them: returns (page_table, lengths) of len(parents) rows, row i a copy
+    of row parents[i] (int32; no row's number: an empty row, -1 throughout) in which pages[i] (int32) is the page of its next token. What the
+    parent's part-filled last page holds is copied there, keys, values and scales of all heads; full pages stay shared, and where pages[i]
+    is no page's number (-1) the last one too (the one row that may go on in it).
+
+    The cache is `paged_append`'s, in 16 or 8 bits, and changed in place; pages are each named once and in no use. All index tensors are
+    read on the GPU only."""
+    name = "paged_fork"
+    for what, t in (("parents", parents), ("pages", pages)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape != parents.shape:
+            raise ValueError("hexmi.paged_fork: %s must be an int32 tensor of one dimension, a value a row" % what)
+    table, lens = _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales)
+    dev, rows = k_pages.device, parents.shape[0]
+    _one_device(name, dev, parents, pages, table_out, lengths_out)
+    from_d, pages_d = _stage(parents, dev), _stage(pages, dev)
+    read = (table, lens, from_d, pages_d, k_pages, v_pages, k_scales, v_scales)
+    to = _index_out(name, "table_out", table_out, (rows, table.shape[1]), read, dev)
+    lens_to = _index_out(name, "lengths_out", lengths_out, (rows,), read + (to,), dev)
+    if rows:
+        args = (k_pages, v_pages, k_scales, v_scales, table, lens, from_d, pages_d, to, lens_to)
+        _run(name, _paged_fork_impl, args, *args)
+    return _finish(to, table_out), _finish(lens_to, lengths_out)
+
+
+def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales=None, window=None, sinks=0, table_out=None):
+    """Moves the pages in use to the front of the cache, and returns (page_table, count): the table with their new names, -1 where an entry is
+    not in use, and an int32 tensor of one element, how many there are; the pages from there on are free. In use is a page that some
+    sequence's row names for positions below its length, within a window those that its last token sees. No more pages
+    than need be are copied: those behind `count`, in rising order, to the free ones before it. The cache, in 16 or 8 bits, is changed in place;
+    table_out may be page_table itself."""
+    name = "paged_compact"
+    window, sinks = _check_window(name, window, sinks)
+    table, lens = _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales)
+    dev = k_pages.device
+    _one_device(name, dev, table_out)
+    same = table_out is not None and table_out.data_ptr() == table.data_ptr() and table_out.stride() == table.stride()
+    to = _index_out(name, "table_out", table_out, table.shape, (None if same else table, lens, k_pages, v_pages, k_scales, v_scales), dev)
+    count = torch.empty(1, dtype=torch.int32, device=dev)
+    args = (k_pages, v_pages, k_scales, v_scales, table, lens, window, sinks, to, count)
+    _run(name, _paged_compact_impl, args, *args)
+    return _finish(to, table_out), count
 
 
 # Above this much multiply-add work the one-launch kernel (32 rows per workgroup, so few workgroups on small

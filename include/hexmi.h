@@ -616,6 +616,94 @@ int hexmi_paged_attention(const hexmi_head_rows *q,
                           float sm_scale, int dtype, void *workspace,
                           int64_t workspace_bytes, hexmi_stream_t stream);
 
+/* The same cache in 8 bits: pages hold OCP e4m3 numbers (dim bytes a key; the
+ * strides of hexmi_paged_batch count bytes then), and every run of `block` slots of a page
+ * (page_size is a multiple of block; a run of a page is block number
+ * s / block) has a scale a head, for keys and for values: a power of two, held
+ * as its biased exponent e + 127 in a byte. Key (value) of head h at slot s of
+ * page p is its number times 2^(k_scales[p * k_page + h * k_head + s / block *
+ * k_block] - 127) (strides in bytes). block: 1 to 64. */
+typedef struct hexmi_paged_scales {
+  uint8_t *k_scales, *v_scales;
+  int64_t k_page, k_head, k_block, v_page, v_head, v_block;
+  int64_t block;
+} hexmi_paged_scales;
+
+/* hexmi_paged_append into a cache in 8 bits. The rows, normed and turned in
+ * fp32, are rounded once, to e4m3: a block's exponent is the least that has the
+ * largest of the call's values of the block (head for head) within 448, in
+ * -15 .. 8 for HEXMI_F16 and -117 .. 120 for HEXMI_BF16 (every number of
+ * the cache is a number of that type then; at the upper end numbers end at
+ * 240). Where older tokens of its sequence stand in the block it does not fall, and
+ * their numbers are rounded again where it rises (which costs only what gets
+ * below e4m3's normal numbers). What a block held of others counts for nothing,
+ * its scale neither. Infinities and NaN become NaN and leave the scale alone.
+ * dim a multiple of 8 up to 256, operand rows and weights on 16-byte
+ * boundaries, pages and their strides on 8-byte ones; HEXMI_ENOTSUP otherwise. Of
+ * two sequences that have new tokens in one block pieces of either are left
+ * there. scales NULL: hexmi_paged_append. */
+int hexmi_paged_append_ex(const hexmi_head_rows *k, const hexmi_head_rows *v,
+                          const hexmi_head_rows *q,
+                          const hexmi_rotation *rotation,
+                          const hexmi_paged_batch *batch,
+                          const hexmi_paged_scales *scales, int dtype,
+                          hexmi_stream_t stream);
+
+/* hexmi_paged_attention of a cache in 8 bits (scales; NULL: in 16) and within a
+ * window (0: none): a token at position p sees the positions j <= p with
+ * j > p - window or j < sinks. What no token of a sequence's new ones sees is
+ * not read, its entries of the table neither, but for whole pages beside what is
+ * seen: those may be none, and what stands there may be anything.
+ * A cache in 8 bits is multiplied as numbers of dtype, exact where its scales
+ * are in hexmi_paged_append_ex's range (dtype fp16 ends at 65504 and has no
+ * steps below 2^-24). Pages on 16-byte boundaries where dim is a multiple of
+ * 16, on 8-byte ones otherwise. No shared pages within a window
+ * (HEXMI_ENOTSUP). Everything else as hexmi_paged_attention. */
+int64_t hexmi_paged_attention_ex_workspace(const hexmi_paged_batch *batch,
+                                           int64_t heads, int64_t shared,
+                                           const hexmi_paged_scales *scales,
+                                           int64_t window, int64_t sinks);
+int hexmi_paged_attention_ex(const hexmi_head_rows *q,
+                             const hexmi_paged_batch *batch,
+                             const hexmi_paged_scales *scales,
+                             const int32_t *shared_pages, int64_t shared,
+                             int64_t window, int64_t sinks, float sm_scale,
+                             int dtype, void *workspace,
+                             int64_t workspace_bytes, hexmi_stream_t stream);
+
+/* Rows that go on from a batch's (a step of a beam search): row i of table_out
+ * [rows, table_cols, leading dim table_out_row] and lengths_out[i] are those of
+ * sequence parents[i] (no sequence's number: an empty row, -1 throughout), and
+ * pages[i], where it is a page's number, becomes the page of the row's next
+ * token: what the parent's part-filled last page holds of its tokens is copied
+ * there (keys, values and scales of all heads), and the entry renamed. A full
+ * last page stays shared, as all before it; a part-filled one does where pages[i] is
+ * no page, and one that is none stays none. pages [rows]: each one once, and no
+ * page that the batch uses (else pieces of either are left there). What the
+ * outputs hold shares no memory with what is read. batch: starts and tokens
+ * are not looked at. dtype: of the pages (16 bits; with scales what they are read as). */
+int hexmi_paged_fork(const hexmi_paged_batch *batch,
+                     const hexmi_paged_scales *scales, const int32_t *parents,
+                     const int32_t *pages, int64_t rows, int32_t *table_out,
+                     int64_t table_out_row, int32_t *lengths_out, int dtype,
+                     hexmi_stream_t stream);
+
+/* The pages in use to the front of the cache: of n pages that a sequence names
+ * for positions below its length (within a window (0: none) those that its
+ * last token sees, sinks among them) those from n on go, in rising order, to the unused
+ * ones below n, in rising order. table_out [sequences, table_cols, leading dim
+ * table_out_row] is the table with their new names, -1 where an entry is not in
+ * use; it may be the table itself. count[0] = n: the pages from n on are free
+ * (and hold what they held). Workspace: 16-byte aligned, not initialised, no state
+ * between calls; two calls that overlap in time need one each. */
+int64_t hexmi_paged_compact_workspace(const hexmi_paged_batch *batch);
+int hexmi_paged_compact(const hexmi_paged_batch *batch,
+                        const hexmi_paged_scales *scales, int64_t window,
+                        int64_t sinks, int32_t *table_out,
+                        int64_t table_out_row, int32_t *count, int dtype,
+                        void *workspace, int64_t workspace_bytes,
+                        hexmi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

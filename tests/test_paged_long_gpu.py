@@ -1,0 +1,682 @@
+"""A paged cache in 8 bits, attention within a window, forks and compaction of pages, against their definitions in 64 bits.
+
+Tolerances, derived: u = eps / 2 is a rounding to the type, e = 2^-24 one to fp32.
+  append     a row is off by 24 e of |a| + |b| before it is rounded (test_paged_gpu.py), to e4m3 by half a step: 2^-4 of the value, half of
+             2^-9 times the scale below the normal numbers. A block's exponent is exact but where the largest value is within 24 e of it of a border;
+             what may come out of either is taken. Older numbers, of four significant bits, are rounded to half a step again. At the type's
+             largest scale numbers end at 240: what is above is off by at most (65504 - 61440) / 65504 < 2^-4 in fp16.
+  attention  numbers times their scales are the type's, so the bound is that of a cache in 16 bits: u (sum w |v| + |o|) for the
+             probabilities' rounding, (dim + 8) e scale sum |q| |k| twice for the scores, 16 e, 2^-25 of a row's largest a key in fp16, u |o|.
+  fork, compact  copies: equal.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+E4M3 = torch.float8_e4m3fn
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+RANGE = {torch.float16: (-15, 8), torch.bfloat16: (-117, 120)}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def values(codes, scales):
+    """Numbers of e4m3 [pages, heads, slots, dim] times their scales, in 64 bits on the CPU."""
+    e = scales.cpu().double() - 127
+    return codes.cpu().double() * torch.exp2(e).repeat_interleave(codes.shape[2] // scales.shape[2], 2)[..., None]
+
+
+def in_order(t, order):
+    """The same tensor with the heads of a token side by side in memory."""
+    return t if order == "head" else t.transpose(1, 2).contiguous().transpose(1, 2)
+
+
+class Long:
+    """A cache and a batch: pages in random order; whatever no new token sees is NaN or has no page, now the one, now the other."""
+
+    def __init__(self, new, context, heads, kv_heads, dim, page, block, dtype, order="head", window=None, sinks=0, seed=0, padding=0, ragged=None,
+                 shared=0):
+        g = _gen(seed)
+        self.new, self.lengths = list(new), [c + n for c, n in zip(context, new)]
+        self.heads, self.kv_heads, self.dim, self.page, self.block, self.dtype = heads, kv_heads, dim, page, block, dtype
+        self.window, self.sinks = window, sinks
+        self.ragged = any(n != 1 for n in new) or padding > 0 if ragged is None else ragged
+        B, T = len(new), sum(new) + padding
+        columns = [-(-n // page) for n in self.lengths]
+        first = shared // page
+        pool = first + sum(max(0, c - first) for c in columns) + 3
+        names = torch.randperm(pool, generator=g)
+        junk = names[-1].item()                                       # a page that is all NaN
+        table = torch.full((B, max(columns + [1]) + 1), -1)
+        self.shared_pages = names[:first].int().cuda() if first else None
+        x = [torch.randn(pool, kv_heads, page, dim, generator=g) for _ in range(2)]
+        if block:
+            blocks = page // block
+            self.scales = [torch.randint(118, 122, (pool, kv_heads, blocks), generator=g, dtype=torch.uint8) for _ in range(2)]
+            x = [(t * 100).clamp(-448, 448).to(E4M3) for t in x]
+            held = [values(t.double(), s) for t, s in zip(x, self.scales)]
+            for t, s in zip(held, self.scales):
+                assert torch.equal(t, t.to(dtype).double())
+        else:
+            self.scales = [None, None]
+            x = [t.to(dtype) for t in x]
+            held = [t.double() for t in x]
+        seen = torch.zeros(pool, page, dtype=torch.bool)
+        used = first
+        self.k64, self.v64 = [], []
+        for b, (n, L) in enumerate(zip(self.new, self.lengths)):
+            table[b, :min(first, columns[b])] = names[:min(first, columns[b])]
+            if columns[b] > first:
+                table[b, first:columns[b]] = names[used:used + columns[b] - first]
+                used += columns[b] - first
+            at = torch.arange(L)
+            mine = (at < sinks) | (at > L - max(n, 1) - window) if window else at >= 0
+            pages = table[b, at // page]
+            seen[pages[mine], at[mine] % page] = True
+            self.k64.append(held[0][pages, :, at % page])
+            self.v64.append(held[1][pages, :, at % page])
+            for c in range(columns[b]):                               # pages that nobody sees
+                if window and not mine[c * page:(c + 1) * page].any():
+                    table[b, c] = (-1, junk, pool, 1 << 30)[(b + c) % 4]
+        if first:
+            seen[names[:first]] = True
+        for t, s in zip(x, self.scales):
+            unseen = ~seen[:, None, :, None].expand(t.shape)
+            if block:
+                t.view(torch.uint8)[unseen] = 0x7f
+            else:
+                t[unseen] = math.nan
+        self.k_pages, self.v_pages = (in_order(t.cuda(), order) for t in x)
+        self.k_scales, self.v_scales = (None if s is None else in_order(s.cuda(), order) for s in self.scales)
+        self.table, self.page_table = table, table.int().cuda()
+        self.lengths_d = torch.tensor(self.lengths, dtype=torch.int32, device="cuda")
+        self.starts = torch.tensor([sum(self.new[:i]) for i in range(B + 1)], dtype=torch.int32, device="cuda") if self.ragged else None
+        self.q = torch.randn(T, heads, dim, generator=g).to(dtype).cuda()
+
+    def kw(self):
+        kw = {"k_scales": self.k_scales, "v_scales": self.v_scales} if self.block else {}
+        return {**kw, "window": self.window, "sinks": self.sinks} if self.window else kw
+
+    def run(self, hexmi, **kw):
+        return hexmi.paged_attention(self.q, self.k_pages, self.v_pages, self.page_table, self.lengths_d, self.starts, **{**self.kw(), **kw})
+
+    def check(self, got, what=""):
+        scale, G, u = 1.0 / math.sqrt(self.dim), self.heads // self.kv_heads, half_step(self.dtype)
+        q = self.q.cpu().double()
+        out, bound = torch.zeros_like(q), torch.zeros_like(q)
+        t = 0
+        for n, L, k, v in zip(self.new, self.lengths, self.k64, self.v64):
+            at, p = torch.arange(L)[None], torch.arange(L - n, L)[:, None]
+            hidden = at > p
+            if self.window:
+                hidden = hidden | (at <= p - self.window) & (at >= self.sinks)
+            for h in range(self.heads if n and L else 0):
+                kh, vh, qh = k[:, h // G], v[:, h // G], q[t:t + n, h]
+                w = torch.softmax((qh @ kh.T * scale).masked_fill(hidden, -math.inf), 1)
+                size = (qh.abs() @ kh.abs().T * scale).masked_fill(hidden, 0).amax(1, keepdim=True)
+                o, a = w @ vh, w @ vh.abs()
+                out[t:t + n, h] = o
+                b = u * (a + o.abs()) + (2 * (self.dim + 8) * E * size + 16 * E) * (a + o.abs()) + u * o.abs()
+                if self.dtype == torch.float16:
+                    b = b + L * 2.0 ** -25 * vh.abs().amax(0) + 2.0 ** -25
+                bound[t:t + n, h] = b
+            t += n
+        assert got.shape == out.shape and got.dtype == self.dtype
+        off = (got.cpu().double() - out).abs()
+        bad = ~(off <= bound)
+        assert not bad.any(), (what, bad.sum().item(), (off / bound.clamp_min(1e-30))[bad].max().item(), bad.nonzero()[:3].tolist())
+
+
+ATTEND = [
+    # new tokens, contexts, heads, kv heads, dim, page, slots a block (0: 16 bits), dtype, order, window, sinks, rows behind the last sequence
+    ([1], [0], 1, 1, 64, 16, 16, "f16", "head", None, 0, 0), ([1, 1, 1], [0, 15, 16], 4, 2, 128, 16, 1, "bf16", "token", None, 0, 0),
+    ([1], [999], 32, 8, 128, 16, 16, "f16", "head", None, 0, 0), ([1] * 10, [15, 16, 17, 31, 32, 33, 62, 63, 64, 65], 8, 2, 128, 32, 8, "bf16", "head", None, 0, 0),
+    ([1] * 5, [127, 128, 255, 256, 257], 12, 12, 64, 64, 64, "bf16", "token", None, 0, 0), ([1] * 3, [500, 3, 77], 20, 1, 128, 3, 3, "f16", "head", None, 0, 0),
+    ([1] * 70, [100] * 70, 4, 4, 64, 100, 50, "f16", "head", None, 0, 0), ([1, 1], [333, 21], 4, 2, 80, 16, 4, "f16", "head", None, 0, 0),
+    ([1, 1], [333, 21], 6, 2, 96, 8, 8, "bf16", "token", None, 0, 0), ([1, 1], [333, 4021], 4, 1, 256, 16, 2, "f16", "head", None, 0, 0),
+    ([1, 1], [90, 200], 5, 1, 8, 7, 7, "f16", "head", None, 0, 0), ([1, 1], [90, 200], 3, 3, 72, 16, 16, "bf16", "head", None, 0, 0),
+    ([1, 1], [90, 700], 4, 2, 136, 16, 16, "f16", "token", None, 0, 0), ([1, 1], [5, 4000], 2, 2, 200, 64, 32, "bf16", "head", None, 0, 0),
+    ([1] * 300, [30] * 300, 2, 1, 64, 16, 16, "bf16", "token", None, 0, 0),
+    ([1, 5, 0, 3], [0, 2, 9, 60], 4, 2, 64, 16, 16, "f16", "head", None, 0, 0), ([200], [0], 8, 2, 128, 16, 8, "bf16", "token", None, 0, 0),
+    ([130, 1, 1, 64], [300, 777, 0, 5], 16, 4, 128, 64, 16, "f16", "head", None, 0, 9), ([63, 64, 65], [1, 0, 64], 3, 3, 128, 32, 32, "bf16", "head", None, 0, 1),
+    ([31, 33], [500, 0], 5, 1, 80, 16, 1, "f16", "token", None, 0, 0), ([70], [70], 6, 2, 96, 7, 7, "bf16", "head", None, 0, 2),
+    ([40, 2], [0, 100], 4, 1, 256, 16, 16, "f16", "head", None, 0, 0), ([129], [1000], 2, 1, 64, 1, 1, "bf16", "head", None, 0, 0),
+    ([12], [7], 4, 2, 24, 16, 16, "f16", "head", None, 0, 0), ([1000, 900], [0, 0], 4, 1, 128, 64, 64, "f16", "head", None, 0, 0),
+    ([300], [0], 4, 4, 160, 64, 16, "bf16", "token", None, 0, 0), ([2], [4090], 8, 1, 128, 64, 32, "f16", "head", None, 0, 0),
+    ([509, 1], [2046, 900], 8, 2, 128, 16, 16, "f16", "head", None, 0, 0),
+    # windows, 16 bits
+    ([1], [0], 2, 1, 64, 16, 0, "f16", "head", 1, 0, 0), ([1] * 4, [0, 1, 2, 700], 4, 2, 128, 16, 0, "bf16", "token", 1, 1, 0),
+    ([1] * 6, [5, 30, 31, 32, 100, 5000], 8, 2, 128, 16, 0, "f16", "head", 32, 0, 0), ([1] * 3, [4000, 70, 300], 32, 8, 128, 64, 0, "bf16", "head", 500, 4, 0),
+    ([1] * 3, [4000, 70, 300], 4, 1, 80, 5, 0, "f16", "token", 129, 7, 0), ([1, 1], [900, 3000], 4, 2, 256, 16, 0, "bf16", "head", 700, 100, 0),
+    ([1] * 70, list(range(0, 700, 10)), 2, 2, 64, 8, 0, "f16", "head", 100, 3, 0), ([1] * 2, [2000, 20000], 2, 1, 96, 256, 0, "f16", "head", 1500, 1, 0),
+    ([200], [0], 8, 2, 128, 16, 0, "bf16", "token", 1, 0, 0), ([300], [0], 4, 1, 64, 16, 0, "f16", "head", 64, 4, 0), ([257], [1000], 4, 2, 128, 16, 0, "f16", "head", 33, 70, 3),
+    ([130, 1, 1, 64], [300, 777, 0, 5], 16, 4, 128, 64, 0, "f16", "head", 100, 10, 9), ([1, 5, 0, 3], [0, 2, 9, 60], 4, 2, 64, 16, 0, "f16", "head", 2, 1, 0),
+    ([1500], [0], 2, 1, 128, 64, 0, "bf16", "head", 200, 4, 0), ([40, 2], [0, 900], 4, 1, 256, 16, 0, "f16", "head", 30, 20, 0),
+    ([60, 70], [3000, 1], 6, 2, 96, 7, 0, "bf16", "token", 1000, 3, 0), ([509, 1], [2046, 900], 8, 2, 128, 16, 0, "f16", "head", 1000, 0, 0),
+    ([3] * 70, [200] * 70, 8, 8, 64, 16, 0, "f16", "head", 50, 5, 5),
+    # windows, 8 bits
+    ([1] * 6, [5, 30, 31, 32, 100, 5000], 8, 2, 128, 16, 16, "f16", "head", 32, 5, 0), ([1] * 3, [4000, 70, 300], 32, 8, 128, 64, 16, "bf16", "token", 500, 4, 0),
+    ([1, 1], [900, 3000], 4, 2, 72, 6, 3, "bf16", "head", 700, 100, 0), ([257], [1000], 4, 2, 128, 16, 4, "f16", "head", 33, 70, 3),
+    ([130, 1, 1, 64], [300, 777, 0, 5], 16, 4, 64, 64, 32, "f16", "head", 100, 10, 9), ([1500], [0], 2, 1, 128, 64, 64, "bf16", "token", 200, 4, 0),
+    ([40, 2], [0, 900], 4, 1, 256, 16, 16, "f16", "head", 30, 20, 0), ([509, 1], [2046, 900], 8, 2, 128, 16, 16, "f16", "head", 1000, 0, 0),
+]
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=lambda c: "x".join(map(str, (len(c[0]), max(c[0]), max(c[1])) + c[2:])))
+def test_attention_against_the_definition(hexmi, case):
+    new, context, heads, kv, dim, page, block, dt, order, window, sinks, padding = case
+    c = Long(new, context, heads, kv, dim, page, block, DTYPES[dt], order, window, sinks, seed=dim + len(new), padding=padding)
+    got = c.run(hexmi)
+    c.check(got)
+    out = torch.full_like(got, 7.0)
+    assert c.run(hexmi, out=out) is out and torch.equal(out, got)
+
+
+@pytest.mark.parametrize("new, context, shared, heads, kv, dim, page, block, dt", [
+    ([1] * 5, [0, 3, 40, 200, 1], 64, 8, 2, 128, 16, 16, "f16"), ([1] * 33, list(range(33)), 1024, 32, 8, 128, 64, 16, "bf16"),
+    ([30, 1, 0, 90], [1, 1, 1, 1], 400, 16, 4, 64, 16, 8, "f16"), ([200, 7], [0, 300], 333, 6, 2, 80, 9, 9, "bf16"),
+    ([1] * 4, [0, 1, 2, 3], 128, 4, 2, 256, 16, 16, "f16"),
+], ids=str)
+def test_shared_prefix_in_8_bits(hexmi, new, context, shared, heads, kv, dim, page, block, dt):
+    c = Long(new, [shared + x for x in context], heads, kv, dim, page, block, DTYPES[dt], seed=dim + len(new), shared=shared)
+    c.check(c.run(hexmi), "each for itself")
+    c.page_table[:, :shared // page] = -7                             # not read
+    c.check(c.run(hexmi, shared_pages=c.shared_pages), "shared")
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_batches(hexmi, seed):
+    rng = random.Random(seed)
+    B, page = rng.randint(1, 6), rng.choice((1, 5, 8, 16, 16, 64, 128))
+    kv = rng.choice((1, 2, 3))
+    block = 0 if rng.random() < 0.3 else rng.choice([b for b in range(1, 65) if page % b == 0])
+    window = rng.choice((1, 3, 17, 64, 100, 333, 2000)) if block == 0 or rng.random() < 0.5 else None
+    new = [rng.choice((1, 1, 0, 2, 33, 150, 300)) for _ in range(B)] if rng.random() < 0.6 else [1] * B
+    c = Long(new, [rng.choice((0, 1, 50, 700, 2500)) for _ in range(B)], kv * rng.choice((1, 2, 5, 17)), kv, rng.choice((16, 64, 64, 128, 104, 192, 256)), page,
+             block, DTYPES[rng.choice(("f16", "bf16"))], rng.choice(("head", "token")), window, rng.choice((0, 1, 4, 90)) if window else 0, seed=seed,
+             padding=rng.choice((0, 0, 3)))
+    c.check(c.run(hexmi))
+
+
+def test_windows_that_hide_nothing_are_none(hexmi):
+    c = Long([40, 1], [300, 777], 8, 2, 128, 16, 0, torch.float16)
+    whole = c.run(hexmi)
+    for window, sinks in ((1 << 70, 0), (1 << 70, 1 << 70), (2000, 0), (1, 2000), (1, 1 << 70)):
+        assert torch.equal(c.run(hexmi, window=window, sinks=sinks), whole), (window, sinks)
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_index_tensors_that_make_no_sense_touch_nothing_outside(hexmi, scaled, ragged):
+    g = _gen(11)
+    pages = [torch.randn(5, 2, 16, 64, generator=g).to(E4M3 if scaled else torch.float16).cuda() for _ in range(2)]
+    kw = {n: torch.full((5, 2, 2), 120, dtype=torch.uint8, device="cuda") for n in ("k_scales", "v_scales")} if scaled else {}
+    q = torch.randn(6, 4, 64, generator=g).half().cuda()
+    B = 4 if ragged else 6
+    lengths = torch.tensor([-(1 << 31), (1 << 31) - 1, 3, 0, 40, 41][:B], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[-(1 << 31), (1 << 31) - 1, 5]] * B, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([3, -9, 1 << 30, 2, 70], dtype=torch.int32, device="cuda") if ragged else None
+    around = torch.full((18, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    out = around[6:12]
+    for window, sinks in ((5, 2), (30, 1 << 50), (None, 0)):
+        hexmi.paged_attention(q, *pages, table, lengths, starts, out=out, window=window, sinks=sinks, **kw)
+        assert (around[:6] == 7).all() and (around[12:] == 7).all()
+        assert ((out == 0) | (out == 7 if ragged else False)).all()
+    if scaled:
+        before = [t.clone() for t in (*pages, *kw.values())]
+        rows = torch.randn(6, 2, 64, generator=g).half().cuda()
+        hexmi.paged_append(rows, rows.clone(), *pages, table, lengths, starts, q=q, inv_freq=hexmi.rope_frequencies(64), **kw)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (*pages, *kw.values())))
+    before = [t.clone() for t in pages]
+    index = torch.tensor([-1, 3, 1 << 30, -(1 << 31), 2, 0, 1], dtype=torch.int32, device="cuda")
+    new_table, new_lengths = hexmi.paged_fork(*pages, table, lengths, index, torch.full_like(index, 1 << 30), **kw)
+    for i, parent in enumerate(index.tolist()):
+        known = 0 <= parent < B
+        assert new_lengths[i].item() == (lengths[parent].item() if known else 0)
+        assert torch.equal(new_table[i], table[parent] if known else torch.full_like(table[0], -1))
+    new_table, count = hexmi.paged_compact(*pages, table, lengths, **kw)
+    assert count.item() == 0 and (new_table == -1).all()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, pages))
+
+
+# ---- appends
+def rows64(x, weight, inv_freq, positions, eps, pairs):
+    """(result, |a| + |b|) of the rows [tokens, heads, dim] in 64 bits on the CPU."""
+    x = x.cpu().double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.cpu().double()
+    size = x.abs()
+    if inv_freq is None:
+        return x, size
+    angle = (positions.cpu().double()[:, None] * inv_freq.cpu())[:, None]
+    c, s, n = angle.cos(), angle.sin(), inv_freq.numel()
+    first = torch.arange(n) * 2 if pairs == "adjacent" else torch.arange(n)
+    second = first + 1 if pairs == "adjacent" else first + n
+    out, a, b = x.clone(), x[..., first], x[..., second]
+    out[..., first], out[..., second] = a * c - b * s, b * c + a * s
+    size[..., first] = size[..., second] = a.abs() + b.abs()
+    return out, size
+
+
+def least_exponent(most, lo, hi):
+    """The least e of lo .. hi with most <= 448 * 2^e."""
+    e = lo
+    while e < hi and most > 448 * 2.0 ** e:
+        e += 1
+    return e
+
+
+def half_steps(value, e):
+    """Half a step of e4m3 times 2^e at a value."""
+    return torch.maximum(value.abs() * 2.0 ** -4, torch.full_like(value, 2.0 ** (e - 10)))
+
+
+def check_appended(pages, scales, before, scales_before, rows, size, new, lengths, table, dtype, ragged):
+    """pages, scales: after a call that put rows [tokens, heads, dim] there; before, scales_before: what stood there."""
+    lo, hi = RANGE[dtype]
+    page = pages.shape[2]
+    block = page // scales.shape[2]
+    now, then = pages.cpu().double(), before.cpu().double()
+    s_now, s_then = scales.cpu().int() - 127, scales_before.cpu().int() - 127
+    touched = torch.zeros(pages.shape[:3], dtype=torch.bool)
+    t = 0
+    for b, (n, L) in enumerate(zip(new, lengths)):
+        for start in range((L - n) // block * block, L, block) if n else ():
+            p = table[b, start // page].item()
+            at = start % page
+            old, end = max(0, L - n - start), min(block, L - start)
+            mine = slice(t + start + old - (L - n), t + start + end - (L - n))
+            touched[p, :, at:at + end] = True
+            for h in range(pages.shape[1]):
+                y, off = rows[mine, h], 24 * E * size[mine, h]
+                most = y.abs().max().item()
+                e = s_now[p, h, at // block].item()
+                could = {least_exponent(m, lo, hi) for m in (most, most - off.max().item(), most + off.max().item())}
+                was = s_then[p, h, at // block].item()
+                if old:
+                    could = {max(x, was) for x in could}
+                assert e in could, (b, start, h, e, could)
+                got = now[p, h, at + old:at + end] * 2.0 ** e
+                wrong = ~((got - y).abs() <= half_steps(y, e) + off)
+                assert not wrong.any(), (b, start, h, (got - y)[wrong][:4], y[wrong][:4])
+                if old:
+                    a, o = then[p, h, at:at + old] * 2.0 ** was, now[p, h, at:at + old] * 2.0 ** e
+                    assert ((a - o).abs() <= (half_steps(a, e) if e > was else torch.zeros(()))).all(), (b, start, h)
+        t += n
+    same = ~touched[..., None].expand(pages.shape)
+    assert torch.equal(pages.cpu().view(torch.uint8)[same], before.cpu().view(torch.uint8)[same])
+
+
+APPEND = [
+    # new tokens, contexts, heads (0: no q), kv heads, dim, rotated columns, page, block, dtype, order, pairs, norms, rows behind the last
+    ([1], [0], 0, 1, 64, 0, 16, 16, "f16", "head", "adjacent", False, 0), ([1] * 5, [0, 15, 16, 17, 100], 4, 2, 128, 128, 16, 16, "f16", "head", "adjacent", False, 0),
+    ([1] * 70, list(range(70)), 32, 8, 128, 128, 16, 8, "bf16", "token", "halves", True, 0), ([1] * 3, [5, 6, 7], 3, 3, 80, 40, 8, 1, "bf16", "head", "halves", True, 0),
+    ([1, 1], [63, 64], 2, 2, 256, 256, 64, 64, "f16", "head", "halves", True, 0), ([1, 1], [63, 9], 5, 5, 8, 8, 32, 32, "f16", "token", "adjacent", True, 0),
+    ([700], [0], 4, 2, 128, 128, 64, 16, "bf16", "token", "halves", True, 0), ([33, 1, 0, 17], [3, 15, 8, 0], 8, 2, 64, 32, 16, 16, "f16", "head", "adjacent", True, 5),
+    ([2, 3, 4, 5] * 9, [14] * 36, 4, 4, 96, 96, 16, 4, "bf16", "head", "halves", False, 1), ([130, 70], [1, 63], 2, 1, 256, 256, 128, 64, "bf16", "head", "halves", True, 0),
+    ([100], [7], 0, 3, 72, 72, 5, 5, "f16", "head", "adjacent", True, 2), ([50, 60], [11, 0], 6, 6, 104, 52, 48, 48, "f16", "token", "halves", True, 0),
+    ([40], [1], 2, 2, 200, 200, 32, 32, "bf16", "head", "adjacent", False, 0), ([5] * 40, [2] * 40, 12, 12, 64, 64, 32, 32, "f16", "head", "halves", False, 3),
+    ([64] * 3, [0, 32, 16], 16, 1, 128, 64, 16, 16, "f16", "head", "halves", True, 0),
+]
+
+
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: "x".join(map(str, (len(c[0]), max(c[0]), max(c[1])) + c[2:])))
+@pytest.mark.parametrize("form", ["slices", "odd"])
+def test_append_against_the_definition(hexmi, case, form):
+    new, context, heads, kv, dim, R, page, block, dt, order, pairs, norms, padding = case
+    g, dtype = _gen(dim + sum(new)), DTYPES[dt]
+    c = Long(new, context, max(heads, kv) // kv * kv, kv, dim, page, block, dtype, order, seed=dim + len(new), padding=padding)
+    T = sum(new) + padding
+    # rows of very different sizes, so that scales rise
+    wide = torch.randn(T + 1, (heads + 2 * kv) * dim + 8, generator=g) * torch.exp2(torch.randint(-6, 5, (T + 1, 1), generator=g).float())
+    wide = wide.to(dtype).cuda()
+    wide = wide.view(-1)[1:1 + T * wide.shape[1]].view(T, -1) if form == "odd" else wide[:T]            # two bytes off the boundaries
+    q, k, v = (wide[:, a:a + n * dim].unflatten(1, (n, dim)) if n else None for a, n in ((0, heads), (heads * dim, kv), ((heads + kv) * dim, kv)))
+    weight = lambda: (1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).cuda() if norms else None
+    kw, qw = weight(), weight() if heads else None
+    freq = hexmi.rope_frequencies(R) if R else None
+    before = [t.clone() for t in (c.k_pages, c.v_pages, c.k_scales, c.v_scales)]
+    got = hexmi.paged_append(k, v, c.k_pages, c.v_pages, c.page_table, c.lengths_d, c.starts, kw, freq, 1e-5, pairs, q, qw, k_scales=c.k_scales,
+                             v_scales=c.v_scales)
+    at = torch.cat([torch.arange(L - n, L) for n, L in zip(new, c.lengths)] + [torch.zeros(padding, dtype=torch.long)])
+    ragged = c.starts is not None
+    check_appended(c.k_pages, c.k_scales, before[0], before[2], *rows64(k, kw, freq, at, 1e-5, pairs), new, c.lengths, c.table, dtype, ragged)
+    check_appended(c.v_pages, c.v_scales, before[1], before[3], v.cpu().double(), torch.zeros(v.shape, dtype=torch.float64), new, c.lengths, c.table,
+                   dtype, ragged)
+    if heads:
+        want, size = rows64(q, qw, freq, at, 1e-5, pairs)
+        want[T - padding:], size[T - padding:] = 0, 0
+        bound = half_step(dtype) * want.abs() + 24 * E * size + torch.finfo(dtype).tiny * half_step(dtype)
+        assert ((got.cpu().double() - want).abs() <= bound).all()
+    else:
+        assert got is None
+
+
+def one_block(hexmi, rows, contexts, dtype, block=16, **kw):
+    """Values put one call after the other into a cache of one head of 64; (numbers, exponents)."""
+    pages = [torch.full((2, 1, 16, 64), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2)]
+    scales = [torch.full((2, 1, 16 // block), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]      # what was there before is nothing
+    table = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    for x, n in zip(rows, contexts):
+        x = x.to(dtype).cuda().view(1, 1, 64)
+        hexmi.paged_append(x, x.clone(), *pages, table, torch.tensor([n + 1], dtype=torch.int32, device="cuda"), k_scales=scales[0], v_scales=scales[1], **kw)
+    for t, s in zip(pages, scales):
+        assert torch.equal(t.view(torch.uint8), pages[0].view(torch.uint8)) and torch.equal(s, scales[0])
+        assert (t[0].view(torch.uint8) == 0x7f).all() and (s[0] == 255).all()
+    return pages[0][1, 0].cpu(), scales[0][1, 0].cpu().int() - 127
+
+
+def test_scales_rise_and_do_not_fall_within_a_block(hexmi):
+    one, two = torch.full((64,), 1.75), torch.full((64,), 0.875)
+    codes, e = one_block(hexmi, [two, one, two, one * 2 ** 6, two], range(5), torch.float16)
+    assert e.item() == -2                                             # 112 = 448 / 4
+    assert torch.equal(codes[:5].float() * 0.25, torch.stack((two, one, two, one * 64, two)))
+    codes, e = one_block(hexmi, [one * 64, two, two], (14, 15, 0), torch.float16)        # the block's first slot again: a new sequence's
+    assert e.item() == -9 and torch.equal(codes[0].float() * 2.0 ** -9, two)
+    # blocks of four: the second one's scale is its own (the first slots are written before, as a sequence's older tokens are)
+    codes, e = one_block(hexmi, [two, two, two, one, one * 4, one], range(6), torch.bfloat16, block=4)
+    assert e[:2].tolist() == [-8, -6]
+    assert torch.equal(codes[3:6].float() * torch.exp2(e[:2].float()).repeat_interleave(4)[3:6, None], torch.stack((one, one * 4, one)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_at_the_ends(hexmi, dtype):
+    lo, hi = RANGE[dtype]
+    most = torch.finfo(dtype).max
+    row = torch.zeros(64)
+    codes, e = one_block(hexmi, [row], [0], dtype)
+    assert e.item() == lo and (codes[0].float() == 0).all()
+    row[:6] = torch.tensor([most, -most, most * 0.75, 1.0, -0.0, most * 0.9375])
+    codes, e = one_block(hexmi, [row], [0], dtype)
+    got = codes[0].double() * 2.0 ** e.item()
+    assert e.item() == hi and torch.equal(got.to(dtype).double(), got)          # numbers of the type, none of them infinite
+    assert ((got - row.to(dtype).double()).abs() <= row.to(dtype).double().abs() * 2.0 ** -4 + 2.0 ** (hi - 10)).all()
+    row = torch.full((64,), 1.0)
+    row[3], row[4], row[5] = math.inf, -math.inf, math.nan
+    codes, e = one_block(hexmi, [row], [0], dtype)
+    assert e.item() == -8 and torch.isnan(codes[0, 3:6].float()).all() and (codes[0, 6:].float() == 256).all() and (codes[0, :3].float() == 256).all()
+    codes, e = one_block(hexmi, [row, torch.full((64,), 8.0)], [0, 1], dtype)     # NaN stays one as the scale rises
+    assert e.item() == -5 and torch.isnan(codes[0, 3:6].float()).all() and (codes[0, 6:].float() == 32).all()
+    tiny = torch.full((64,), 2.0 ** (lo - 9))
+    codes, e = one_block(hexmi, [tiny], [0], dtype)
+    assert e.item() == lo and (codes[0].float() == 2.0 ** -9).all()
+    # every border between two exponents: 448 * 2^e and the next number
+    for x in (1.75, 1.0, 1.5, 0.4375):
+        above = torch.nextafter(torch.tensor(x, dtype=torch.float32), torch.tensor(9.0)) if dtype == torch.float32 else torch.tensor(x) * (1 + torch.finfo(dtype).eps)
+        for y in (torch.tensor(x), above):
+            y = y.to(dtype).float()
+            _, e = one_block(hexmi, [torch.full((64,), y.item())], [0], dtype)
+            assert e.item() == least_exponent(y.item(), lo, hi), (x, y.item())
+
+
+def test_every_number_of_e4m3_is_rounded_to_even(hexmi):
+    """All numbers and the middles between neighbours, at a scale of 1 (the largest is 448)."""
+    numbers = torch.arange(127, dtype=torch.uint8).view(E4M3).double()
+    middles = (numbers[1:] + numbers[:-1]) / 2
+    all_of = torch.cat((numbers, middles, -numbers, -middles))
+    for i in range(0, all_of.numel(), 60):
+        row = torch.zeros(64, dtype=torch.float64)
+        row[:min(60, all_of.numel() - i)] = all_of[i:i + 60]
+        row[63] = 448
+        x = row.to(torch.float16)
+        assert torch.equal(x.double(), row)
+        codes, e = one_block(hexmi, [x], [0], torch.float16)
+        assert e.item() == 0 and torch.equal(codes[0].view(torch.uint8), row.float().to(E4M3).view(torch.uint8))
+
+
+# ---- forks and compaction
+def fork_reference(c, parents, pages):
+    """(table, lengths, copies (from, to, slots))."""
+    table, lengths, copies = [], [], []
+    for parent, page in zip(parents, pages):
+        if not 0 <= parent < len(c.lengths):
+            table.append([-1] * c.table.shape[1])
+            lengths.append(0)
+            continue
+        row, L = c.table[parent].tolist(), c.lengths[parent]
+        column, filled = min(L, len(row) * c.page) // c.page, min(L, len(row) * c.page) % c.page
+        if 0 <= page < c.k_pages.shape[0] and column < len(row) and (filled == 0 or 0 <= row[column] < c.k_pages.shape[0]):
+            if filled:
+                copies.append((row[column], page, filled))
+            row[column] = page
+        table.append(row)
+        lengths.append(L)
+    return torch.tensor(table, dtype=torch.int32), torch.tensor(lengths, dtype=torch.int32), copies
+
+
+def raw(t):
+    return t.contiguous().view(torch.uint8) if t.dtype == E4M3 else t.contiguous().view(torch.int16) if t.dtype != torch.uint8 else t
+
+
+FORK = [
+    # contexts, rows, kv heads, dim, page, block (0: 16 bits), dtype, order
+    ([0], 1, 1, 64, 16, 0, "f16", "head"), ([600, 601, 615, 15], 4, 8, 128, 16, 0, "f16", "head"), ([599, 31, 32, 33, 0], 200, 2, 80, 16, 0, "bf16", "token"),
+    ([100, 2000, 255, 256], 50, 8, 128, 256, 32, "bf16", "token"), ([100, 2000, 255], 7, 3, 96, 128, 16, "f16", "head"), ([9, 5, 3], 30, 1, 8, 5, 5, "f16", "head"),
+    ([40] * 70, 70, 2, 72, 7, 1, "bf16", "head"), ([40, 3], 5, 2, 36, 16, 0, "f16", "head"), ([40, 3], 5, 2, 20, 16, 2, "f16", "token"), ([40, 3], 5, 3, 7, 16, 16, "f16", "head"),
+]
+
+
+@pytest.mark.parametrize("case", FORK, ids=lambda c: "x".join(map(str, (len(c[0]), max(c[0])) + c[1:])))
+def test_fork_against_the_definition(hexmi, case):
+    context, rows, kv, dim, page, block, dt, order = case
+    rng = random.Random(rows)
+    c = Long([1] * len(context), context, kv, kv, dim, page, block, DTYPES[dt], order, seed=rows)
+    pool = c.k_pages.shape[0]
+    tensors = [t for t in (c.k_pages, c.v_pages, c.k_scales, c.v_scales) if t is not None]
+    grown = [in_order(torch.cat((t.contiguous(), t[:1].expand(rows, *t.shape[1:]))), order) for t in tensors]      # fresh pages behind
+    c.k_pages, c.v_pages = grown[:2]
+    scales = dict(zip(("k_scales", "v_scales"), grown[2:]))
+    parents = [rng.randrange(len(context)) if rng.random() < 0.9 else rng.choice((-1, len(context), 1 << 30)) for _ in range(rows)]
+    pages = [pool + i if rng.random() < 0.85 else rng.choice((-1, pool + rows, 1 << 30)) for i in range(rows)]
+    table, lengths, copies = fork_reference(c, parents, pages)
+    want = [t.clone() for t in grown]
+    for a, b, filled in copies:
+        for t in want[:2]:
+            raw_t = t.view(torch.uint8) if block else t
+            raw_t[b, :, :filled] = raw_t[a, :, :filled]
+        for t in want[2:]:
+            t[b, :, :-(-filled // block)] = t[a, :, :-(-filled // block)]
+    index = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    got = hexmi.paged_fork(c.k_pages, c.v_pages, c.page_table, c.lengths_d, index(parents), index(pages), **scales)
+    assert torch.equal(got[0].cpu(), table) and torch.equal(got[1].cpu(), lengths)
+    for a, b in zip(grown, want):
+        assert torch.equal(raw(a), raw(b))
+    # into tensors of the caller's, one of them the table itself
+    outs = torch.full_like(got[0], 9), torch.full_like(got[1], 9)
+    again = hexmi.paged_fork(c.k_pages, c.v_pages, c.page_table, c.lengths_d, index(parents), index(pages), table_out=outs[0], lengths_out=outs[1], **scales)
+    assert again[0] is outs[0] and again[1] is outs[1] and torch.equal(outs[0], got[0]) and torch.equal(outs[1], got[1])
+    if rows == len(context):
+        hexmi.paged_fork(c.k_pages, c.v_pages, c.page_table, c.lengths_d, index(parents), index(pages), table_out=c.page_table, lengths_out=c.lengths_d, **scales)
+        assert torch.equal(c.page_table, got[0]) and torch.equal(c.lengths_d, got[1])
+
+
+def compact_reference(table, lengths, pool, page, window, sinks):
+    used = [[0 <= c < pool and i * page < min(L, len(row) * page) and (not window or i * page < sinks or (i + 1) * page > min(L, len(row) * page) - window)
+             for i, c in enumerate(row)] for row, L in zip(table, lengths)]
+    marked = {c for row, u in zip(table, used) for c, x in zip(row, u) if x}
+    n = len(marked)
+    moves = dict(zip(sorted(p for p in marked if p >= n), sorted(set(range(n)) - marked)))
+    return [[moves.get(c, c) if x else -1 for c, x in zip(row, u)] for row, u in zip(table, used)], n, moves
+
+
+COMPACT = [
+    # lengths, pool, columns, kv heads, dim, page, block, dtype, order, window, sinks
+    ([], 5, 3, 1, 64, 16, 0, "f16", "head", None, 0), ([0, 0], 5, 3, 1, 64, 16, 0, "f16", "head", None, 0), ([40, 16, 17, 0, 48], 20, 3, 2, 128, 16, 0, "f16", "head", None, 0),
+    ([100, 90, 7], 64, 8, 2, 80, 16, 16, "bf16", "token", None, 0), ([100, 90, 7], 32, 8, 2, 80, 16, 4, "bf16", "head", None, 0), ([1000] * 30, 2000, 64, 2, 64, 16, 0, "bf16", "head", None, 0),
+    ([1000, 77, 3000], 700, 200, 3, 20, 16, 2, "f16", "head", 100, 20), ([1000, 77, 3000], 33333, 200, 1, 8, 16, 16, "f16", "token", 1, 0), ([128], 8, 8, 1, 64, 16, 0, "f16", "head", None, 0),
+    ([64 * 16], 64, 64, 1, 64, 16, 0, "f16", "head", None, 0), ([500, 400], 200, 500, 2, 7, 1, 1, "f16", "head", 50, 3), ([9] * 100, 100, 1, 1, 16, 9, 0, "f16", "head", None, 0),
+]
+
+
+@pytest.mark.parametrize("case", COMPACT, ids=lambda c: "x".join(map(str, (len(c[0]), sum(c[0])) + c[1:])))
+def test_compact_against_the_definition(hexmi, case):
+    lengths, pool, columns, kv, dim, page, block, dt, order, window, sinks = case
+    g, rng = _gen(pool), random.Random(pool)
+    shape = (pool, kv, page, dim)
+    pages = [in_order((torch.randint(0, 256, shape, generator=g, dtype=torch.uint8).view(E4M3) if block else torch.randn(shape, generator=g).to(DTYPES[dt])).cuda(), order)
+             for _ in range(2)]
+    scales = {n: torch.randint(0, 256, (pool, kv, page // block), generator=g, dtype=torch.uint8).cuda() for n in ("k_scales", "v_scales")} if block else {}
+    # some pages are several sequences', some none, some no page's number; entries past a length are whatever
+    names = torch.randperm(pool, generator=g).tolist()
+    table = [[rng.choice((names[(b * columns + i) % pool], names[(b * columns + i) % pool], names[i % pool], names[(b * columns + i) % pool], -1 if rng.random() < 0.2 else names[0]))
+              if rng.random() < 0.97 else rng.choice((-1, pool, 1 << 30)) for i in range(columns)] for b in range(len(lengths))]
+    if len(lengths) == 1 or len(lengths) == 100:
+        table = [[names[(b * columns + i) % pool] for i in range(columns)] for b in range(len(lengths))]        # every page in use
+    want, n, moves = compact_reference(table, lengths, pool, page, window, sinks)
+    held = [t.clone() for t in (*pages, *scales.values())]
+    for t in held:
+        flat = t.view(torch.uint8) if t.dtype == E4M3 else t
+        source = flat.clone()
+        for a, b in moves.items():
+            flat[b] = source[a]
+    page_table = torch.tensor(table, dtype=torch.int32, device="cuda").view(len(lengths), columns)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    kw = {**scales, "window": window, "sinks": sinks}
+    got, count = hexmi.paged_compact(*pages, page_table, lens, **kw)
+    assert count.tolist() == [n] and got.tolist() == want
+    for a, b in zip((*pages, *scales.values()), held):
+        assert torch.equal(raw(a), raw(b))
+    # nothing is left to move, and the table may be its own result
+    kept = got.clone()
+    result, count = hexmi.paged_compact(*pages, got, lens, table_out=got, **kw)
+    assert result is got and count.tolist() == [n] and torch.equal(got, kept)
+    for a, b in zip((*pages, *scales.values()), held):
+        assert torch.equal(raw(a), raw(b))
+
+
+# ---- a run of them
+def step(hexmi, state, x, freq, graph=False):
+    q = hexmi.paged_append(x[:, 4:6], x[:, 6:], state["k"], state["v"], state["table"], state["lengths"], inv_freq=freq, q=x[:, :4], k_scales=state["ks"],
+                           v_scales=state["vs"])
+    return hexmi.paged_attention(q, state["k"], state["v"], state["table"], state["lengths"], window=40, sinks=4, k_scales=state["ks"], v_scales=state["vs"])
+
+
+def small_state(seed, rows=3):
+    g = _gen(seed)
+    state = {"k": (torch.randn(40, 2, 16, 64, generator=g) * 50).to(E4M3).cuda(), "v": (torch.randn(40, 2, 16, 64, generator=g) * 50).to(E4M3).cuda(),
+             "ks": torch.full((40, 2, 2), 121, dtype=torch.uint8, device="cuda"), "vs": torch.full((40, 2, 2), 122, dtype=torch.uint8, device="cuda"),
+             "lengths": torch.tensor([30, 47, 80][:rows], dtype=torch.int32, device="cuda"),
+             "table": torch.randperm(40, generator=g)[:rows * 8].view(rows, 8).int().cuda()}
+    return state
+
+
+def test_beams_that_fork_and_compact_go_on_as_without(hexmi):
+    """Decode steps of three rows; every row forked into two, the pages compacted, and on: the same as rows that kept pages of their own."""
+    freq = hexmi.rope_frequencies(64)
+    g = _gen(1)
+    xs = [torch.randn(3, 8, 64, generator=g).half().cuda() for _ in range(40)]
+    a = small_state(5)
+    apart = {n: t.clone() for n, t in a.items()}
+    for x in xs[:5]:
+        for s in (a, apart):
+            s["lengths"] += 1
+        assert torch.equal(step(hexmi, a, x, freq), step(hexmi, apart, x, freq))
+    fresh = torch.tensor([p for p in range(40) if p not in set(a["table"].flatten().tolist())][:6], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([2, 0, 1, 1, 0, 2], dtype=torch.int32, device="cuda")
+    table, lengths = hexmi.paged_fork(a["k"], a["v"], a["table"], a["lengths"], parents, fresh, k_scales=a["ks"], v_scales=a["vs"])
+    a["table"], a["lengths"] = table, lengths
+    for i, x in enumerate(xs[5:12]):
+        both = torch.randn(6, 8, 64, generator=g).half().cuda()
+        a["lengths"] += 1
+        apart["lengths"] += 1
+        got = step(hexmi, a, both, freq)
+        if i == 3:                                                    # in the middle: the table renamed, pages moved
+            a["table"], count = hexmi.paged_compact(a["k"], a["v"], a["table"], a["lengths"], k_scales=a["ks"], v_scales=a["vs"], window=40, sinks=4)
+            assert 0 < count.item() <= 40
+            again = hexmi.paged_attention(torch.ones(6, 4, 64, device="cuda").half(), a["k"], a["v"], a["table"], a["lengths"], window=40, sinks=4,
+                                          k_scales=a["ks"], v_scales=a["vs"])
+            assert torch.isfinite(again).all()
+            free = iter(range(count.item(), 40))                      # every row's next pages
+            for r in range(6):
+                for col in range((a["lengths"][r].item() + 15) // 16, 8):
+                    a["table"][r, col] = next(free, -1)
+        if i == 0:
+            # rows 1, 2 and 0 of the fork go on as rows 0, 1 and 2 of the batch apart
+            first = step(hexmi, apart, both[[1, 2, 0]], freq)
+            assert torch.equal(got[[1, 2, 0]], first)
+        else:
+            assert torch.equal(got[[1, 2, 0]], step(hexmi, apart, both[[1, 2, 0]], freq)), i
+
+
+def test_a_captured_step_is_replayed(hexmi):
+    """Append, attention within a window, fork and compaction in one graph, replayed as lengths and tables change, with eager work between."""
+    freq = hexmi.rope_frequencies(64)
+    g = _gen(2)
+    state, x = small_state(6), torch.zeros(3, 8, 64, dtype=torch.float16, device="cuda")
+    parents, pages = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    def all_of(s):
+        out = step(hexmi, s, x, freq)
+        table, lengths = hexmi.paged_fork(s["k"], s["v"], s["table"], s["lengths"], parents, pages, k_scales=s["ks"], v_scales=s["vs"])
+        packed, count = hexmi.paged_compact(s["k"], s["v"], table, lengths, k_scales=s["ks"], v_scales=s["vs"], window=40, sinks=4)
+        return out, table, lengths, packed, count
+
+    warm = {n: t.clone() for n, t in state.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        all_of(warm)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = all_of(state)
+    fresh = small_state(6)
+    for name in state:
+        state[name].copy_(fresh[name])
+    eager = {n: t.clone() for n, t in state.items()}
+    free = [p for p in range(40) if p not in set(fresh["table"].flatten().tolist())]
+    for i in range(5):
+        x.copy_(torch.randn(3, 8, 64, generator=g).half())
+        parents.copy_(torch.tensor([i % 3, 2, 0], dtype=torch.int32))
+        pages.copy_(torch.tensor(free[3 * i % 12:3 * i % 12 + 3], dtype=torch.int32))
+        for s in (state, eager):
+            s["lengths"] += 1
+        graph.replay()
+        want = all_of(eager)
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            assert torch.equal(a, b), i
+        for name in state:
+            assert torch.equal(raw(state[name]) if name in "kv" else state[name], raw(eager[name]) if name in "kv" else eager[name]), (i, name)
+
+
+def test_calls_on_two_streams(hexmi):
+    c = [Long([1] * 4, [700, 33, 2000, 90], 8, 2, 128, 16, 16, torch.float16, seed=s, window=300, sinks=4) for s in (1, 2)]
+    want = [x.run(hexmi) for x in c]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(c[i].run(hexmi))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_through_the_dispatcher_and_host_index_tensors(hexmi):
+    c = Long([3, 1], [40, 90], 4, 2, 64, 16, 8, torch.float16, window=30, sinks=2, seed=3)
+    got = c.run(hexmi)
+    c.page_table, c.lengths_d, c.starts = c.page_table.cpu(), c.lengths_d.cpu(), c.starts.cpu()
+    assert torch.equal(c.run(hexmi), got)
+    previous = hexmi.through_dispatcher(True)
+    try:
+        assert torch.equal(c.run(hexmi), got)
+        index = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+        a = hexmi.paged_fork(c.k_pages, c.v_pages, c.page_table, c.lengths_d, index, torch.full_like(index, -1), c.k_scales, c.v_scales)
+        b = hexmi.paged_compact(c.k_pages, c.v_pages, c.page_table, c.lengths_d, c.k_scales, c.v_scales)
+    finally:
+        hexmi.through_dispatcher(previous)
+    assert torch.equal(a[0].cpu(), c.page_table[[1, 0]]) and b[0].shape == c.page_table.shape
