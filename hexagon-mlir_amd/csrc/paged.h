@@ -73,6 +73,21 @@ template <> inline constexpr int kMostExponent<f16> = 8;
 // 2^e of a normal number
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
+// eight numbers of e4m3 times a power of two, in T
+template <typename T>
+__device__ __forceinline__ auto widened(uint32_t lo, uint32_t hi, float scale) {
+  if constexpr (std::is_same_v<T, f16>) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true),
+                c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),
+                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+}
+
 // The sequence of row t: the last b with starts[b] <= t, by the 64 lanes of a wave together (t the same for all): 64 places are asked
 // at once, so 64 sequences take one read and 4096 two. -1: none (below starts[0], from starts[sequences] on).
 __device__ __forceinline__ int sequence_of(const Pages& p, int t, int lane) {
@@ -131,6 +146,19 @@ template <int D, int COLS, bool PADDED> constexpr int copied_column(int c, int d
 template <typename T> constexpr float kLift = 0.0f;
 template <> inline constexpr float kLift<f16> = 7.0f;
 
+// What a cache holds and which of it a token sees: 16 bits, all up to its own position; the same within a window; 8 bits, within a window
+// that may be as wide as any cache. Kernels of their own, so that the first pays for neither.
+struct Whole {
+  static constexpr bool kScaled = false, kWindow = false;
+};
+struct Windowed {
+  static constexpr bool kScaled = false, kWindow = true;
+};
+struct Scaled {
+  static constexpr bool kScaled = true, kWindow = true;
+};
+constexpr int kNoWindow = 0x7fffffff;
+
 // What attention over the pages takes beside them (paged_attn.hip, paged_decode.hip).
 struct PagedAttnArgs {
   const void *q, *k, *v;
@@ -140,6 +168,8 @@ struct PagedAttnArgs {
   int prefix, heads, group, dim;               // group: query heads of a key head
   float scale;                                 // sm_scale * log2 e
   Divider by_group;
+  int window, sinks, view;                     // of a windowed kind; view: the most keys that a token sees, kNoWindow for any
+  Scales scales;                               // of a scaled one
 };
 // Sums that several workgroups hold of a row: slot i of row (token * heads + head) has the row's unnormalised output, dim floats at
 // o + (i * rows + row) * dim, and (maximum in log2 units, sum) at ml[i * rows + row]; sum 0: no key, and o is not written.
@@ -175,14 +205,23 @@ struct DecodeArgs {
   int own;                                     // otherwise the slot of the sequences' own keys
   bool join_all;                               // own is the last slot, and every unit is joined with the prefix's sums
 };
-PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix);
+PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix, int64_t view);
 int64_t paged_decode_workspace(const PagedDecodePlan& plan, int64_t dim);
 // One new token a sequence, or those sequences of a batch that have one, with the tiles (none: splits and shared_splits 0) of the prefix and the
 // others. Rows whose sums are to be joined (tiles.sums) are left there, but for one token a sequence throughout.
 int paged_decode(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, int dtype, void* workspace, const TileArgs& tiles,
                  hipStream_t s);
-// tiles and `grid` workers in one launch (paged_shared.hip)
-int paged_shared_decode(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
+// The kernels of a kind, each instantiated in a file of its own or in one of the kind's: tiles (paged_tile.h), decode workers (paged_decode.h),
+// both in one launch (paged_shared.h).
+template <typename Kind> int launch_paged_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, int dtype, hipStream_t s);
+template <typename Kind>
+int launch_paged_workers(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned grid, int dtype, hipStream_t s);
+template <typename Kind>
+int launch_paged_shared(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
                         hipStream_t s);
+// f of the kind that a call is of
+template <typename F> int with_kind(const PagedAttnArgs& a, F&& f) {
+  return a.scales.k ? f(Scaled{}) : a.view != kNoWindow ? f(Windowed{}) : f(Whole{});
+}
 
 }  // namespace hexmi

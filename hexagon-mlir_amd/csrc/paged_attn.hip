@@ -6,14 +6,6 @@
 namespace hexmi {
 namespace {
 
-template <typename T, int D, int COLS, bool PADDED, typename Shape>
-__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : D == 64 ? 3 : 2)
-void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
-  __shared__ __attribute__((aligned(16))) T lds[Shape::lds_elements(D)];
-  __shared__ float m_lds[Shape::kGroups][Shape::kRows], l_lds[Shape::kGroups][Shape::kRows];
-  paged_tile<T, D, COLS, PADDED, Shape>(a, p, w, blockIdx.x, gridDim.x, lds, m_lds, l_lds);
-}
-
 // A row's sums of all slots (at most 32) joined: 32 threads a row, a thread the columns d and, past 128, d + 128.
 template <typename T>
 __global__ __launch_bounds__(256)
@@ -61,19 +53,6 @@ void paged_join_kernel(PagedAttnArgs a, RowSums sums) {
     if (d + h * 128 < a.dim) store4o<T>(to + d + h * 128, out[h][0] * inv, out[h][1] * inv, out[h][2] * inv, out[h][3] * inv);
 }
 
-template <typename T>
-int launch_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, hipStream_t s) {
-  const unsigned grid = (unsigned)(((int64_t)w.tiles * w.splits + (int64_t)w.shared_tiles * w.shared_splits) * p.kv_heads);
-  auto launch = [&](auto width, auto shape) {
-    typedef decltype(width) W;
-    typedef decltype(shape) Shape;
-    hipLaunchKernelGGL((paged_tile_kernel<T, W::D, W::COLS, W::PADDED, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);
-    return launch_status();
-  };
-  return w.deep ? with_width<128>(a.dim, [&](auto width) { return launch(width, DeepTile{}); })
-                : with_width<256>(a.dim, [&](auto width) { return launch(width, WideTile{}); });
-}
-
 // What a call launches: the prefix's tiles (prefix_splits 0: none), then one token a sequence (decode) or tiles of the sequences' own keys
 // (splits), then the join of the tiles' sums.
 struct Plan {
@@ -94,10 +73,10 @@ int parts_of(int64_t units, int64_t keys, int64_t wanted, int64_t least, int64_t
 // sequence. As wide / 8192 columns of 16, 32 heads of 128 over 8, us: one prompt of 40 tokens 7.6 / 14.1, of 400 14.6 / 22.6, of 1000 26.9 / 37.2 (parts
 // that nothing fills, and their join), of 2000 54.9 / 54.8; 64 decoding behind 99 10.5 / 12.7; one behind 999, 64 behind 99 .. 16383, 509
 // tokens beside 15 single ones and 4 x 4096 are level.
-Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
+Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t view) {
   Plan plan = {};
   const int64_t group = heads / b.kv_heads, prefix = shared * b.page_size, rows = b.tokens * group, cus = hexmi_num_cus();
-  const int64_t own = b.table_cols * b.page_size - prefix;
+  const int64_t there = b.table_cols * b.page_size, own = (there < view ? there : view) - prefix;
   plan.decode = b.starts == nullptr;
   plan.rows = b.tokens * heads;
   const int64_t wide = (rows + WideTile::kRows - 1) / WideTile::kRows * b.kv_heads;
@@ -124,7 +103,7 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
     plan.prefix_splits = parts_of(full * b.kv_heads, prefix, wanted, plan.decode ? 128 : 256, plan.decode ? (sets < 31 ? sets : 31) : 16);
   }
   if (plan.workers) {
-    plan.one = plan_paged_decode(b, heads, prefix);
+    plan.one = plan_paged_decode(b, heads, prefix, view);
     plan.decode_bytes = (paged_decode_workspace(plan.one, b.dim) + 15) / 16 * 16;
   }
   if (!plan.decode) {
@@ -136,12 +115,24 @@ Plan plan_of(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
 }
 
 }  // namespace
+
+template int launch_paged_tiles<Whole>(const PagedAttnArgs&, const Pages&, const TileArgs&, int, hipStream_t);
+
 }  // namespace hexmi
 
 using namespace hexmi;
 
 namespace {
-int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
+// What a call sees of its cache: window 0: all of it.
+struct Seen {
+  int window, sinks;
+  int64_t view;
+};
+Seen seen_of(const hexmi_paged_batch& b, int64_t window, int64_t sinks) {
+  const int w = window_of(window, sinks, b.table_cols * b.page_size);
+  return w ? Seen{w, (int)sinks, (int64_t)w + sinks} : Seen{0, 0, kNoWindow};
+}
+int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t view) {
   const int rc = check_batch(b);
   if (rc != HEXMI_OK) return rc;
   if (heads < 1 || heads % b.kv_heads != 0 || shared < 0 || shared > b.table_cols) return HEXMI_EINVAL;
@@ -152,23 +143,20 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared) {
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   if (b.tokens == 0) return HEXMI_OK;          // nothing to launch: there is no plan of it (plan_of divides by the tiles)
-  const Plan plan = plan_of(b, heads, shared);
+  const Plan plan = plan_of(b, heads, shared, view);
   if (plan.slots() > 0 && plan.rows > limit / 32) return HEXMI_ENOTSUP;         // 32 threads a row join them
   const int64_t workers = b.sequences > limit / 1024 / units ? limit : b.sequences * units;
   return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads + workers <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
 }
-}  // namespace
-
-extern "C" int64_t hexmi_paged_attention_workspace(const hexmi_paged_batch* batch, int64_t heads, int64_t shared) {
-  if (!batch || check(*batch, heads, shared) != HEXMI_OK || batch->tokens == 0) return 0;
-  const Plan plan = plan_of(*batch, heads, shared);
+int64_t workspace_of(const hexmi_paged_batch* batch, int64_t heads, int64_t shared, int64_t view) {
+  if (!batch || check(*batch, heads, shared, view) != HEXMI_OK || batch->tokens == 0) return 0;
+  const Plan plan = plan_of(*batch, heads, shared, view);
   return plan.decode_bytes + plan.sum_bytes;
 }
-
-extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const int32_t* shared_pages, int64_t shared,
-                                     float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
-  if (!q || !batch || (shared > 0 && !shared_pages) || workspace_bytes < 0) return HEXMI_EINVAL;
-  int rc = check(*batch, q->heads, shared);
+int attend(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, const int32_t* shared_pages, int64_t shared,
+           const Seen& seen, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
+  if ((shared > 0 && !shared_pages) || workspace_bytes < 0) return HEXMI_EINVAL;
+  int rc = check(*batch, q->heads, shared, seen.view);
   if (rc != HEXMI_OK) return rc;
   if (!(sm_scale > 0.0f) || sm_scale > 2e38f) return HEXMI_EINVAL;
   if (dtype != HEXMI_F16 && dtype != HEXMI_BF16) return HEXMI_ENOTSUP;
@@ -176,18 +164,22 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   if (!q->x || !q->out || !batch->k_pages || !batch->v_pages ||
       (batch->sequences > 0 && (!batch->lengths || (batch->table_cols > 0 && !batch->page_table))))
     return HEXMI_EINVAL;
-  const int64_t strides[] = {q->token, q->head, q->out_token, q->out_head, batch->k_page, batch->k_head, batch->k_slot, batch->v_page,
-                             batch->v_head, batch->v_slot};
-  for (int64_t s : strides)
+  const int step = scales && batch->dim % 16 == 0 ? 16 : 8;         // elements between rows: 16 bytes, or the 8 that eight columns are
+  for (int64_t s : {q->token, q->head, q->out_token, q->out_head})
     if (s % 8 != 0) return HEXMI_ENOTSUP;
+  for (int64_t s : {batch->k_page, batch->k_head, batch->k_slot, batch->v_page, batch->v_head, batch->v_slot})
+    if (s % step != 0) return HEXMI_ENOTSUP;
   if (batch->k_slot < 0 || batch->k_slot > 1 << 26 || batch->v_slot < 0 || batch->v_slot > 1 << 26) return HEXMI_ENOTSUP;      // 32-bit offsets within a page
-  if (!aligned_to(q->x, 16) || !aligned_to(q->out, 16) || !aligned_to(batch->k_pages, 16) || !aligned_to(batch->v_pages, 16)) return HEXMI_ENOTSUP;
-  const Plan plan = plan_of(*batch, q->heads, shared);
+  const size_t boundary = scales ? step : 16;
+  if (!aligned_to(q->x, 16) || !aligned_to(q->out, 16) || !aligned_to(batch->k_pages, boundary) || !aligned_to(batch->v_pages, boundary))
+    return HEXMI_ENOTSUP;
+  const Plan plan = plan_of(*batch, q->heads, shared, seen.view);
   const int64_t need = plan.decode_bytes + plan.sum_bytes;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return HEXMI_EINVAL;
   const int64_t group = q->heads / batch->kv_heads;
   const PagedAttnArgs a = {q->x, batch->k_pages, batch->v_pages, q->out, q->token, q->head, q->out_token, q->out_head, shared_pages,
-                           (int)(shared * batch->page_size), (int)q->heads, (int)group, (int)batch->dim, sm_scale * kLog2e, divider(group)};
+                           (int)(shared * batch->page_size), (int)q->heads, (int)group, (int)batch->dim, sm_scale * kLog2e, divider(group),
+                           seen.window ? seen.window : kNoWindow, seen.sinks, (int)seen.view, scales ? scales_of(*scales) : Scales{}};
   const Pages p = pages_of(*batch);
   float* o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.decode_bytes);
   const RowSums sums = {o, reinterpret_cast<float2*>(o + plan.slots() * plan.rows * batch->dim), plan.rows, plan.slots()};
@@ -195,12 +187,40 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
   begin_call();
   const TileArgs tiles = {plan.deep, plan.workers, plan.prefix_tiles, plan.prefix_splits, (int)plan.tiles, plan.splits, sums};
   rc = plan.workers ? paged_decode(plan.one, a, p, dtype, workspace, tiles, s)
-       : dtype == HEXMI_F16 ? launch_tiles<f16>(a, p, tiles, s) : launch_tiles<bf16>(a, p, tiles, s);
+                    : with_kind(a, [&](auto kind) { return launch_paged_tiles<decltype(kind)>(a, p, tiles, dtype, s); });
   if (rc != HEXMI_OK || plan.decode || sums.slots == 0) return rc;
   const unsigned blocks = (unsigned)((plan.rows + 7) / 8);
   if (dtype == HEXMI_F16) hipLaunchKernelGGL((paged_join_kernel<f16>), dim3(blocks), dim3(256), 0, s, a, sums);
   else hipLaunchKernelGGL((paged_join_kernel<bf16>), dim3(blocks), dim3(256), 0, s, a, sums);
   return launch_status();
+}
+}  // namespace
+
+extern "C" int64_t hexmi_paged_attention_workspace(const hexmi_paged_batch* batch, int64_t heads, int64_t shared) {
+  return workspace_of(batch, heads, shared, kNoWindow);
+}
+
+extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const int32_t* shared_pages, int64_t shared,
+                                     float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
+  if (!q || !batch) return HEXMI_EINVAL;
+  return attend(q, batch, nullptr, shared_pages, shared, Seen{0, 0, kNoWindow}, sm_scale, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t hexmi_paged_attention_ex_workspace(const hexmi_paged_batch* batch, int64_t heads, int64_t shared,
+                                                      const hexmi_paged_scales* scales, int64_t window, int64_t sinks) {
+  if (!batch || window < 0 || sinks < 0 || check_batch(*batch) != HEXMI_OK) return 0;
+  (void)scales;                                // a cache in 8 bits is cut as one in 16
+  return workspace_of(batch, heads, shared, seen_of(*batch, window, sinks).view);
+}
+
+extern "C" int hexmi_paged_attention_ex(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi_paged_scales* scales,
+                                        const int32_t* shared_pages, int64_t shared, int64_t window, int64_t sinks, float sm_scale, int dtype,
+                                        void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
+  if (!q || !batch || window < 0 || sinks < 0) return HEXMI_EINVAL;
+  int rc = check_batch(*batch);
+  if (rc != HEXMI_OK || (scales && (rc = check_scales(*batch, *scales)) != HEXMI_OK)) return rc;
+  if (window > 0 && shared > 0) return HEXMI_ENOTSUP;
+  return attend(q, batch, scales, shared_pages, shared, seen_of(*batch, window, sinks), sm_scale, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int hexmi_paged_tile_column(int64_t dim, int64_t chunk) {

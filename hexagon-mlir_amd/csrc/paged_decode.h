@@ -22,7 +22,9 @@
 namespace hexmi {
 namespace {
 
+constexpr int kWaves = 4;                      // of a workgroup that only decodes
 constexpr int kTileKeys = 32;                  // of a wave; a workgroup's W waves take a block of W * kTileKeys
+constexpr int kBlockKeys = kWaves * kTileKeys;
 
 template <typename T> struct Mfma16;
 template <> struct Mfma16<f16> {
@@ -52,8 +54,10 @@ template <int W> __device__ __forceinline__ int blocks_of_keys(int keys) {
   return keys > W * kTileKeys ? (keys + W * kTileKeys - 1) / (W * kTileKeys) : 1;
 }
 // of sequence b, none where it has other than one new token (the tiles take those)
-template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix) {
-  return new_tokens_of(p, b) == 1 ? blocks_of_keys<W>(length_of(p, b) - prefix) : 0;
+// view: the most keys that its token sees
+__device__ __forceinline__ int at_most(int n, int most) { return n < most ? n : most; }
+template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix, int view) {
+  return new_tokens_of(p, b) == 1 ? blocks_of_keys<W>(at_most(length_of(p, b), view) - prefix) : 0;
 }
 // the sum over the lanes up to this one
 __device__ __forceinline__ int sum_up_to(int v) {
@@ -74,23 +78,23 @@ struct BlockList {
   int of_64, all;                              // blocks of the first 64 sequences, of all (one unit's)
 };
 template <int W>
-__device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int lane) {
+__device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int view, int lane) {
   BlockList l;
   l.length = lane < p.sequences ? length_of(p, lane) : 0;
-  l.blocks = lane < p.sequences && new_tokens_of(p, lane) == 1 ? blocks_of_keys<W>(l.length - prefix) : 0;
+  l.blocks = lane < p.sequences && new_tokens_of(p, lane) == 1 ? blocks_of_keys<W>(at_most(l.length, view) - prefix) : 0;
   l.up_to = sum_up_to(l.blocks);
   l.of_64 = of_last_lane(l.up_to);
   int more = 0;
-  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix) : 0;
+  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, view) : 0;
   l.all = l.of_64 + (p.sequences > kWave ? of_last_lane(sum_up_to(more)) : 0);
   return l;
 }
 // The sequence that block `at` of the list belongs to, with `units` units a sequence, and the blocks (of one unit) before it.
 template <int W>
-__device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, int units, int at, int lane, int& before) {
+__device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, int view, int units, int at, int lane, int& before) {
   before = 0;
   for (int b0 = 0;; b0 += kWave) {
-    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
+    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, view) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
     const uint64_t past = __ballot((before + sum) * units > at);
     if (past || b0 + kWave >= p.sequences) {   // `at` is below the end: there is one
       const int first = past ? __ffsll((unsigned long long)past) - 1 : 0;
@@ -103,8 +107,8 @@ __device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, i
 __device__ __forceinline__ int length_at(const BlockList& l, const Pages& p, int b) {
   return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.length, b & (kWave - 1)) : length_of(p, b));
 }
-template <int W> __device__ __forceinline__ int blocks_at(const BlockList& l, const Pages& p, int prefix, int b) {
-  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.blocks, b & (kWave - 1)) : blocks_of<W>(p, b, prefix));
+template <int W> __device__ __forceinline__ int blocks_at(const BlockList& l, const Pages& p, int prefix, int view, int b) {
+  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.blocks, b & (kWave - 1)) : blocks_of<W>(p, b, prefix, view));
 }
 // worker w's run of `total` blocks
 __device__ __forceinline__ int run_start(int total, int workers, int w) {
@@ -138,11 +142,19 @@ __device__ __forceinline__ void keep_sums(const DecodeArgs& w, int64_t row, int 
 // D, COLS, PADDED: HeadWidth. A lane whose columns lie past the head reads the head's first ones instead: the query has zeros there, and what
 // comes of V there is not stored.
 // worker: of w.workers, or the unit where that is 0.
-template <typename T, int D, int COLS, bool PADDED, int W>
+// The keys that a token sees within a window are its sinks and the last of its sequence, gone through as if they stood side by side.
+// A scaled cache: keys and values are widened to T (exact, see kLeastExponent) on the way from their registers to the matrix cores and to LDS.
+// A lane's 16 bytes are 16 columns of a row, so where a head is whole 64s the columns go to the products in another order, the query's too.
+template <typename T, typename Kind, int D, int COLS, bool PADDED, int W>
 __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned worker, char* lds,
                                                     float (*m_lds)[16], float (*l_lds)[16]) {
   typedef typename MfmaT<T>::Frag Frag;
   constexpr int DS = COLS / 32, DT = COLS / 16, kPitch = COLS + 4;
+  constexpr bool kWide = Kind::kScaled && COLS % 64 == 0 && !PADDED;
+  constexpr int LS = kWide ? DS / 2 : DS;                           // loads of a row
+  typedef std::conditional_t<Kind::kScaled && !kWide, u32x2, u32x4> Raw;
+  typedef std::conditional_t<Kind::kScaled, uint8_t, T> Held;
+  const int view = Kind::kWindow ? a.view : kNoWindow;
   constexpr int kWaveBytes = decode_wave_bytes(D, COLS), kBlock = W * kTileKeys;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane / 16, n = lane % 16;
@@ -150,7 +162,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
   // This lane's bytes of V in LDS, rows of D columns in 16-byte chunks: chunk g of row n, where it puts, and columns 4 (n % 4) .. of row
   // 4 g + n / 4, from where it takes (ds_read_b64_tr_b16: a group of 16 lanes asks for 4 rows x 16 columns, and a lane gets a column).
   // Other chunks are these with the chunk's number XORed in.
-  const int put_at = wave * kWaveBytes + n * (D * 2) + (g ^ swz_pairs<D>(n)) * 16;
+  const int put_at = wave * kWaveBytes + n * (D * 2) + ((kWide ? 2 * g : g) ^ swz_pairs<D>(n)) * 16;
   const int take_row = 4 * g + (n >> 2), take_at = wave * kWaveBytes + take_row * (D * 2) + (((n & 3) >> 1) ^ swz_pairs<D>(take_row)) * 16 + (n & 1) * 8;
   float* o_lds = reinterpret_cast<float*>(lds + wave * kWaveBytes);
   const int units = p.kv_heads * w.row_tiles;
@@ -163,21 +175,22 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     unit = worker - b * units;
     list.length = 0;
     cur = 0;
-    end = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix));
+    end = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix, view));
   } else {
-    list = block_list<W>(p, a.prefix, lane);
+    list = block_list<W>(p, a.prefix, view, lane);
     total = list.all * units;
     cur = run_start(total, w.workers, worker);
     end = run_start(total, w.workers, worker + 1);
     if (wave == 0 && lane == 0) w.begun[worker].last = -1;
     if (cur >= end) return;
-    b = sequence_at<W>(list, p, a.prefix, units, cur, lane, before);
+    b = sequence_at<W>(list, p, a.prefix, view, units, cur, lane, before);
   }
   const int start = cur;
 
   while (cur < end) {
-    const int length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
-    const int blocks = w.workers ? blocks_at<W>(list, p, a.prefix, b) : end - cur, local = cur - before * units;
+    const int whole_length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
+    const int length = at_most(whole_length, view), skip = whole_length - length;      // keys that are seen; those between the sinks and the others
+    const int blocks = w.workers ? blocks_at<W>(list, p, a.prefix, view, b) : end - cur, local = cur - before * units;
     if (local >= blocks * units) {             // on to the next sequence
       before += blocks;
       ++b;
@@ -197,7 +210,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
       const T* q = static_cast<const T*>(a.q) + token * a.q_token + (head0 + (n < rows ? n : rows - 1)) * a.q_head;
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds) {
-        const int c = ds * 32 + g * 8;
+        const int c = kWide ? ds / 2 * 64 + g * 16 + ds % 2 * 8 : ds * 32 + g * 8;
         const bool live = !PADDED || c < dim;
         col[ds] = live ? c : 0;
         qf[ds] = *reinterpret_cast<const Frag*>(q + col[ds]);
@@ -214,11 +227,14 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     int key_end = a.prefix + (block0 + count) * kBlock;
     key_end = key_end < length ? key_end : length;
     const int32_t* table = p.table + b * p.table_row;
-    const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
-    const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
+    const Held* k_head = static_cast<const Held*>(a.k) + kvh * p.k_head;
+    const Held* v_head = static_cast<const Held*>(a.v) + kvh * p.v_head;
     // where keys key0 + n and key0 + 16 + n stand; past the end: the last key again, without weight
     struct Keys { int page[2]; };
-    auto clamped = [&](int key) __attribute__((always_inline)) { return key < key_end ? key : key_end - 1; };
+    auto clamped = [&](int key) __attribute__((always_inline)) {
+      const int c = key < key_end ? key : key_end - 1;
+      return Kind::kWindow ? c + (c >= a.sinks ? skip : 0) : c;
+    };
     auto find = [&](int key0) __attribute__((always_inline)) {
       Keys k;
 #pragma unroll
@@ -226,18 +242,35 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
       return k;
     };
     auto there = [&](int page) __attribute__((always_inline)) { return page >= 0 && page < p.num_pages; };
-    auto load = [&](const Keys& at, int key0, const T* base, int64_t page_stride, int64_t slot_stride, u32x4 (*r)[DS]) __attribute__((always_inline)) {
+    auto load = [&](const Keys& at, int key0, const Held* base, int64_t page_stride, int64_t slot_stride, Raw (*r)[LS]) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int key = clamped(key0 + t * 16 + n), slot = key - divided(key, p.size) * p.page_size;
-        const T* row = base + (there(at.page[t]) ? at.page[t] : 0) * page_stride + slot * slot_stride;
+        const Held* row = base + (there(at.page[t]) ? at.page[t] : 0) * page_stride + slot * slot_stride;
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) r[t][ds] = *reinterpret_cast<const u32x4*>(row + col[ds]);
+        for (int i = 0; i < LS; ++i) r[t][i] = *reinterpret_cast<const Raw*>(row + col[kWide ? 2 * i : i]);
       }
     };
+    // Scales: a lane asks for one of its row's four, g % 2 the row (n, 16 + n), g / 2 keys' or values'; the swaps give all to all.
+    const uint8_t* scale_head = nullptr;
+    int64_t scale_page = 0, scale_block = 0;
+    if constexpr (Kind::kScaled) {
+      const Scales& sc = a.scales;
+      scale_head = g < 2 ? sc.k + kvh * sc.k_head : sc.v + kvh * sc.v_head;
+      scale_page = g < 2 ? sc.k_page : sc.v_page;
+      scale_block = g < 2 ? sc.k_block : sc.v_block;
+    }
+    auto load_scale = [&](const Keys& at, int key0) __attribute__((always_inline)) {
+      const int key = clamped(key0 + (g & 1) * 16 + n), slot = key - divided(key, p.size) * p.page_size;
+      auto pick = [](bool second, int v0, int v1) { return second ? v1 : v0; };      // (values, not places: no scratch)
+      const int page = pick(g & 1, at.page[0], at.page[1]);
+      return (uint32_t)scale_head[(there(page) ? page : 0) * scale_page + divided(slot, a.scales.by_block) * scale_block];
+    };
     if (key_first < key_end) {
-      u32x4 kr[2][DS], vr[2][DS];
+      Raw kr[2][LS], vr[2][LS];
       Keys now = find(key_first), next = find(key_first + kBlock);
+      uint32_t own_scale = 0;
+      if constexpr (Kind::kScaled) own_scale = load_scale(now, key_first);
       load(now, key_first, k_head, p.k_page, p.k_slot, kr);
       load(now, key_first, v_head, p.v_page, p.v_slot, vr);
       for (int key0 = key_first; key0 < key_end; key0 += kBlock) {
@@ -245,17 +278,33 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
         // what the constants of a chunk are XORed into; kept from becoming a register each
         int to = put_at, from = take_at;
         asm volatile("" : "+v"(to), "+v"(from));
+        float k_scale0 = 1.0f, k_scale1 = 1.0f, v_scale0 = 1.0f, v_scale1 = 1.0f;
+        if constexpr (Kind::kScaled) {
+          float first, second;
+          swap16(__builtin_bit_cast(float, own_scale << 23), first, second);
+          swap32(first, k_scale0, v_scale0);
+          swap32(second, k_scale1, v_scale1);
+        }
         f32x4 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds)
+        for (int i = 0; i < LS; ++i)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) s[t] = Mfma16<T>::run(__builtin_bit_cast(Frag, kr[t][ds]), qf[ds], s[t]);
+          for (int t = 0; t < 2; ++t) {
+            if constexpr (Kind::kScaled) {
+#pragma unroll
+              for (int h = 0; h < (kWide ? 2 : 1); ++h)
+                s[t] = Mfma16<T>::run(widened<T>(kr[t][i][2 * h], kr[t][i][2 * h + 1], t ? k_scale1 : k_scale0), qf[kWide ? 2 * i + h : i], s[t]);
+            } else {
+              s[t] = Mfma16<T>::run(__builtin_bit_cast(Frag, kr[t][i]), qf[i], s[t]);
+            }
+          }
         const bool ok0 = there(now.page[0]) && key0 + n < key_end, ok1 = there(now.page[1]) && key0 + 16 + n < key_end;
         const bool whole = __ballot(ok0 && ok1) == ~0ull;
         __builtin_amdgcn_sched_barrier(0);
         load(next, key0 + kBlock, k_head, p.k_page, p.k_slot, kr);
+        if constexpr (Kind::kScaled) own_scale = load_scale(next, key0 + kBlock);
         __builtin_amdgcn_sched_barrier(0);
         if (!whole) {                                                // what stands where no key is may be anything: no weight, and zeros of V
           const uint32_t k0 = (uint32_t)__ballot(ok0), k1 = (uint32_t)__ballot(ok1);
@@ -265,15 +314,26 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
             if (!(k1 >> (4 * g + i) & 1)) s[1][i] = -INFINITY;
           }
 #pragma unroll
-          for (int ds = 0; ds < DS; ++ds) {
-            if (!ok0) vr[0][ds] = u32x4{0u, 0u, 0u, 0u};
-            if (!ok1) vr[1][ds] = u32x4{0u, 0u, 0u, 0u};
+          for (int i = 0; i < LS; ++i) {
+            if (!ok0) vr[0][i] = Raw{};
+            if (!ok1) vr[1][i] = Raw{};
           }
+          if (!ok0) v_scale0 = 1.0f;                                 // (a scale may be a NaN's)
+          if (!ok1) v_scale1 = 1.0f;
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int ds = 0; ds < DS; ++ds) *reinterpret_cast<u32x4*>(lds + (to ^ (ds * 64)) + t * (16 * D * 2)) = vr[t][ds];
+          for (int i = 0; i < LS; ++i) {
+            if constexpr (Kind::kScaled) {
+#pragma unroll
+              for (int h = 0; h < (kWide ? 2 : 1); ++h)
+                *reinterpret_cast<Frag*>(lds + (to ^ (kWide ? i * 128 + h * 16 : i * 64)) + t * (16 * D * 2)) =
+                    widened<T>(vr[t][i][2 * h], vr[t][i][2 * h + 1], t ? v_scale1 : v_scale0);
+            } else {
+              *reinterpret_cast<u32x4*>(lds + (to ^ (i * 64)) + t * (16 * D * 2)) = vr[t][i];
+            }
+          }
         __builtin_amdgcn_sched_barrier(0);
         load(next, key0 + kBlock, v_head, p.v_page, p.v_slot, vr);
         __builtin_amdgcn_sched_barrier(0);
@@ -359,5 +419,26 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
   }
 }
 
+template <typename T, typename Kind, int D, int COLS, bool PADDED>
+__global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
+void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * decode_wave_bytes(D, COLS)];
+  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
+  paged_decode_worker<T, Kind, D, COLS, PADDED, kWaves>(a, p, w, blockIdx.x, lds, m_lds, l_lds);
+}
+
 }  // namespace
+
+template <typename Kind>
+int launch_paged_workers(const PagedAttnArgs& a, const Pages& p, const DecodeArgs& w, unsigned grid, int dtype, hipStream_t s) {
+  return with_width<256>(a.dim, [&](auto width) {
+    typedef decltype(width) W;
+    if (dtype == HEXMI_F16)
+      hipLaunchKernelGGL((paged_decode_kernel<f16, Kind, W::D, W::COLS, W::PADDED>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);
+    else
+      hipLaunchKernelGGL((paged_decode_kernel<bf16, Kind, W::D, W::COLS, W::PADDED>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);
+    return launch_status();
+  });
+}
+
 }  // namespace hexmi

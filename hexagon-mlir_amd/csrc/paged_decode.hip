@@ -5,16 +5,6 @@
 namespace hexmi {
 namespace {
 
-constexpr int kWaves = 4, kBlockKeys = kWaves * kTileKeys;
-
-template <typename T, int D, int COLS, bool PADDED>
-__global__ __launch_bounds__(kWaves * kWave, D == 256 ? 1 : 2)
-void paged_decode_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
-  __shared__ __attribute__((aligned(16))) char lds[kWaves * decode_wave_bytes(D, COLS)];
-  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
-  paged_decode_worker<T, D, COLS, PADDED, kWaves>(a, p, w, blockIdx.x, lds, m_lds, l_lds);
-}
-
 // The units that several workers share: block (w, row) takes the one that worker w began. With join_all every unit is joined with the
 // prefix's sums: block (unit, row).
 template <typename T>
@@ -29,10 +19,10 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     u = blockIdx.x - b * units;
     if (w.workers) {
       const int lane = threadIdx.x % kWave;
-      const BlockList list = block_list<kWaves>(p, a.prefix, lane);
+      const BlockList list = block_list<kWaves>(p, a.prefix, a.view, lane);
       int before = 0;
-      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<kWaves>(p, x, a.prefix);
-      const int blocks = blocks_at<kWaves>(list, p, a.prefix, b), total = list.all * units;
+      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<kWaves>(p, x, a.prefix, a.view);
+      const int blocks = blocks_at<kWaves>(list, p, a.prefix, a.view, b), total = list.all * units;
       const int first = of_last_lane(sum_up_to(before)) * units + u * blocks;
       w0 = worker_of(total, w.workers, first);
       w1 = worker_of(total, w.workers, first + blocks - 1);
@@ -127,17 +117,13 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
            hipStream_t s) {
   const unsigned grid = plan.workers ? plan.workers : (unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles);
   if (tiles.shared_splits || tiles.splits) {
-    const int rc = paged_shared_decode(a, p, tiles, w, grid, dtype, s);
+    const int rc = with_kind(a, [&](auto kind) { return launch_paged_shared<decltype(kind)>(a, p, tiles, w, grid, dtype, s); });
     if (rc != HEXMI_OK || (!w.join_all && plan.workers < 2)) return rc;
     const dim3 joins(w.join_all ? (unsigned)((int64_t)p.sequences * p.kv_heads * plan.row_tiles) : plan.workers - 1, plan.rows);
     hipLaunchKernelGGL((paged_decode_join_kernel<T>), joins, dim3(256), 0, s, a, p, w);
     return launch_status();
   }
-  const int rc = with_width<256>(a.dim, [&](auto width) {
-    typedef decltype(width) W;
-    hipLaunchKernelGGL((paged_decode_kernel<T, W::D, W::COLS, W::PADDED>), dim3(grid), dim3(kWaves * kWave), 0, s, a, p, w);
-    return launch_status();
-  });
+  const int rc = with_kind(a, [&](auto kind) { return launch_paged_workers<decltype(kind)>(a, p, w, grid, dtype, s); });
   if (rc != HEXMI_OK || plan.workers < 2) return rc;
   hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(plan.workers - 1, plan.rows), dim3(256), 0, s, a, p, w);
   return launch_status();
@@ -145,9 +131,11 @@ int launch(const PagedDecodePlan& plan, const PagedAttnArgs& a, const Pages& p, 
 
 }  // namespace
 
-PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix) {
+template int launch_paged_workers<Whole>(const PagedAttnArgs&, const Pages&, const DecodeArgs&, unsigned, int, hipStream_t);
+
+PagedDecodePlan plan_paged_decode(const hexmi_paged_batch& b, int64_t heads, int64_t prefix, int64_t view) {
   const int64_t group = heads / b.kv_heads, tiles = (group + 15) / 16, units = b.sequences * b.kv_heads * tiles;
-  const int64_t most = b.table_cols * b.page_size - prefix, blocks = most > kBlockKeys ? (most + kBlockKeys - 1) / kBlockKeys : 1;
+  const int64_t there = b.table_cols * b.page_size, most = (there < view ? there : view) - prefix, blocks = most > kBlockKeys ? (most + kBlockKeys - 1) / kBlockKeys : 1;
   const int rows = (int)(group < 16 ? group : 16);
   if (blocks <= 1) return {0, (int)tiles, rows};
   // A block each while they are fewer than the compute units; then four and more, so that a worker's sums are few beside its keys, on as

@@ -82,7 +82,7 @@ __device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
 // zeros there or they are not multiplied, and what comes of V there is not stored.
 // A workgroup's tile: number block_id of a launch whose tiles are `grid` workgroups; lds: Shape::lds_elements(D); m_lds, l_lds: of every
 // group's rows.
-template <typename T, int D, int COLS, bool PADDED, typename Shape>
+template <typename T, typename Kind, int D, int COLS, bool PADDED, typename Shape>
 __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, unsigned block_id, unsigned grid,
                                            T* lds, float (*m_lds)[Shape::kRows], float (*l_lds)[Shape::kRows]) {
   typedef typename MfmaT<T>::Frag Frag;
@@ -106,6 +106,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   const int part = unit % splits, tile = tiles - 1 - (int)(unit / splits % tiles), kvh = unit / splits / tiles;
 
   int token0 = 0, rows, row0, new_tokens = 0, begin = 0, end;
+  int hidden = 0;                                                   // keys from the sinks' end to there no row of the tile sees
   int64_t length = 0;
   bool none = false;                                                // rows of no sequence
   const int most = p.table_cols * p.page_size;
@@ -130,25 +131,36 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     end = none ? 0 : keys_of(length, new_tokens, divided(last, a.by_group), most);
     begin = a.prefix;
     table = p.table + (none ? 0 : b) * p.table_row;
+    if (Kind::kWindow && !none) hidden = keys_of(length, new_tokens, divided(row0, a.by_group), most) - a.window;
   }
   end = __builtin_amdgcn_readfirstlane(end);
-  const int blocks = end > begin ? (end - begin + kKeys - 1) / kKeys : 0, share = (blocks + splits - 1) / splits;
+  // Blocks are counted without those in which nothing is seen: block `sink_blocks` is the one that the window begins in.
+  hidden = Kind::kWindow ? __builtin_amdgcn_readfirstlane(hidden) : 0;
+  const int sink_blocks = Kind::kWindow ? a.sinks / kKeys + (a.sinks % kKeys != 0) : 0;
+  const int left_out = Kind::kWindow && hidden / kKeys > sink_blocks ? hidden / kKeys - sink_blocks : 0;
+  auto key_at = [&](int block) __attribute__((always_inline)) {
+    return begin + (Kind::kWindow && block >= sink_blocks ? block + left_out : block) * kKeys;
+  };
+  const int blocks = end > begin ? (end - begin + kKeys - 1) / kKeys - left_out : 0, share = (blocks + splits - 1) / splits;
   const int block0 = part * share, block1 = block0 + share < blocks ? block0 + share : blocks;
 
   const int first = block0 + group;                                 // this group's blocks: first, first + kGroups, ..
 
   // ---- copies: instruction j of a wave takes kRowsOfOne rows, a lane 16 bytes of one
-  const T* k_head = static_cast<const T*>(a.k) + kvh * p.k_head;
-  const T* v_head = static_cast<const T*>(a.v) + kvh * p.v_head;
+  typedef std::conditional_t<Kind::kScaled, uint8_t, T> Held;
+  const Held* k_head = static_cast<const Held*>(a.k) + kvh * p.k_head;
+  const Held* v_head = static_cast<const Held*>(a.v) + kvh * p.v_head;
   const int lin = row_wave * kWave + lane, copy_row = lin / CPR, lds_at = row_wave * kWave * 8;
   // The table's entry for key kKeys block + lane. No branch: it is asked for a block ahead, and what it is worth is looked at then (a load
   // behind a branch would be waited for where the branch ends).
   auto find = [&](int block) __attribute__((always_inline)) {
-    const int key = begin + block * kKeys + lane % kKeys;
+    const int key = key_at(block) + lane % kKeys;
     return table[divided(key < end ? key : end - 1, p.size)];       // end > begin: only asked then
   };
   auto page_at = [&](int block, int entry) __attribute__((always_inline)) {     // -1: no key there
-    return block < block1 && begin + block * kKeys + lane % kKeys < end && entry >= 0 && entry < p.num_pages ? entry : -1;
+    const int key = key_at(block) + lane % kKeys;
+    const bool unseen = Kind::kWindow && key >= a.sinks && key < hidden;
+    return block < block1 && key < end && !unseen && entry >= 0 && entry < p.num_pages ? entry : -1;
   };
   // One block into LDS, by copies that the compiler does not know of: it would wait for all of them before it reads LDS transposed, in the
   // middle of the block before. They are waited for ahead of the barrier that ends that block. Where every key is there and the rows of an
@@ -160,10 +172,48 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
     return copied_column<D, COLS, PADDED>(c, dim);
   };
+  // A scaled cache comes by way of registers: asked for when the block before is begun, widened to T and put into LDS when it is done.
+  struct Coming {
+    u32x2 k[NI], v[NI];
+    uint32_t k_scale, v_scale;                                      // of the lane's key
+  };
+  auto ask = [&](int block, int page_of_lane) __attribute__((always_inline)) {
+    Coming c;
+    const int key_of_lane = key_at(block) + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
+    const int64_t page = page_of_lane < 0 ? 0 : page_of_lane;       // no key: what stands in the first page, and zeros in its place
+    const int64_t k_at = page * p.k_page + slot_of_lane * p.k_slot, v_at = page * p.v_page + slot_of_lane * p.v_slot;
+    const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
+    c.k_scale = (a.scales.k + kvh * a.scales.k_head)[page * a.scales.k_page + block_of_lane * a.scales.k_block];
+    c.v_scale = (a.scales.v + kvh * a.scales.v_head)[page * a.scales.v_page + block_of_lane * a.scales.v_block];
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int r = copy_row + j * kRowStep;
+        const int64_t at = v ? v_at : k_at;
+        const uint32_t lo = __shfl((int)(uint32_t)at, r), hi = __shfl((int)(at >> 32), r);
+        (v ? c.v : c.k)[j] = *reinterpret_cast<const u32x2*>((v ? v_head : k_head) + (int64_t)((uint64_t)hi << 32 | lo) + column(v, r));
+      }
+    return c;
+  };
+  auto put = [&](const Coming& c, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    const uint32_t k_scale = page_of_lane < 0 ? 127 : c.k_scale, v_scale = page_of_lane < 0 ? 0x80000000u | 127 : c.v_scale;     // the top bit: none
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int r = copy_row + j * kRowStep;
+      const uint32_t ks = __shfl((int)k_scale, r), vs = __shfl((int)v_scale, r);
+      const Frag k = widened<T>(c.k[j][0], c.k[j][1], __builtin_bit_cast(float, ks << 23));
+      Frag v = widened<T>(c.v[j][0], c.v[j][1], __builtin_bit_cast(float, (vs & 255) << 23));
+      if (vs >> 31) v = Frag{};
+      *reinterpret_cast<Frag*>(k_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) = k;
+      *reinterpret_cast<Frag*>(v_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) = v;
+    }
+  };
   auto copy = [&](int block, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    if constexpr (!Kind::kScaled) {
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
       // a lane works out where its key stands, for all of the block's at once; an instruction takes its first row's
-      const int key_of_lane = begin + block * kKeys + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
+      const int key_of_lane = key_at(block) + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
       const int64_t k_at = page_of_lane * p.k_page + slot_of_lane * p.k_slot, v_at = page_of_lane * p.v_page + slot_of_lane * p.v_slot;
       auto first_of = [&](int64_t at, int j) __attribute__((always_inline)) {
         const int row = row_wave * kRowsOfOne + j * kRowStep;
@@ -187,7 +237,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     }
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int r = copy_row + j * kRowStep, key = begin + block * kKeys + r, page = __shfl(page_of_lane, r);
+      const int r = copy_row + j * kRowStep, key = key_at(block) + r, page = __shfl(page_of_lane, r);
       const int slot = key - divided(key, p.size) * p.page_size;
       T *k_to = k_dst + lds_at + j * (kRowWaves * kWave * 8), *v_to = v_dst + lds_at + j * (kRowWaves * kWave * 8);
       if (page >= 0) {
@@ -197,13 +247,17 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
         *reinterpret_cast<u32x4*>(v_to + lane * 8) = u32x4{0u, 0u, 0u, 0u};
       }
     }
+    }
   };
   int page = -1, next = -1;
   if (block0 < block1) {                                            // on their way while the rows are looked up
     page = find(first);
     next = find(first + kGroups);
     page = page_at(first, page);
-    if (first < block1) copy(first, page, k_lds0, v_lds0);
+    if (first < block1) {
+      if constexpr (Kind::kScaled) put(ask(first, page), page, k_lds0, v_lds0);
+      else copy(first, page, k_lds0, v_lds0);
+    }
   }
 
   // this lane's row: its token, its queries and the keys it sees
@@ -257,9 +311,11 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
 
   auto process = [&](int block, uint64_t there, int next_page, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
-    const int key0 = begin + block * kKeys;
-    if (block + kGroups < block1) copy(block + kGroups, next_page, k_dst, v_dst);
+    const int key0 = key_at(block);
+    if constexpr (!Kind::kScaled)
+      if (block + kGroups < block1) copy(block + kGroups, next_page, k_dst, v_dst);
     if (block >= block1 || key0 >= most_keys) return;               // wave-uniform; the barriers are outside
+    if (Kind::kWindow && key0 >= a.sinks && key0 + kKeys <= least_keys - a.window) return;
     f32x16 s[JT];
 #pragma unroll
     for (int jt = 0; jt < JT; ++jt)
@@ -310,14 +366,15 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     read_v(0, vf0);
     __builtin_amdgcn_sched_barrier(0);
     // s[jt][r] is the score of key key0 + 32 jt + 8 (r / 4) + 4 half + r % 4
-    if (there != ~0ull || key0 + kKeys > least_keys) {
+    if (there != ~0ull || key0 + kKeys > least_keys || (Kind::kWindow && key0 + kKeys > a.sinks && key0 < most_keys - a.window)) {
       const uint32_t bits[2] = {(uint32_t)there >> (4 * half), (uint32_t)(there >> 32) >> (4 * half)};
 #pragma unroll
       for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r / 4) + r % 4;
-          if (!(bits[jt] >> at & 1) || key0 + jt * 32 + at + 4 * half >= keys) s[jt][r] = -INFINITY;
+          const int key = key0 + jt * 32 + at + 4 * half;
+          if (!(bits[jt] >> at & 1) || key >= keys || (Kind::kWindow && key >= a.sinks && key < keys - a.window)) s[jt][r] = -INFINITY;
         }
     }
     float mx = -INFINITY, mx1 = -INFINITY;
@@ -374,20 +431,27 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     asm volatile("" : "+v"(f));
     qf[ds] = __builtin_bit_cast(Frag, f);
   }
-  for (int block = first, at = block0; at < block1; block += 2 * kGroups, at += 2 * kGroups) {      // as many turns for every group
+  // one block: its copies are here, the next one's are asked for
+  auto walk = [&](int block, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    uint64_t there = __ballot(page >= 0);
+    const uint64_t there = __ballot(page >= 0);
     page = page_at(block + kGroups, next);
     next = find(block + 2 * kGroups);
-    process(block, there, page, k_lds0, v_lds0, k_lds1, v_lds1);
+    if constexpr (Kind::kScaled) {
+      const bool comes = block + kGroups < block1;
+      Coming c = {};
+      if (comes) c = ask(block + kGroups, page);
+      process(block, there, page, k_src, v_src, k_dst, v_dst);
+      if (comes) put(c, page, k_dst, v_dst);
+    } else {
+      process(block, there, page, k_src, v_src, k_dst, v_dst);
+    }
+  };
+  for (int block = first, at = block0; at < block1; block += 2 * kGroups, at += 2 * kGroups) {      // as many turns for every group
+    walk(block, k_lds0, v_lds0, k_lds1, v_lds1);
     if (at + kGroups >= block1) break;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    there = __ballot(page >= 0);
-    page = page_at(block + 2 * kGroups, next);
-    next = find(block + 3 * kGroups);
-    process(block + kGroups, there, page, k_lds1, v_lds1, k_lds0, v_lds0);
+    walk(block + kGroups, k_lds1, v_lds1, k_lds0, v_lds0);
   }
   __syncthreads();
 
@@ -468,5 +532,30 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   }
 }
 
+template <typename T, typename Kind, int D, int COLS, bool PADDED, typename Shape>
+__global__ __launch_bounds__(Shape::kThreads, D == 256 ? 1 : D == 64 ? 3 : 2)
+void paged_tile_kernel(PagedAttnArgs a, Pages p, TileArgs w) {
+  __shared__ __attribute__((aligned(16))) T lds[Shape::lds_elements(D)];
+  __shared__ float m_lds[Shape::kGroups][Shape::kRows], l_lds[Shape::kGroups][Shape::kRows];
+  paged_tile<T, Kind, D, COLS, PADDED, Shape>(a, p, w, blockIdx.x, gridDim.x, lds, m_lds, l_lds);
+}
+
 }  // namespace
+
+template <typename Kind>
+int launch_paged_tiles(const PagedAttnArgs& a, const Pages& p, const TileArgs& w, int dtype, hipStream_t s) {
+  const unsigned grid = (unsigned)(((int64_t)w.tiles * w.splits + (int64_t)w.shared_tiles * w.shared_splits) * p.kv_heads);
+  auto launch = [&](auto width, auto shape) {
+    typedef decltype(width) W;
+    typedef decltype(shape) Shape;
+    if (dtype == HEXMI_F16)
+      hipLaunchKernelGGL((paged_tile_kernel<f16, Kind, W::D, W::COLS, W::PADDED, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);
+    else
+      hipLaunchKernelGGL((paged_tile_kernel<bf16, Kind, W::D, W::COLS, W::PADDED, Shape>), dim3(grid), dim3(Shape::kThreads), 0, s, a, p, w);
+    return launch_status();
+  };
+  return w.deep ? with_width<128>(a.dim, [&](auto width) { return launch(width, DeepTile{}); })
+                : with_width<256>(a.dim, [&](auto width) { return launch(width, WideTile{}); });
+}
+
 }  // namespace hexmi
