@@ -343,12 +343,17 @@ const at::Tensor* index(PyObject* o, int64_t dims, const at::Tensor& like) {
   const at::Tensor* t = contiguous(o);
   return t && t->dim() == dims && t->scalar_type() == at::kInt && t->device() == like.device() ? t : nullptr;
 }
+// pages [pages, kv heads, page size, dim] of a type, keys and values alike
+bool pages_of(PyObject* ko, PyObject* vo, at::ScalarType type, const at::Tensor*& k, const at::Tensor*& v) {
+  k = dense(ko);
+  v = k ? dense(vo) : nullptr;
+  return v && k->dim() == 4 && k->sizes() == v->sizes() && k->scalar_type() == type && v->scalar_type() == type && v->device() == k->device() &&
+         k->stride(3) == 1 && v->stride(3) == 1;
+}
 // k_pages, v_pages, page_table, lengths, starts or None. written: whether the pages are, and not only read
-bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, bool written, hexmi_paged_batch& b) {
-  const at::Tensor *k = dense(a[0]), *v = k ? dense(a[1]) : nullptr;
-  if (!v || k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != rows.scalar_type() || v->scalar_type() != k->scalar_type() ||
-      k->device() != rows.device() || v->device() != k->device() || k->size(3) != dim || k->stride(3) != 1 || v->stride(3) != 1)
-    return false;
+bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, at::ScalarType held, bool written, hexmi_paged_batch& b) {
+  const at::Tensor *k, *v;
+  if (!pages_of(a[0], a[1], held, k, v) || k->device() != rows.device() || k->size(3) != dim) return false;
   const at::Tensor *table = index(a[2], 2, rows), *lengths = index(a[3], 1, rows), *starts = nullptr;
   if (!table || !lengths || table->size(0) != lengths->size(0)) return false;
   if (a[4] != Py_None) {
@@ -362,6 +367,42 @@ bool batch_of(PyObject* const* a, const at::Tensor& rows, int64_t dim, bool writ
        k->size(0), k->size(2), k->size(1), dim, static_cast<const int32_t*>(in(table)), table->size(1), table->size(1),
        static_cast<const int32_t*>(in(lengths)), static_cast<const int32_t*>(in(starts)), lengths->size(0), rows.size(0)};
   return true;
+}
+// k_scales and v_scales beside a batch's pages, or None both; written as the pages are
+struct ScalesOf {
+  bool given = false;
+  hexmi_paged_scales s = {};
+  const hexmi_paged_scales* get() const { return given ? &s : nullptr; }
+};
+bool scales_of(PyObject* ko, PyObject* vo, const hexmi_paged_batch& b, const at::Tensor& like, bool written, ScalesOf& r) {
+  if (ko == Py_None && vo == Py_None) return true;
+  const at::Tensor *k = dense(ko), *v = k ? dense(vo) : nullptr;
+  if (!v || k->dim() != 3 || k->sizes() != v->sizes() || k->scalar_type() != at::kByte || v->scalar_type() != at::kByte ||
+      k->device() != like.device() || v->device() != k->device() || k->size(0) != b.num_pages || k->size(1) != b.kv_heads ||
+      b.page_size % k->size(2) != 0 || b.page_size / k->size(2) > 64)
+    return false;
+  auto place = [&](const at::Tensor* t) { return static_cast<uint8_t*>(written ? t->mutable_data_ptr() : const_cast<void*>(in(t))); };
+  r.given = true;
+  r.s = {place(k), place(v), stride(*k, 0), stride(*k, 1), stride(*k, 2), stride(*v, 0), stride(*v, 1), stride(*v, 2), b.page_size / k->size(2)};
+  return true;
+}
+// window or None, sinks; 0: none. Numbers past any position are left to ops.py.
+bool window_of(PyObject* wo, PyObject* so, int64_t& window, int64_t& sinks) {
+  auto whole = [](PyObject* o, int64_t& v) {
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    return over == 0 && v >= 0 && v <= int64_t(1) << 40;
+  };
+  window = 0;
+  if (!whole(so, sinks) || (wo != Py_None && (!whole(wo, window) || window == 0))) return false;
+  return wo != Py_None || sinks == 0;
+}
+bool on_boundaries(const at::Tensor* t) {      // rows of 16-bit numbers, the last dimension theirs
+  if (!t) return true;
+  for (int64_t d = 0; d + 1 < t->dim(); ++d)
+    if (stride(*t, (int)d) % 8 != 0) return false;
+  return reinterpret_cast<uintptr_t>(in(t)) % 16 == 0;
 }
 bool in_storage_of(const void* p, const at::Tensor& t) {
   const auto* base = static_cast<const char*>(t.storage().data());
@@ -410,17 +451,20 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 // paged_append(k, v, k_pages, v_pages, page_table, lengths, starts or None, k_weight or None, inv_freq or None, eps, pairs, q or None,
-// q_weight or None): q's rows, or True
+// q_weight or None, k_scales or None, v_scales or None): q's rows, or True
 PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    const at::Tensor* k = n == 13 ? dense(a[0]) : nullptr;
+    const at::Tensor* k = n == 15 ? dense(a[0]) : nullptr;
     if (!k || (k->scalar_type() != at::kHalf && k->scalar_type() != at::kBFloat16) || !(k = head_rows(a[0], k->scalar_type()))) HEXMI_NOT_PLAIN;
     const at::ScalarType type = k->scalar_type();
     const int64_t D = k->size(2);
     const at::Tensor *v = head_rows(a[1], type), *q = nullptr, *kw, *qw;
     hexmi_paged_batch batch;
     hexmi_rotation turn;
-    if (!v || v->sizes() != k->sizes() || v->device() != k->device() || !batch_of(a + 2, *k, D, true, batch) || batch.kv_heads != k->size(1) ||
+    ScalesOf scales;
+    const at::ScalarType held = a[13] == Py_None ? type : at::kFloat8_e4m3fn;
+    if (!v || v->sizes() != k->sizes() || v->device() != k->device() || !batch_of(a + 2, *k, D, held, true, batch) || batch.kv_heads != k->size(1) ||
+        !scales_of(a[13], a[14], batch, *k, true, scales) ||
         !optional(a[7], kw, {D}, type, *k) || !rotation_of(a[8], a[9], a[10], *k, D, turn) || !optional(a[12], qw, {D}, type, *k))
       HEXMI_NOT_PLAIN;
     if (a[11] != Py_None) {
@@ -433,6 +477,9 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       for (const void* pages : {batch.k_pages, batch.v_pages})
         if (t && t->numel() && in_storage_of(pages, *t)) HEXMI_NOT_PLAIN;
     if (batch.k_pages == batch.v_pages) HEXMI_NOT_PLAIN;
+    if (scales.given && (D % 8 != 0 || D > 256)) HEXMI_NOT_PLAIN;
+    for (const at::Tensor* t : {k, v, q, kw, qw})
+      if (scales.given && !on_boundaries(t)) HEXMI_NOT_PLAIN;
     const Launch at(*k);
     if (!at.ok) HEXMI_NOT_PLAIN;
     const hexmi_head_rows kr = rows_of(k, nullptr, kw), vr = rows_of(v, nullptr, nullptr);
@@ -442,34 +489,98 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       qo = fresh(q->sizes(), type, *q);
       qr = rows_of(q, &qo, qw);
     }
-    const int status = unlocked(hexmi_paged_append, &kr, &vr, q ? &qr : nullptr, &turn, &batch, code_of(type), at.stream);
-    if (status != HEXMI_OK || q) return finish(status, "hexmi_paged_append", std::move(qo));
+    const int status = unlocked(hexmi_paged_append_ex, &kr, &vr, q ? &qr : nullptr, &turn, &batch, scales.get(), code_of(type), at.stream);
+    if (status != HEXMI_OK || q) return finish(status, scales.given ? "hexmi_paged_append_ex" : "hexmi_paged_append", std::move(qo));
     Py_RETURN_TRUE;
   });
 }
 
-// paged_attention(q, k_pages, v_pages, page_table, lengths, starts or None, sm_scale or None, shared_pages or None)
+// paged_attention(q, k_pages, v_pages, page_table, lengths, starts or None, sm_scale or None, shared_pages or None, k_scales or None,
+// v_scales or None, window or None, sinks)
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    const at::Tensor* q = n == 8 ? dense(a[0]) : nullptr;
+    const at::Tensor* q = n == 12 ? dense(a[0]) : nullptr;
     if (!q || (q->scalar_type() != at::kHalf && q->scalar_type() != at::kBFloat16) || !(q = head_rows(a[0], q->scalar_type()))) HEXMI_NOT_PLAIN;
     const int64_t H = q->size(1), D = q->size(2);
     if (D % 8 != 0 || D > 256 || stride(*q, 0) % 8 != 0 || stride(*q, 1) % 8 != 0 || reinterpret_cast<uintptr_t>(in(q)) % 16 != 0) HEXMI_NOT_PLAIN;
     hexmi_paged_batch batch;
-    if (!batch_of(a + 1, *q, D, false, batch) || H % batch.kv_heads != 0) HEXMI_NOT_PLAIN;
+    ScalesOf scales;
+    int64_t window, sinks;
+    if (!batch_of(a + 1, *q, D, a[8] == Py_None ? q->scalar_type() : at::kFloat8_e4m3fn, false, batch) || H % batch.kv_heads != 0 ||
+        !scales_of(a[8], a[9], batch, *q, false, scales) || !window_of(a[10], a[11], window, sinks))
+      HEXMI_NOT_PLAIN;
     double scale = 1.0 / std::sqrt((double)D);
     if ((a[6] != Py_None && !number(a[6], scale)) || !(scale > 0.0 && scale <= 2e38)) HEXMI_NOT_PLAIN;
     const at::Tensor* shared = nullptr;
-    if (a[7] != Py_None && (!(shared = index(a[7], 1, *q)) || shared->size(0) > batch.table_cols)) HEXMI_NOT_PLAIN;
+    if (a[7] != Py_None && (window || !(shared = index(a[7], 1, *q)) || shared->size(0) > batch.table_cols)) HEXMI_NOT_PLAIN;
     const Launch at(*q);
     if (!at.ok) HEXMI_NOT_PLAIN;
     at::Tensor out = fresh(q->sizes(), q->scalar_type(), *q);
     const hexmi_head_rows qr = rows_of(q, &out, nullptr);
-    const int64_t pages = shared ? shared->size(0) : 0, bytes = hexmi_paged_attention_workspace(&batch, H, pages);
+    const int64_t pages = shared ? shared->size(0) : 0;
+    const int64_t bytes = hexmi_paged_attention_ex_workspace(&batch, H, pages, scales.get(), window, sinks);
     const at::Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, *q) : at::Tensor();
-    return finish(unlocked(hexmi_paged_attention, &qr, &batch, static_cast<const int32_t*>(in(shared)), pages, (float)scale,
-                           code_of(q->scalar_type()), bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, at.stream),
-                  "hexmi_paged_attention", std::move(out));
+    return finish(unlocked(hexmi_paged_attention_ex, &qr, &batch, scales.get(), static_cast<const int32_t*>(in(shared)), pages, window, sinks,
+                           (float)scale, code_of(q->scalar_type()), bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, at.stream),
+                  scales.given || window ? "hexmi_paged_attention_ex" : "hexmi_paged_attention", std::move(out));
+  });
+}
+
+// k_pages, v_pages, page_table, lengths, k_scales or None, v_scales or None of a call that copies pages
+bool cache_of(PyObject* const* a, const at::Tensor*& k, hexmi_paged_batch& batch, ScalesOf& scales) {
+  k = dense(a[0]);
+  if (!k) return false;
+  const at::ScalarType held = a[4] == Py_None ? k->scalar_type() : at::kFloat8_e4m3fn;
+  if (a[4] == Py_None && held != at::kHalf && held != at::kBFloat16) return false;
+  const at::Tensor* v;
+  if (!pages_of(a[0], a[1], held, k, v)) return false;
+  const at::Tensor *table = index(a[2], 2, *k), *lengths = index(a[3], 1, *k);
+  if (!table || !lengths || table->size(0) != lengths->size(0)) return false;
+  batch = {k->mutable_data_ptr(), v->mutable_data_ptr(), stride(*k, 0), stride(*k, 1), stride(*k, 2), stride(*v, 0), stride(*v, 1), stride(*v, 2),
+           k->size(0), k->size(2), k->size(1), k->size(3), static_cast<const int32_t*>(in(table)), table->size(1), table->size(1),
+           static_cast<const int32_t*>(in(lengths)), nullptr, lengths->size(0), lengths->size(0)};
+  return batch.k_pages != batch.v_pages && scales_of(a[4], a[5], batch, *k, true, scales);
+}
+
+// paged_fork(k_pages, v_pages, page_table, lengths, k_scales or None, v_scales or None, parents, pages): (table, lengths)
+PyObject* paged_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *k, *parents, *pages;
+    hexmi_paged_batch batch;
+    ScalesOf scales;
+    if (n != 8 || !cache_of(a, k, batch, scales) || !(parents = index(a[6], 1, *k)) || !(pages = index(a[7], 1, *k)) ||
+        parents->size(0) != pages->size(0))
+      HEXMI_NOT_PLAIN;
+    const Launch at(*k);
+    if (!at.ok) HEXMI_NOT_PLAIN;
+    const int64_t rows = parents->size(0);
+    at::Tensor table = fresh({rows, batch.table_cols}, at::kInt, *k), lengths = fresh({rows}, at::kInt, *k);
+    const int status = unlocked(hexmi_paged_fork, &batch, scales.get(), static_cast<const int32_t*>(in(parents)), static_cast<const int32_t*>(in(pages)),
+                                rows, static_cast<int32_t*>(table.mutable_data_ptr()), batch.table_cols,
+                                static_cast<int32_t*>(lengths.mutable_data_ptr()), scales.given ? HEXMI_F16 : code_of(k->scalar_type()), at.stream);
+    if (status != HEXMI_OK) return finish(status, "hexmi_paged_fork", std::move(table));
+    return pair(std::move(table), std::move(lengths));
+  });
+}
+
+// paged_compact(k_pages, v_pages, page_table, lengths, k_scales or None, v_scales or None, window or None, sinks): (table, count)
+PyObject* paged_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* k;
+    hexmi_paged_batch batch;
+    ScalesOf scales;
+    int64_t window, sinks;
+    if (n != 8 || !cache_of(a, k, batch, scales) || !window_of(a[6], a[7], window, sinks)) HEXMI_NOT_PLAIN;
+    const Launch at(*k);
+    if (!at.ok) HEXMI_NOT_PLAIN;
+    at::Tensor table = fresh({batch.sequences, batch.table_cols}, at::kInt, *k), count = fresh({1}, at::kInt, *k);
+    const int64_t bytes = hexmi_paged_compact_workspace(&batch);
+    const at::Tensor ws = fresh({bytes}, at::kByte, *k);
+    const int status = unlocked(hexmi_paged_compact, &batch, scales.get(), window, sinks, static_cast<int32_t*>(table.mutable_data_ptr()),
+                                batch.table_cols, static_cast<int32_t*>(count.mutable_data_ptr()),
+                                scales.given ? HEXMI_F16 : code_of(k->scalar_type()), ws.mutable_data_ptr(), bytes, at.stream);
+    if (status != HEXMI_OK) return finish(status, "hexmi_paged_compact", std::move(table));
+    return pair(std::move(table), std::move(count));
   });
 }
 
@@ -525,6 +636,7 @@ PyMODINIT_FUNC PyInit__front() {
   if (!(HEXMI_OPERATOR(softmax) && HEXMI_OPERATOR(rms_norm) && HEXMI_OPERATOR(layer_norm) && HEXMI_OPERATOR(matmul) &&
         HEXMI_OPERATOR(w8a16_matmul) && HEXMI_OPERATOR(flash_attention) && HEXMI_OPERATOR(attention) && HEXMI_OPERATOR(unary) &&
         HEXMI_OPERATOR(binary) && HEXMI_OPERATOR(qk_norm_rope) && HEXMI_OPERATOR(paged_append) && HEXMI_OPERATOR(paged_attention) &&
+        HEXMI_OPERATOR(paged_fork) && HEXMI_OPERATOR(paged_compact) &&
         PyModule_AddStringConstant(m, "torch_version", HEXMI_TORCH_VERSION) == 0))
     Py_CLEAR(m);
 #undef HEXMI_OPERATOR

@@ -471,7 +471,7 @@ class _Front:
     def __getattr__(self, name):
         _lib.lib()
         names = ("softmax", "rms_norm", "layer_norm", "matmul", "w8a16_matmul", "flash_attention", "attention", "unary", "binary",
-                 "qk_norm_rope", "paged_append", "paged_attention")
+                 "qk_norm_rope", "paged_append", "paged_attention", "paged_fork", "paged_compact")
         if name not in names:
             raise AttributeError(name)
         try:
@@ -1061,8 +1061,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     biased exponent e + 127 of the power of two that the numbers of each page_size / blocks slots (1 to 64) of a page are multiplied by. A
     block's exponent is the least that has the largest of the call's values in it within 448; it does not fall below what older tokens
     of the sequence in the block have, and their numbers are rounded again where it rises. dim a multiple of 8 up to 256."""
-    if q_out is None and k_scales is None and v_scales is None and not _THROUGH_DISPATCHER:
-        y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight)
+    if q_out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight, k_scales, v_scales)
         if y is not None:
             return y if q is not None else None
     name = "paged_append"
@@ -1126,8 +1126,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
     k_scales, v_scales: a cache in 8 bits, as `paged_append` has it. window: a token at position p sees the positions j <= p with
     j > p - window or j < sinks; pages that hold none of what a sequence's new tokens see are not read, and their entries of the table
     may be anything (-1, once `paged_compact` has freed them). No shared pages within a window."""
-    if out is None and k_scales is None and v_scales is None and window is None and not sinks and not _THROUGH_DISPATCHER:
-        y = _front.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages)
+    if out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, sm_scale, shared_pages, k_scales, v_scales, window, sinks)
         if y is not None:
             return y
     name = "paged_attention"
@@ -1197,6 +1197,10 @@ def paged_fork(k_pages, v_pages, page_table, lengths, parents, pages, k_scales=N
 
     The cache is `paged_append`'s, in 16 or 8 bits, and changed in place; pages are each named once and in no use. All index tensors are
     read on the GPU only."""
+    if table_out is None and lengths_out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_fork(k_pages, v_pages, page_table, lengths, k_scales, v_scales, parents, pages)
+        if y is not None:
+            return y
     name = "paged_fork"
     for what, t in (("parents", parents), ("pages", pages)):
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape != parents.shape:
@@ -1220,6 +1224,10 @@ def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales
     sequence's row names for positions below its length, within a window those that its last token sees. No more pages
     than need be are copied: those behind `count`, in rising order, to the free ones before it. The cache, in 16 or 8 bits, is changed in place;
     table_out may be page_table itself."""
+    if table_out is None and not _THROUGH_DISPATCHER:
+        y = _front.paged_compact(k_pages, v_pages, page_table, lengths, k_scales, v_scales, window, sinks)
+        if y is not None:
+            return y
     name = "paged_compact"
     window, sinks = _check_window(name, window, sinks)
     table, lens = _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales)
