@@ -9,6 +9,8 @@
 namespace hexmi {
 namespace {
 
+constexpr int kUnitGroups = 2048;              // workgroups wanted for keys and values
+
 // Units (a sequence's new tokens of one block): those of sequence b are numbered from first_unit(b) on, b = -1 .. sequences (first_row). n
 // tokens stand in at most floor((n - 2) / block) + 2 blocks and floor(x1 / block) - floor(x0 / block) >= floor(n / block) for x1 = x0 + n, so
 // two more for each sequence are enough; some numbers are no unit.
@@ -70,88 +72,90 @@ __device__ __forceinline__ u32x2 codes_again(u32x2 c, int by) {
   return c;
 }
 
-// LPR lanes take a row, eight columns each. HALVES, PIECES: head_rows.hip.
+// Where a unit's tokens stand: rows token0 .. token0 + n - 1 (n <= 0: none) at positions from `position` on, all in one block of a page.
+struct Unit {
+  int token0, n, page, slot, block, old;       // old: slots of the block, before `slot`, that older tokens of the sequence have
+  int64_t position;
+};
+__device__ __forceinline__ Unit unit_at(const Pages& p, const Scales& sc, int unit, int lane) {
+  Unit u = {0, 0, -1, 0, 0, 0, 0};
+  int b = unit, n = 1, nth = 0;
+  if (p.starts) {
+    b = __builtin_amdgcn_readfirstlane(sequence_of_unit(p, sc, unit, lane));
+    if (b < 0 || b >= p.sequences) return u;
+    u.token0 = first_row(p, b);
+    n = first_row(p, b + 1) - u.token0;
+    nth = unit - first_unit(p, sc, b);
+    if (n <= 0) return u;                      // starts may fall
+  } else {
+    u.token0 = b;
+  }
+  const int64_t first = (int64_t)p.lengths[b] - n;
+  const int r = first >= 0 ? (int)first - divided((int)first, sc.by_block) * sc.block : (int)((first % sc.block + sc.block) % sc.block);
+  const int skip = nth > 0 ? nth * sc.block - r : 0, next = (nth + 1) * sc.block - r;       // tokens before the unit's own, up to its last
+  u.token0 += skip;
+  u.n = (next < n ? next : n) - skip;
+  u.position = first + skip;
+  if (u.n <= 0 || u.position < 0 || u.position >= (int64_t)p.table_cols * p.page_size) return u;
+  const int column = divided((int)u.position, p.size), page = p.table[b * p.table_row + column];
+  if (page < 0 || page >= p.num_pages) return u;
+  u.page = page;
+  u.slot = (int)u.position - column * p.page_size;
+  u.block = divided(u.slot, sc.by_block);
+  u.old = u.slot - u.block * sc.block;
+  return u;
+}
+
+// Workgroups from kv_grid on take the queries, as head_rows_kernel does; the others a unit and a share of its heads. LPR lanes take a row, eight
+// columns each (HALVES, PIECES: head_rows.h). A wave holds kHeld times the rows that it has at once, so that rows of a block are read and
+// turned once; larger blocks are gone through twice.
 template <typename T, int LPR, bool HALVES, bool PIECES>
-__global__ __launch_bounds__(256)
-void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, int shares, Divider by_heads) {
+__global__ __launch_bounds__(256, 4)
+void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, int shares, int q_waves) {
+  constexpr int kRowsAtOnce = kWave / LPR, kHeld = 4;
+  __shared__ __attribute__((aligned(16))) HeadRowsLds<T, LPR, HALVES> lds;
   extern __shared__ __attribute__((aligned(16))) f32x2 angle[];    // [tokens of the block][columns / 2]
-  __shared__ __attribute__((aligned(16))) T beside[HALVES ? 4 : 1][HALVES ? kWave * 8 : 8];
-  constexpr int kRowsAtOnce = kWave / LPR;
+  if (blockIdx.x >= kv_grid) {
+    HeadArgs q = a;
+    q.heads[1] = q.heads[2] = 0;
+    head_rows_of<T, LPR, HALVES, PIECES, true>(q, p, q_waves, blockIdx.x - kv_grid, gridDim.x - kv_grid, lds);
+    return;
+  }
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c0 = lane % LPR * 8, group = lane / LPR, half = a.columns / 2;
   const bool live = c0 < a.dim, turns = c0 < a.columns;
-  const int unit = blockIdx.x / shares, share = blockIdx.x - unit * shares;
-
-  // ---- the tokens: rows token0 .. token0 + m - 1 at positions from `position` on, in one block, or none of them has a page
-  int b, token0, n;
-  if (!p.starts) {
-    b = unit;
-    token0 = b;
-    n = 1;
-  } else {
-    b = __builtin_amdgcn_readfirstlane(sequence_of_unit(p, sc, unit, lane));
-    token0 = first_row(p, b);
-    n = first_row(p, b + 1) - token0;
-  }
-  const bool none = b < 0 || b >= p.sequences;
-  int64_t position = none ? 0 : (int64_t)p.lengths[b] - n;
-  const int64_t most = (int64_t)p.table_cols * p.page_size;
-  int first = 0;                                                    // tokens before the unit's own
-  const int nth = p.starts ? unit - first_unit(p, sc, b) : 0;
-  {
-    const int r = position >= 0 && position < 0x7fffffff ? (int)position - divided((int)position, sc.by_block) * sc.block
-                                                         : (int)((position % sc.block + sc.block) % sc.block);
-    if (nth > 0) first = sc.block - r + (nth - 1) * sc.block;
-    if (first >= n) return;
-    const int next = sc.block - r + nth * sc.block;
-    n = (next < n ? next : n) - first;
-  }
-  token0 += first;
-  position += first;
-  int page = -1, slot = 0, block = 0, old = 0;                      // old: slots of the block that older tokens of the sequence have
-  if (!none && position >= 0 && position < most) {
-    const int column = divided((int)position, p.size);
-    page = p.table[b * p.table_row + column];
-    if (page < 0 || page >= p.num_pages) page = -1;
-    slot = (int)position - column * p.page_size;
-    block = divided(slot, sc.by_block);
-    old = slot - block * sc.block;
-  }
-  for (int i = threadIdx.x; i < n * half; i += 256) {
+  const int share = blockIdx.x % shares;
+  const Unit u = unit_at(p, sc, blockIdx.x / shares, lane);
+  if (u.n <= 0 || u.page < 0) return;
+  for (int i = threadIdx.x; i < u.n * half; i += 256) {
     const int t = i / half;
     float sn, cs;
-    sincos_turns((double)(position + t) * a.inv_freq[i - t * half] * 0.15915494309189533577, sn, cs);       // 1 / (2 pi)
+    sincos_turns((double)(u.position + t) * a.inv_freq[i - t * half] * 0.15915494309189533577, sn, cs);       // 1 / (2 pi)
     angle[i] = f32x2{cs, sn};
   }
   __syncthreads();
 
-  // ---- row (token t, head h) of a kind, normed and turned
-  auto fetch = [&](const Kind& kind, int t, int h) __attribute__((always_inline)) {
-    Eight<T> x = load_eight(static_cast<const T*>(kind.x) + (token0 + t) * kind.token + h * kind.head + (live ? c0 : 0));
-    if (!live) x = {};
-    return x;
-  };
-  auto turned = [&](const Kind& kind, int columns, int t, const Eight<T>& x, float* y) __attribute__((always_inline)) {
+  // row x of keys, token t of the unit, normed and turned
+  auto turned = [&](int t, const Eight<T>& x, float* y) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = column(x, e);
-    const T* w = static_cast<const T*>(kind.weight);
-    Eight<T> wt = {};
+    const T* w = static_cast<const T*>(a.kind[1].weight);
     float scale = 1.0f;
     if (w) {
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(y[e], y[e], sum);
       scale = rms_scale(fmaf(row_sum<LPR>(sum), 1.0f / (float)a.dim, a.eps));
+      Eight<T> wt = {};
       if (live) wt = load_eight(w + c0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = y[e] * scale * column(wt, e);
     }
-    if (columns == 0) return;
     const f32x2* at = angle + t * half;
     if constexpr (HALVES) {
-      *reinterpret_cast<Eight<T>*>(&beside[wave][lane * 8]) = x;
+      *reinterpret_cast<Eight<T>*>(&lds.beside[wave][lane * 8]) = x;
       asm volatile("" ::: "memory");                                // a wave's LDS accesses are in order
-      const T* row = &beside[wave][group * LPR * 8];
+      const T* row = &lds.beside[wave][group * LPR * 8];
       if (turns) {
         if constexpr (PIECES) {
           const bool second = c0 >= half;
@@ -170,7 +174,7 @@ void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, int shares, Divider by_h
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int c = c0 + e;
-            if (c >= columns) continue;
+            if (c >= a.columns) continue;
             const bool second = c >= half;
             const int other = second ? c - half : c + half;
             float v = to_f32<T>(row[other]);
@@ -184,94 +188,108 @@ void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, int shares, Divider by_h
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (c0 + 2 * e >= columns) continue;
+        if (c0 + 2 * e >= a.columns) continue;
         const f32x2 cs = at[c0 / 2 + e];
-        const float u = y[2 * e], v = y[2 * e + 1];
-        y[2 * e] = fmaf(u, cs[0], -(v * cs[1]));
-        y[2 * e + 1] = fmaf(v, cs[0], u * cs[1]);
+        const float x0 = y[2 * e], x1 = y[2 * e + 1];
+        y[2 * e] = fmaf(x0, cs[0], -(x1 * cs[1]));
+        y[2 * e + 1] = fmaf(x1, cs[0], x0 * cs[1]);
       }
     }
   };
-  auto most_of = [&](const float* y) __attribute__((always_inline)) {
-    float m = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]) < INFINITY ? fabsf(y[e]) : 0.0f);
-    return m;
-  };
 
-  // ---- jobs: rows of queries kRowsAtOnce at a time; keys, then values, a head at a time (of one token kRowsAtOnce heads)
-  const int q_jobs = (n * a.heads[0] + kRowsAtOnce - 1) / kRowsAtOnce;
-  const int each = n == 1 ? (p.kv_heads + kRowsAtOnce - 1) / kRowsAtOnce : p.kv_heads, jobs = q_jobs + (page < 0 ? 0 : 2 * each);
-  for (int job = share * 4 + wave; job < jobs; job += shares * 4) {
-    if (job < q_jobs) {
-      const Kind& kind = a.kind[0];
-      const int at = job * kRowsAtOnce + group, rows = n * a.heads[0], r = at < rows ? at : rows - 1;
-      const int t = divided(r, by_heads), h = r - t * a.heads[0];
-      float y[8];
-      turned(kind, a.columns, t, fetch(kind, t, h), y);
-      if (!live || at >= rows) continue;
-      Eight<T> out;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(out.w)[e] = from_f32<T>(none ? 0.0f : y[e]);
-      store_eight(static_cast<T*>(kind.out) + (token0 + t) * kind.out_token + h * kind.out_head + c0, out);
-      continue;
-    }
-    const bool v = job - q_jobs >= each;
+  // ---- jobs: keys, then values, a head at a time (of one token kRowsAtOnce heads)
+  const bool one = u.n == 1;
+  const int each = one ? (p.kv_heads + kRowsAtOnce - 1) / kRowsAtOnce : p.kv_heads;
+  const int passes = one ? 1 : (u.n + kRowsAtOnce - 1) / kRowsAtOnce;
+  for (int job = share * 4 + wave; job < 2 * each; job += shares * 4) {
+    const bool v = job >= each;
     const Kind& kind = v ? a.kind[2] : a.kind[1];
-    const int in_kind = job - q_jobs - (v ? each : 0), columns = v ? 0 : a.columns;
-    const bool one = n == 1;
+    const int in_kind = v ? job - each : job;
     const int at_head = one ? in_kind * kRowsAtOnce + group : in_kind, head = at_head < p.kv_heads ? at_head : p.kv_heads - 1;
+    const bool is_head = live && at_head < p.kv_heads;
+    const T* rows = static_cast<const T*>(kind.x) + u.token0 * kind.token + head * kind.head + (live ? c0 : 0);
+    auto token_of = [&](int pass) __attribute__((always_inline)) {  // past the last: the last again
+      const int t = one ? 0 : pass * kRowsAtOnce + group;
+      return t < u.n ? t : u.n - 1;
+    };
+    float y[kHeld][8];
     float largest = 0.0f;
-    for (int t0 = 0; t0 < n; t0 += kRowsAtOnce) {
-      const int t = one ? 0 : t0 + group < n ? t0 + group : n - 1;
-      float y[8];
-      turned(kind, columns, t, fetch(kind, t, head), y);
-      largest = fmaxf(largest, most_of(y));
+    auto hold = [&](int first) __attribute__((always_inline)) {     // passes first .. first + kHeld - 1, those that there are
+      Eight<T> x[kHeld];
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (first + i < passes) x[i] = load_eight(rows + token_of(first + i) * kind.token);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (first + i >= passes) continue;
+        if (!live) x[i] = {};
+        if (v) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[i][e] = column(x[i], e);
+        } else {
+          turned(token_of(first + i), x[i], y[i]);
+        }
+      }
+    };
+    for (int first = 0; first < passes; first += kHeld) {
+      hold(first);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (first + i >= passes) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(y[i][e]) < INFINITY ? fabsf(y[i][e]) : 0.0f);
+      }
     }
     largest = one ? row_max<LPR>(largest) : wave_max(largest);
-    uint8_t* scale = v ? sc.v + page * sc.v_page + head * sc.v_head + block * sc.v_block : sc.k + page * sc.k_page + head * sc.k_head + block * sc.k_block;
-    uint8_t* codes = v ? static_cast<uint8_t*>(a.kind[2].out) + page * p.v_page + head * p.v_head
-                       : static_cast<uint8_t*>(a.kind[1].out) + page * p.k_page + head * p.k_head;
+    uint8_t* scale = v ? sc.v + u.page * sc.v_page + head * sc.v_head + u.block * sc.v_block
+                       : sc.k + u.page * sc.k_page + head * sc.k_head + u.block * sc.k_block;
     const int64_t slot_stride = v ? p.v_slot : p.k_slot;
+    uint8_t* codes = static_cast<uint8_t*>(kind.out) + u.slot * slot_stride + c0 + (v ? u.page * p.v_page + head * p.v_head : u.page * p.k_page + head * p.k_head);
     int e = exponent_of(largest);
     e = e < kLeastExponent<T> ? kLeastExponent<T> : e < kMostExponent<T> ? e : kMostExponent<T>;
-    if (old > 0) {
+    if (u.old > 0) {
       const int before = (int)*scale - 127;
       if (before > e) e = before < kMostExponent<T> ? before : kMostExponent<T>;
-      if (e > before && live && at_head < p.kv_heads)               // older tokens' numbers again
-        for (int s = one ? 0 : group; s < old; s += one ? 1 : kRowsAtOnce) {
-          u32x2* c = reinterpret_cast<u32x2*>(codes + (slot - old + s) * slot_stride + c0);
+      if (e > before && is_head)                                    // older tokens' numbers again
+        for (int s = one ? 0 : group; s < u.old; s += one ? 1 : kRowsAtOnce) {
+          u32x2* c = reinterpret_cast<u32x2*>(codes + (s - u.old) * slot_stride);
           *c = codes_again(*c, before - e);
         }
     }
     const float by = power_of_two(-e), limit = e == kMostExponent<T> ? 240.0f : 448.0f;
-    for (int t0 = 0; t0 < n; t0 += kRowsAtOnce) {
-      const int t = one ? 0 : t0 + group < n ? t0 + group : n - 1;
-      float y[8];
-      turned(kind, columns, t, fetch(kind, t, head), y);
-      if (live && at_head < p.kv_heads && (one || t0 + group < n))
-        *reinterpret_cast<u32x2*>(codes + (slot + t) * slot_stride + c0) = to_codes(y, by, limit);
+    for (int first = 0; first < passes; first += kHeld) {
+      if (passes > kHeld) hold(first);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int t = one ? 0 : (first + i) * kRowsAtOnce + group;
+        if (first + i < passes && is_head && t < u.n) *reinterpret_cast<u32x2*>(codes + t * slot_stride) = to_codes(y[i], by, limit);
+      }
     }
-    if (c0 == 0 && at_head < p.kv_heads && (one || group == 0)) *scale = (uint8_t)(e + 127);
+    if (c0 == 0 && is_head && (one || group == 0)) *scale = (uint8_t)(e + 127);
   }
 }
 
 template <typename T, int LPR>
 int launch_rows(const HeadArgs& a, const Pages& p, const Scales& sc, hipStream_t s) {
+  constexpr int64_t rows_at_once = kWave / LPR;
   const int64_t units = p.starts ? (int64_t)p.tokens / sc.block + 2 * ((int64_t)p.sequences + 2) : p.sequences;
-  const int64_t rows_at_once = kWave / LPR, jobs = (a.heads[0] + rows_at_once - 1) / rows_at_once + 2 * (a.heads[1] + rows_at_once - 1) / rows_at_once;
-  int64_t shares = 1024 / units, most = (jobs + 3) / 4;
+  const int64_t jobs = 2 * (p.starts ? p.kv_heads : (p.kv_heads + rows_at_once - 1) / rows_at_once), most = (jobs + 3) / 4;
+  int64_t shares = kUnitGroups / (units > 0 ? units : 1);
   shares = shares < 1 ? 1 : shares < most ? shares : most;
-  if (!grid_fits(units * shares, 256)) return HEXMI_ENOTSUP;
-  const unsigned lds = (unsigned)((p.starts ? sc.block : 1) * (a.columns / 2) * sizeof(f32x2));
-  const dim3 grid((unsigned)(units * shares));
-  const Divider by_heads = divider(a.heads[0] > 0 ? a.heads[0] : 1);
+  HeadArgs q = a;
+  q.heads[1] = q.heads[2] = 0;
+  const int64_t q_waves = a.heads[0] > 0 ? waves_per_token<LPR>(q) : 0;
+  const int64_t q_blocks = (a.tokens * q_waves + 3) / 4, q_grid = q_blocks < (1 << 22) ? q_blocks : 1 << 22;
+  if (!grid_fits(units * shares + q_grid, 256)) return HEXMI_ENOTSUP;
+  const unsigned lds = (unsigned)((p.starts ? sc.block : 1) * (a.columns / 2) * sizeof(f32x2)), kv_grid = (unsigned)(units * shares);
+  const dim3 grid((unsigned)(units * shares + q_grid));
+  if (grid.x == 0) return HEXMI_OK;
   if (!a.halves || a.columns == 0)
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, false, false>), grid, dim3(256), lds, s, a, p, sc, (int)shares, by_heads);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, false, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
   else if (a.columns % 16 == 0)
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, true>), grid, dim3(256), lds, s, a, p, sc, (int)shares, by_heads);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, true>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
   else
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, false>), grid, dim3(256), lds, s, a, p, sc, (int)shares, by_heads);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
   return launch_status();
 }
 template <typename T>
