@@ -172,6 +172,12 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
     return copied_column<D, COLS, PADDED>(c, dim);
   };
+  // what the lane of instruction j's first row has
+  auto of_first_row = [&](int64_t at, int j) __attribute__((always_inline)) {
+    const int row = row_wave * kRowsOfOne + j * kRowStep;
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, row), hi = __builtin_amdgcn_readlane((int)(at >> 32), row);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+  };
   // A scaled cache comes by way of registers: asked for when the block before is begun, widened to T and put into LDS when it is done.
   struct Coming {
     u32x2 k[NI], v[NI];
@@ -185,6 +191,17 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
     c.k_scale = (a.scales.k + kvh * a.scales.k_head)[page * a.scales.k_page + block_of_lane * a.scales.k_block];
     c.v_scale = (a.scales.v + kvh * a.scales.v_head)[page * a.scales.v_page + block_of_lane * a.scales.v_block];
+    if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const Held* from = (v ? v_head : k_head) + of_first_row(v ? v_at : k_at, j);
+          const uint32_t off = lane / CPR * (uint32_t)(v ? p.v_slot : p.k_slot) + column(v, copy_row + j * kRowStep);
+          (v ? c.v : c.k)[j] = *reinterpret_cast<const u32x2*>(from + off);
+        }
+      return c;
+    }
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -196,7 +213,20 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       }
     return c;
   };
+  const bool one_scale = Kind::kScaled && one_page && a.scales.block % kRowsOfOne == 0;
   auto put = [&](const Coming& c, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    if (one_scale && __ballot(page_of_lane >= 0) == ~0ull) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int row = row_wave * kRowsOfOne + j * kRowStep;
+        const uint32_t ks = __builtin_amdgcn_readlane((int)c.k_scale, row), vs = __builtin_amdgcn_readlane((int)c.v_scale, row);
+        *reinterpret_cast<Frag*>(k_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) =
+            widened<T>(c.k[j][0], c.k[j][1], __builtin_bit_cast(float, ks << 23));
+        *reinterpret_cast<Frag*>(v_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) =
+            widened<T>(c.v[j][0], c.v[j][1], __builtin_bit_cast(float, vs << 23));
+      }
+      return;
+    }
     const uint32_t k_scale = page_of_lane < 0 ? 127 : c.k_scale, v_scale = page_of_lane < 0 ? 0x80000000u | 127 : c.v_scale;     // the top bit: none
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -215,11 +245,6 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       // a lane works out where its key stands, for all of the block's at once; an instruction takes its first row's
       const int key_of_lane = key_at(block) + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
       const int64_t k_at = page_of_lane * p.k_page + slot_of_lane * p.k_slot, v_at = page_of_lane * p.v_page + slot_of_lane * p.v_slot;
-      auto first_of = [&](int64_t at, int j) __attribute__((always_inline)) {
-        const int row = row_wave * kRowsOfOne + j * kRowStep;
-        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, row), hi = __builtin_amdgcn_readlane((int)(at >> 32), row);
-        return (int64_t)((uint64_t)hi << 32 | lo);
-      };
       constexpr int kStep = kRowWaves * kWave * 16;                 // bytes of LDS between a wave's instructions
 #pragma unroll
       for (int v = 0; v < 2; ++v)
@@ -228,8 +253,8 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
           const T* head = v ? v_head : k_head;
           const int64_t at = v ? v_at : k_at;
           const int step = lane / CPR * (int)(v ? p.v_slot : p.k_slot);
-          copy_two_to_lds_asm<kStep>(reinterpret_cast<const char*>(head + first_of(at, j)), (step + column(v, copy_row + j * kRowStep)) * 2,
-                                     reinterpret_cast<const char*>(head + first_of(at, j + 1)),
+          copy_two_to_lds_asm<kStep>(reinterpret_cast<const char*>(head + of_first_row(at, j)), (step + column(v, copy_row + j * kRowStep)) * 2,
+                                     reinterpret_cast<const char*>(head + of_first_row(at, j + 1)),
                                      (step + column(v, copy_row + (j + 1) * kRowStep)) * 2,
                                      reinterpret_cast<char*>((v ? v_dst : k_dst) + lds_at) + j * kStep);
         }
