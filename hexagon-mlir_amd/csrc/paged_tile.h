@@ -72,6 +72,9 @@ __device__ __forceinline__ Run run_of_tile(const Pages& p, int group, int tile, 
   return run;
 }
 
+// A tile of keys in 8 bits: rows of D bytes, 16-byte chunks, XOR swizzled so that the 16 rows that a read takes at a time stand on all banks
+template <int D> __device__ __forceinline__ int swz_k8tile(int row) { return D == 64 ? (row >> 2) & 3 : D == 128 ? (row >> 1) & 7 : row & 15; }
+
 // keys that token i of a sequence's n sees, whatever the index tensors hold
 __device__ __forceinline__ int keys_of(int64_t length, int n, int i, int most) {
   const int64_t keys = length - n + i + 1;
@@ -169,6 +172,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   constexpr int kRowsOfOne = kWave / CPR;
   const bool one_page = p.page_size % kRowsOfOne == 0;
   auto column = [&](bool v, int r) __attribute__((always_inline)) {
+    if (Kind::kScaled && !v) return copied_column<D, COLS, PADDED>(((lin % CPR / 2) ^ swz_k8tile<D>(r)) * 16 + lin % 2 * 8, dim);
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
     return copied_column<D, COLS, PADDED>(c, dim);
   };
@@ -213,29 +217,30 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
       }
     return c;
   };
+  uint32_t k_scale_now = 127;                                       // of key lane % kKeys of the block that is in LDS
   const bool one_scale = Kind::kScaled && one_page && a.scales.block % kRowsOfOne == 0;
   auto put = [&](const Coming& c, int page_of_lane, T* k_dst, T* v_dst) __attribute__((always_inline)) {
+    // keys as they are, values widened
+    k_scale_now = c.k_scale;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) reinterpret_cast<u32x2*>(k_dst)[row_wave * kWave + lane + j * kRowWaves * kWave] = c.k[j];
     if (one_scale && __ballot(page_of_lane >= 0) == ~0ull) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int row = row_wave * kRowsOfOne + j * kRowStep;
-        const uint32_t ks = __builtin_amdgcn_readlane((int)c.k_scale, row), vs = __builtin_amdgcn_readlane((int)c.v_scale, row);
-        *reinterpret_cast<Frag*>(k_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) =
-            widened<T>(c.k[j][0], c.k[j][1], __builtin_bit_cast(float, ks << 23));
+        const uint32_t vs = __builtin_amdgcn_readlane((int)c.v_scale, row);
         *reinterpret_cast<Frag*>(v_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) =
             widened<T>(c.v[j][0], c.v[j][1], __builtin_bit_cast(float, vs << 23));
       }
       return;
     }
-    const uint32_t k_scale = page_of_lane < 0 ? 127 : c.k_scale, v_scale = page_of_lane < 0 ? 0x80000000u | 127 : c.v_scale;     // the top bit: none
+    const uint32_t v_scale = page_of_lane < 0 ? 0x80000000u | 127 : c.v_scale;     // the top bit: none
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int r = copy_row + j * kRowStep;
-      const uint32_t ks = __shfl((int)k_scale, r), vs = __shfl((int)v_scale, r);
-      const Frag k = widened<T>(c.k[j][0], c.k[j][1], __builtin_bit_cast(float, ks << 23));
+      const uint32_t vs = __shfl((int)v_scale, r);
       Frag v = widened<T>(c.v[j][0], c.v[j][1], __builtin_bit_cast(float, (vs & 255) << 23));
       if (vs >> 31) v = Frag{};
-      *reinterpret_cast<Frag*>(k_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) = k;
       *reinterpret_cast<Frag*>(v_dst + lds_at + j * (kRowWaves * kWave * 8) + lane * 8) = v;
     }
   };
@@ -295,7 +300,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
-      const int c = ds * 16 + half * 8;
+      const int c = Kind::kScaled ? ds / 2 * 32 + half * 16 + ds % 2 * 8 : ds * 16 + half * 8;      // as the keys' columns come
       if (!PADDED || c < dim) qf[ds] = *reinterpret_cast<const Frag*>(q + c);
       else qf[ds] = Frag{};
     }
@@ -346,7 +351,33 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[jt][r] = 0.0f;
-    {
+    if constexpr (Kind::kScaled) {
+      // 16 columns of a key a read, widened for two products
+      constexpr int kAhead = 2, PS = DS / 2;
+      float scale[JT];
+      if constexpr (JT == 2) swap32(__builtin_bit_cast(float, k_scale_now << 23), scale[0], scale[1]);
+      else scale[0] = __builtin_bit_cast(float, k_scale_now << 23);
+      auto read_k = [&](int jt, int i) __attribute__((always_inline)) {
+        const int r = jt * 32 + lane % 32, c = (i * 2 + half) ^ swz_k8tile<D>(r);
+        return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(k_src) + r * D + c * 16);
+      };
+      u32x4 kf[JT][PS];
+#pragma unroll
+      for (int i = 0; i < kAhead && i < PS; ++i)
+#pragma unroll
+        for (int jt = 0; jt < JT; ++jt) kf[jt][i] = read_k(jt, i);
+#pragma unroll
+      for (int i = 0; i < PS; ++i) {
+        if (i + kAhead < PS)
+#pragma unroll
+          for (int jt = 0; jt < JT; ++jt) kf[jt][i + kAhead] = read_k(jt, i + kAhead);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int jt = 0; jt < JT; ++jt) s[jt] = MfmaT<T>::run(widened<T>(kf[jt][i][2 * h], kf[jt][i][2 * h + 1], scale[jt]), qf[2 * i + h], s[jt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
       constexpr int kAhead = 3;
       auto read_k = [&](int jt, int ds) __attribute__((always_inline)) {
         const int r = jt * 32 + lane % 32, c = (ds * 2 + half) ^ swz_ktile<D == 64 ? 64 : 128>(r);
