@@ -19,19 +19,30 @@ struct CopyArgs {
   int pieces;                                  // of a row
 };
 
+// pieces first, first + step, .. of all of the first `slots` slots of page `from` to page `to`, in the order of memory: heads within slots or slots
+// within heads, what stands side by side as one run. Four are on their way at a time.
 template <typename Piece>
 __device__ __forceinline__ void copy_rows(const Side& side, int from, int to, int heads, int slots, int pieces, int first, int step) {
-  // the order of memory: slots within heads, or heads within slots
   const bool slots_inside = side.slot < side.head;
-  const int inner = slots_inside ? slots : heads;
-  const int64_t inner_stride = slots_inside ? side.slot : side.head, outer_stride = slots_inside ? side.head : side.slot;
+  const int64_t row = pieces * (int64_t)sizeof(Piece), inner_stride = slots_inside ? side.slot : side.head, outer_stride = slots_inside ? side.head : side.slot;
+  const int inner = slots_inside ? slots : heads, all = heads * slots * pieces;
+  const bool runs = inner_stride == row;
+  const int run = runs ? inner * pieces : pieces;
   const char* src = side.pages + from * side.page;
   char* dst = side.pages + to * side.page;
-  const int64_t all = (int64_t)heads * slots * pieces;
-  for (int64_t i = first; i < all; i += step) {
-    const int64_t r = i / pieces, o = r / inner;
-    const int64_t at = o * outer_stride + (r - o * inner) * inner_stride + (i - r * pieces) * sizeof(Piece);
-    *reinterpret_cast<Piece*>(dst + at) = *reinterpret_cast<const Piece*>(src + at);
+  constexpr int kAtOnce = 4;
+  for (int i0 = first; i0 < all; i0 += kAtOnce * step) {
+    Piece x[kAtOnce];
+    int64_t at[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * step, o = i / run;
+      at[u] = (runs ? o * outer_stride : o / inner * outer_stride + o % inner * inner_stride) + (i - o * run) * (int64_t)sizeof(Piece);
+      if (i < all) x[u] = *reinterpret_cast<const Piece*>(src + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (i0 + u * step < all) *reinterpret_cast<Piece*>(dst + at[u]) = x[u];
   }
 }
 __device__ __forceinline__ void copy_scales(const CopyArgs& c, int side, int from, int to, int heads, int blocks, int first, int step) {
@@ -69,7 +80,10 @@ void fork_kernel(CopyArgs c, Pages p, const int32_t* parents, const int32_t* pag
   }
 }
 
-// ---- compact: mark (a bit a page), number what is to go and where to, move and rename
+// ---- compact: mark (a bit a page), number what is to go and where to, move and rename. Few entries and pages go to one workgroup, and two
+// launches do.
+constexpr int kFewEntries = 8192, kFewWords = 8192;
+constexpr int kMovePieces = 1024;              // of a page, a workgroup at a time
 struct CompactSpace {
   uint32_t* marks;                             // [words]
   int32_t *renamed, *sources, *targets;        // [pages]
@@ -95,27 +109,31 @@ __device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, i
   const int page = p.table[b * p.table_row + column];
   return page >= 0 && page < p.num_pages ? page : -1;
 }
+// entry i of the table, row by row
+__device__ __forceinline__ int used_page(const Pages& p, const View& w, int64_t i) {
+  const int b = (int)(i / p.table_cols);
+  return used_page(p, w, b, (int)(i - (int64_t)b * p.table_cols));
+}
 __global__ __launch_bounds__(256)
 void mark_kernel(Pages p, View w, uint32_t* marks, int64_t entries) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
-    const int b = (int)(i / p.table_cols), page = used_page(p, w, b, (int)(i - (int64_t)b * p.table_cols));
+    const int page = used_page(p, w, i);
     if (page < 0) continue;
     const uint32_t bit = 1u << page % 32;
     if (!(__hip_atomic_load(marks + page / 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit)) atomicOr(marks + page / 32, bit);
   }
 }
 
-// One workgroup: a thread takes a run of words, twice.
-__global__ __launch_bounds__(1024)
-void number_kernel(CompactSpace s, int num_pages, int32_t* count) {
+// By a workgroup of 1024: how many pages are marked, which of them go where, and their new names. A thread takes a run of words, twice.
+__device__ __forceinline__ void number_pages(const uint32_t* marks, const CompactSpace& s, int num_pages, int32_t* count) {
   __shared__ int sums[16], used_below, total;
   const int words = (int)words_of(num_pages), each = (words + 1023) / 1024;
   const int w0 = (int)threadIdx.x * each < words ? (int)threadIdx.x * each : words, w1 = w0 + each < words ? w0 + each : words;
   int n = 0;
-  for (int w = w0; w < w1; ++w) n += __popc(s.marks[w]);
+  for (int w = w0; w < w1; ++w) n += __popc(marks[w]);
   // the sum over the threads before this one
-  int up_to = n;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int up_to = n;
   for (int d = 1; d < kWave; d *= 2) {
     const int v = __shfl_up(up_to, d);
     if (lane >= d) up_to += v;
@@ -131,50 +149,68 @@ void number_kernel(CompactSpace s, int num_pages, int32_t* count) {
   // used pages below `front`: the thread whose run holds it says
   if (front / 32 >= w0 && front / 32 < w1) {
     int below = before;
-    for (int w = w0; w < front / 32; ++w) below += __popc(s.marks[w]);
-    used_below = below + __popc(s.marks[front / 32] & ((1u << front % 32) - 1));
+    for (int w = w0; w < front / 32; ++w) below += __popc(marks[w]);
+    used_below = below + __popc(marks[front / 32] & ((1u << front % 32) - 1));
   } else if (threadIdx.x == 0 && front / 32 >= words) {
     used_below = total;                                             // all pages are in use
   }
   __syncthreads();
-  const int moved = used_below;
+  const int moved = used_below, moves = front - moved;
   int used = before;
   for (int w = w0; w < w1; ++w) {
-    const uint32_t marks = s.marks[w];
-    const int page0 = w * 32, last = num_pages - page0 < 32 ? num_pages - page0 : 32;
-    for (int i = 0; i < last; ++i) {
-      const int page = page0 + i;
-      if (marks >> i & 1) {
-        if (page >= front) s.sources[used - moved] = page;
-        ++used;
-      } else if (page < front) {
-        s.targets[page - used] = page;
-      }
+    const uint32_t word = marks[w];
+    const int page0 = w * 32;
+    // of a word's pages those below `front` that are free, and those from it on that are in use
+    const uint32_t below = front >= page0 + 32 ? ~0u : front <= page0 ? 0u : (1u << (front - page0)) - 1;
+    for (uint32_t free = ~word & below; free; free &= free - 1) {
+      const int i = __ffs(free) - 1;
+      s.targets[page0 + i - used - __popc(word & ((1u << i) - 1))] = page0 + i;
     }
+    for (uint32_t go = word & ~below; go; go &= go - 1) {
+      const int i = __ffs(go) - 1;
+      s.sources[used + __popc(word & ((1u << i) - 1)) - moved] = page0 + i;
+    }
+    used += __popc(word);
   }
   if (threadIdx.x == 0) {
-    *s.moves = front - moved;
+    *s.moves = moves;
     *count = front;
   }
+  __syncthreads();                                                  // sources and targets are the workgroup's own
+  for (int i = threadIdx.x; i < moves; i += 1024) s.renamed[s.sources[i]] = s.targets[i];
 }
-__global__ __launch_bounds__(256)
-void name_kernel(CompactSpace s) {
-  const int moves = *s.moves;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < moves; i += gridDim.x * 256) s.renamed[s.sources[i]] = s.targets[i];
+__global__ __launch_bounds__(1024)
+void number_kernel(CompactSpace s, int num_pages, int32_t* count) { number_pages(s.marks, s, num_pages, count); }
+
+// All of it by one workgroup, the marks in LDS.
+__global__ __launch_bounds__(1024)
+void mark_and_number_kernel(Pages p, View w, CompactSpace s, int32_t* count, int entries) {
+  __shared__ uint32_t marks[kFewWords];
+  const int words = (int)words_of(p.num_pages);
+  for (int i = threadIdx.x; i < words; i += 1024) marks[i] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < entries; i += 1024) {
+    const int page = used_page(p, w, i);
+    if (page >= 0) atomicOr(marks + page / 32, 1u << page % 32);
+  }
+  __syncthreads();
+  number_pages(marks, s, p.num_pages, count);
 }
 
 template <typename Piece>
 __global__ __launch_bounds__(256)
-void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int64_t entries) {
+void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int64_t entries, int parts) {
   const int front = *count, moves = *s.moves;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
     const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols), page = used_page(p, w, b, column);
     table_out[b * table_out_row + column] = page >= front ? s.renamed[page] : page;
   }
-  for (int64_t i = blockIdx.x; i < 2 * (int64_t)moves; i += gridDim.x) {
-    const int move = (int)(i / 2), side = (int)(i - 2 * (int64_t)move), from = s.sources[move], to = s.targets[move];
-    copy_rows<Piece>(c.side[side], from, to, p.kv_heads, p.page_size, c.pieces, threadIdx.x, 256);
-    if (c.block) copy_scales(c, side, from, to, p.kv_heads, divided(p.page_size, c.by_block), threadIdx.x, 256);
+  for (int64_t i = blockIdx.x; i < 2 * (int64_t)moves * parts; i += gridDim.x) {
+    const int64_t unit = i / parts;
+    const int part = (int)(i - unit * parts), move = (int)(unit / 2), side = (int)(unit - 2 * (int64_t)move), from = s.sources[move], to = s.targets[move];
+    copy_rows<Piece>(c.side[side], from, to, p.kv_heads, p.page_size, c.pieces, part * 256 + threadIdx.x, parts * 256);
+    if (c.block) copy_scales(c, side, from, to, p.kv_heads, divided(p.page_size, c.by_block), part * 256 + threadIdx.x, parts * 256);
   }
 }
 
@@ -200,6 +236,7 @@ int check_cache(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales
     for (int64_t x : {(int64_t)reinterpret_cast<uintptr_t>(s.pages), s.page, s.head, s.slot, b.dim * size})
       while (x % piece != 0) piece /= 2;
   c.pieces = (int)(b.dim * size / piece);
+  if (b.kv_heads * b.page_size > 0x3fffffff / c.pieces) return HEXMI_ENOTSUP;     // pieces of a page are counted in 32 bits
   if (scales) {
     c.scales[0] = scales->k_scales;
     c.scales[1] = scales->v_scales;
@@ -279,12 +316,19 @@ extern "C" int hexmi_paged_compact(const hexmi_paged_batch* batch, const hexmi_p
   const int64_t words = words_of(batch->num_pages);
   auto blocks = [](int64_t n, int64_t most) { return dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)); };
   begin_call();
-  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, space.marks, words);
-  if (entries > 0) hipLaunchKernelGGL(mark_kernel, blocks(entries, 4096), dim3(256), 0, s, p, view, space.marks, entries);
-  hipLaunchKernelGGL(number_kernel, dim3(1), dim3(1024), 0, s, space, (int)batch->num_pages, count);
-  hipLaunchKernelGGL(name_kernel, blocks(batch->num_pages, 256), dim3(256), 0, s, space);
+  if (entries <= kFewEntries && words <= kFewWords) {
+    hipLaunchKernelGGL(mark_and_number_kernel, dim3(1), dim3(1024), 0, s, p, view, space, count, (int)entries);
+  } else {
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, space.marks, words);
+    if (entries > 0) hipLaunchKernelGGL(mark_kernel, blocks(entries, 4096), dim3(256), 0, s, p, view, space.marks, entries);
+    hipLaunchKernelGGL(number_kernel, dim3(1), dim3(1024), 0, s, space, (int)batch->num_pages, count);
+  }
+  // a workgroup for some KiB of a page; no more than half of the pages move
+  const int64_t page_pieces = batch->kv_heads * batch->page_size * c.pieces, parts = (page_pieces + kMovePieces - 1) / kMovePieces;
+  const int64_t units = batch->num_pages * parts > (entries + 255) / 256 ? batch->num_pages * parts : (entries + 255) / 256;
   return with_piece(piece, [&](auto x) {
-    hipLaunchKernelGGL((move_kernel<decltype(x)>), dim3(2048), dim3(256), 0, s, c, p, view, space, count, table_out, table_out_row, entries);
+    hipLaunchKernelGGL((move_kernel<decltype(x)>), dim3((unsigned)(units < 2048 ? units : 2048)), dim3(256), 0, s, c, p, view, space, count, table_out,
+                       table_out_row, entries, (int)parts);
     return launch_status();
   });
 }
