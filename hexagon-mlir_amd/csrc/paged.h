@@ -219,6 +219,13 @@ int launch_paged_workers(const PagedAttnArgs& a, const Pages& p, const DecodeArg
 template <typename Kind>
 int launch_paged_shared(const PagedAttnArgs& a, const Pages& p, const TileArgs& tiles, const DecodeArgs& w, unsigned grid, int dtype,
                         hipStream_t s);
+#define HEXMI_PAGED_KIND(EXTERN, KIND)                                                                                              \
+  EXTERN template int launch_paged_tiles<KIND>(const PagedAttnArgs&, const Pages&, const TileArgs&, int, hipStream_t);                \
+  EXTERN template int launch_paged_workers<KIND>(const PagedAttnArgs&, const Pages&, const DecodeArgs&, unsigned, int, hipStream_t);  \
+  EXTERN template int launch_paged_shared<KIND>(const PagedAttnArgs&, const Pages&, const TileArgs&, const DecodeArgs&, unsigned, int, hipStream_t);
+HEXMI_PAGED_KIND(extern, Whole)
+HEXMI_PAGED_KIND(extern, Windowed)
+HEXMI_PAGED_KIND(extern, Scaled)
 // f of the kind that a call is of
 template <typename F> int with_kind(const PagedAttnArgs& a, F&& f) {
   return a.scales.k ? f(Scaled{}) : a.view != kNoWindow ? f(Windowed{}) : f(Whole{});

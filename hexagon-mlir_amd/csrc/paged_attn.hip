@@ -139,7 +139,7 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t vie
   if (b.dim % 8 != 0 || b.dim > 256 || heads > 65535) return HEXMI_ENOTSUP;
   // rows, the blocks of all sequences and heads, and a launch's threads stay below 2^31
   const int64_t group = heads / b.kv_heads, limit = 0x7fffffff, units = b.kv_heads * ((group + 15) / 16);
-  const int64_t blocks = (b.table_cols * b.page_size + 127) / 128 + 1;
+  const int64_t blocks = (b.table_cols * b.page_size + 127) / 128 + 2;
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   if (b.tokens == 0) return HEXMI_OK;          // nothing to launch: there is no plan of it (plan_of divides by the tiles)

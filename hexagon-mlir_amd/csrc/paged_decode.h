@@ -54,10 +54,18 @@ template <int W> __device__ __forceinline__ int blocks_of_keys(int keys) {
   return keys > W * kTileKeys ? (keys + W * kTileKeys - 1) / (W * kTileKeys) : 1;
 }
 // of sequence b, none where it has other than one new token (the tiles take those)
-// view: the most keys that its token sees
+// View: the most keys that its token sees, and the blocks that a unit counts for beside its own when the work is dealt: to begin one costs
+// a worker about the time of a block in 8 bits.
+struct Dealt {
+  int view, extra;
+};
+constexpr int kExtraBlocks = 1;                // of a cache in 8 bits; in 16, none
 __device__ __forceinline__ int at_most(int n, int most) { return n < most ? n : most; }
-template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix, int view) {
-  return new_tokens_of(p, b) == 1 ? blocks_of_keys<W>(at_most(length_of(p, b), view) - prefix) : 0;
+template <int W> __device__ __forceinline__ int dealt_blocks(int length, int prefix, const Dealt& d) {
+  return blocks_of_keys<W>(at_most(length, d.view) - prefix) + d.extra;
+}
+template <int W> __device__ __forceinline__ int blocks_of(const Pages& p, int b, int prefix, const Dealt& d) {
+  return new_tokens_of(p, b) == 1 ? dealt_blocks<W>(length_of(p, b), prefix, d) : 0;
 }
 // the sum over the lanes up to this one
 __device__ __forceinline__ int sum_up_to(int v) {
@@ -78,23 +86,23 @@ struct BlockList {
   int of_64, all;                              // blocks of the first 64 sequences, of all (one unit's)
 };
 template <int W>
-__device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, int view, int lane) {
+__device__ __forceinline__ BlockList block_list(const Pages& p, int prefix, const Dealt& d, int lane) {
   BlockList l;
   l.length = lane < p.sequences ? length_of(p, lane) : 0;
-  l.blocks = lane < p.sequences && new_tokens_of(p, lane) == 1 ? blocks_of_keys<W>(at_most(l.length, view) - prefix) : 0;
+  l.blocks = lane < p.sequences && new_tokens_of(p, lane) == 1 ? dealt_blocks<W>(l.length, prefix, d) : 0;
   l.up_to = sum_up_to(l.blocks);
   l.of_64 = of_last_lane(l.up_to);
   int more = 0;
-  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, view) : 0;
+  for (int b0 = kWave; b0 < p.sequences; b0 += kWave) more += b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, d) : 0;
   l.all = l.of_64 + (p.sequences > kWave ? of_last_lane(sum_up_to(more)) : 0);
   return l;
 }
 // The sequence that block `at` of the list belongs to, with `units` units a sequence, and the blocks (of one unit) before it.
 template <int W>
-__device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, int view, int units, int at, int lane, int& before) {
+__device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, int prefix, const Dealt& d, int units, int at, int lane, int& before) {
   before = 0;
   for (int b0 = 0;; b0 += kWave) {
-    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, view) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
+    const int n = b0 == 0 ? l.blocks : b0 + lane < p.sequences ? blocks_of<W>(p, b0 + lane, prefix, d) : 0, sum = b0 == 0 ? l.up_to : sum_up_to(n);
     const uint64_t past = __ballot((before + sum) * units > at);
     if (past || b0 + kWave >= p.sequences) {   // `at` is below the end: there is one
       const int first = past ? __ffsll((unsigned long long)past) - 1 : 0;
@@ -107,8 +115,8 @@ __device__ __forceinline__ int sequence_at(const BlockList& l, const Pages& p, i
 __device__ __forceinline__ int length_at(const BlockList& l, const Pages& p, int b) {
   return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.length, b & (kWave - 1)) : length_of(p, b));
 }
-template <int W> __device__ __forceinline__ int blocks_at(const BlockList& l, const Pages& p, int prefix, int view, int b) {
-  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.blocks, b & (kWave - 1)) : blocks_of<W>(p, b, prefix, view));
+template <int W> __device__ __forceinline__ int blocks_at(const BlockList& l, const Pages& p, int prefix, const Dealt& d, int b) {
+  return __builtin_amdgcn_readfirstlane(b < kWave ? __builtin_amdgcn_readlane(l.blocks, b & (kWave - 1)) : blocks_of<W>(p, b, prefix, d));
 }
 // worker w's run of `total` blocks
 __device__ __forceinline__ int run_start(int total, int workers, int w) {
@@ -154,7 +162,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
   constexpr int LS = kWide ? DS / 2 : DS;                           // loads of a row
   typedef std::conditional_t<Kind::kScaled && !kWide, u32x2, u32x4> Raw;
   typedef std::conditional_t<Kind::kScaled, uint8_t, T> Held;
-  const int view = Kind::kWindow ? a.view : kNoWindow;
+  const Dealt dealt = {Kind::kWindow ? a.view : kNoWindow, Kind::kScaled ? kExtraBlocks : 0};
   constexpr int kWaveBytes = decode_wave_bytes(D, COLS), kBlock = W * kTileKeys;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane / 16, n = lane % 16;
@@ -175,22 +183,22 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     unit = worker - b * units;
     list.length = 0;
     cur = 0;
-    end = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix, view));
+    end = __builtin_amdgcn_readfirstlane(blocks_of<W>(p, b, a.prefix, dealt));
   } else {
-    list = block_list<W>(p, a.prefix, view, lane);
+    list = block_list<W>(p, a.prefix, dealt, lane);
     total = list.all * units;
     cur = run_start(total, w.workers, worker);
     end = run_start(total, w.workers, worker + 1);
     if (wave == 0 && lane == 0) w.begun[worker].last = -1;
     if (cur >= end) return;
-    b = sequence_at<W>(list, p, a.prefix, view, units, cur, lane, before);
+    b = sequence_at<W>(list, p, a.prefix, dealt, units, cur, lane, before);
   }
   const int start = cur;
 
   while (cur < end) {
     const int whole_length = w.workers ? length_at(list, p, b) : __builtin_amdgcn_readfirstlane(length_of(p, b));
-    const int length = at_most(whole_length, view), skip = whole_length - length;      // keys that are seen; those between the sinks and the others
-    const int blocks = w.workers ? blocks_at<W>(list, p, a.prefix, view, b) : end - cur, local = cur - before * units;
+    const int length = at_most(whole_length, dealt.view), skip = whole_length - length;      // keys that are seen; those between the sinks and the others
+    const int blocks = w.workers ? blocks_at<W>(list, p, a.prefix, dealt, b) : end - cur, local = cur - before * units;
     if (local >= blocks * units) {             // on to the next sequence
       before += blocks;
       ++b;
@@ -223,8 +231,9 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
     float m = -INFINITY, neg_m = 0.0f, l = 0.0f;
 
     // ---- keys: this wave's tiles of the run
-    const int key_first = a.prefix + (block0 * W + wave) * kTileKeys;
-    int key_end = a.prefix + (block0 + count) * kBlock;
+    auto own_block = [&](int block) __attribute__((always_inline)) { return block > dealt.extra ? block - dealt.extra : 0; };
+    const int key_first = a.prefix + (own_block(block0) * W + wave) * kTileKeys;
+    int key_end = a.prefix + own_block(block0 + count) * kBlock;
     key_end = key_end < length ? key_end : length;
     const int32_t* table = p.table + b * p.table_row;
     const Held* k_head = static_cast<const Held*>(a.k) + kvh * p.k_head;

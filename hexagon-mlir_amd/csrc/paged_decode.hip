@@ -19,10 +19,11 @@ void paged_decode_join_kernel(PagedAttnArgs a, Pages p, DecodeArgs w) {
     u = blockIdx.x - b * units;
     if (w.workers) {
       const int lane = threadIdx.x % kWave;
-      const BlockList list = block_list<kWaves>(p, a.prefix, a.view, lane);
+      const Dealt dealt = {a.view, a.scales.k ? kExtraBlocks : 0};
+      const BlockList list = block_list<kWaves>(p, a.prefix, dealt, lane);
       int before = 0;
-      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<kWaves>(p, x, a.prefix, a.view);
-      const int blocks = blocks_at<kWaves>(list, p, a.prefix, a.view, b), total = list.all * units;
+      for (int x = lane; x < b; x += kWave) before += x < kWave ? list.blocks : blocks_of<kWaves>(p, x, a.prefix, dealt);
+      const int blocks = blocks_at<kWaves>(list, p, a.prefix, dealt, b), total = list.all * units;
       const int first = of_last_lane(sum_up_to(before)) * units + u * blocks;
       w0 = worker_of(total, w.workers, first);
       w1 = worker_of(total, w.workers, first + blocks - 1);
