@@ -9,7 +9,9 @@
 namespace hexmi {
 namespace {
 
-constexpr int kUnitGroups = 2048;              // workgroups wanted for keys and values
+// Workgroups wanted for keys and values: a unit's heads are shared while they are fewer. 1024 / 2048 / 4096: prompts of 8100 tokens 46.5 / 50.9 /
+// 51.2 us (every share works out the angles again); keys and values by workgroups of their own 51 (their rows stand side by side).
+constexpr int kUnitGroups = 1024;
 
 // Units (a sequence's new tokens of one block): those of sequence b are numbered from first_unit(b) on, b = -1 .. sequences (first_row). n
 // tokens stand in at most floor((n - 2) / block) + 2 blocks and floor(x1 / block) - floor(x0 / block) >= floor(n / block) for x1 = x0 + n, so
@@ -106,26 +108,32 @@ __device__ __forceinline__ Unit unit_at(const Pages& p, const Scales& sc, int un
   return u;
 }
 
-// Workgroups from kv_grid on take the queries, as head_rows_kernel does; the others a unit and a share of its heads. LPR lanes take a row, eight
-// columns each (HALVES, PIECES: head_rows.h). A wave holds kHeld times the rows that it has at once, so that rows of a block are read and
+// kv_grid workgroups take a unit and a share of its heads each, q_grid the queries, as head_rows_kernel does; eights of both kinds by turns
+// (workgroup ids go round robin to the 8 XCDs), so that neither waits for the other: prompts of 8100 tokens 46.6 us, one kind behind the other
+// 56. LPR lanes take a row, eight columns each (HALVES, PIECES: head_rows.h). A wave holds kHeld times the rows that it has at once, so that rows of a block are read and
 // turned once; larger blocks are gone through twice.
 template <typename T, int LPR, bool HALVES, bool PIECES>
 __global__ __launch_bounds__(256, 4)
-void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, int shares, int q_waves) {
+void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, unsigned q_grid, int shares, int q_waves) {
   constexpr int kRowsAtOnce = kWave / LPR, kHeld = 4;
   __shared__ __attribute__((aligned(16))) HeadRowsLds<T, LPR, HALVES> lds;
   extern __shared__ __attribute__((aligned(16))) f32x2 angle[];    // [tokens of the block][columns / 2]
-  if (blockIdx.x >= kv_grid) {
+  const uint32_t eight = blockIdx.x / 8, kv_eights = (kv_grid + 7) / 8, eights = gridDim.x / 8;
+  const uint32_t before = (uint32_t)((uint64_t)eight * kv_eights / eights);      // eights of keys and values before this one
+  const bool is_q = (uint32_t)((uint64_t)(eight + 1) * kv_eights / eights) == before;
+  const uint32_t id = (is_q ? eight - before : before) * 8 + blockIdx.x % 8;
+  if (is_q) {
     HeadArgs q = a;
     q.heads[1] = q.heads[2] = 0;
-    head_rows_of<T, LPR, HALVES, PIECES, true>(q, p, q_waves, blockIdx.x - kv_grid, gridDim.x - kv_grid, lds);
+    if (id < q_grid) head_rows_of<T, LPR, HALVES, PIECES, true>(q, p, q_waves, id, q_grid, lds);
     return;
   }
+  if (id >= kv_grid) return;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c0 = lane % LPR * 8, group = lane / LPR, half = a.columns / 2;
   const bool live = c0 < a.dim, turns = c0 < a.columns;
-  const int share = blockIdx.x % shares;
-  const Unit u = unit_at(p, sc, blockIdx.x / shares, lane);
+  const int share = id % shares;
+  const Unit u = unit_at(p, sc, id / shares, lane);
   if (u.n <= 0 || u.page < 0) return;
   for (int i = threadIdx.x; i < u.n * half; i += 256) {
     const int t = i / half;
@@ -280,16 +288,16 @@ int launch_rows(const HeadArgs& a, const Pages& p, const Scales& sc, hipStream_t
   q.heads[1] = q.heads[2] = 0;
   const int64_t q_waves = a.heads[0] > 0 ? waves_per_token<LPR>(q) : 0;
   const int64_t q_blocks = (a.tokens * q_waves + 3) / 4, q_grid = q_blocks < (1 << 22) ? q_blocks : 1 << 22;
-  if (!grid_fits(units * shares + q_grid, 256)) return HEXMI_ENOTSUP;
+  if (!grid_fits(units * shares + q_grid + 16, 256)) return HEXMI_ENOTSUP;
   const unsigned lds = (unsigned)((p.starts ? sc.block : 1) * (a.columns / 2) * sizeof(f32x2)), kv_grid = (unsigned)(units * shares);
-  const dim3 grid((unsigned)(units * shares + q_grid));
+  const dim3 grid((kv_grid + 7) / 8 * 8 + (unsigned)(q_grid + 7) / 8 * 8);
   if (grid.x == 0) return HEXMI_OK;
   if (!a.halves || a.columns == 0)
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, false, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, false, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (unsigned)q_grid, (int)shares, (int)q_waves);
   else if (a.columns % 16 == 0)
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, true>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, true>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (unsigned)q_grid, (int)shares, (int)q_waves);
   else
-    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (int)shares, (int)q_waves);
+    hipLaunchKernelGGL((scaled_rows_kernel<T, LPR, true, false>), grid, dim3(256), lds, s, a, p, sc, kv_grid, (unsigned)q_grid, (int)shares, (int)q_waves);
   return launch_status();
 }
 template <typename T>

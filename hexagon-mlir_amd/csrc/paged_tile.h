@@ -137,14 +137,13 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     if (Kind::kWindow && !none) hidden = keys_of(length, new_tokens, divided(row0, a.by_group), most) - a.window;
   }
   end = __builtin_amdgcn_readfirstlane(end);
-  // Blocks are counted without those in which nothing is seen: block `sink_blocks` is the one that the window begins in.
+  // The keys that are walked: the sinks and those from the first that the tile's first row sees, as if they stood side by side, cut at whole 16s
+  // so that an instruction's rows are neighbours all the same.
   hidden = Kind::kWindow ? __builtin_amdgcn_readfirstlane(hidden) : 0;
-  const int sink_blocks = Kind::kWindow ? a.sinks / kKeys + (a.sinks % kKeys != 0) : 0;
-  const int left_out = Kind::kWindow && hidden / kKeys > sink_blocks ? hidden / kKeys - sink_blocks : 0;
-  auto key_at = [&](int block) __attribute__((always_inline)) {
-    return begin + (Kind::kWindow && block >= sink_blocks ? block + left_out : block) * kKeys;
-  };
-  const int blocks = end > begin ? (end - begin + kKeys - 1) / kKeys - left_out : 0, share = (blocks + splits - 1) / splits;
+  const int sinks16 = Kind::kWindow ? (a.sinks + 15) & ~15 : 0;
+  const int left_out = Kind::kWindow && (hidden & ~15) > sinks16 ? (hidden & ~15) - sinks16 : 0;
+  auto key_at = [&](int walked) __attribute__((always_inline)) { return begin + walked + (Kind::kWindow && walked >= sinks16 ? left_out : 0); };
+  const int blocks = end > begin ? (end - begin - left_out + kKeys - 1) / kKeys : 0, share = (blocks + splits - 1) / splits;
   const int block0 = part * share, block1 = block0 + share < blocks ? block0 + share : blocks;
 
   const int first = block0 + group;                                 // this group's blocks: first, first + kGroups, ..
@@ -157,11 +156,11 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   // The table's entry for key kKeys block + lane. No branch: it is asked for a block ahead, and what it is worth is looked at then (a load
   // behind a branch would be waited for where the branch ends).
   auto find = [&](int block) __attribute__((always_inline)) {
-    const int key = key_at(block) + lane % kKeys;
+    const int key = key_at(block * kKeys + lane % kKeys);
     return table[divided(key < end ? key : end - 1, p.size)];       // end > begin: only asked then
   };
   auto page_at = [&](int block, int entry) __attribute__((always_inline)) {     // -1: no key there
-    const int key = key_at(block) + lane % kKeys;
+    const int key = key_at(block * kKeys + lane % kKeys);
     const bool unseen = Kind::kWindow && key >= a.sinks && key < hidden;
     return block < block1 && key < end && !unseen && entry >= 0 && entry < p.num_pages ? entry : -1;
   };
@@ -189,7 +188,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   };
   auto ask = [&](int block, int page_of_lane) __attribute__((always_inline)) {
     Coming c;
-    const int key_of_lane = key_at(block) + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
+    const int key_of_lane = key_at(block * kKeys + lane % kKeys), slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
     const int64_t page = page_of_lane < 0 ? 0 : page_of_lane;       // no key: what stands in the first page, and zeros in its place
     const int64_t k_at = page * p.k_page + slot_of_lane * p.k_slot, v_at = page * p.v_page + slot_of_lane * p.v_slot;
     const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
@@ -248,7 +247,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     if constexpr (!Kind::kScaled) {
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
       // a lane works out where its key stands, for all of the block's at once; an instruction takes its first row's
-      const int key_of_lane = key_at(block) + lane % kKeys, slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
+      const int key_of_lane = key_at(block * kKeys + lane % kKeys), slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
       const int64_t k_at = page_of_lane * p.k_page + slot_of_lane * p.k_slot, v_at = page_of_lane * p.v_page + slot_of_lane * p.v_slot;
       constexpr int kStep = kRowWaves * kWave * 16;                 // bytes of LDS between a wave's instructions
 #pragma unroll
@@ -267,7 +266,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     }
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int r = copy_row + j * kRowStep, key = key_at(block) + r, page = __shfl(page_of_lane, r);
+      const int r = copy_row + j * kRowStep, key = key_at(block * kKeys + r), page = __shfl(page_of_lane, r);
       const int slot = key - divided(key, p.size) * p.page_size;
       T *k_to = k_dst + lds_at + j * (kRowWaves * kWave * 8), *v_to = v_dst + lds_at + j * (kRowWaves * kWave * 8);
       if (page >= 0) {
@@ -341,11 +340,11 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   float m_i = -INFINITY, neg_m = 0.0f, l_i = 0.0f;
 
   auto process = [&](int block, uint64_t there, int next_page, const T* k_src, const T* v_src, T* k_dst, T* v_dst) __attribute__((always_inline)) {
-    const int key0 = key_at(block);
+    const int walked0 = block * kKeys, key0 = key_at(walked0);
     if constexpr (!Kind::kScaled)
       if (block + kGroups < block1) copy(block + kGroups, next_page, k_dst, v_dst);
     if (block >= block1 || key0 >= most_keys) return;               // wave-uniform; the barriers are outside
-    if (Kind::kWindow && key0 >= a.sinks && key0 + kKeys <= least_keys - a.window) return;
+    if (Kind::kWindow && walked0 >= sinks16 && key0 + kKeys <= least_keys - a.window) return;
     f32x16 s[JT];
 #pragma unroll
     for (int jt = 0; jt < JT; ++jt)
@@ -422,14 +421,16 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     read_v(0, vf0);
     __builtin_amdgcn_sched_barrier(0);
     // s[jt][r] is the score of key key0 + 32 jt + 8 (r / 4) + 4 half + r % 4
-    if (there != ~0ull || key0 + kKeys > least_keys || (Kind::kWindow && key0 + kKeys > a.sinks && key0 < most_keys - a.window)) {
+    const int last_key = key_at(walked0 + kKeys - 1);
+    if (there != ~0ull || last_key >= least_keys ||
+        (Kind::kWindow && last_key >= a.sinks && (key0 > a.sinks ? key0 : a.sinks) < most_keys - a.window)) {
       const uint32_t bits[2] = {(uint32_t)there >> (4 * half), (uint32_t)(there >> 32) >> (4 * half)};
 #pragma unroll
       for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r / 4) + r % 4;
-          const int key = key0 + jt * 32 + at + 4 * half;
+          const int key = key_at(walked0 + jt * 32 + at + 4 * half);
           if (!(bits[jt] >> at & 1) || key >= keys || (Kind::kWindow && key >= a.sinks && key < keys - a.window)) s[jt][r] = -INFINITY;
         }
     }
