@@ -186,14 +186,19 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     u32x2 k[NI], v[NI];
     uint32_t k_scale, v_scale;                                      // of the lane's key
   };
+  const uint8_t *k_scales = a.scales.k + kvh * a.scales.k_head, *v_scales = a.scales.v + kvh * a.scales.v_head;
   auto ask = [&](int block, int page_of_lane) __attribute__((always_inline)) {
     Coming c;
     const int key_of_lane = key_at(block * kKeys + lane % kKeys), slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
-    const int64_t page = page_of_lane < 0 ? 0 : page_of_lane;       // no key: what stands in the first page, and zeros in its place
-    const int64_t k_at = page * p.k_page + slot_of_lane * p.k_slot, v_at = page * p.v_page + slot_of_lane * p.v_slot;
+    const int page = page_of_lane < 0 ? 0 : page_of_lane;           // no key: what stands in the first page, and zeros in its place
+    // strides of a scaled cache are below 2^32: two instructions a place
+    auto place = [&](int64_t page_stride, int at, int64_t stride) __attribute__((always_inline)) {
+      return (int64_t)((uint64_t)(uint32_t)page * (uint32_t)page_stride + (uint64_t)(uint32_t)at * (uint32_t)stride);
+    };
+    const int64_t k_at = place(p.k_page, slot_of_lane, p.k_slot), v_at = place(p.v_page, slot_of_lane, p.v_slot);
     const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
-    c.k_scale = (a.scales.k + kvh * a.scales.k_head)[page * a.scales.k_page + block_of_lane * a.scales.k_block];
-    c.v_scale = (a.scales.v + kvh * a.scales.v_head)[page * a.scales.v_page + block_of_lane * a.scales.v_block];
+    c.k_scale = k_scales[place(a.scales.k_page, block_of_lane, a.scales.k_block)];
+    c.v_scale = v_scales[place(a.scales.v_page, block_of_lane, a.scales.v_block)];
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
 #pragma unroll
       for (int v = 0; v < 2; ++v)
@@ -521,7 +526,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     next = find(block + 2 * kGroups);
     if constexpr (Kind::kScaled) {
       const bool comes = block + kGroups < block1;
-      Coming c = {};
+      Coming c;
       if (comes) c = ask(block + kGroups, page);
       process(block, there, page, k_src, v_src, k_dst, v_dst);
       if (comes) put(c, page, k_dst, v_dst);
