@@ -251,11 +251,16 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
       return k;
     };
     auto there = [&](int page) __attribute__((always_inline)) { return page >= 0 && page < p.num_pages; };
+    // strides of a scaled cache are below 2^32
+    auto place = [&](int page, int64_t page_stride, int at, int64_t stride) __attribute__((always_inline)) {
+      if constexpr (Kind::kScaled) return (int64_t)((uint64_t)(uint32_t)page * (uint32_t)page_stride + (uint64_t)(uint32_t)at * (uint32_t)stride);
+      else return page * page_stride + at * stride;
+    };
     auto load = [&](const Keys& at, int key0, const Held* base, int64_t page_stride, int64_t slot_stride, Raw (*r)[LS]) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int key = clamped(key0 + t * 16 + n), slot = key - divided(key, p.size) * p.page_size;
-        const Held* row = base + (there(at.page[t]) ? at.page[t] : 0) * page_stride + slot * slot_stride;
+        const Held* row = base + place(there(at.page[t]) ? at.page[t] : 0, page_stride, slot, slot_stride);
 #pragma unroll
         for (int i = 0; i < LS; ++i) r[t][i] = *reinterpret_cast<const Raw*>(row + col[kWide ? 2 * i : i]);
       }
@@ -273,7 +278,7 @@ __device__ __forceinline__ void paged_decode_worker(const PagedAttnArgs& a, cons
       const int key = clamped(key0 + (g & 1) * 16 + n), slot = key - divided(key, p.size) * p.page_size;
       auto pick = [](bool second, int v0, int v1) { return second ? v1 : v0; };      // (values, not places: no scratch)
       const int page = pick(g & 1, at.page[0], at.page[1]);
-      return (uint32_t)scale_head[(there(page) ? page : 0) * scale_page + divided(slot, a.scales.by_block) * scale_block];
+      return (uint32_t)scale_head[place(there(page) ? page : 0, scale_page, divided(slot, a.scales.by_block), scale_block)];
     };
     if (key_first < key_end) {
       Raw kr[2][LS], vr[2][LS];
