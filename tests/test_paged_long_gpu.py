@@ -680,3 +680,84 @@ def test_through_the_dispatcher_and_host_index_tensors(hexmi):
     finally:
         hexmi.through_dispatcher(previous)
     assert torch.equal(a[0].cpu(), c.page_table[[1, 0]]) and b[0].shape == c.page_table.shape
+
+
+def test_caches_past_32_bits(hexmi):
+    """Pages that stand past 4 GiB of their tensors: append, attention, fork and compaction as over a small cache."""
+    g = _gen(9)
+    size, dim, rows = 128, 256, 4
+    far = (1 << 32) // (size * dim) + 100
+    big = {n: torch.zeros(far, 1, size, dim, dtype=torch.uint8, device="cuda").view(E4M3) for n in ("k", "v")}
+    small = {n: torch.zeros(40, 1, size, dim, dtype=torch.uint8, device="cuda").view(E4M3) for n in ("k", "v")}
+    scales = {c: {n: torch.full((pool, 1, 4), 121, dtype=torch.uint8, device="cuda") for n in ("k_scales", "v_scales")} for c, pool in (("big", far), ("small", 40))}
+    at = far - 40                                                     # page p of the small cache is page at + p of the large one
+    assert at * size * dim > 1 << 32
+    for n in ("k", "v"):
+        x = torch.randint(0, 0x70, (40, 1, size, dim), generator=g, dtype=torch.uint8).cuda()
+        small[n].view(torch.uint8).copy_(x)
+        big[n].view(torch.uint8)[at:].copy_(x)
+    table = torch.randperm(40, generator=g)[:rows * 5].view(rows, 5).int().cuda()
+    lengths = torch.tensor([300, 640, 1, 511], dtype=torch.int32, device="cuda")
+    free = torch.tensor([p for p in range(40) if p not in set(table.flatten().tolist())][:rows], dtype=torch.int32, device="cuda")
+    x = torch.randn(rows, 4, dim, generator=g).half().cuda()
+    freq = hexmi.rope_frequencies(dim)
+    results = []
+    for pages, kw, add in ((small, scales["small"], 0), (big, scales["big"], at)):
+        q = hexmi.paged_append(x[:, 2:3], x[:, 3:], pages["k"], pages["v"], table + add, lengths, inv_freq=freq, q=x[:, :2], **kw)
+        out = [hexmi.paged_attention(q, pages["k"], pages["v"], table + add, lengths, **kw)]
+        starts = torch.tensor([0, 1, 4, 4, 4], dtype=torch.int32, device="cuda")
+        out.append(hexmi.paged_attention(q, pages["k"], pages["v"], table + add, lengths, starts, window=200, sinks=3, **kw))
+        new_table, new_lengths = hexmi.paged_fork(pages["k"], pages["v"], table + add, lengths, torch.tensor([3, 0, 1, 1], dtype=torch.int32, device="cuda"), free + add, **kw)
+        out += [new_table - add, new_lengths, raw(pages["k"][add:add + 40]).clone(), raw(pages["v"][add:add + 40]).clone(), kw["k_scales"][add:add + 40].clone()]
+        packed, count = hexmi.paged_compact(pages["k"], pages["v"], new_table, new_lengths, **kw)
+        out += [count, hexmi.paged_attention(q, pages["k"], pages["v"], packed, new_lengths, **kw)]
+        results.append(out)
+    for i, (a, b) in enumerate(zip(*results)):
+        assert torch.equal(torch.where(a < 0, torch.full_like(a, -1), a) if i == 2 else a, torch.where(b < 0, torch.full_like(b, -1), b) if i == 2 else b), i
+
+
+def test_lengths_past_the_table_end_with_it(hexmi):
+    c = Long([3, 1], [60, 77], 4, 2, 64, 16, 0, torch.float16, window=20, sinks=5, seed=8, ragged=True)
+    table = c.page_table[:, :5].contiguous()                          # 80 positions
+    at_end = torch.tensor([80, 80], dtype=torch.int32, device="cuda")
+    pages = torch.randn(2, *c.k_pages.shape, generator=_gen(1)).half().cuda()
+    one = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    q = c.q[:2].contiguous()
+    want = hexmi.paged_attention(q, pages[0], pages[1], table.clamp(0, 3), at_end, one, window=20, sinks=5)
+    got = hexmi.paged_attention(q, pages[0], pages[1], table.clamp(0, 3), at_end + 1000, one, window=20, sinks=5)
+    assert torch.equal(got, want)
+    assert torch.equal(hexmi.paged_attention(q, pages[0], pages[1], table.clamp(0, 3), at_end + 1000, window=20, sinks=5),
+                       hexmi.paged_attention(q, pages[0], pages[1], table.clamp(0, 3), at_end, window=20, sinks=5))
+
+
+def test_pages_with_room_between_them(hexmi):
+    """Strides of pages, heads, slots and scales that are not the tensors' own."""
+    c = Long([40, 1, 1], [100, 300, 9], 4, 2, 64, 16, 8, torch.bfloat16, seed=4, window=90, sinks=2)
+    want = c.run(hexmi)
+    for name in ("k_pages", "v_pages"):
+        t = getattr(c, name)
+        wide = torch.full((t.shape[0], t.shape[1] + 1, 2 * t.shape[2], t.shape[3] + 16), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3)
+        view = wide[:, 1:, ::2, 16:]
+        view.view(torch.uint8).copy_(t.view(torch.uint8))
+        setattr(c, name, view)
+    for name in ("k_scales", "v_scales"):
+        t = getattr(c, name)
+        wide = torch.full((2 * t.shape[0], t.shape[1], t.shape[2], 3), 255, dtype=torch.uint8, device="cuda")
+        view = wide[1::2, :, :, 1]
+        view.copy_(t)
+        setattr(c, name, view)
+    assert torch.equal(c.run(hexmi), want)
+    rows = torch.randn(3, 2, 64, generator=_gen(3)).bfloat16().cuda()
+    close = Long([1] * 3, [100, 300, 9], 4, 2, 64, 16, 8, torch.bfloat16, seed=4)
+    apart = Long([1] * 3, [100, 300, 9], 4, 2, 64, 16, 8, torch.bfloat16, seed=4)
+    wide = torch.zeros(apart.k_pages.shape[0], 2, 32, 80, dtype=torch.uint8, device="cuda").view(E4M3)
+    wide[:, :, ::2, 16:].view(torch.uint8).copy_(apart.k_pages.view(torch.uint8))
+    apart.k_pages = wide[:, :, ::2, 16:]
+    for x in (close, apart):
+        hexmi.paged_append(rows, rows.clone(), x.k_pages, x.v_pages, x.page_table, x.lengths_d, k_scales=x.k_scales, v_scales=x.v_scales)
+    assert torch.equal(raw(close.k_pages), raw(apart.k_pages)) and torch.equal(close.k_scales, apart.k_scales)
+    assert (wide[:, :, 1::2].float() == 0).all() and (wide[..., :16].float() == 0).all()
+    index = torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda")
+    got = [hexmi.paged_fork(x.k_pages, x.v_pages, x.page_table, x.lengths_d, index, torch.full_like(index, -1), x.k_scales, x.v_scales) for x in (close, apart)]
+    packed = [hexmi.paged_compact(x.k_pages, x.v_pages, *t, x.k_scales, x.v_scales) for x, t in zip((close, apart), got)]
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.equal(packed[0][0], packed[1][0]) and torch.equal(raw(close.k_pages), raw(apart.k_pages))
