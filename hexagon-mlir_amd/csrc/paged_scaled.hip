@@ -2,8 +2,11 @@
 // power-of-two scale for each block of slots and head; the queries' rows beside them.
 //
 // A block's scale is known when all of the call's rows in it are, so a workgroup takes the new tokens of one block of one sequence and a share
-// of the heads: the angles of its tokens are worked out once, into LDS, and a wave takes a head's keys or values of the block, first for the
-// largest value, then to write them (the rows come out of the caches the second time).
+// of the heads: the angles of its tokens are worked out once, into LDS, and a wave takes a head's keys or values of the block, held in registers
+// while the largest value is found. A scale is a power of two so that it can rise while a block fills: older numbers keep their bits then, but
+// for what falls below e4m3's normal numbers.
+// Bound by its launch up to some hundred tokens (64 tokens x 32 + 8 heads of 128 5.1 us), then by rows in flight: prompts of 8100 tokens, normed
+// and turned, 46.8 us (3.6 TB/s; a copy of that size 34).
 #include "head_rows.h"
 
 namespace hexmi {

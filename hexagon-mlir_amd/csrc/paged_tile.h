@@ -15,6 +15,9 @@
 // instructions take, and two workgroups a compute unit hide that in part. Measured on the way: copies that the compiler knows of (it waits
 // for them before it reads LDS transposed) 609; a lane's own address for every row 687. Few rows are bound by what is one behind the other:
 // launch and look-up about 5 us, 1 to 2 us a block (its copies are all waited for before the next block is begun), the join 4 to 5.
+//
+// A cache in 8 bits (Scaled) keeps its keys as they are in LDS, half of the reads, and widens them as they are multiplied, four instructions a
+// product; its values are widened on their way there. That is bound by instruction issue: prompts of 4 x 4096 637 us.
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"
