@@ -324,7 +324,7 @@ extern "C" int hexmi_paged_append_ex(const hexmi_head_rows* k, const hexmi_head_
   if ((dtype != HEXMI_F16 && dtype != HEXMI_BF16) || batch->dim % 8 != 0 || batch->dim > 256) return HEXMI_ENOTSUP;
   if (batch->tokens == 0) return HEXMI_OK;
   if (batch->sequences > 0 && (!batch->lengths || (batch->table_cols > 0 && !batch->page_table))) return HEXMI_EINVAL;
-  if (!batch->k_pages || !batch->v_pages) return HEXMI_EINVAL;
+  if (!batch->k_pages || !batch->v_pages || scales->k_scales == scales->v_scales) return HEXMI_EINVAL;
   if ((rc = take(a, 0, q, true)) != HEXMI_OK || (rc = take(a, 1, k, false)) != HEXMI_OK || (rc = take(a, 2, v, false)) != HEXMI_OK) return rc;
   for (int i = 0; i < 3; ++i) {
     const Kind& r = a.kind[i];

@@ -477,7 +477,7 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       for (const void* pages : {batch.k_pages, batch.v_pages})
         if (t && t->numel() && in_storage_of(pages, *t)) HEXMI_NOT_PLAIN;
     if (batch.k_pages == batch.v_pages) HEXMI_NOT_PLAIN;
-    if (scales.given && (D % 8 != 0 || D > 256)) HEXMI_NOT_PLAIN;
+    if (scales.given && (D % 8 != 0 || D > 256 || scales.s.k_scales == scales.s.v_scales)) HEXMI_NOT_PLAIN;
     for (const at::Tensor* t : {k, v, q, kw, qw})
       if (scales.given && !on_boundaries(t)) HEXMI_NOT_PLAIN;
     const Launch at(*k);

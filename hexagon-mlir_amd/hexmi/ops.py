@@ -1072,6 +1072,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     if k_pages.dim() != 4 or k.dim() != 3 or k.shape[1:] != (k_pages.shape[1], k_pages.shape[3]) or v.shape != k.shape:
         raise ValueError("hexmi.paged_append: k and v are [tokens, kv heads, dim], the pages [pages, kv heads, page size, dim]")
     dim, tokens = k.shape[2], k.shape[0]
+    if scaled and k_scales.data_ptr() == v_scales.data_ptr():
+        raise ValueError("hexmi.paged_append: keys and values need scales of their own")
     if scaled and (dim % 8 != 0 or dim > 256):
         raise ValueError("hexmi.paged_append: a cache in 8 bits takes a dim that is a multiple of 8 up to 256")
     _head_operands(name, k, k_weight, dim, k.dtype)

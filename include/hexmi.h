@@ -639,7 +639,8 @@ typedef struct hexmi_paged_scales {
  * below e4m3's normal numbers). What a block held of others counts for nothing,
  * its scale neither. Infinities and NaN become NaN and leave the scale alone.
  * dim a multiple of 8 up to 256, operand rows and weights on 16-byte
- * boundaries, pages and their strides on 8-byte ones; HEXMI_ENOTSUP otherwise. Of
+ * boundaries, pages and their strides on 8-byte ones; HEXMI_ENOTSUP otherwise;
+ * keys and values have pages and scales of their own. Of
  * two sequences that have new tokens in one block pieces of either are left
  * there. scales NULL: hexmi_paged_append. */
 int hexmi_paged_append_ex(const hexmi_head_rows *k, const hexmi_head_rows *v,

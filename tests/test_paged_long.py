@@ -64,6 +64,15 @@ def test_append_in_8_bits_refuses_other_dims():
             hexmi.paged_append(*(torch.zeros(2, 2, dim, dtype=torch.float16) for _ in range(2)), **a)
 
 
+def test_append_refuses_scales_that_are_one_tensor():
+    scales = torch.zeros(3, 2, 1, dtype=torch.uint8)
+    rows = torch.zeros(2, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="scales of their own"):
+        hexmi.paged_append(rows, rows.clone(), **batch(k_scales=scales, v_scales=scales))
+    s = c_scales(v_scales=4096)
+    assert _lib.lib().hexmi_paged_append_ex(c_rows(), c_rows(), None, TURN, c_batch(), s, _lib.F16, None) == _lib.EINVAL
+
+
 @pytest.mark.parametrize("window, sinks", [(0, 0), (-1, 0), (2.0, 0), (True, 0), (5, -1), (5, 1.0), (None, 4), (torch.tensor(4), 0)])
 def test_window_refusals(window, sinks):
     with pytest.raises(ValueError, match="window"):
@@ -116,7 +125,7 @@ def c_rows(heads=2, **kw):
 
 
 def c_scales(**kw):
-    return _lib.PagedScales(**{**dict(k_scales=4096, v_scales=4096, k_page=2, k_head=1, k_block=1, v_page=2, v_head=1, v_block=1, block=16), **kw})
+    return _lib.PagedScales(**{**dict(k_scales=4096, v_scales=8192, k_page=2, k_head=1, k_block=1, v_page=2, v_head=1, v_block=1, block=16), **kw})
 
 
 TURN = _lib.Rotation(inv_freq=4096, columns=64, pairs=0, eps=1e-5)

@@ -216,6 +216,26 @@ def test_windows_that_hide_nothing_are_none(hexmi):
         assert torch.equal(c.run(hexmi, window=window, sinks=sinks), whole), (window, sinks)
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 1, 40]])
+def test_scales_at_the_ends_of_their_range(hexmi, dt, new):
+    """Values with the least exponent (in fp16 subnormal numbers among them), keys with a large one beside small queries."""
+    dtype = DTYPES[dt]
+    c = Long(new, [300, 20, 77], 4, 2, 64, 16, 8, dtype, seed=6)
+    least, large = RANGE[dtype][0], 7
+    for i, (name, e) in enumerate((("k", large), ("v", least))):
+        old = c.scales[i].double() - 127
+        whole = []
+        for b, t in enumerate(getattr(c, name + "64")):
+            at = torch.arange(t.shape[0])
+            whole.append(t * torch.exp2(e - old[c.table[b, at // 16], :, at % 16 // 8])[..., None])
+            assert torch.equal(whole[-1], whole[-1].to(dtype).double())
+        setattr(c, name + "64", whole)
+        getattr(c, name + "_scales").fill_(e + 127)
+    c.q.mul_(2.0 ** -12)
+    c.check(c.run(hexmi))
+
+
 @pytest.mark.parametrize("scaled", [False, True])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_index_tensors_that_make_no_sense_touch_nothing_outside(hexmi, scaled, ragged):
