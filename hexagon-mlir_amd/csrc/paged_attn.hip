@@ -170,8 +170,10 @@ int attend(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi
   for (int64_t s : {batch->k_page, batch->k_head, batch->k_slot, batch->v_page, batch->v_head, batch->v_slot})
     if (s % step != 0) return HEXMI_ENOTSUP;
   if (batch->k_slot < 0 || batch->k_slot > 1 << 26 || batch->v_slot < 0 || batch->v_slot > 1 << 26) return HEXMI_ENOTSUP;      // 32-bit offsets within a page
-  if (scales)
-    for (int64_t s : {batch->k_page, batch->v_page, scales->k_page, scales->k_block, scales->v_page, scales->v_block})
+  const hexmi_paged_scales none = {};
+  const hexmi_paged_scales& sc = scales ? *scales : none;
+  if (scales || seen.window)
+    for (int64_t s : {batch->k_page, batch->v_page, sc.k_page, sc.k_block, sc.v_page, sc.v_block})
       if (s < 0 || s > 0xffffffffll) return HEXMI_ENOTSUP;          // 32 bits
   const size_t boundary = scales ? step : 16;
   if (!aligned_to(q->x, 16) || !aligned_to(q->out, 16) || !aligned_to(batch->k_pages, boundary) || !aligned_to(batch->v_pages, boundary))

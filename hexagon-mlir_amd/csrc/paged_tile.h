@@ -178,6 +178,11 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
     return copied_column<D, COLS, PADDED>(c, dim);
   };
+  // strides of a windowed kind are below 2^32: two instructions a place
+  auto place = [&](int page, int64_t page_stride, int at, int64_t stride) __attribute__((always_inline)) {
+    if constexpr (Kind::kWindow) return (int64_t)((uint64_t)(uint32_t)page * (uint32_t)page_stride + (uint64_t)(uint32_t)at * (uint32_t)stride);
+    else return page * page_stride + at * stride;
+  };
   // what the lane of instruction j's first row has
   auto of_first_row = [&](int64_t at, int j) __attribute__((always_inline)) {
     const int row = row_wave * kRowsOfOne + j * kRowStep;
@@ -194,14 +199,10 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     Coming c;
     const int key_of_lane = key_at(block * kKeys + lane % kKeys), slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
     const int page = page_of_lane < 0 ? 0 : page_of_lane;           // no key: what stands in the first page, and zeros in its place
-    // strides of a scaled cache are below 2^32: two instructions a place
-    auto place = [&](int64_t page_stride, int at, int64_t stride) __attribute__((always_inline)) {
-      return (int64_t)((uint64_t)(uint32_t)page * (uint32_t)page_stride + (uint64_t)(uint32_t)at * (uint32_t)stride);
-    };
-    const int64_t k_at = place(p.k_page, slot_of_lane, p.k_slot), v_at = place(p.v_page, slot_of_lane, p.v_slot);
+    const int64_t k_at = place(page, p.k_page, slot_of_lane, p.k_slot), v_at = place(page, p.v_page, slot_of_lane, p.v_slot);
     const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
-    c.k_scale = k_scales[place(a.scales.k_page, block_of_lane, a.scales.k_block)];
-    c.v_scale = v_scales[place(a.scales.v_page, block_of_lane, a.scales.v_block)];
+    c.k_scale = k_scales[place(page, a.scales.k_page, block_of_lane, a.scales.k_block)];
+    c.v_scale = v_scales[place(page, a.scales.v_page, block_of_lane, a.scales.v_block)];
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
 #pragma unroll
       for (int v = 0; v < 2; ++v)
@@ -256,7 +257,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
       // a lane works out where its key stands, for all of the block's at once; an instruction takes its first row's
       const int key_of_lane = key_at(block * kKeys + lane % kKeys), slot_of_lane = key_of_lane - divided(key_of_lane, p.size) * p.page_size;
-      const int64_t k_at = page_of_lane * p.k_page + slot_of_lane * p.k_slot, v_at = page_of_lane * p.v_page + slot_of_lane * p.v_slot;
+      const int64_t k_at = place(page_of_lane, p.k_page, slot_of_lane, p.k_slot), v_at = place(page_of_lane, p.v_page, slot_of_lane, p.v_slot);
       constexpr int kStep = kRowWaves * kWave * 16;                 // bytes of LDS between a wave's instructions
 #pragma unroll
       for (int v = 0; v < 2; ++v)

@@ -198,3 +198,12 @@ def test_fork_and_compact_entries_refuse_before_they_launch():
     need = lib.hexmi_paged_compact_workspace(c_batch())
     assert need > 0 and compact(room=need - 1) == _lib.EINVAL
     assert lib.hexmi_paged_compact_workspace(c_batch(num_pages=0)) == 0 and lib.hexmi_paged_compact_workspace(None) == 0
+
+
+@pytest.mark.parametrize("change", [dict(k_page=1 << 32), dict(v_page=-2048)])
+def test_strides_past_32_bits_are_refused_within_a_window(change):
+    f = _lib.lib().hexmi_paged_attention_ex
+    for scales, window in ((None, 5), (c_scales(), 0)):
+        assert f(c_rows(heads=4), c_batch(**change), scales, None, 0, window, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
+    for change in (dict(k_page=1 << 32), dict(v_block=-1)):
+        assert f(c_rows(heads=4), c_batch(), c_scales(**change), None, 0, 0, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
