@@ -73,6 +73,11 @@ template <> inline constexpr int kMostExponent<f16> = 8;
 // 2^e of a normal number
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
+// the least e with most <= 448 * 2^e = 1.75 * 2^(e + 8)
+__device__ __forceinline__ int exponent_of(float most) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, most);
+  return (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+}
 // eight numbers of e4m3 times a power of two, in T
 template <typename T>
 __device__ __forceinline__ auto widened(uint32_t lo, uint32_t hi, float scale) {

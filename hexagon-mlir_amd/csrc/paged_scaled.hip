@@ -47,11 +47,6 @@ __device__ __forceinline__ float row_max(float v) {
   return v;
 }
 
-// the least e with most <= 448 * 2^e = 1.75 * 2^(e + 8)
-__device__ __forceinline__ int exponent_of(float most) {
-  const uint32_t bits = __builtin_bit_cast(uint32_t, most);
-  return (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
-}
 // eight values (finite, or NaN for what is not) times `by`, rounded to e4m3, at most `limit`
 __device__ __forceinline__ u32x2 to_codes(const float* y, float by, float limit) {
   float v[8];

@@ -75,6 +75,7 @@ __device__ __forceinline__ Run run_of_tile(const Pages& p, int group, int tile, 
   return run;
 }
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 // A tile of keys in 8 bits: rows of D bytes, 16-byte chunks, XOR swizzled so that the 16 rows that a read takes at a time stand on all banks
 template <int D> __device__ __forceinline__ int swz_k8tile(int row) { return D == 64 ? (row >> 2) & 3 : D == 128 ? (row >> 1) & 7 : row & 15; }
 
@@ -303,8 +304,56 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   const bool live = row < rows;
   const int in_seq = divided(live ? row : rows - 1, a.by_group), head = kvh * a.group + (live ? row : rows - 1) - in_seq * a.group;
   const int token = token0 + in_seq;
+  // bf16 queries over keys in 8 bits: a query is t = 2^e (a + b / 16) with a and b in e4m3, exact but for what is below 2^-13 of a row's largest
+  // value (off by 2^-21 of that): e4m3 has half of bf16's eight bits, and what a leaves is within half of its last one. So keys are multiplied
+  // as they are, with the scales of both as the instruction's own.
+  constexpr bool kSplit = Kind::kScaled && std::is_same_v<T, bf16> && COLS % 64 == 0;
+  constexpr int SS = kSplit ? COLS / 64 : 1;
+  i32x8 q_high[SS], q_low[SS];                                      // columns 64 i + 32 half ..
+  int q_scale = 0;
+  if constexpr (kSplit) {
+    const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
+    Frag f[SS][4];
+    float largest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SS; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int c = i * 64 + half * 32 + w * 8;
+        f[i][w] = Frag{};
+        if (!PADDED || c < dim) f[i][w] = *reinterpret_cast<const Frag*>(q + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = fabsf((float)f[i][w][e]);
+          largest = fmaxf(largest, x < INFINITY ? x : 0.0f);
+        }
+      }
+    largest = fmaxf(largest, other_half(largest));
+    int e = exponent_of(largest);
+    e = e < -110 ? -110 : e;
+    q_scale = e + 127;
+    const float by = power_of_two(-e);
+#pragma unroll
+    for (int i = 0; i < SS; ++i)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {                                 // four columns a word
+        float x[4], rest[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float v = (float)f[i][w / 2][w % 2 * 4 + c];
+          x[c] = fabsf(v) < INFINITY ? v * by : NAN;
+        }
+        int word = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        word = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], word, true);
+        q_high[i][w] = word;
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+        rest[0] = x[0] - lo[0], rest[1] = x[1] - lo[1], rest[2] = x[2] - hi[0], rest[3] = x[3] - hi[1];
+        word = __builtin_amdgcn_cvt_pk_fp8_f32(rest[0] * 16.0f, rest[1] * 16.0f, 0, false);
+        q_low[i][w] = __builtin_amdgcn_cvt_pk_fp8_f32(rest[2] * 16.0f, rest[3] * 16.0f, word, true);
+      }
+  }
   Frag qf[DS];                                                      // row lane % 32, columns 16 ds + 8 half ..
-  {
+  if constexpr (!kSplit) {
     const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
@@ -359,7 +408,38 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[jt][r] = 0.0f;
-    if constexpr (Kind::kScaled) {
+    if constexpr (kSplit) {
+      int scale[JT] = {(int)k_scale_now};
+      if constexpr (JT == 2) {
+        float lower, upper;
+        swap32(__builtin_bit_cast(float, k_scale_now), lower, upper);
+        scale[0] = __builtin_bit_cast(int, lower);
+        scale[JT - 1] = __builtin_bit_cast(int, upper);
+      }
+      auto read_k = [&](int jt, int i) __attribute__((always_inline)) {      // 32 columns of a key
+        const int r = jt * 32 + lane % 32;
+        const char* row = reinterpret_cast<const char*>(k_src) + r * D;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(row + ((i * 4 + half * 2) ^ swz_k8tile<D>(r)) * 16);
+        const u32x4 y = *reinterpret_cast<const u32x4*>(row + ((i * 4 + half * 2 + 1) ^ swz_k8tile<D>(r)) * 16);
+        return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+      };
+      i32x8 kf[JT][SS];
+#pragma unroll
+      for (int jt = 0; jt < JT; ++jt) kf[jt][0] = read_k(jt, 0);
+#pragma unroll
+      for (int i = 0; i < SS; ++i) {
+        if (i + 1 < SS)
+#pragma unroll
+          for (int jt = 0; jt < JT; ++jt) kf[jt][i + 1] = read_k(jt, i + 1);
+#pragma unroll
+        for (int jt = 0; jt < JT; ++jt)
+          s[jt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[jt][i], q_high[i], s[jt], 0, 0, 0, scale[jt], 0, q_scale);
+#pragma unroll
+        for (int jt = 0; jt < JT; ++jt)
+          s[jt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[jt][i], q_low[i], s[jt], 0, 0, 0, scale[jt], 0, q_scale - 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (Kind::kScaled) {
       // 16 columns of a key a read, widened for two products
       constexpr int kAhead = 2, PS = DS / 2;
       float scale[JT];
@@ -516,7 +596,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
 
   // the queries are here before the walk begins: their first use must not wait inside it, with copies on their way
 #pragma unroll
-  for (int ds = 0; ds < DS; ++ds) {
+  for (int ds = 0; ds < (kSplit ? 0 : DS); ++ds) {
     u32x4 f = __builtin_bit_cast(u32x4, qf[ds]);
     asm volatile("" : "+v"(f));
     qf[ds] = __builtin_bit_cast(Frag, f);

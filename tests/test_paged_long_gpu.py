@@ -236,6 +236,47 @@ def test_scales_at_the_ends_of_their_range(hexmi, dt, new):
     c.check(c.run(hexmi))
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 72, 128, 256])
+def test_queries_of_very_different_sizes(hexmi, dt, dim):
+    """Columns of a query from 2^-20 to 1 of its largest, over keys in 8 bits. A bf16 query is multiplied as the sum of two numbers of e4m3: a
+    value x of a row whose largest is m is off by half of the second one's last step, 2^-10 / 16 of the row's scale, which is at least m / 448
+    and at most m / 224: by 2^-14 / 224 m < 2^-21 m, so a score by scale 2^-21 m sum |k|, and the weights by twice that."""
+    c = Long([90, 1, 1], [40, 300, 9], 4, 2, dim, 16, 8, DTYPES[dt], seed=12)
+    g = _gen(13)
+    c.q = (c.q.cpu().double() * torch.exp2(torch.randint(-20, 1, c.q.shape, generator=g).double())).to(c.dtype).cuda()
+    got = c.run(hexmi).cpu().double()
+    t, G, scale, u = 0, 2, 1 / math.sqrt(dim), half_step(c.dtype)
+    for n, L, k, v in zip(c.new, c.lengths, c.k64, c.v64):
+        hidden = torch.arange(L)[None] > torch.arange(L - n, L)[:, None]
+        for h in range(4):
+            q, kh, vh = c.q[t:t + n, h].cpu().double(), k[:, h // G], v[:, h // G]
+            w = torch.softmax((q @ kh.T * scale).masked_fill(hidden, -math.inf), 1)
+            o, a = w @ vh, w @ vh.abs()
+            size = (q.abs() @ kh.abs().T * scale).amax(1, keepdim=True)
+            off = scale * 2.0 ** -21 * q.abs().amax(1, keepdim=True) * kh.abs().sum(1).amax()
+            bound = u * (a + o.abs()) + (2 * (dim + 8) * E * size + 2 * off + 16 * E) * (a + o.abs()) + u * o.abs()
+            if dt == "f16":
+                bound = bound + L * 2.0 ** -25 * vh.abs().amax(0) + 2.0 ** -25
+            assert ((got[t:t + n, h] - o).abs() <= bound).all(), (n, h)
+        t += n
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("block, window", [(8, None), (8, 50), (0, 50)])
+def test_queries_that_are_not_finite_stay_in_their_rows(hexmi, dt, block, window):
+    c = Long([90, 1, 1], [40, 300, 9], 4, 2, 64, 16, block, DTYPES[dt], seed=14, window=window, sinks=2 if window else 0)
+    want = c.run(hexmi)
+    rows = [(3, 1, math.nan), (70, 0, math.inf), (90, 2, -math.inf), (91, 3, math.nan)]
+    for t, h, x in rows:
+        c.q[t, h, 5] = x
+    got = c.run(hexmi)
+    hit = torch.zeros(92, 4, dtype=torch.bool, device="cuda")
+    for t, h, _ in rows:
+        hit[t, h] = True
+    assert torch.isnan(got[hit].float()).all() and torch.equal(got[~hit], want[~hit])
+
+
 @pytest.mark.parametrize("scaled", [False, True])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_index_tensors_that_make_no_sense_touch_nothing_outside(hexmi, scaled, ragged):
