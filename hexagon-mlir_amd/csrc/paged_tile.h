@@ -16,8 +16,9 @@
 // for them before it reads LDS transposed) 609; a lane's own address for every row 687. Few rows are bound by what is one behind the other:
 // launch and look-up about 5 us, 1 to 2 us a block (its copies are all waited for before the next block is begun), the join 4 to 5.
 //
-// A cache in 8 bits (Scaled) keeps its keys as they are in LDS, half of the reads, and widens them as they are multiplied, four instructions a
-// product; its values are widened on their way there. That is bound by instruction issue: prompts of 4 x 4096 637 us.
+// A cache in 8 bits (Scaled) keeps its keys as they are in LDS, half of the reads. bf16 queries are split into two numbers of e4m3 and multiplied
+// with them as they are; fp16's would take three, so for those keys are widened, four instructions a product. Values are widened on their way to
+// LDS. Bound by instruction issue: prompts of 4 x 4096, bf16, 631 us (keys widened 656, in 16 bits 596).
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"

@@ -657,7 +657,8 @@ int hexmi_paged_append_ex(const hexmi_head_rows *k, const hexmi_head_rows *v,
  * seen: those may be none, and what stands there may be anything.
  * A cache in 8 bits is multiplied as numbers of dtype, exact where its scales
  * are in hexmi_paged_append_ex's range (dtype fp16 ends at 65504 and has no
- * steps below 2^-24). Pages on 16-byte boundaries where dim is a multiple of
+ * steps below 2^-24); bf16 queries are multiplied with its keys to within 2^-21 of
+ * the row's largest value. Pages on 16-byte boundaries where dim is a multiple of
  * 16, on 8-byte ones otherwise; with scales or a window strides of pages, slots
  * and blocks from 0 to 2^32 - 1. No shared pages within a window (HEXMI_ENOTSUP). A position past the
  * table's columns counts as the last of them. Everything else as
