@@ -18,7 +18,7 @@
 //
 // A cache in 8 bits (Scaled) keeps its keys as they are in LDS, half of the reads. bf16 queries are split into two numbers of e4m3 and multiplied
 // with them as they are; fp16's would take three, so for those keys are widened, four instructions a product. Values are widened on their way to
-// LDS. Bound by instruction issue: prompts of 4 x 4096, bf16, 631 us (keys widened 656, in 16 bits 596).
+// LDS. Bound by instruction issue: prompts of 4 x 4096, bf16, 603 us (in 16 bits 574; keys widened 656 for 631, eight columns a lane 616).
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"
@@ -176,7 +176,6 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
   constexpr int kRowsOfOne = kWave / CPR;
   const bool one_page = p.page_size % kRowsOfOne == 0;
   auto column = [&](bool v, int r) __attribute__((always_inline)) {
-    if (Kind::kScaled && !v) return copied_column<D, COLS, PADDED>(((lin % CPR / 2) ^ swz_k8tile<D>(r)) * 16 + lin % 2 * 8, dim);
     const int c = ((lin % CPR) ^ (v ? swz_vtile<D == 64 ? 64 : 128>(r) : swz_ktile<D == 64 ? 64 : 128>(r))) * 8;
     return copied_column<D, COLS, PADDED>(c, dim);
   };
@@ -192,8 +191,17 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     return (int64_t)((uint64_t)hi << 32 | lo);
   };
   // A scaled cache comes by way of registers: asked for when the block before is begun, widened to T and put into LDS when it is done.
+  // Keys 16 columns a lane, 8 of a padded head, whose rows may end within 16.
+  constexpr int kPiece = PADDED ? 8 : 16, PPR = D / kPiece, NK = kKeys * PPR / kWave / kRowWaves, kKeyRows = kWave / PPR, kKeyStep = kRowWaves * kKeyRows;
+  typedef std::conditional_t<PADDED, u32x2, u32x4> Piece;
+  const bool one_page_of_keys = p.page_size % kKeyRows == 0;
+  auto key_column = [&](int r) __attribute__((always_inline)) {
+    const int i = lin % PPR;
+    return copied_column<D, COLS, PADDED>(PADDED ? ((i / 2) ^ swz_k8tile<D>(r)) * 16 + i % 2 * 8 : (i ^ swz_k8tile<D>(r)) * 16, dim);
+  };
   struct Coming {
-    u32x2 k[NI], v[NI];
+    Piece k[NK];
+    u32x2 v[NI];
     uint32_t k_scale, v_scale;                                      // of the lane's key
   };
   const uint8_t *k_scales = a.scales.k + kvh * a.scales.k_head, *v_scales = a.scales.v + kvh * a.scales.v_head;
@@ -205,26 +213,37 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     const int block_of_lane = divided(slot_of_lane, a.scales.by_block);
     c.k_scale = k_scales[place(page, a.scales.k_page, block_of_lane, a.scales.k_block)];
     c.v_scale = v_scales[place(page, a.scales.v_page, block_of_lane, a.scales.v_block)];
-    if (one_page && __ballot(page_of_lane >= 0) == ~0ull) {
+    const bool whole = __ballot(page_of_lane >= 0) == ~0ull;
+    auto of_row = [&](int64_t at, int row) __attribute__((always_inline)) {
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, row), hi = __builtin_amdgcn_readlane((int)(at >> 32), row);
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    };
+    auto of_lanes_row = [&](int64_t at, int row) __attribute__((always_inline)) {
+      const uint32_t lo = __shfl((int)(uint32_t)at, row), hi = __shfl((int)(at >> 32), row);
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    };
+    if (one_page_of_keys && whole) {
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const Held* from = (v ? v_head : k_head) + of_first_row(v ? v_at : k_at, j);
-          const uint32_t off = lane / CPR * (uint32_t)(v ? p.v_slot : p.k_slot) + column(v, copy_row + j * kRowStep);
-          (v ? c.v : c.k)[j] = *reinterpret_cast<const u32x2*>(from + off);
-        }
-      return c;
-    }
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int r = copy_row + j * kRowStep;
-        const int64_t at = v ? v_at : k_at;
-        const uint32_t lo = __shfl((int)(uint32_t)at, r), hi = __shfl((int)(at >> 32), r);
-        (v ? c.v : c.k)[j] = *reinterpret_cast<const u32x2*>((v ? v_head : k_head) + (int64_t)((uint64_t)hi << 32 | lo) + column(v, r));
+      for (int j = 0; j < NK; ++j) {
+        const int row0 = row_wave * kKeyRows + j * kKeyStep;
+        c.k[j] = *reinterpret_cast<const Piece*>(k_head + of_row(k_at, row0) + (lane / PPR * (uint32_t)p.k_slot + key_column(row0 + lane / PPR)));
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        const int r = row_wave * kKeyRows + j * kKeyStep + lane / PPR;
+        c.k[j] = *reinterpret_cast<const Piece*>(k_head + of_lanes_row(k_at, r) + key_column(r));
+      }
+    }
+    if (one_page && whole) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        c.v[j] = *reinterpret_cast<const u32x2*>(v_head + of_first_row(v_at, j) + (lane / CPR * (uint32_t)p.v_slot + column(true, copy_row + j * kRowStep)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        c.v[j] = *reinterpret_cast<const u32x2*>(v_head + of_lanes_row(v_at, copy_row + j * kRowStep) + column(true, copy_row + j * kRowStep));
+    }
     return c;
   };
   uint32_t k_scale_now = 127;                                       // of key lane % kKeys of the block that is in LDS
@@ -233,7 +252,7 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
     // keys as they are, values widened
     k_scale_now = c.k_scale;
 #pragma unroll
-    for (int j = 0; j < NI; ++j) reinterpret_cast<u32x2*>(k_dst)[row_wave * kWave + lane + j * kRowWaves * kWave] = c.k[j];
+    for (int j = 0; j < NK; ++j) reinterpret_cast<Piece*>(k_dst)[row_wave * kWave + lane + j * kRowWaves * kWave] = c.k[j];
     if (one_scale && __ballot(page_of_lane >= 0) == ~0ull) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
