@@ -60,9 +60,8 @@ __device__ __forceinline__ u32x2 to_codes(const float* y, float by, float limit)
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
   return u32x2{(uint32_t)lo, (uint32_t)hi};
 }
-// eight numbers of e4m3 times 2^by (by <= 0), rounded again
-__device__ __forceinline__ u32x2 codes_again(u32x2 c, int by) {
-  const float f = by < -126 ? 0.0f : power_of_two(by);
+// eight numbers of e4m3 times f (at most 1, or NaN), rounded again
+__device__ __forceinline__ u32x2 codes_again(u32x2 c, float f) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
@@ -254,15 +253,21 @@ void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, unsign
     int e = exponent_of(largest);
     e = e < kLeastExponent<T> ? kLeastExponent<T> : e < kMostExponent<T> ? e : kMostExponent<T>;
     if (u.old > 0) {
-      const int before = (int)*scale - 127;
-      if (before > e) e = before < kMostExponent<T> ? before : kMostExponent<T>;
-      if (e > before && is_head)                                    // older tokens' numbers again
+      // An exponent above T's range (a cache that was filled as another type) stays, so that its numbers keep their values. 255 is none: what
+      // it scales is NaN, and becomes e4m3's.
+      const int held = *scale, before = held - 127;
+      if (before > e && held != 255) e = before;
+      if (e != before && is_head) {                                 // older tokens' numbers again
+        const float f = held == 255 ? NAN : before - e < -126 ? 0.0f : power_of_two(before - e);
         for (int s = one ? 0 : group; s < u.old; s += one ? 1 : kRowsAtOnce) {
           u32x2* c = reinterpret_cast<u32x2*>(codes + (s - u.old) * slot_stride);
-          *c = codes_again(*c, before - e);
+          *c = codes_again(*c, f);
         }
+      }
     }
-    const float by = power_of_two(-e), limit = e == kMostExponent<T> ? 240.0f : 448.0f;
+    // from the type's largest exponent on numbers end at 240 times it, at a whole multiple of e4m3's least (2^-9)
+    const float by = e < 127 ? power_of_two(-e) : 0x1p-127f;
+    const float limit = e < kMostExponent<T> ? 448.0f : floorf(240.0f * 512.0f * power_of_two(kMostExponent<T> - e)) * 0x1p-9f;
     for (int first = 0; first < passes; first += kHeld) {
       if (passes > kHeld) hold(first);
 #pragma unroll

@@ -1060,7 +1060,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, starts=None, k_wei
     A cache in 8 bits: pages of float8_e4m3fn, and k_scales, v_scales uint8 [pages, kv heads, blocks] (any strides, changed in place), the
     biased exponent e + 127 of the power of two that the numbers of each page_size / blocks slots (1 to 64) of a page are multiplied by. A
     block's exponent is the least that has the largest of the call's values in it within 448; it does not fall below what older tokens
-    of the sequence in the block have, and their numbers are rounded again where it rises. dim a multiple of 8 up to 256."""
+    of the sequence in the block have, and their numbers are rounded again where it rises. dim a multiple of 8 up to 256.
+    What one type filled another may go on with: an older exponent beyond the type's range (fp16: above 8) stays as it is."""
     if q_out is None and not _THROUGH_DISPATCHER:
         y = _front.paged_append(k, v, k_pages, v_pages, page_table, lengths, starts, k_weight, inv_freq, eps, pairs, q, q_weight, k_scales, v_scales)
         if y is not None:

@@ -636,7 +636,9 @@ typedef struct hexmi_paged_scales {
  * the cache is a number of that type then; at the upper end numbers end at
  * 240). Where older tokens of its sequence stand in the block it does not fall, and
  * their numbers are rounded again where it rises (which costs only what gets
- * below e4m3's normal numbers). What a block held of others counts for nothing,
+ * below e4m3's normal numbers); so an older exponent above that range (a cache
+ * that was filled as another type) stays, and new numbers end where they are
+ * still the type's. (255 is no exponent: what it scales becomes NaN.) What a block held of others counts for nothing,
  * its scale neither. Infinities and NaN become NaN and leave the scale alone.
  * dim a multiple of 8 up to 256, operand rows and weights on 16-byte
  * boundaries, pages and their strides on 8-byte ones; HEXMI_ENOTSUP otherwise;

@@ -481,6 +481,58 @@ def test_values_at_the_ends(hexmi, dtype):
             assert e.item() == least_exponent(y.item(), lo, hi), (x, y.item())
 
 
+@pytest.mark.parametrize("dt, befores", [("f16", (7, 8, 9, 10, 13, 20, 21, 22, 25, 60, 127)), ("bf16", (119, 120, 121, 124, 127))])
+@pytest.mark.parametrize("new", [1, 3, 9])
+def test_older_exponents_above_the_range_stay(hexmi, dt, befores, new):
+    """A block that another type filled, with an exponent that this one's appends do not reach: it does not fall, the older numbers stay as they
+    are, and the new ones are numbers of the type. Rounding is e4m3's own, so all of it is exact."""
+    dtype, g = DTYPES[dt], _gen(21)
+    hi = RANGE[dtype][1]
+    for before in befores:
+        old, kv, dim = 5, 3, 64
+        codes = torch.randint(0, 0x7f, (2, kv, 16, dim), generator=g, dtype=torch.uint8)
+        k_pages, v_pages = codes.view(E4M3).cuda(), codes.view(E4M3).cuda()
+        scales = [torch.full((2, kv, 1), before + 127, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        largest = torch.finfo(dtype).max
+        y = (torch.randn(new, kv, dim, generator=g) * torch.exp2(torch.randint(-20, 2, (new, kv, 1), generator=g).float()) * (largest / 16)).clamp(-largest, largest)
+        y[0, 0, 0], y[0, 0, 1] = largest, -largest
+        y = y.to(dtype)
+        starts = None if new == 1 else torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        hexmi.paged_append(y.cuda(), y.cuda(), k_pages, v_pages, torch.tensor([[1]], dtype=torch.int32, device="cuda"),
+                           torch.tensor([old + new], dtype=torch.int32, device="cuda"), starts, k_scales=scales[0], v_scales=scales[1])
+        e = max(before, hi)                                           # the largest value asks for the type's largest exponent
+        limit = 448.0 if e < hi else math.floor(240 * 512 * 2.0 ** (hi - e)) / 512
+        for pages, s in zip((k_pages, v_pages), scales):
+            got = pages.cpu().view(torch.uint8)
+            at = s.cpu().int()[1, :, 0] - 127
+            want_e = [max(before, least_exponent(y[:, h].abs().max().item(), *RANGE[dtype])) for h in range(kv)]
+            assert at.tolist() == want_e and (s[0] == before + 127).all(), (before, at)
+            for h in range(kv):
+                if want_e[h] == before:
+                    assert torch.equal(got[1, h, :old], codes[1, h, :old]), before
+                if want_e[h] < hi:
+                    continue
+                x = (y[:, h].double() * 2.0 ** -want_e[h]).clamp(-limit, limit)
+                put = got[1, h, old:old + new].view(E4M3)
+                assert torch.equal(put.float(), x.float().to(E4M3).float()), (before, h)
+                back = put.double() * 2.0 ** want_e[h]
+                assert torch.equal(back.to(dtype).double(), back) and torch.isfinite(back.to(dtype)).all(), before
+            assert torch.equal(got[:, :, old + new:], codes[:, :, old + new:]) and torch.equal(got[0], codes[0])
+
+
+def test_an_older_exponent_of_255_is_none(hexmi):
+    """What it scales is NaN and becomes so; the new numbers are as in a fresh block."""
+    codes = torch.randint(0, 0x7f, (1, 1, 16, 64), generator=_gen(22), dtype=torch.uint8)
+    pages = [codes.view(E4M3).cuda() for _ in range(2)]
+    scales = [torch.full((1, 1, 1), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    x = torch.full((1, 1, 64), 1.75, dtype=torch.float16, device="cuda")
+    hexmi.paged_append(x, x.clone(), *pages, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda"),
+                       k_scales=scales[0], v_scales=scales[1])
+    for t, s in zip(pages, scales):
+        assert s.item() == 127 - 8 and torch.isnan(t[0, 0, :3].float()).all() and (t[0, 0, 3].float() == 448).all()
+        assert torch.equal(t.cpu().view(torch.uint8)[0, 0, 4:], codes[0, 0, 4:])
+
+
 def test_every_number_of_e4m3_is_rounded_to_even(hexmi):
     """All numbers and the middles between neighbours, at a scale of 1 (the largest is 448)."""
     numbers = torch.arange(127, dtype=torch.uint8).view(E4M3).double()
