@@ -22,6 +22,7 @@
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"
+#include "paged_seen.h"
 
 namespace hexmi {
 namespace {
@@ -547,16 +548,10 @@ __device__ __forceinline__ void paged_tile(const PagedAttnArgs& a, const Pages& 
         // half as much so: a prompt of 16001 within 1024 356 -> 336 us). Without one few blocks are, and the compares need no registers.
         int seen_up_to = keys;
         asm volatile("" : "+v"(seen_up_to));                            // worked out here, and not kept over the walk
-        auto below = [](int n) __attribute__((always_inline)) {         // the first n bits of 32
-          const int m = n < 0 ? 0 : n < 32 ? n : 32;
-          return (uint32_t)(0xffffffffull >> (32 - m));
-        };
 #pragma unroll
         for (int jt = 0; jt < JT; ++jt) {
           const int first = begin + walked0 + jt * 32 + left_out;       // of the 32, counted from what the row sees
-          uint32_t seen = below(seen_up_to - first);
-          if (Kind::kWindow) seen &= ~below(seen_up_to - a.window - first) | below(a.sinks - walked0 - jt * 32);
-          seen = (seen & (uint32_t)(there >> 32 * jt)) >> (4 * half);
+          const uint32_t seen = (seen_of_32(seen_up_to, first, a.window, a.sinks - walked0 - jt * 32) & (uint32_t)(there >> 32 * jt)) >> (4 * half);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int at = 8 * (r / 4) + r % 4;

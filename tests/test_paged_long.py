@@ -1,4 +1,8 @@
 """Refusals of a paged cache in 8 bits, of windows, forks and compaction, and of their C entry points. No GPU."""
+import os
+import shutil
+import subprocess
+
 import pytest
 import torch
 
@@ -207,3 +211,39 @@ def test_strides_past_32_bits_are_refused_within_a_window(change):
         assert f(c_rows(heads=4), c_batch(**change), scales, None, 0, window, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
     for change in (dict(k_page=1 << 32), dict(v_block=-1)):
         assert f(c_rows(heads=4), c_batch(), c_scales(**change), None, 0, 0, 0, 1.0, _lib.F16, 4096, 1 << 40, None) == _lib.ENOTSUP
+
+
+SEEN = r"""
+#include <cstdio>
+#include "paged_seen.h"
+int main() {
+  const int at[] = {0, 1, 2, 31, 32, 33, 63, 64, 500, 4096, 0x3fffffff, 0x7ffffbe0, 0x7fffffff}, sinks[] = {-0x7fffffff, -1, 0, 1, 31, 32, 33, 0x7fffffff};
+  for (int keys : at)
+    for (int first : at)
+      for (int window : at)
+        for (int s : sinks) {
+          if (window == 0) continue;
+          unsigned want = 0;
+          for (long long i = 0; i < 32; ++i) {
+            const long long key = (long long)first + i;
+            if (key < keys && (key >= (long long)keys - window || i < s)) want |= 1u << i;
+          }
+          if (hexmi::seen_of_32(keys, first, window, s) != want) return printf("%d %d %d %d\n", keys, first, window, s), 1;
+        }
+  return 0;
+}
+"""
+
+
+def test_which_keys_a_row_sees_is_worked_out_without_overflow(tmp_path):
+    """The bits of 32 keys against their definition in 64 bits, with the checks of undefined behaviour on: rows of few keys beside blocks of far
+    ones, windows as wide as any cache."""
+    compiler = shutil.which("g++")
+    if compiler is None:
+        pytest.skip("no C++ compiler for host code")
+    source, program = tmp_path / "seen.cpp", tmp_path / "seen"
+    source.write_text(SEEN)
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hexagon-mlir_amd", "csrc")
+    subprocess.run([compiler, "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", csrc, str(source), "-o", str(program)], check=True)
+    run = subprocess.run([str(program)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout + run.stderr
