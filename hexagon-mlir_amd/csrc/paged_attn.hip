@@ -132,14 +132,14 @@ Seen seen_of(const hexmi_paged_batch& b, int64_t window, int64_t sinks) {
   const int w = window_of(window, sinks, b.table_cols * b.page_size);
   return w ? Seen{w, (int)sinks, (int64_t)w + sinks} : Seen{0, 0, kNoWindow};
 }
-int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t view) {
+int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t view, bool scaled) {
   const int rc = check_batch(b);
   if (rc != HEXMI_OK) return rc;
   if (heads < 1 || heads % b.kv_heads != 0 || shared < 0 || shared > b.table_cols) return HEXMI_EINVAL;
   if (b.dim % 8 != 0 || b.dim > 256 || heads > 65535) return HEXMI_ENOTSUP;
-  // rows, the blocks of all sequences and heads, and a launch's threads stay below 2^31
+  // rows, the blocks of all sequences and heads (of a cache in 8 bits one more a unit, kExtraBlocks), and a launch's threads stay below 2^31
   const int64_t group = heads / b.kv_heads, limit = 0x7fffffff, units = b.kv_heads * ((group + 15) / 16);
-  const int64_t blocks = (b.table_cols * b.page_size + 127) / 128 + 2;
+  const int64_t blocks = (b.table_cols * b.page_size + 127) / 128 + (scaled ? 2 : 1);
   if (b.tokens > limit / heads || b.sequences > limit / units / blocks) return HEXMI_ENOTSUP;
   if (!b.starts) return b.sequences <= limit / 256 / units ? HEXMI_OK : HEXMI_ENOTSUP;
   if (b.tokens == 0) return HEXMI_OK;          // nothing to launch: there is no plan of it (plan_of divides by the tiles)
@@ -148,15 +148,15 @@ int check(const hexmi_paged_batch& b, int64_t heads, int64_t shared, int64_t vie
   const int64_t workers = b.sequences > limit / 1024 / units ? limit : b.sequences * units;
   return (plan.tiles * plan.splits + (int64_t)plan.prefix_tiles * plan.prefix_splits) * b.kv_heads + workers <= limit / 512 ? HEXMI_OK : HEXMI_ENOTSUP;
 }
-int64_t workspace_of(const hexmi_paged_batch* batch, int64_t heads, int64_t shared, int64_t view) {
-  if (!batch || check(*batch, heads, shared, view) != HEXMI_OK || batch->tokens == 0) return 0;
+int64_t workspace_of(const hexmi_paged_batch* batch, int64_t heads, int64_t shared, int64_t view, bool scaled) {
+  if (!batch || check(*batch, heads, shared, view, scaled) != HEXMI_OK || batch->tokens == 0) return 0;
   const Plan plan = plan_of(*batch, heads, shared, view);
   return plan.decode_bytes + plan.sum_bytes;
 }
 int attend(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, const int32_t* shared_pages, int64_t shared,
            const Seen& seen, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
   if ((shared > 0 && !shared_pages) || workspace_bytes < 0) return HEXMI_EINVAL;
-  int rc = check(*batch, q->heads, shared, seen.view);
+  int rc = check(*batch, q->heads, shared, seen.view, scales != nullptr);
   if (rc != HEXMI_OK) return rc;
   if (!(sm_scale > 0.0f) || sm_scale > 2e38f) return HEXMI_EINVAL;
   if (dtype != HEXMI_F16 && dtype != HEXMI_BF16) return HEXMI_ENOTSUP;
@@ -202,7 +202,7 @@ int attend(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi
 }  // namespace
 
 extern "C" int64_t hexmi_paged_attention_workspace(const hexmi_paged_batch* batch, int64_t heads, int64_t shared) {
-  return workspace_of(batch, heads, shared, kNoWindow);
+  return workspace_of(batch, heads, shared, kNoWindow, false);
 }
 
 extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const int32_t* shared_pages, int64_t shared,
@@ -214,8 +214,7 @@ extern "C" int hexmi_paged_attention(const hexmi_head_rows* q, const hexmi_paged
 extern "C" int64_t hexmi_paged_attention_ex_workspace(const hexmi_paged_batch* batch, int64_t heads, int64_t shared,
                                                       const hexmi_paged_scales* scales, int64_t window, int64_t sinks) {
   if (!batch || window < 0 || sinks < 0 || check_batch(*batch) != HEXMI_OK) return 0;
-  (void)scales;                                // a cache in 8 bits is cut as one in 16
-  return workspace_of(batch, heads, shared, seen_of(*batch, window, sinks).view);
+  return workspace_of(batch, heads, shared, seen_of(*batch, window, sinks).view, scales != nullptr);      // a cache in 8 bits is cut as one in 16
 }
 
 extern "C" int hexmi_paged_attention_ex(const hexmi_head_rows* q, const hexmi_paged_batch* batch, const hexmi_paged_scales* scales,

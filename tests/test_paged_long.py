@@ -118,6 +118,21 @@ def test_index_results_are_checked():
     assert ops._index_out("paged_fork", "table_out", good, (2, 3), (good[1:],), dev) is not good
 
 
+def test_batches_of_16_bits_are_as_large_as_before_there_were_8():
+    """What a unit counts for beside its own blocks of 128 keys belongs to a cache in 8 bits: in 16, 2090000 sequences of 1026 blocks and one more
+    each stay below 2^31."""
+    lib, q = _lib.lib(), c_rows(heads=1)
+    of = lambda blocks: c_batch(kv_heads=1, table_cols=blocks * 8, table_row=blocks * 8, sequences=2090000, tokens=65536, starts=4096)
+    need = lambda blocks, s=None: lib.hexmi_paged_attention_ex_workspace(of(blocks), 1, 0, s, 0, 0)
+    assert need(1026) > 0 and need(1027) == 0 and need(1025, c_scales()) > 0 and need(1026, c_scales()) == 0
+    assert lib.hexmi_paged_attention_workspace(of(1026), 1, 0) == need(1026)
+    # past that check (to a workspace that is too small), and not
+    assert lib.hexmi_paged_attention(q, of(1026), None, 0, 1.0, _lib.F16, 4096, 1, None) == _lib.EINVAL
+    assert lib.hexmi_paged_attention(q, of(1027), None, 0, 1.0, _lib.F16, 4096, 1, None) == _lib.ENOTSUP
+    for blocks, status in ((1025, _lib.EINVAL), (1026, _lib.ENOTSUP)):
+        assert lib.hexmi_paged_attention_ex(q, of(blocks), c_scales(), None, 0, 0, 0, 1.0, _lib.F16, 4096, 1, None) == status
+
+
 def c_batch(**kw):
     b = dict(k_pages=4096, v_pages=4096, k_page=2048, k_head=1024, k_slot=64, v_page=2048, v_head=1024, v_slot=64, num_pages=3, page_size=16,
              kv_heads=2, dim=64, page_table=4096, table_row=2, table_cols=2, lengths=4096, starts=None, sequences=2, tokens=2)
