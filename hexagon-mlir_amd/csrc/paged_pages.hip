@@ -101,12 +101,13 @@ void clear_kernel(uint32_t* marks, int64_t words) {
 
 struct View {
   int window, sinks;                           // window 0: all
+  int ahead;                                   // positions past a length that count too
 };
 // the page that entry (b, column) of the table names, -1: none in use
 __device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, int column) {
   const int length = length_of(p, b);
   const int first = column * p.page_size;
-  if (first >= length) return -1;
+  if (first - w.ahead >= length) return -1;
   if (w.window > 0 && first >= w.sinks && first + p.page_size <= length - w.window) return -1;
   const int page = p.table[b * p.table_row + column];
   return page >= 0 && page < p.num_pages ? page : -1;
@@ -304,16 +305,23 @@ extern "C" int64_t hexmi_paged_compact_workspace(const hexmi_paged_batch* batch)
 
 extern "C" int hexmi_paged_compact(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int64_t window, int64_t sinks, int32_t* table_out,
                                    int64_t table_out_row, int32_t* count, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
+  return hexmi_paged_compact_ex(batch, scales, window, sinks, 0, table_out, table_out_row, count, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int64_t window, int64_t sinks, int64_t ahead,
+                                      int32_t* table_out, int64_t table_out_row, int32_t* count, int dtype, void* workspace, int64_t workspace_bytes,
+                                      hexmi_stream_t stream) {
   CopyArgs c;
   int piece;
   const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
   if (rc != HEXMI_OK) return rc;
   const int64_t entries = batch->sequences * batch->table_cols;
-  if (window < 0 || sinks < 0 || !count || (entries > 0 && !table_out)) return HEXMI_EINVAL;
+  if (window < 0 || sinks < 0 || ahead < 0 || !count || (entries > 0 && !table_out)) return HEXMI_EINVAL;
   if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < hexmi_paged_compact_workspace(batch)) return HEXMI_EINVAL;
   const Pages p = pages_of(*batch);
   const CompactSpace space = space_of(workspace, batch->num_pages);
-  const View view = {window_of(window, sinks, batch->table_cols * batch->page_size), (int)(sinks < 0x7fffffff ? sinks : 0x7fffffff)};
+  const int64_t positions = batch->table_cols * batch->page_size;
+  const View view = {window_of(window, sinks, positions), (int)(sinks < 0x7fffffff ? sinks : 0x7fffffff), (int)(ahead < positions ? ahead : positions)};
   const hipStream_t s = as_stream(stream);
   const int64_t words = words_of(batch->num_pages);
   auto blocks = [](int64_t n, int64_t most) { return dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)); };

@@ -101,7 +101,7 @@ _LIBDEF.define("paged_attention_ex(Tensor q, Tensor k_pages, Tensor v_pages, Ten
 _LIBDEF.define("paged_fork(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
                "Tensor lengths, Tensor parents, Tensor pages, Tensor(e!) table_out, Tensor(f!) lengths_out) -> ()")
 _LIBDEF.define("paged_compact(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
-               "Tensor lengths, int? window, int sinks, Tensor(e!) table_out, Tensor(f!) count) -> ()")
+               "Tensor lengths, int? window, int sinks, Tensor(e!) table_out, Tensor(f!) count, int ahead=0) -> ()")
 
 
 def _row_workspace(rows, cols, block_cols, x):
@@ -371,14 +371,14 @@ def _paged_fork_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, 
                    "hexmi_paged_fork")
 
 
-def _paged_compact_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, window, sinks, table_out, count):
+def _paged_compact_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, window, sinks, table_out, count, ahead=0):
     batch = _paged_batch(lengths.shape[0], k_pages, v_pages, page_table, lengths, None)
     with _on(k_pages.device):
         need = _lib.lib().hexmi_paged_compact_workspace(batch)
         ws = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
-        _lib.check(_lib.lib().hexmi_paged_compact(batch, _paged_scales(k_pages, k_scales, v_scales), window or 0, sinks, _p(table_out),
-                                                  table_out.stride(0), _p(count), _page_type(k_pages, k_scales), _p(ws), need, _stream()),
-                   "hexmi_paged_compact")
+        _lib.check(_lib.lib().hexmi_paged_compact_ex(batch, _paged_scales(k_pages, k_scales, v_scales), window or 0, sinks, ahead, _p(table_out),
+                                                     table_out.stride(0), _p(count), _page_type(k_pages, k_scales), _p(ws), need, _stream()),
+                   "hexmi_paged_compact_ex" if ahead else "hexmi_paged_compact")
 
 
 for _name, _fn in (("softmax", _softmax_impl), ("rms_norm", _rms_norm_impl), ("layer_norm", _layer_norm_impl),
@@ -1196,7 +1196,8 @@ def paged_fork(k_pages, v_pages, page_table, lengths, parents, pages, k_scales=N
     """Rows that go on from a batch's, as a step of a beam search has them: returns (page_table, lengths) of len(parents) rows, row i a copy
     of row parents[i] (int32; no row's number: an empty row, -1 throughout) in which pages[i] (int32) is the page of its next token. What the
     parent's part-filled last page holds is copied there, keys, values and scales of all heads; full pages stay shared, and where pages[i]
-    is no page's number (-1) the last one too (the one row that may go on in it).
+    is no page's number (-1) the last one too (the one row that may go on in it). Where the parent's last page is full, pages[i] stands past
+    the row's length: `paged_compact` keeps it with ahead=1, and without takes it for free.
 
     The cache is `paged_append`'s, in 16 or 8 bits, and changed in place; pages are each named once and in no use. All index tensors are
     read on the GPU only."""
@@ -1221,25 +1222,28 @@ def paged_fork(k_pages, v_pages, page_table, lengths, parents, pages, k_scales=N
     return _finish(to, table_out), _finish(lens_to, lengths_out)
 
 
-def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales=None, window=None, sinks=0, table_out=None):
+def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales=None, window=None, sinks=0, table_out=None, ahead=0):
     """Moves the pages in use to the front of the cache, and returns (page_table, count): the table with their new names, -1 where an entry is
     not in use, and an int32 tensor of one element, how many there are; the pages from there on are free. In use is a page that some
-    sequence's row names for positions below its length, within a window those that its last token sees. No more pages
+    sequence's row names for positions below its length, within a window those that its last token sees; with `ahead`, those of that many
+    positions past its length too (1: the pages that `paged_fork` put there for the next tokens, which are taken for free without). No more pages
     than need be are copied: those behind `count`, in rising order, to the free ones before it. The cache, in 16 or 8 bits, is changed in place;
     table_out may be page_table itself."""
-    if table_out is None and not _THROUGH_DISPATCHER:
+    if table_out is None and type(ahead) is int and ahead == 0 and not _THROUGH_DISPATCHER:
         y = _front.paged_compact(k_pages, v_pages, page_table, lengths, k_scales, v_scales, window, sinks)
         if y is not None:
             return y
     name = "paged_compact"
     window, sinks = _check_window(name, window, sinks)
+    if isinstance(ahead, bool) or not isinstance(ahead, int) or ahead < 0:
+        raise ValueError("hexmi.paged_compact: ahead is a number of positions from 0")
     table, lens = _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales)
     dev = k_pages.device
     _one_device(name, dev, table_out)
     same = table_out is not None and table_out.data_ptr() == table.data_ptr() and table_out.stride() == table.stride()
     to = _index_out(name, "table_out", table_out, table.shape, (None if same else table, lens, k_pages, v_pages, k_scales, v_scales), dev)
     count = torch.empty(1, dtype=torch.int32, device=dev)
-    args = (k_pages, v_pages, k_scales, v_scales, table, lens, window, sinks, to, count)
+    args = (k_pages, v_pages, k_scales, v_scales, table, lens, window, sinks, to, count, min(ahead, 1 << 40))
     _run(name, _paged_compact_impl, args, *args)
     return _finish(to, table_out), count
 

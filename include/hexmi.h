@@ -685,7 +685,9 @@ int hexmi_paged_attention_ex(const hexmi_head_rows *q,
  * there (keys, values and scales of all heads), and the entry renamed. A full
  * last page stays shared, as all before it; a part-filled one does where pages[i] is
  * no page, and one that is none stays none. pages [rows]: each one once, and no
- * page that the batch uses (else pieces of either are left there). What the
+ * page that the batch uses (else pieces of either are left there). The page of
+ * a next token that begins one stands past the row's length: a compaction keeps it
+ * with `ahead` 1 (hexmi_paged_compact_ex), and without takes it for free. What the
  * outputs hold shares no memory with what is read. batch: starts and tokens
  * are not looked at. dtype: of the pages (16 bits; with scales what they are read as). */
 int hexmi_paged_fork(const hexmi_paged_batch *batch,
@@ -709,6 +711,17 @@ int hexmi_paged_compact(const hexmi_paged_batch *batch,
                         int64_t table_out_row, int32_t *count, int dtype,
                         void *workspace, int64_t workspace_bytes,
                         hexmi_stream_t stream);
+
+/* hexmi_paged_compact where tables name pages for tokens that are still to
+ * come: those of the `ahead` positions past each length are in use too. After
+ * hexmi_paged_fork 1: where a row's last page is full, the page of its next token
+ * stands past its length, and hexmi_paged_compact takes it for free. */
+int hexmi_paged_compact_ex(const hexmi_paged_batch *batch,
+                           const hexmi_paged_scales *scales, int64_t window,
+                           int64_t sinks, int64_t ahead, int32_t *table_out,
+                           int64_t table_out_row, int32_t *count, int dtype,
+                           void *workspace, int64_t workspace_bytes,
+                           hexmi_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -219,6 +219,14 @@ def test_fork_and_compact_entries_refuse_before_they_launch():
     assert lib.hexmi_paged_compact_workspace(c_batch(num_pages=0)) == 0 and lib.hexmi_paged_compact_workspace(None) == 0
 
 
+@pytest.mark.parametrize("ahead", [-1, 1.0, True, None])
+def test_compact_refuses_what_is_no_number_of_positions(ahead):
+    with pytest.raises(ValueError, match="ahead"):
+        hexmi.paged_compact(**batch(), ahead=ahead)
+    if ahead == -1:
+        assert _lib.lib().hexmi_paged_compact_ex(c_batch(), c_scales(), 0, 0, ahead, 4096, 2, 4096, _lib.F16, 4096, 1 << 40, None) == _lib.EINVAL
+
+
 @pytest.mark.parametrize("change", [dict(k_page=1 << 32), dict(v_page=-2048)])
 def test_strides_past_32_bits_are_refused_within_a_window(change):
     f = _lib.lib().hexmi_paged_attention_ex

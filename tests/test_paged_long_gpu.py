@@ -668,6 +668,43 @@ def test_compact_against_the_definition(hexmi, case):
         assert torch.equal(raw(a), raw(b))
 
 
+def kept_reference(table, lengths, pool, page, window, sinks, ahead):
+    """compact_reference where `ahead` positions past a length count too."""
+    positions = [min(max(L, 0), len(row) * page) for row, L in zip(table, lengths)]
+    used = [[0 <= c < pool and i * page < n + ahead and (not window or i * page < sinks or (i + 1) * page > n - window) for i, c in enumerate(row)]
+            for row, n in zip(table, positions)]
+    marked = {c for row, u in zip(table, used) for c, x in zip(row, u) if x}
+    n = len(marked)
+    moves = dict(zip(sorted(p for p in marked if p >= n), sorted(set(range(n)) - marked)))
+    return [[moves.get(c, c) if x else -1 for c, x in zip(row, u)] for row, u in zip(table, used)], n, moves
+
+
+@pytest.mark.parametrize("ahead", [1, 2, 16, 17, 40, 1 << 50])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (20, 3)])
+def test_compact_keeps_pages_ahead(hexmi, ahead, window, sinks):
+    rng, pool, page = random.Random(ahead), 60, 16
+    lengths = [0, 15, 16, 17, 32, 47, 96, 200, -5]                    # the table ends at 96
+    table = [rng.sample(range(pool), 6) for _ in lengths]
+    table[2][1], table[3][2] = -1, pool                               # no page there yet
+    x = [torch.randn(pool, 2, page, 64, generator=_gen(1)).half().cuda() for _ in range(2)]
+    before = [t.clone() for t in x]
+    want, n, moves = kept_reference(table, lengths, pool, page, window, sinks, ahead)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    got, count = hexmi.paged_compact(*x, index(table), index(lengths), window=window, sinks=sinks, ahead=ahead)
+    assert got.tolist() == want and count.tolist() == [n]
+    for now, then in zip(x, before):
+        held = then.clone()
+        for a, b in moves.items():
+            held[b] = then[a]
+        assert torch.equal(now, held)
+    previous = hexmi.through_dispatcher(True)
+    try:
+        again, _ = hexmi.paged_compact(*before, index(table), index(lengths), window=window, sinks=sinks, ahead=ahead)
+    finally:
+        hexmi.through_dispatcher(previous)
+    assert torch.equal(again, got)
+
+
 # ---- a run of them
 def step(hexmi, state, x, freq, graph=False):
     q = hexmi.paged_append(x[:, 4:6], x[:, 6:], state["k"], state["v"], state["table"], state["lengths"], inv_freq=freq, q=x[:, :4], k_scales=state["ks"],
@@ -720,6 +757,29 @@ def test_beams_that_fork_and_compact_go_on_as_without(hexmi):
             assert torch.equal(got[[1, 2, 0]], first)
         else:
             assert torch.equal(got[[1, 2, 0]], step(hexmi, apart, both[[1, 2, 0]], freq)), i
+
+
+def test_a_fork_at_the_end_of_a_page_keeps_its_page_through_a_compaction(hexmi):
+    """Rows whose next token begins the page that the fork gave them: appends and attention go on as without the compaction."""
+    freq, g = hexmi.rope_frequencies(64), _gen(3)
+    a = small_state(7)
+    a["lengths"].copy_(torch.tensor([48, 33, 64], dtype=torch.int32))
+    for r in range(3):                                                # no page is named past a length
+        a["table"][r, (a["lengths"][r].item() + 15) // 16:] = -1
+    used = set(a["table"].flatten().tolist())
+    fresh = torch.tensor([p for p in range(39, -1, -1) if p not in used][:5], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([0, 2, 0, 1, 2], dtype=torch.int32, device="cuda")
+    a["table"], a["lengths"] = hexmi.paged_fork(a["k"], a["v"], a["table"], a["lengths"], parents, fresh, k_scales=a["ks"], v_scales=a["vs"])
+    apart = {n: t.clone() for n, t in a.items()}
+    a["table"], count = hexmi.paged_compact(a["k"], a["v"], a["table"], a["lengths"], k_scales=a["ks"], v_scales=a["vs"], window=40, sinks=4, ahead=1)
+    assert not torch.equal(a["k"].view(torch.uint8), apart["k"].view(torch.uint8)) and a["table"].max().item() < count.item()
+    for i in range(16):                                               # the tokens of the new page
+        x = torch.randn(5, 8, 64, generator=g).half().cuda()
+        for s in (a, apart):
+            s["lengths"] += 1
+        assert torch.equal(step(hexmi, a, x, freq), step(hexmi, apart, x, freq)), i
+        if a["lengths"][3].item() == 48:
+            break
 
 
 def test_a_captured_step_is_replayed(hexmi):
