@@ -102,6 +102,8 @@ void clear_kernel(uint32_t* marks, int64_t words) {
 struct View {
   int window, sinks;                           // window 0: all
   int ahead;                                   // positions past a length that count too
+  const int32_t* shared_pages;                 // the first `shared` pages of every sequence, whatever the table says there
+  int shared;
 };
 // the page that entry (b, column) of the table names, -1: none in use
 __device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, int column) {
@@ -109,11 +111,16 @@ __device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, i
   const int first = column * p.page_size;
   if (first - w.ahead >= length) return -1;
   if (w.window > 0 && first >= w.sinks && first + p.page_size <= length - w.window) return -1;
-  const int page = p.table[b * p.table_row + column];
+  const int page = column < w.shared ? w.shared_pages[column] : p.table[b * p.table_row + column];
   return page >= 0 && page < p.num_pages ? page : -1;
 }
-// entry i of the table, row by row
+// entry i of the table, row by row, and then of the shared pages, which are in use in any case
 __device__ __forceinline__ int used_page(const Pages& p, const View& w, int64_t i) {
+  const int64_t in_table = (int64_t)p.sequences * p.table_cols;
+  if (i >= in_table) {
+    const int page = w.shared_pages[i - in_table];
+    return page >= 0 && page < p.num_pages ? page : -1;
+  }
   const int b = (int)(i / p.table_cols);
   return used_page(p, w, b, (int)(i - (int64_t)b * p.table_cols));
 }
@@ -203,11 +210,18 @@ void mark_and_number_kernel(Pages p, View w, CompactSpace s, int32_t* count, int
 
 template <typename Piece>
 __global__ __launch_bounds__(256)
-void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int64_t entries, int parts) {
+void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int32_t* shared_out,
+                 int64_t entries, int parts) {
   const int front = *count, moves = *s.moves;
+  const int64_t in_table = entries - w.shared;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
-    const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols), page = used_page(p, w, b, column);
-    table_out[b * table_out_row + column] = page >= front ? s.renamed[page] : page;
+    const int page = used_page(p, w, i), name = page >= front ? s.renamed[page] : page;
+    if (i >= in_table) {
+      shared_out[i - in_table] = name;
+      continue;
+    }
+    const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols);
+    table_out[b * table_out_row + column] = name;
   }
   for (int64_t i = blockIdx.x; i < 2 * (int64_t)moves * parts; i += gridDim.x) {
     const int64_t unit = i / parts;
@@ -305,23 +319,27 @@ extern "C" int64_t hexmi_paged_compact_workspace(const hexmi_paged_batch* batch)
 
 extern "C" int hexmi_paged_compact(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int64_t window, int64_t sinks, int32_t* table_out,
                                    int64_t table_out_row, int32_t* count, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
-  return hexmi_paged_compact_ex(batch, scales, window, sinks, 0, table_out, table_out_row, count, dtype, workspace, workspace_bytes, stream);
+  return hexmi_paged_compact_ex(batch, scales, nullptr, 0, window, sinks, 0, table_out, table_out_row, nullptr, count, dtype, workspace, workspace_bytes,
+                                stream);
 }
 
-extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int64_t window, int64_t sinks, int64_t ahead,
-                                      int32_t* table_out, int64_t table_out_row, int32_t* count, int dtype, void* workspace, int64_t workspace_bytes,
-                                      hexmi_stream_t stream) {
+extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, const int32_t* shared_pages, int64_t shared,
+                                      int64_t window, int64_t sinks, int64_t ahead, int32_t* table_out, int64_t table_out_row, int32_t* shared_out,
+                                      int32_t* count, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
   CopyArgs c;
   int piece;
   const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
   if (rc != HEXMI_OK) return rc;
-  const int64_t entries = batch->sequences * batch->table_cols;
-  if (window < 0 || sinks < 0 || ahead < 0 || !count || (entries > 0 && !table_out)) return HEXMI_EINVAL;
+  if (window < 0 || sinks < 0 || ahead < 0 || !count || (batch->sequences * batch->table_cols > 0 && !table_out)) return HEXMI_EINVAL;
+  if (shared < 0 || shared > batch->table_cols || (shared > 0 && (!shared_pages || !shared_out))) return HEXMI_EINVAL;
+  if (window > 0 && shared > 0) return HEXMI_ENOTSUP;
+  const int64_t entries = batch->sequences * batch->table_cols + shared;
   if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < hexmi_paged_compact_workspace(batch)) return HEXMI_EINVAL;
   const Pages p = pages_of(*batch);
   const CompactSpace space = space_of(workspace, batch->num_pages);
   const int64_t positions = batch->table_cols * batch->page_size;
-  const View view = {window_of(window, sinks, positions), (int)(sinks < 0x7fffffff ? sinks : 0x7fffffff), (int)(ahead < positions ? ahead : positions)};
+  const View view = {window_of(window, sinks, positions), (int)(sinks < 0x7fffffff ? sinks : 0x7fffffff), (int)(ahead < positions ? ahead : positions),
+                     shared_pages, (int)shared};
   const hipStream_t s = as_stream(stream);
   const int64_t words = words_of(batch->num_pages);
   auto blocks = [](int64_t n, int64_t most) { return dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)); };
@@ -338,7 +356,7 @@ extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexm
   const int64_t units = batch->num_pages * parts > (entries + 255) / 256 ? batch->num_pages * parts : (entries + 255) / 256;
   return with_piece(piece, [&](auto x) {
     hipLaunchKernelGGL((move_kernel<decltype(x)>), dim3((unsigned)(units < 2048 ? units : 2048)), dim3(256), 0, s, c, p, view, space, count, table_out,
-                       table_out_row, entries, (int)parts);
+                       table_out_row, shared_out, entries, (int)parts);
     return launch_status();
   });
 }

@@ -106,7 +106,7 @@ SIGNATURES = {
     "hexmi_paged_fork": (_int, [_batch, _scales, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _int, _ptr]),
     "hexmi_paged_compact_workspace": (_i64, [_batch]),
     "hexmi_paged_compact": (_int, [_batch, _scales, _i64, _i64, _ptr, _i64, _ptr, _int, _ptr, _i64, _ptr]),
-    "hexmi_paged_compact_ex": (_int, [_batch, _scales, _i64, _i64, _i64, _ptr, _i64, _ptr, _int, _ptr, _i64, _ptr]),
+    "hexmi_paged_compact_ex": (_int, [_batch, _scales, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _int, _ptr, _i64, _ptr]),
 }
 
 # measurement probes of include/hexmi_calibrate.h: exported by the library, not part of the operator ABI

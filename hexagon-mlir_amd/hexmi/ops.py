@@ -101,7 +101,8 @@ _LIBDEF.define("paged_attention_ex(Tensor q, Tensor k_pages, Tensor v_pages, Ten
 _LIBDEF.define("paged_fork(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
                "Tensor lengths, Tensor parents, Tensor pages, Tensor(e!) table_out, Tensor(f!) lengths_out) -> ()")
 _LIBDEF.define("paged_compact(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scales, Tensor(d!)? v_scales, Tensor page_table, "
-               "Tensor lengths, int? window, int sinks, Tensor(e!) table_out, Tensor(f!) count, int ahead=0) -> ()")
+               "Tensor lengths, int? window, int sinks, Tensor(e!) table_out, Tensor(f!) count, int ahead=0, "
+               "Tensor? shared_pages=None, Tensor(g!)? shared_out=None) -> ()")
 
 
 def _row_workspace(rows, cols, block_cols, x):
@@ -371,14 +372,16 @@ def _paged_fork_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, 
                    "hexmi_paged_fork")
 
 
-def _paged_compact_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, window, sinks, table_out, count, ahead=0):
+def _paged_compact_impl(k_pages, v_pages, k_scales, v_scales, page_table, lengths, window, sinks, table_out, count, ahead=0,
+                        shared_pages=None, shared_out=None):
     batch = _paged_batch(lengths.shape[0], k_pages, v_pages, page_table, lengths, None)
     with _on(k_pages.device):
         need = _lib.lib().hexmi_paged_compact_workspace(batch)
         ws = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
-        _lib.check(_lib.lib().hexmi_paged_compact_ex(batch, _paged_scales(k_pages, k_scales, v_scales), window or 0, sinks, ahead, _p(table_out),
-                                                     table_out.stride(0), _p(count), _page_type(k_pages, k_scales), _p(ws), need, _stream()),
-                   "hexmi_paged_compact_ex" if ahead else "hexmi_paged_compact")
+        _lib.check(_lib.lib().hexmi_paged_compact_ex(batch, _paged_scales(k_pages, k_scales, v_scales), _p(shared_pages),
+                                                     0 if shared_pages is None else shared_pages.shape[0], window or 0, sinks, ahead, _p(table_out),
+                                                     table_out.stride(0), _p(shared_out), _p(count), _page_type(k_pages, k_scales), _p(ws), need,
+                                                     _stream()), "hexmi_paged_compact_ex")
 
 
 for _name, _fn in (("softmax", _softmax_impl), ("rms_norm", _rms_norm_impl), ("layer_norm", _layer_norm_impl),
@@ -1035,6 +1038,11 @@ def _check_scales(name, k_pages, k_scales, v_scales):
     return True
 
 
+def _check_shared_pages(name, shared_pages, page_table):
+    if shared_pages is not None and (shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] > page_table.shape[-1]):
+        raise ValueError("hexmi.%s: shared_pages must be an int32 tensor of one dimension, no longer than the table is wide" % name)
+
+
 def _check_window(name, window, sinks):
     """(window, sinks) as the library takes them; numbers past any position are one as good as another."""
     if window is None and sinks:
@@ -1117,7 +1125,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
     hold both.
 
     shared_pages int32 [n]: the first n pages of every sequence are these (a prompt that all have in common), and their keys are gone
-    through once for all of them; the result is the same without, if the table names them.
+    through once for all of them; the result is the same without, if the table names them. `paged_compact` has to be told of them too.
 
     How the work is cut goes by the width of page_table: one much wider than the longest sequence costs a small batch 2 to 10 us, and sums in
     another order.
@@ -1149,8 +1157,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, sm_sc
         sm_scale = 1.0 / math.sqrt(q.shape[2])
     if not 0 < sm_scale <= 2e38:
         raise ValueError("hexmi.paged_attention: sm_scale must be positive")
-    if shared_pages is not None and (shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] > page_table.shape[-1]):
-        raise ValueError("hexmi.paged_attention: shared_pages must be an int32 tensor of one dimension, no longer than the table is wide")
+    _check_shared_pages(name, shared_pages, page_table)
     table, lens, begin = _paged_operands(name, q.shape[0], k_pages, v_pages, page_table, lengths, starts)
     dev = k_pages.device
     _one_device(name, dev, q, shared_pages, out)
@@ -1222,14 +1229,19 @@ def paged_fork(k_pages, v_pages, page_table, lengths, parents, pages, k_scales=N
     return _finish(to, table_out), _finish(lens_to, lengths_out)
 
 
-def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales=None, window=None, sinks=0, table_out=None, ahead=0):
+def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales=None, window=None, sinks=0, table_out=None, ahead=0,
+                  shared_pages=None):
     """Moves the pages in use to the front of the cache, and returns (page_table, count): the table with their new names, -1 where an entry is
     not in use, and an int32 tensor of one element, how many there are; the pages from there on are free. In use is a page that some
     sequence's row names for positions below its length, within a window those that its last token sees; with `ahead`, those of that many
     positions past its length too (1: the pages that `paged_fork` put there for the next tokens, which are taken for free without). No more pages
     than need be are copied: those behind `count`, in rising order, to the free ones before it. The cache, in 16 or 8 bits, is changed in place;
-    table_out may be page_table itself."""
-    if table_out is None and type(ahead) is int and ahead == 0 and not _THROUGH_DISPATCHER:
+    table_out may be page_table itself.
+
+    shared_pages int32 [n]: the first n pages of every sequence are these, as `paged_attention` has them. They are in use whatever the lengths,
+    what the table says in those columns is not read, and (page_table, count, shared_pages) is returned, the last with their new names. A prefix
+    that neither is given nor stands in the table is taken for free. Not within a window, as in the attention."""
+    if table_out is None and shared_pages is None and type(ahead) is int and ahead == 0 and not _THROUGH_DISPATCHER:
         y = _front.paged_compact(k_pages, v_pages, page_table, lengths, k_scales, v_scales, window, sinks)
         if y is not None:
             return y
@@ -1237,15 +1249,21 @@ def paged_compact(k_pages, v_pages, page_table, lengths, k_scales=None, v_scales
     window, sinks = _check_window(name, window, sinks)
     if isinstance(ahead, bool) or not isinstance(ahead, int) or ahead < 0:
         raise ValueError("hexmi.paged_compact: ahead is a number of positions from 0")
+    if window is not None and shared_pages is not None:
+        raise ValueError("hexmi.paged_compact: no shared pages within a window (name them in page_table)")
+    _check_shared_pages(name, shared_pages, page_table)
     table, lens = _pages_to_copy(name, k_pages, v_pages, page_table, lengths, k_scales, v_scales)
     dev = k_pages.device
-    _one_device(name, dev, table_out)
+    _one_device(name, dev, table_out, shared_pages)
+    sd = _stage(shared_pages, dev)
     same = table_out is not None and table_out.data_ptr() == table.data_ptr() and table_out.stride() == table.stride()
-    to = _index_out(name, "table_out", table_out, table.shape, (None if same else table, lens, k_pages, v_pages, k_scales, v_scales), dev)
+    to = _index_out(name, "table_out", table_out, table.shape, (None if same else table, lens, k_pages, v_pages, k_scales, v_scales, sd), dev)
+    shared_to = None if sd is None else torch.empty_like(sd)
     count = torch.empty(1, dtype=torch.int32, device=dev)
-    args = (k_pages, v_pages, k_scales, v_scales, table, lens, window, sinks, to, count, min(ahead, 1 << 40))
+    args = (k_pages, v_pages, k_scales, v_scales, table, lens, window, sinks, to, count, min(ahead, 1 << 40), sd, shared_to)
     _run(name, _paged_compact_impl, args, *args)
-    return _finish(to, table_out), count
+    to = _finish(to, table_out)
+    return (to, count) if sd is None else (to, count, shared_to)
 
 
 # Above this much multiply-add work the one-launch kernel (32 rows per workgroup, so few workgroups on small

@@ -702,7 +702,8 @@ int hexmi_paged_fork(const hexmi_paged_batch *batch,
  * ones below n, in rising order. table_out [sequences, table_cols, leading dim
  * table_out_row] is the table with their new names, -1 where an entry is not in
  * use; it may be the table itself. count[0] = n: the pages from n on are free
- * (and hold what they held). Workspace: 16-byte aligned, not initialised, no state
+ * (and hold what they held). Pages that are in use beside the table's (a shared prefix,
+ * those of tokens to come): hexmi_paged_compact_ex. Workspace: 16-byte aligned, not initialised, no state
  * between calls; two calls that overlap in time need one each. */
 int64_t hexmi_paged_compact_workspace(const hexmi_paged_batch *batch);
 int hexmi_paged_compact(const hexmi_paged_batch *batch,
@@ -712,14 +713,25 @@ int hexmi_paged_compact(const hexmi_paged_batch *batch,
                         void *workspace, int64_t workspace_bytes,
                         hexmi_stream_t stream);
 
-/* hexmi_paged_compact where tables name pages for tokens that are still to
- * come: those of the `ahead` positions past each length are in use too. After
- * hexmi_paged_fork 1: where a row's last page is full, the page of its next token
- * stands past its length, and hexmi_paged_compact takes it for free. */
+/* hexmi_paged_compact where more than the table's positions below the lengths is
+ * in use.
+ * shared_pages [shared]: the first pages of every sequence, as
+ * hexmi_paged_attention has them. They are in use whatever the lengths, what the table
+ * says in those columns is not read, and shared_out [shared], which shares no
+ * memory with what is read, has their new names (-1 for one that is no page); so do
+ * the table's columns. Without, a prefix that the table does not name is
+ * taken for free, and one that it does moves while the caller's list keeps the old
+ * names. Not within a window (HEXMI_ENOTSUP), as the attention.
+ * ahead: where tables name pages for tokens that are still to come, those
+ * of that many positions past each length are in use too. After hexmi_paged_fork
+ * 1: where a row's last page is full, the page of its next token stands past its
+ * length, and hexmi_paged_compact takes it for free. */
 int hexmi_paged_compact_ex(const hexmi_paged_batch *batch,
-                           const hexmi_paged_scales *scales, int64_t window,
-                           int64_t sinks, int64_t ahead, int32_t *table_out,
-                           int64_t table_out_row, int32_t *count, int dtype,
+                           const hexmi_paged_scales *scales,
+                           const int32_t *shared_pages, int64_t shared,
+                           int64_t window, int64_t sinks, int64_t ahead,
+                           int32_t *table_out, int64_t table_out_row,
+                           int32_t *shared_out, int32_t *count, int dtype,
                            void *workspace, int64_t workspace_bytes,
                            hexmi_stream_t stream);
 

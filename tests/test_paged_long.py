@@ -224,7 +224,19 @@ def test_compact_refuses_what_is_no_number_of_positions(ahead):
     with pytest.raises(ValueError, match="ahead"):
         hexmi.paged_compact(**batch(), ahead=ahead)
     if ahead == -1:
-        assert _lib.lib().hexmi_paged_compact_ex(c_batch(), c_scales(), 0, 0, ahead, 4096, 2, 4096, _lib.F16, 4096, 1 << 40, None) == _lib.EINVAL
+        assert _lib.lib().hexmi_paged_compact_ex(c_batch(), c_scales(), None, 0, 0, 0, ahead, 4096, 2, None, 4096, _lib.F16, 4096, 1 << 40, None) == _lib.EINVAL
+
+
+def test_compact_refuses_bad_shared_pages():
+    for bad in (torch.zeros(1), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="hexmi.paged_compact: shared_pages"):
+            hexmi.paged_compact(**batch(), shared_pages=bad)
+    with pytest.raises(ValueError, match="no shared pages within a window"):
+        hexmi.paged_compact(**batch(), shared_pages=torch.zeros(1, dtype=torch.int32), window=5)
+    f = _lib.lib().hexmi_paged_compact_ex
+    call = lambda pages, n, out, window=0: f(c_batch(), c_scales(), pages, n, window, 0, 0, 4096, 2, out, 4096, _lib.F16, 4096, 1 << 40, None)
+    assert call(None, 1, 4096) == call(4096, 1, None) == call(4096, 3, 4096) == call(4096, -1, 4096) == _lib.EINVAL
+    assert call(4096, 1, 4096, window=5) == _lib.ENOTSUP
 
 
 @pytest.mark.parametrize("change", [dict(k_page=1 << 32), dict(v_page=-2048)])

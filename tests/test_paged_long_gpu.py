@@ -705,6 +705,50 @@ def test_compact_keeps_pages_ahead(hexmi, ahead, window, sinks):
     assert torch.equal(again, got)
 
 
+@pytest.mark.parametrize("ahead", [0, 1])
+@pytest.mark.parametrize("columns", ["none", "stale", "named"])
+@pytest.mark.parametrize("shared", [[], [40, 3], [57, 41, 41, -1, 60, 2]], ids=len)
+def test_compact_of_a_shared_prefix_against_the_definition(hexmi, shared, columns, ahead):
+    """The prefix's pages are in use whatever the lengths, and what the table says in their columns does not count."""
+    rng, pool, page = random.Random(len(shared)), 60, 16
+    lengths = [0, 31, 32, 97, 128, 1, -5]
+    others = [p for p in range(pool) if p not in shared]
+    table = [rng.sample(others, 8) for _ in lengths]
+    for row in table:
+        row[:len(shared)] = {"none": [-7] * len(shared), "stale": rng.sample(others, len(shared)), "named": shared}[columns]
+    x = [torch.randn(pool, 1, page, 64, generator=_gen(1)).half().cuda() for _ in range(2)]
+    before = [t.clone() for t in x]
+    # the same as a table that names them, with a row of their own
+    want, n, moves = kept_reference([shared + row[len(shared):] for row in table] + [shared], lengths + [len(shared) * page], pool, page, None, 0, ahead)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    got, count, names = hexmi.paged_compact(*x, index(table), index(lengths), shared_pages=index(shared), ahead=ahead)
+    assert got.tolist() == want[:-1] and count.tolist() == [n] and names.tolist() == want[-1]
+    for now, then in zip(x, before):
+        held = then.clone()
+        for a, b in moves.items():
+            held[b] = then[a]
+        assert torch.equal(now, held)
+    # into the table itself, through the dispatcher, and with the prefix on the host
+    previous = hexmi.through_dispatcher(True)
+    try:
+        t = index(table)
+        again = hexmi.paged_compact(*before, t, index(lengths), shared_pages=torch.tensor(shared, dtype=torch.int32), ahead=ahead, table_out=t)
+    finally:
+        hexmi.through_dispatcher(previous)
+    assert again[0] is t and all(torch.equal(a, b) for a, b in zip(again, (got, count, names)))
+    assert all(torch.equal(a, b) for a, b in zip(x, before))
+
+
+def test_compact_of_a_shared_prefix_and_no_sequence(hexmi):
+    x = [torch.randn(9, 1, 4, 8, generator=_gen(1)).half().cuda() for _ in range(2)]
+    before = [t.clone() for t in x]
+    table = torch.zeros(0, 5, dtype=torch.int32, device="cuda")
+    got, count, names = hexmi.paged_compact(*x, table, torch.zeros(0, dtype=torch.int32, device="cuda"),
+                                            shared_pages=torch.tensor([8, 1], dtype=torch.int32, device="cuda"))
+    assert got.shape == (0, 5) and count.item() == 2 and names.tolist() == [0, 1]
+    assert all(torch.equal(a[0], b[8]) and torch.equal(a[1:], b[1:]) for a, b in zip(x, before))
+
+
 # ---- a run of them
 def step(hexmi, state, x, freq, graph=False):
     q = hexmi.paged_append(x[:, 4:6], x[:, 6:], state["k"], state["v"], state["table"], state["lengths"], inv_freq=freq, q=x[:, :4], k_scales=state["ks"],
@@ -780,6 +824,33 @@ def test_a_fork_at_the_end_of_a_page_keeps_its_page_through_a_compaction(hexmi):
         assert torch.equal(step(hexmi, a, x, freq), step(hexmi, apart, x, freq)), i
         if a["lengths"][3].item() == 48:
             break
+
+
+@pytest.mark.parametrize("new, context, shared, dim, page, block, dt", [
+    ([1] * 5, [0, 3, 40, 200, 1], 64, 128, 16, 16, "f16"), ([30, 1, 0, 90], [1, 1, 1, 1], 400, 64, 16, 8, "bf16"), ([1] * 3, [5, 90, 20], 96, 64, 32, 0, "f16"),
+], ids=str)
+@pytest.mark.parametrize("named", [False, True])
+def test_a_shared_prefix_through_a_compaction(hexmi, new, context, shared, dim, page, block, dt, named):
+    """A cache of which the first pages are nobody's: the prefix moves with the rest, and attention is the same behind it."""
+    c = Long(new, [shared + x for x in context], 4, 2, dim, page, block, DTYPES[dt], seed=dim, shared=shared)
+    tensors = [t for t in (c.k_pages, c.v_pages, c.k_scales, c.v_scales) if t is not None]
+    grown = [torch.cat((t[:1].expand(7, *t.shape[1:]), t)) for t in tensors]
+    c.k_pages, c.v_pages = grown[:2]
+    if block:
+        c.k_scales, c.v_scales = grown[2:]
+    c.page_table, c.shared_pages = torch.where(c.page_table >= 0, c.page_table + 7, c.page_table), c.shared_pages + 7
+    want = c.run(hexmi, shared_pages=c.shared_pages)
+    c.check(want)
+    if not named:
+        c.page_table[:, :shared // page] = -7
+    scales = {"k_scales": c.k_scales, "v_scales": c.v_scales} if block else {}
+    old = c.shared_pages
+    c.page_table, count, c.shared_pages = hexmi.paged_compact(c.k_pages, c.v_pages, c.page_table, c.lengths_d, shared_pages=old, **scales)
+    assert not torch.equal(c.shared_pages, old) and c.page_table.max().item() < count.item() and c.shared_pages.max().item() < count.item()
+    for t in (c.k_pages, c.v_pages):                                  # what is free now may be anything
+        t[count.item():].view(torch.uint8 if block else torch.int16).fill_(0x7f if block else 0x7fff)
+    assert torch.equal(c.run(hexmi, shared_pages=c.shared_pages), want)
+    c.check(c.run(hexmi), "each for itself")                          # the table names them now
 
 
 def test_a_captured_step_is_replayed(hexmi):
