@@ -424,6 +424,27 @@ def test_append_against_the_definition(hexmi, case, form):
         assert got is None
 
 
+MANY = [61, 62, 63, 64, 65, 127, 300, 4100]
+
+
+@pytest.mark.parametrize("sequences", MANY)
+@pytest.mark.parametrize("block", [2, 16])
+def test_append_of_many_sequences(hexmi, sequences, block):
+    """Which sequence a block of new tokens belongs to is looked up 64 starts at a time: ragged batches around that and far beyond, sequences without
+    new tokens and rows behind the last among them."""
+    new = [(1, 0, 3, 17, 0, 1)[(5 * i + i // 7) % 6] for i in range(sequences)]
+    context = [(0, 3, 15, 30, 7)[i % 5] for i in range(sequences)]
+    case = (new, context, 2, 1, 64, 64, 16, block, "f16", "head", "adjacent", False, 5)
+    test_append_against_the_definition(hexmi, case, "slices")
+
+
+@pytest.mark.parametrize("sequences", MANY)
+def test_all_sequences_but_one_without_new_tokens(hexmi, sequences):
+    for at in (0, sequences // 2, sequences - 1):
+        new = [40 if i == at else 0 for i in range(sequences)]
+        test_append_against_the_definition(hexmi, (new, [5] * sequences, 0, 1, 64, 0, 16, 16, "bf16", "head", "adjacent", False, 0), "slices")
+
+
 def one_block(hexmi, rows, contexts, dtype, block=16, **kw):
     """Values put one call after the other into a cache of one head of 64; (numbers, exponents)."""
     pages = [torch.full((2, 1, 16, 64), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2)]
