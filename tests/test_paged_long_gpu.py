@@ -726,6 +726,45 @@ def test_compact_keeps_pages_ahead(hexmi, ahead, window, sinks):
     assert torch.equal(again, got)
 
 
+LARGE = [
+    # sequences, columns, pool, page, window, sinks, shared pages: one workgroup marks up to 8192 entries and 262144 pages, shared ones among them
+    (1, 8192, 9000, 1, None, 0, 0), (1, 8193, 9000, 1, None, 0, 0), (64, 128, 5000, 4, None, 0, 0), (64, 129, 20000, 4, 70, 9, 0), (300, 40, 7001, 2, None, 0, 0),
+    (2, 4096, 9000, 1, None, 0, 1), (3, 50, 262144, 1, None, 0, 0), (3, 50, 262145, 1, None, 0, 2), (700, 300, 262175, 1, 100, 0, 0), (1, 8193, 33, 1, None, 0, 0),
+    (9000, 1, 9000, 1, None, 0, 0), (0, 8193, 40, 1, None, 0, 8193),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "x".join(map(str, c)))
+def test_compact_of_many_entries_and_pages(hexmi, case):
+    """Around the sizes from which marks are made by many workgroups, in a workspace that held ones."""
+    from hexmi import _lib, ops
+    B, columns, pool, page, window, sinks, shared = case
+    rng, g = random.Random(B + pool), _gen(pool)
+    lengths = [rng.choice((0, rng.randint(0, columns * page), columns * page)) for _ in range(B)] or []
+    if B in (1, 9000):
+        lengths = [columns * page] * B
+    # the upper half of the pool is named more often, some pages by several rows
+    table = [[rng.randrange(pool // 2, pool) if rng.random() < 0.8 else rng.choice((-1, pool, rng.randrange(pool))) for _ in range(columns)] for _ in range(B)]
+    prefix = [rng.randrange(pool) for _ in range(shared)]
+    want, n, moves = kept_reference([prefix + row[shared:] for row in table] + [prefix], lengths + [shared * page], pool, page, window, sinks, 0)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    x = [torch.randint(-(1 << 15), 1 << 15, (pool, 1, page, 8), generator=g, dtype=torch.int16).view(torch.float16).cuda() for _ in range(2)]
+    held = [t.clone() for t in x]
+    if moves:
+        source, target = (torch.tensor(list(v), device="cuda") for v in (moves.keys(), moves.values()))
+        for t in held:
+            t[target] = t[source]
+    page_table, lens, prefix_d = index(table).view(B, columns), index(lengths), index(prefix)
+    out, names, count = torch.full_like(page_table, 9), torch.full_like(prefix_d, 9), torch.full((1,), 9, dtype=torch.int32, device="cuda")
+    batch = ops._paged_batch(B, *x, page_table, lens, None)
+    ws = torch.full((_lib.lib().hexmi_paged_compact_workspace(batch),), 255, dtype=torch.uint8, device="cuda")
+    _lib.check(_lib.lib().hexmi_paged_compact_ex(batch, None, prefix_d.data_ptr() if shared else None, shared, window or 0, sinks, 0, out.data_ptr(), columns,
+                                                 names.data_ptr() if shared else None, count.data_ptr(), _lib.F16, ws.data_ptr(), ws.numel(),
+                                                 torch.cuda.current_stream().cuda_stream), "hexmi_paged_compact_ex")
+    assert count.item() == n and out.tolist() == want[:-1] and names.tolist() == want[-1]
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(x, held))
+
+
 @pytest.mark.parametrize("ahead", [0, 1])
 @pytest.mark.parametrize("columns", ["none", "stale", "named"])
 @pytest.mark.parametrize("shared", [[], [40, 3], [57, 41, 41, -1, 60, 2]], ids=len)
