@@ -231,8 +231,8 @@ void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* cou
   }
 }
 
-// HEXMI_OK, or why a cache is refused; the copies' arguments and the bytes of their pieces
-int check_cache(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int dtype, int64_t table_out_row, CopyArgs& c, int& piece) {
+// HEXMI_OK, or why a cache is refused; the copies' arguments and the bytes of their pieces. One row of a result is as good with any stride.
+int check_cache(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales, int dtype, int64_t rows_out, int64_t table_out_row, CopyArgs& c, int& piece) {
   if (!batch) return HEXMI_EINVAL;
   hexmi_paged_batch b = *batch;
   b.starts = nullptr;
@@ -244,7 +244,7 @@ int check_cache(const hexmi_paged_batch* batch, const hexmi_paged_scales* scales
   if (!b.k_pages || !b.v_pages || (b.sequences > 0 && (!b.lengths || (b.table_cols > 0 && !b.page_table)))) return HEXMI_EINVAL;
   const int size = scales ? 1 : 2;
   if (b.dim > (1 << 20)) return HEXMI_ENOTSUP;
-  if (table_out_row < b.table_cols) return HEXMI_EINVAL;
+  if (rows_out > 1 && table_out_row < b.table_cols) return HEXMI_EINVAL;
   c = {};
   c.side[0] = {static_cast<char*>(b.k_pages), b.k_page * size, b.k_head * size, b.k_slot * size};
   c.side[1] = {static_cast<char*>(b.v_pages), b.v_page * size, b.v_head * size, b.v_slot * size};
@@ -293,7 +293,7 @@ extern "C" int hexmi_paged_fork(const hexmi_paged_batch* batch, const hexmi_page
                                 int64_t rows, int32_t* table_out, int64_t table_out_row, int32_t* lengths_out, int dtype, hexmi_stream_t stream) {
   CopyArgs c;
   int piece;
-  const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
+  const int rc = check_cache(batch, scales, dtype, rows, table_out_row, c, piece);
   if (rc != HEXMI_OK) return rc;
   if (rows < 0) return HEXMI_EINVAL;
   if (rows == 0) return HEXMI_OK;
@@ -328,7 +328,7 @@ extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexm
                                       int32_t* count, int dtype, void* workspace, int64_t workspace_bytes, hexmi_stream_t stream) {
   CopyArgs c;
   int piece;
-  const int rc = check_cache(batch, scales, dtype, table_out_row, c, piece);
+  const int rc = check_cache(batch, scales, dtype, batch ? batch->sequences : 0, table_out_row, c, piece);
   if (rc != HEXMI_OK) return rc;
   if (window < 0 || sinks < 0 || ahead < 0 || !count || (batch->sequences * batch->table_cols > 0 && !table_out)) return HEXMI_EINVAL;
   if (shared < 0 || shared > batch->table_cols || (shared > 0 && (!shared_pages || !shared_out))) return HEXMI_EINVAL;

@@ -1065,3 +1065,23 @@ def test_pages_with_room_between_them(hexmi):
     got = [hexmi.paged_fork(x.k_pages, x.v_pages, x.page_table, x.lengths_d, index, torch.full_like(index, -1), x.k_scales, x.v_scales) for x in (close, apart)]
     packed = [hexmi.paged_compact(x.k_pages, x.v_pages, *t, x.k_scales, x.v_scales) for x, t in zip((close, apart), got)]
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.equal(packed[0][0], packed[1][0]) and torch.equal(raw(close.k_pages), raw(apart.k_pages))
+
+
+def test_a_table_of_one_row_of_any_stride(hexmi):
+    """A column turned into a row is contiguous, whatever its row stride says: read, written in place and as the result."""
+    c = Long([1], [100], 2, 2, 64, 16, 8, torch.float16, seed=5)
+    want_attention = c.run(hexmi)
+    kw = {"k_scales": c.k_scales, "v_scales": c.v_scales}
+    plain = [t.clone() for t in (c.k_pages, c.v_pages)]
+    parents, pages = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    fork = hexmi.paged_fork(*plain, c.page_table, c.lengths_d, parents, pages, **kw)
+    compact = hexmi.paged_compact(*plain, c.page_table, c.lengths_d, k_scales=c.k_scales.clone(), v_scales=c.v_scales.clone())
+    row = c.page_table.clone().view(-1, 1).T
+    assert row.stride() == (1, 1) and row.is_contiguous()
+    c.page_table = row
+    assert torch.equal(c.run(hexmi), want_attention)
+    out = torch.zeros_like(row).view(-1, 1).T
+    table, lengths = hexmi.paged_fork(c.k_pages, c.v_pages, row, c.lengths_d, parents, pages, table_out=out, **kw)
+    assert table is out and torch.equal(out, fork[0]) and torch.equal(lengths, fork[1])
+    table, count = hexmi.paged_compact(c.k_pages, c.v_pages, row, c.lengths_d, table_out=row, **kw)
+    assert table is row and torch.equal(row, compact[0]) and torch.equal(count, compact[1])
