@@ -1085,3 +1085,66 @@ def test_a_table_of_one_row_of_any_stride(hexmi):
     assert table is out and torch.equal(out, fork[0]) and torch.equal(lengths, fork[1])
     table, count = hexmi.paged_compact(c.k_pages, c.v_pages, row, c.lengths_d, table_out=row, **kw)
     assert table is row and torch.equal(row, compact[0]) and torch.equal(count, compact[1])
+
+
+@pytest.mark.parametrize("new", [[1] * 4, [5, 0, 40, 1]])
+def test_append_in_8_bits_into_rows_of_the_callers(hexmi, new):
+    """q's rows into q itself, into rows off the boundaries, into the keys' rows (read by others), and through the dispatcher: all the same."""
+    g, freq = _gen(15), hexmi.rope_frequencies(64)
+    T = sum(new)
+    rows = torch.randn(T, 6, 64, generator=g).half().cuda()
+
+    def call(q_out=None, x=None):
+        c = Long(new, [30, 3, 9, 100], 2, 2, 64, 16, 8, torch.float16, seed=3, ragged=len(set(new)) > 1)
+        x = rows.clone() if x is None else x
+        q_out = q_out(x) if callable(q_out) else q_out
+        y = hexmi.paged_append(x[:, 2:4], x[:, 4:], c.k_pages, c.v_pages, c.page_table, c.lengths_d, c.starts, inv_freq=freq, q=x[:, :2], q_out=q_out,
+                               k_scales=c.k_scales, v_scales=c.v_scales)
+        assert q_out is None or y is q_out
+        return [y.clone(), raw(c.k_pages), raw(c.v_pages), c.k_scales, c.v_scales]
+
+    want = call()
+    odd = torch.zeros(T * 2 * 64 + 1, dtype=torch.float16, device="cuda")[1:].view(T, 2, 64)
+    for q_out in (lambda x: x[:, :2], odd, lambda x: x[:, 2:4], lambda x: x[:, 1:3], torch.zeros(T, 2, 64, dtype=torch.float16)):
+        got = call(q_out)
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
+    previous = hexmi.through_dispatcher(True)
+    try:
+        got = call()
+    finally:
+        hexmi.through_dispatcher(previous)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_what_is_only_read_stays_shared(hexmi):
+    """Attention over copy-on-write pages and scales in 8 bits, and within a window, copies neither; a fork, which writes, has its own."""
+    c = Long([1] * 3, [40, 90, 7], 4, 2, 64, 16, 8, torch.float16, seed=4, window=30, sinks=2)
+    want = c.run(hexmi)
+    plain = {n: getattr(c, n) for n in ("k_pages", "v_pages", "k_scales", "v_scales")}
+    for n, t in plain.items():
+        setattr(c, n, torch._lazy_clone(t))
+    assert torch.equal(c.run(hexmi), want)
+    assert all(torch._C._is_cow_tensor(getattr(c, n)) for n in plain)
+    before = {n: (raw(t) if n in ("k_pages", "v_pages") else t).clone() for n, t in plain.items()}
+    parents, pages = torch.tensor([1], dtype=torch.int32, device="cuda"), torch.tensor([c.k_pages.shape[0] - 1], dtype=torch.int32, device="cuda")
+    hexmi.paged_fork(c.k_pages, c.v_pages, c.page_table, c.lengths_d, parents, pages, c.k_scales, c.v_scales)
+    for n, t in before.items():
+        assert torch.equal(raw(plain[n]) if n in ("k_pages", "v_pages") else plain[n], t), n
+
+
+@pytest.mark.parametrize("block", [2, 8])
+def test_tokens_before_the_first_position_are_left_out(hexmi, block):
+    """More new tokens than a length has positions: those below 0 leave nothing and see nothing, the others are as alone."""
+    g = _gen(6)
+    rows = torch.randn(25, 6, 64, generator=g).half().cuda()
+    results = []
+    for first, n in ((0, 25), (18, 7)):
+        c = Long([7], [0], 2, 2, 64, 16, block, torch.float16, seed=3, ragged=True)
+        starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        x = rows[first:]
+        hexmi.paged_append(x[:, 2:4], x[:, 4:], c.k_pages, c.v_pages, c.page_table, c.lengths_d, starts, k_scales=c.k_scales, v_scales=c.v_scales)
+        kw = {"k_scales": c.k_scales, "v_scales": c.v_scales}
+        out = hexmi.paged_attention(x[:, :2], c.k_pages, c.v_pages, c.page_table, c.lengths_d, starts, window=5, sinks=1, **kw)
+        results.append([out[18 - first:], raw(c.k_pages), raw(c.v_pages), c.k_scales, c.v_scales])
+        assert (out[:18 - first] == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
