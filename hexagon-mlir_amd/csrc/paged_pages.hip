@@ -114,24 +114,26 @@ __device__ __forceinline__ int used_page(const Pages& p, const View& w, int b, i
   const int page = column < w.shared ? w.shared_pages[column] : p.table[b * p.table_row + column];
   return page >= 0 && page < p.num_pages ? page : -1;
 }
-// entry i of the table, row by row, and then of the shared pages, which are in use in any case
+// entry i of the table, row by row
 __device__ __forceinline__ int used_page(const Pages& p, const View& w, int64_t i) {
-  const int64_t in_table = (int64_t)p.sequences * p.table_cols;
-  if (i >= in_table) {
-    const int page = w.shared_pages[i - in_table];
-    return page >= 0 && page < p.num_pages ? page : -1;
-  }
   const int b = (int)(i / p.table_cols);
   return used_page(p, w, b, (int)(i - (int64_t)b * p.table_cols));
 }
+// shared page i, in use in any case
+__device__ __forceinline__ int shared_page(const Pages& p, const View& w, int i) {
+  const int page = w.shared_pages[i];
+  return page >= 0 && page < p.num_pages ? page : -1;
+}
 __global__ __launch_bounds__(256)
 void mark_kernel(Pages p, View w, uint32_t* marks, int64_t entries) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
-    const int page = used_page(p, w, i);
-    if (page < 0) continue;
+  auto mark = [&](int page) __attribute__((always_inline)) {
+    if (page < 0) return;
     const uint32_t bit = 1u << page % 32;
     if (!(__hip_atomic_load(marks + page / 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit)) atomicOr(marks + page / 32, bit);
-  }
+  };
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = first; i < entries; i += step) mark(used_page(p, w, i));
+  for (int64_t i = first; i < w.shared; i += step) mark(shared_page(p, w, (int)i));
 }
 
 // By a workgroup of 1024: how many pages are marked, which of them go where, and their new names. A thread takes a run of words, twice.
@@ -204,6 +206,10 @@ void mark_and_number_kernel(Pages p, View w, CompactSpace s, int32_t* count, int
     const int page = used_page(p, w, i);
     if (page >= 0) atomicOr(marks + page / 32, 1u << page % 32);
   }
+  for (int i = threadIdx.x; i < w.shared; i += 1024) {
+    const int page = shared_page(p, w, i);
+    if (page >= 0) atomicOr(marks + page / 32, 1u << page % 32);
+  }
   __syncthreads();
   number_pages(marks, s, p.num_pages, count);
 }
@@ -213,15 +219,13 @@ __global__ __launch_bounds__(256)
 void move_kernel(CopyArgs c, Pages p, View w, CompactSpace s, const int32_t* count, int32_t* table_out, int64_t table_out_row, int32_t* shared_out,
                  int64_t entries, int parts) {
   const int front = *count, moves = *s.moves;
-  const int64_t in_table = entries - w.shared;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
-    const int page = used_page(p, w, i), name = page >= front ? s.renamed[page] : page;
-    if (i >= in_table) {
-      shared_out[i - in_table] = name;
-      continue;
-    }
-    const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols);
-    table_out[b * table_out_row + column] = name;
+    const int b = (int)(i / p.table_cols), column = (int)(i - (int64_t)b * p.table_cols), page = used_page(p, w, b, column);
+    table_out[b * table_out_row + column] = page >= front ? s.renamed[page] : page;
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < w.shared; i += (int64_t)gridDim.x * 256) {
+    const int page = shared_page(p, w, (int)i);
+    shared_out[i] = page >= front ? s.renamed[page] : page;
   }
   for (int64_t i = blockIdx.x; i < 2 * (int64_t)moves * parts; i += gridDim.x) {
     const int64_t unit = i / parts;
@@ -333,7 +337,7 @@ extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexm
   if (window < 0 || sinks < 0 || ahead < 0 || !count || (batch->sequences * batch->table_cols > 0 && !table_out)) return HEXMI_EINVAL;
   if (shared < 0 || shared > batch->table_cols || (shared > 0 && (!shared_pages || !shared_out))) return HEXMI_EINVAL;
   if (window > 0 && shared > 0) return HEXMI_ENOTSUP;
-  const int64_t entries = batch->sequences * batch->table_cols + shared;
+  const int64_t entries = batch->sequences * batch->table_cols, all = entries + shared;
   if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < hexmi_paged_compact_workspace(batch)) return HEXMI_EINVAL;
   const Pages p = pages_of(*batch);
   const CompactSpace space = space_of(workspace, batch->num_pages);
@@ -344,16 +348,16 @@ extern "C" int hexmi_paged_compact_ex(const hexmi_paged_batch* batch, const hexm
   const int64_t words = words_of(batch->num_pages);
   auto blocks = [](int64_t n, int64_t most) { return dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)); };
   begin_call();
-  if (entries <= kFewEntries && words <= kFewWords) {
+  if (all <= kFewEntries && words <= kFewWords) {
     hipLaunchKernelGGL(mark_and_number_kernel, dim3(1), dim3(1024), 0, s, p, view, space, count, (int)entries);
   } else {
     hipLaunchKernelGGL(clear_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, space.marks, words);
-    if (entries > 0) hipLaunchKernelGGL(mark_kernel, blocks(entries, 4096), dim3(256), 0, s, p, view, space.marks, entries);
+    if (all > 0) hipLaunchKernelGGL(mark_kernel, blocks(all, 4096), dim3(256), 0, s, p, view, space.marks, entries);
     hipLaunchKernelGGL(number_kernel, dim3(1), dim3(1024), 0, s, space, (int)batch->num_pages, count);
   }
   // a workgroup for some KiB of a page; no more than half of the pages move
   const int64_t page_pieces = batch->kv_heads * batch->page_size * c.pieces, parts = (page_pieces + kMovePieces - 1) / kMovePieces;
-  const int64_t units = batch->num_pages * parts > (entries + 255) / 256 ? batch->num_pages * parts : (entries + 255) / 256;
+  const int64_t units = batch->num_pages * parts > (all + 255) / 256 ? batch->num_pages * parts : (all + 255) / 256;
   return with_piece(piece, [&](auto x) {
     hipLaunchKernelGGL((move_kernel<decltype(x)>), dim3((unsigned)(units < 2048 ? units : 2048)), dim3(256), 0, s, c, p, view, space, count, table_out,
                        table_out_row, shared_out, entries, (int)parts);
