@@ -1148,3 +1148,49 @@ def test_tokens_before_the_first_position_are_left_out(hexmi, block):
         results.append([out[18 - first:], raw(c.k_pages), raw(c.v_pages), c.k_scales, c.v_scales])
         assert (out[:18 - first] == 0).all()
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_a_captured_compaction_behind_a_prefix_is_replayed(hexmi):
+    """A fork and a compaction that keeps its pages and a shared prefix, in one graph, replayed as tables, lengths and prefix change."""
+    g = _gen(8)
+    pool, page, cols = 50, 8, 6
+    pages = [torch.randn(pool, 2, page, 64, generator=g).half().cuda() for _ in range(2)]
+    table, lengths = torch.zeros(4, cols, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    prefix, parents, fresh = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (2, 5, 5))
+
+    def both(x, t, n, shared):
+        t, n = hexmi.paged_fork(*x, t, n, parents, fresh)
+        return (t, n, *hexmi.paged_compact(*x, t, n, ahead=1, shared_pages=shared))
+
+    warm = [t.clone() for t in pages]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(warm, table, lengths, prefix)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = both(pages, table, lengths, prefix)
+    for i in range(5):
+        order = torch.randperm(pool, generator=g).int()
+        prefix.copy_(order[:2])
+        fresh.copy_(order[2:7])
+        parents.copy_(torch.randint(-1, 5, (5,), generator=g).int())
+        table.copy_(order[7:7 + 4 * cols].view(4, cols))
+        lengths.copy_(torch.randint(2, cols + 1, (4,), generator=g).int() * page - (torch.arange(4) % 2 * 3).int())
+        for t in pages:
+            t.copy_(torch.randn(t.shape, generator=g).half())
+        eager = [t.clone() for t in pages]
+        graph.replay()
+        want = both(eager, table, lengths, prefix)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results, want)), i
+        assert all(torch.equal(a, b) for a, b in zip(pages, eager)), i
+
+
+def test_the_registered_compaction_takes_its_former_arguments(hexmi):
+    x = [torch.randn(6, 1, 4, 8, generator=_gen(1)).half().cuda() for _ in range(2)]
+    table, lengths = torch.tensor([[5, 1]], dtype=torch.int32, device="cuda"), torch.tensor([8], dtype=torch.int32, device="cuda")
+    out, count = torch.empty_like(table), torch.empty(1, dtype=torch.int32, device="cuda")
+    torch.ops.hexmi.paged_compact(*x, None, None, table, lengths, None, 0, out, count)
+    assert count.item() == 2 and out.tolist() == [[0, 1]]
