@@ -47,13 +47,23 @@ __device__ __forceinline__ float row_max(float v) {
   return v;
 }
 
-// eight values (finite, or NaN for what is not) times `by`, rounded to e4m3, at most `limit`
-__device__ __forceinline__ u32x2 to_codes(const float* y, float by, float limit) {
+// Eight values, ones that are not finite as NaN, over 2^e, rounded to e4m3. Numbers end at 240 times T's largest exponent, which is within 448 2^e
+// where e is below that; where an older exponent leaves fewer bits of it than there are, at the next multiple of 2^(e - 9) below.
+template <typename T>
+__device__ __forceinline__ u32x2 to_codes(const float* y, int e) {
+  constexpr int kOver = kMostExponent<T> + 14;
+  constexpr float kMost = 240.0f * (kMostExponent<T> == 8 ? 0x1p8f : 0x1p120f);
+  static_assert(kMostExponent<T> == 8 || kMostExponent<T> == 120);
+  const float by = __builtin_amdgcn_ldexpf(1.0f, -e);
   float v[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = y[e] * by;
-    v[e] = fabsf(y[e]) < INFINITY ? fminf(fmaxf(x, -limit), limit) : NAN;
+  for (int i = 0; i < 8; ++i) v[i] = fabsf(y[i]) < INFINITY ? fminf(fmaxf(y[i], -kMost), kMost) * by : NAN;
+  if constexpr (kOver < 128) {
+    if (e >= kOver) {
+      const float most = floorf(kMost * by * 512.0f) * 0x1p-9f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] > most ? most : v[i] < -most ? -most : v[i];
+    }
   }
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
@@ -258,22 +268,19 @@ void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, unsign
       const int held = *scale, before = held - 127;
       if (before > e && held != 255) e = before;
       if (e != before && is_head) {                                 // older tokens' numbers again
-        const float f = held == 255 ? NAN : before - e < -126 ? 0.0f : power_of_two(before - e);
+        const float f = held == 255 ? NAN : __builtin_amdgcn_ldexpf(1.0f, before - e);
         for (int s = one ? 0 : group; s < u.old; s += one ? 1 : kRowsAtOnce) {
           u32x2* c = reinterpret_cast<u32x2*>(codes + (s - u.old) * slot_stride);
           *c = codes_again(*c, f);
         }
       }
     }
-    // from the type's largest exponent on numbers end at 240 times it, at a whole multiple of e4m3's least (2^-9)
-    const float by = e < 127 ? power_of_two(-e) : 0x1p-127f;
-    const float limit = e < kMostExponent<T> ? 448.0f : floorf(240.0f * 512.0f * power_of_two(kMostExponent<T> - e)) * 0x1p-9f;
     for (int first = 0; first < passes; first += kHeld) {
       if (passes > kHeld) hold(first);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         const int t = one ? 0 : (first + i) * kRowsAtOnce + group;
-        if (first + i < passes && is_head && t < u.n) *reinterpret_cast<u32x2*>(codes + t * slot_stride) = to_codes(y[i], by, limit);
+        if (first + i < passes && is_head && t < u.n) *reinterpret_cast<u32x2*>(codes + t * slot_stride) = to_codes<T>(y[i], e);
       }
     }
     if (c0 == 0 && is_head && (one || group == 0)) *scale = (uint8_t)(e + 127);
