@@ -55,7 +55,9 @@ template <int W> __device__ __forceinline__ int blocks_of_keys(int keys) {
 }
 // of sequence b, none where it has other than one new token (the tiles take those)
 // View: the most keys that its token sees, and the blocks that a unit counts for beside its own when the work is dealt: to begin one costs
-// a worker about the time of a block in 8 bits.
+// a worker about the time of a block in 8 bits. None / 1 / 2, us: 64 sequences of 100 to 16384 over 8 heads 99.1 / 93.5 / 95.5, 128 of 50 to 2000
+// 53.4 / 45.6 / 46.5, 8 of 100 to 4000 14.0 / 13.7 / 13.5, heads of 80 45.0 / 43.5 / 46.6; the other way round heads of 64 78.6 / 80.8 / 80.8 and
+// lengths that are all the same, 32 x 1000 19.9 / 21.0 / 21.6 (16 x 2048 x 32 heads 65.5 / 65.3 / 65.5).
 struct Dealt {
   int view, extra;
 };

@@ -6,14 +6,17 @@
 // while the largest value is found. A scale is a power of two so that it can rise while a block fills: older numbers keep their bits then, but
 // for what falls below e4m3's normal numbers.
 // Bound by its launch up to some hundred tokens (64 tokens x 32 + 8 heads of 128 5.1 us), then by rows in flight: prompts of 8100 tokens, normed
-// and turned, 46.8 us (3.6 TB/s; a copy of that size 34).
+// and turned, 46.8 us (3.6 TB/s; a copy of that size 34). That is with blocks of 16: 32 and 64 slots, which a wave does not hold and goes through
+// twice, take 69 and 79 us, heads of 256 80 in blocks of 16 and 211 of 64; 600 tokens 10 us, in blocks of 64 32.
 #include "head_rows.h"
 
 namespace hexmi {
 namespace {
 
 // Workgroups wanted for keys and values: a unit's heads are shared while they are fewer. 1024 / 2048 / 4096: prompts of 8100 tokens 46.5 / 50.9 /
-// 51.2 us (every share works out the angles again); keys and values by workgroups of their own 51 (their rows stand side by side).
+// 51.2 us (every share works out the angles again); keys and values by workgroups of their own 51 (their rows stand side by side). 512 / 1024 / 2048
+// over other batches, us: 32 x 100 29.2 / 23.0 / 23.5, blocks of 64 81.9 / 77.3 / 77.5, 32 key heads of 64 77 / 63 / 61, 16000 tokens 99.6 / 99.3 /
+// 97.0, up to 600 tokens and one key head level; heads of 256 69.7 / 77.7 / 77.8.
 constexpr int kUnitGroups = 1024;
 
 // Units (a sequence's new tokens of one block): those of sequence b are numbered from first_unit(b) on, b = -1 .. sequences (first_row). n

@@ -10,7 +10,7 @@
 // The prefix is one sequence that all rows of the batch attend: its keys go through LDS once for kRows rows, whatever sequences they are
 // of. Its sums, and those of tiles whose keys are cut over several workgroups because there are few, go through the workspace.
 //
-// What bounds it. Prompts of 4 x 4096, 32 heads over 8 of 128, bf16: 587 us, 0.93 PFLOP/s (a matrix product of 8192^3 1.12). Without the
+// What bounds it. Prompts of 4 x 4096, 32 heads over 8 of 128, bf16: 589 us, 0.92 PFLOP/s (a matrix product of 8192^3 1.60). Without the
 // copies it takes 432 us, with nothing but them 332: a wave reads all of a block out of LDS for its 32 rows, as many cycles as the matrix
 // instructions take, and two workgroups a compute unit hide that in part. Measured on the way: copies that the compiler knows of (it waits
 // for them before it reads LDS transposed) 609; a lane's own address for every row 687. Few rows are bound by what is one behind the other:
@@ -18,7 +18,8 @@
 //
 // A cache in 8 bits (Scaled) keeps its keys as they are in LDS, half of the reads. bf16 queries are split into two numbers of e4m3 and multiplied
 // with them as they are; fp16's would take three, so for those keys are widened, four instructions a product. Values are widened on their way to
-// LDS. Bound by instruction issue: prompts of 4 x 4096, bf16, 603 us (in 16 bits 574; keys widened 656 for 631, eight columns a lane 616).
+// LDS. Bound by instruction issue: prompts of 4 x 4096, bf16, 612 us (fp16 656; in 16 bits 589). Measured on the way, in turns: keys widened for
+// bf16 too 656 for 631, eight columns a lane 616 for 603.
 #pragma once
 #include "flash_attn_tiles.h"
 #include "paged.h"
