@@ -7,7 +7,7 @@
 // for what falls below e4m3's normal numbers.
 // Bound by its launch up to some hundred tokens (64 tokens x 32 + 8 heads of 128 5.1 us), then by rows in flight: prompts of 8100 tokens, normed
 // and turned, 46.8 us (3.6 TB/s; a copy of that size 34). That is with blocks of 16: 32 and 64 slots, which a wave does not hold and goes through
-// twice, take 69 and 79 us, heads of 256 80 in blocks of 16 and 211 of 64; 600 tokens 10 us, in blocks of 64 32.
+// twice, take 65 and 79 us, heads of 256 76 in blocks of 16 and 212 of 64; 600 tokens 10 us, in blocks of 64 32.
 #include "head_rows.h"
 
 namespace hexmi {
@@ -15,8 +15,8 @@ namespace {
 
 // Workgroups wanted for keys and values: a unit's heads are shared while they are fewer. 1024 / 2048 / 4096: prompts of 8100 tokens 46.5 / 50.9 /
 // 51.2 us (every share works out the angles again); keys and values by workgroups of their own 51 (their rows stand side by side). 512 / 1024 / 2048
-// over other batches, us: 32 x 100 29.2 / 23.0 / 23.5, blocks of 64 81.9 / 77.3 / 77.5, 32 key heads of 64 77 / 63 / 61, 16000 tokens 99.6 / 99.3 /
-// 97.0, up to 600 tokens and one key head level; heads of 256 69.7 / 77.7 / 77.8.
+// over other batches, us: 32 x 100 25.8 / 21.9 / 22.5, blocks of 64 81.5 / 77.1 / 77.3, up to 600 tokens and one key head level; the other way round
+// 32 key heads of 64 76 / 59 / 54, 16000 tokens 92.0 / 92.2 / 87.8, heads of 256 68.5 / 73.5 / 73.2.
 constexpr int kUnitGroups = 1024;
 
 // Units (a sequence's new tokens of one block): those of sequence b are numbered from first_unit(b) on, b = -1 .. sequences (first_row). n
@@ -121,7 +121,8 @@ __device__ __forceinline__ Unit unit_at(const Pages& p, const Scales& sc, int un
 // kv_grid workgroups take a unit and a share of its heads each, q_grid the queries, as head_rows_kernel does; eights of both kinds by turns
 // (workgroup ids go round robin to the 8 XCDs), so that neither waits for the other: prompts of 8100 tokens 46.6 us, one kind behind the other
 // 56. LPR lanes take a row, eight columns each (HALVES, PIECES: head_rows.h). A wave holds kHeld times the rows that it has at once, so that rows of a block are read and
-// turned once; larger blocks are gone through twice.
+// turned once; larger blocks are gone through twice. 2 / 4 / 8 times, us: prompts of 8100 tokens 56.2 / 47.6 / 57.2 (more registers, fewer waves), blocks of
+// 64 81.4 / 77.1 / 84.6, 600 tokens 12.9 / 10.2 / 12.0, 32 x 100 26.6 / 22.1 / 28.4, heads of 64 57.9 / 58.9 / 83.6; but heads of 256 74.9 / 73.7 / 66.5.
 template <typename T, int LPR, bool HALVES, bool PIECES>
 __global__ __launch_bounds__(256, 4)
 void scaled_rows_kernel(HeadArgs a, Pages p, Scales sc, unsigned kv_grid, unsigned q_grid, int shares, int q_waves) {
